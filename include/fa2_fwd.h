@@ -230,6 +230,120 @@ FA2_API int fa2_default_config(int32_t head_dim, int32_t* block_m, int32_t* bloc
  */
 FA2_API int fa2_should_pack_gqa(int32_t n_q, int32_t group, int32_t block_m);
 
+/*
+ * ---- Serving: packed sequences, a paged K/V cache and rotary positions. No counterpart in the
+ * reference (its README.md:308-315 lists variable lengths and decoding as out of scope).
+ *
+ * Rows of several sequences lie back to back: sequence s owns rows cu[s] .. cu[s + 1] - 1 of a packed
+ * tensor [n_tokens, heads, head_dim] (cu: int32, n_seq + 1 ascending entries on the device; rows past
+ * cu[n_seq] belong to none and are left as they are). Lengths, page tables and positions are read on the
+ * device by the launch itself: nothing is copied to the host, a captured launch follows what they hold at
+ * each replay, and no value of theirs makes a launch read or write outside the tensors.
+ * Strides are element strides with a unit head_dim stride; 16-bit pointers are 16-byte aligned and their
+ * strides non-negative multiples of 8 elements, K and V rows at most 2^22 elements apart.
+ */
+
+/* Element type of a cache that holds e4m3 (OCP, no infinities), with a scale byte per row. */
+#define FA2_DTYPE_E4M3 2
+
+/*
+ * A paged cache: k and v [n_pages, h_kv, page_size, head_dim], strides [page, head, token]. cache_dtype is
+ * FA2_DTYPE_F16, FA2_DTYPE_BF16 or FA2_DTYPE_E4M3; with e4m3, strides are multiples of 16 bytes and
+ * k_scale and v_scale [n_pages, h_kv, page_size] hold a byte e per row, whose values are e4m3 * 2^(e - 127)
+ * (e8m0). page_size is a power of two of at least 16, and a page holds at least 1 KiB of each head's
+ * rows (so head_dim 16 takes pages of 32 tokens, or 64 in e4m3, and head_dim 32 pages of 32 in e4m3).
+ */
+typedef struct fa2_cache {
+  void* k;
+  void* v;
+  void* k_scale;
+  void* v_scale;
+  int64_t k_stride[3], v_stride[3];
+  int64_t k_scale_stride[3], v_scale_stride[3];
+  int32_t n_pages, h_kv, page_size, head_dim, cache_dtype;
+} fa2_cache;
+
+/*
+ * Sequences over a paged cache, all device pointers: lens[s] tokens of sequence s are in the cache, the
+ * sequence's packed rows being the last of them; token p lies in page table[s * table_stride + p / page_size]
+ * at row p % page_size. max_pages: entries per row of the table.
+ */
+typedef struct fa2_sequences {
+  const int32_t* cu;
+  const int32_t* lens;
+  const int32_t* table;
+  int64_t table_stride;
+  int32_t n_seq, n_tokens, max_pages;
+} fa2_sequences;
+
+/*
+ * Rotation of a row's first 2 * half values (a multiple of 16, at most head_dim; the rest are copied):
+ * pairs (i, i + half), or (2 i, 2 i + 1) when interleaved, by the angle position * freqs[i] (device
+ * float64[half], radians), times scale. Angles are formed in float64.
+ */
+typedef struct fa2_rotation {
+  const double* freqs;
+  int32_t half, interleaved;
+  double scale;
+} fa2_rotation;
+
+/*
+ * fa2_rotary - out = x rotated. x and out [batch, heads, n, head_dim], strides [b, h, n]; out may be x.
+ * positions: device int32 or int64 (position_bytes 4 or 8), strides [b, n] (0 repeats).
+ */
+FA2_API int fa2_rotary(const void* x, void* out, const int64_t x_stride[3], const int64_t o_stride[3],
+                       const void* positions, int32_t position_bytes, const int64_t p_stride[2],
+                       const fa2_rotation* rotation, int32_t batch, int32_t heads, int32_t n,
+                       int32_t head_dim, int32_t dtype, void* stream);
+
+/*
+ * fa2_cache_write - every packed row's k and v [n_tokens, h_kv, head_dim] (strides [token, head]) into its
+ * place in the cache. With a rotation k is rotated by its position in the sequence first, and q
+ * [n_tokens, h_q, head_dim], if not null, into q_out (which may be q). 16-bit caches are of the rows' own
+ * type. An e4m3 row is written as the nearest e4m3 values of x / 2^e, e the least integer with
+ * max|x| <= 448 * 2^e over the row's finite values (and e at most 8, |x| at most 61440, in fp16, or e at most
+ * 120 in bf16); NaN and infinities are stored as NaN. Rows without a place (before a sequence's start, past the
+ * table, in a page that the cache does not have) are not written; q is rotated all the same, except
+ * rows of no sequence or before a sequence's start, which are left as they are. Two rows with one place are the
+ * caller's to avoid: which of them stays, in whole or in parts, is not defined.
+ */
+FA2_API int fa2_cache_write(const fa2_cache* cache, const fa2_sequences* seq, const void* k, const void* v,
+                            const int64_t k_stride[2], const int64_t v_stride[2],
+                            const void* q, void* q_out, const int64_t q_stride[2],
+                            const int64_t qo_stride[2], int32_t h_q, const fa2_rotation* rotation,
+                            int32_t dtype, void* stream);
+
+/*
+ * fa2_cache_read - the mirror of fa2_cache_write: every packed row's k and v out of the cache, as dtype
+ * (a 16-bit cache's own). A place past the table or in a page that the cache does not have
+ * reads as zeros; rows of no sequence or before a sequence's start are left as they are.
+ */
+FA2_API int fa2_cache_read(const fa2_cache* cache, const fa2_sequences* seq, void* k, void* v,
+                           const int64_t k_stride[2], const int64_t v_stride[2], int32_t dtype, void* stream);
+
+/*
+ * fa2_attn_packed - attention within each of n_seq packed sequences: q and out [n_tokens, h_q, head_dim], k
+ * and v [kv_tokens, h_kv, head_dim], strides [token, head]. cu_kv gives the sequences of k and v (NULL: cu,
+ * and kv_tokens == n_tokens). causal: aligned at the end, the sequence's last row sees its last key, row i
+ * keys up to i + n_kv - n_q. A row that sees no key gets 0 and a log-sum-exp of -inf.
+ * lse: NULL, or float[h_q * n_tokens], natural logarithm, row h * n_tokens + t.
+ */
+FA2_API int fa2_attn_packed(const void* q, const void* k, const void* v, void* out,
+                            const int64_t q_stride[2], const int64_t k_stride[2],
+                            const int64_t v_stride[2], const int64_t o_stride[2],
+                            const int32_t* cu, const int32_t* cu_kv, int32_t n_seq, int32_t n_tokens,
+                            int32_t kv_tokens, int32_t h_q, int32_t h_kv, int32_t head_dim, int32_t dtype,
+                            int32_t causal, float qk_scale, float* lse, void* stream);
+
+/*
+ * fa2_attn_paged - attention of every sequence's packed rows over its lens[s] tokens in the cache (their own k
+ * and v written there first: fa2_cache_write), masks and lse as in fa2_attn_packed. dtype is q's and out's type, and
+ * a 16-bit cache's; e4m3 values are read in that type. A sequence that a page outside the cache reaches gets NaN in the rows that see it.
+ */
+FA2_API int fa2_attn_paged(const void* q, void* out, const int64_t q_stride[2], const int64_t o_stride[2],
+                           const fa2_cache* cache, const fa2_sequences* seq, int32_t h_q, int32_t dtype,
+                           int32_t causal, float qk_scale, float* lse, void* stream);
+
 /* Thread-local description of the last failure in this thread ("" if none). */
 FA2_API const char* fa2_last_error(void);
 

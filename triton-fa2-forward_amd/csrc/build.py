@@ -3,8 +3,9 @@ measurement library libfa2_ablate.so beside it.
 
     python triton-fa2-forward_amd/csrc/build.py [-j 8] [--verbose]
 
-Compiles attn_fwd_inst.hip once per (dtype, head_dim) pair plus the split-KV combine pass
-(attn_fwd_combine.hip), the key-norm pass (attn_key_norm.hip) and the C-ABI file fa2_fwd.hip,
+Compiles attn_fwd_inst.hip and attn_ragged_inst.hip once per (dtype, head_dim) pair plus the split-KV
+combine pass (attn_fwd_combine.hip), the key-norm pass (attn_key_norm.hip), the rotary and cache kernels
+(serve_cache.hip) and the C-ABI file fa2_fwd.hip,
 in parallel, with hipcc for gfx950 only, and links them into
 triton-fa2-forward_amd/fa2/libfa2_fwd.so next to the Python front end that loads it. Beside it goes
 fa2/_torch_call.so, the front end's native common call (fa2_torch.cpp, against the installed torch). Then builds
@@ -144,7 +145,10 @@ def build_variant(name, defines, jobs=8, verbose=False):
             cmds.append([cc, *flags, f"-DFA2_DT={dt}", f"-DFA2_D={d}", "-c",
                          os.path.join(CSRC, "attn_fwd_inst.hip"), "-o",
                          os.path.join(obj_dir, f"attn_fwd_dt{dt}_d{d}.o")])
-    for name_ in ("attn_fwd_combine", "attn_fwd_wavesplit", "attn_key_norm", "fa2_fwd", "fa2_scratch"):
+            cmds.append([cc, *flags, f"-DFA2_DT={dt}", f"-DFA2_D={d}", "-c",
+                         os.path.join(CSRC, "attn_ragged_inst.hip"), "-o",
+                         os.path.join(obj_dir, f"attn_ragged_dt{dt}_d{d}.o")])
+    for name_ in ("attn_fwd_combine", "attn_fwd_wavesplit", "attn_key_norm", "serve_cache", "fa2_fwd", "fa2_scratch"):
         cmds.append([cc, *flags, "-c", os.path.join(CSRC, name_ + ".hip"), "-o",
                      os.path.join(obj_dir, name_ + ".o")])
     with ThreadPoolExecutor(max_workers=max(1, jobs)) as ex:
@@ -162,16 +166,22 @@ def build(jobs=8, verbose=False):
     """Compile every kernel instance and link both libraries. Returns the product .so path."""
     os.makedirs(OBJ_DIR, exist_ok=True)
     cc = hipcc()
-    units, ablate_units = [], []
+    units, serve_units, ablate_units = [], [], []
     for dt in DTYPES:
         for d in HEAD_DIMS:
             obj = os.path.join(OBJ_DIR, f"attn_fwd_dt{dt}_d{d}.o")
             units.append([cc, *common_flags(), "-Rpass-analysis=kernel-resource-usage",
                           f"-DFA2_DT={dt}", f"-DFA2_D={d}", "-c",
                           os.path.join(CSRC, "attn_fwd_inst.hip"), "-o", obj])
+            obj = os.path.join(OBJ_DIR, f"attn_ragged_dt{dt}_d{d}.o")
+            serve_units.append([cc, *common_flags(), "-Rpass-analysis=kernel-resource-usage",
+                                f"-DFA2_DT={dt}", f"-DFA2_D={d}", "-c",
+                                os.path.join(CSRC, "attn_ragged_inst.hip"), "-o", obj])
             obj = os.path.join(OBJ_DIR, f"attn_fwd_ablate_dt{dt}_d{d}.o")
             ablate_units.append([cc, *common_flags(), f"-DFA2_DT={dt}", f"-DFA2_D={d}", "-c",
                                  os.path.join(CSRC, "attn_fwd_ablate_inst.hip"), "-o", obj])
+    serve_units.append([cc, *common_flags(), "-c", os.path.join(CSRC, "serve_cache.hip"),
+                        "-o", os.path.join(OBJ_DIR, "serve_cache.o")])
     shared = []
     for name in ("attn_fwd_wavesplit", "attn_fwd_combine", "attn_key_norm"):
         remarks = ["-Rpass-analysis=kernel-resource-usage"] if name == "attn_fwd_wavesplit" else []
@@ -193,7 +203,7 @@ def build(jobs=8, verbose=False):
                   "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM", f'-DFA2_BUILT_FOR="{torch_build_id()}"', "-I", INCLUDE,
                   *(f for p in torch_paths()[0] for f in ("-isystem", p)), "-c",
                   os.path.join(CSRC, "fa2_torch.cpp"), "-o", torch_obj]
-    everything = units + shared + [api, scratch] + ablate_units + [ablate_api, ablate_split, ceiling, torch_call]
+    everything = units + shared + serve_units + [api, scratch] + ablate_units + [ablate_api, ablate_split, ceiling, torch_call]
     with ThreadPoolExecutor(max_workers=max(1, jobs)) as ex:
         errs = list(ex.map(lambda cmd: _run(cmd, verbose), everything))
 
@@ -211,7 +221,7 @@ def build(jobs=8, verbose=False):
         os.replace(path + ".tmp", path)
 
     shared_objs = [u[-1] for u in shared]
-    link([u[-1] for u in units] + shared_objs + [api[-1], scratch[-1]], LIB_PATH)
+    link([u[-1] for u in units + serve_units] + shared_objs + [api[-1], scratch[-1]], LIB_PATH)
     link([u[-1] for u in ablate_units] + shared_objs + [ablate_api[-1], ablate_split[-1], ceiling[-1]],
          ABLATE_LIB_PATH)
     _run(["g++", "-shared", "-fPIC", "-o", TORCH_CALL_PATH + ".tmp", torch_obj,

@@ -1,0 +1,76 @@
+// serve_common.hpp - device helpers of the serving kernels: which sequence a packed row belongs to,
+// where a token lies in the cache, and the conversion between 16-bit rows and e4m3 rows.
+#pragma once
+
+#include "attn_fwd_common.hpp"
+#include "serve_params.hpp"
+
+namespace fa2 {
+
+template <int DT>
+__device__ __forceinline__ float to_f32(uint16_t x) {
+  if constexpr (DT == 0) return (float)__builtin_bit_cast(_Float16, x);
+  return __uint_as_float((uint32_t)x << 16);
+}
+
+// cu[i], held to [0, n_tokens]: no row outside the tensors is ever addressed, whatever cu holds.
+__device__ __forceinline__ int row_bound(const int32_t* cu, int i, int n_tokens) {
+  return min(max(cu[i], 0), n_tokens);
+}
+
+// The largest s in [0, n_seq) with cu[s] <= t, for ascending cu (some s in [0, n_seq) otherwise). All 64
+// lanes of a wave ask for one t; each round tests 64 sequences at once, so a call of up to 64
+// sequences waits for one load, up to 4096 for two.
+__device__ __forceinline__ int find_sequence(const int32_t* cu, int n_seq, int t, int lane) {
+  int lo = 0, n = n_seq;  // the answer lies in [lo, lo + n)
+  while (n > 1) {
+    const int step = (n + 63) / 64;
+    const int i = lane * step;
+    const uint64_t below = __builtin_amdgcn_ballot_w64(i < n && cu[lo + (i < n ? i : 0)] <= t);
+    const int c = max(__builtin_popcountll(below) - 1, 0);
+    lo += c * step;
+    n = min(step, n - c * step);
+  }
+  return lo;
+}
+
+// A packed row's sequence and position in it; seq < 0: the row belongs to none, or its place is before
+// the sequence's start (more rows than tokens).
+struct Place {
+  int seq;
+  int pos;
+  int page;  // -1: past the table, or not a page of the cache
+};
+__device__ __forceinline__ Place find_place(const Sequences& q, int t, int lane) {
+  Place p = {-1, 0, -1};
+  if (t >= q.n_tokens) return p;
+  const int s = find_sequence(q.cu, q.n_seq, t, lane);
+  const int end = row_bound(q.cu, s + 1, q.n_tokens);
+  if (t < row_bound(q.cu, s, q.n_tokens) || t >= end) return p;
+  const int64_t pos = (int64_t)max(q.lens[s], 0) - (end - t);
+  if (pos < 0) return p;
+  p.seq = s;
+  p.pos = (int)pos;
+  const int slot = p.pos >> q.page_shift;
+  if (slot < q.max_pages) {
+    const int page = q.table[s * q.table_stride + slot];
+    if ((unsigned)page < (unsigned)q.n_pages) p.page = page;
+  }
+  return p;
+}
+
+// 2^(byte - 127) of an e8m0 scale byte (255: NaN)
+__device__ __forceinline__ float e8m0_to_f32(uint32_t b) {
+  return __uint_as_float(b == 0 ? 0x00400000u : b == 255u ? 0x7fc00000u : b << 23);
+}
+
+// 4 e4m3 values of a word times scale, rounded to the 16-bit type (exactly, but where the product leaves
+// the type's range): two packed pairs.
+template <int DT>
+__device__ __forceinline__ u32x2 e4m3_to_16(uint32_t w, float scale) {
+  const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false);
+  const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+  return u32x2{Elem<DT>::pack2(lo[0] * scale, lo[1] * scale), Elem<DT>::pack2(hi[0] * scale, hi[1] * scale)};
+}
+
+}  // namespace fa2

@@ -1,0 +1,35 @@
+// serve_launch.hpp - launchers of the serving kernels. Each returns a hipError_t value.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include "serve_params.hpp"
+
+namespace fa2 {
+
+// Tokens of one workgroup of the rotary and cache kernels: as many as its 256 lanes take rows of at once.
+int serve_tokens_per_wg(int lanes_per_token);
+
+int launch_rotary(int dtype, int head_dim, const RotaryParams& p, unsigned grid, hipStream_t stream);
+int launch_cache(bool write, int dtype, int head_dim, bool e4m3, const CacheParams& p, unsigned grid,
+                 hipStream_t stream);
+
+// Where K and V of a ragged attention launch lie: packed rows, 16-bit pages, e4m3 pages.
+constexpr int kSourcePacked = 0, kSourcePages = 1, kSourceE4m3 = 2;
+
+template <int DT, int D>
+int launch_ragged(const RaggedParams& p, int source, unsigned grid, hipStream_t stream);
+
+#define FA2_DECLARE_RAGGED(DT, D) \
+  extern template int launch_ragged<DT, D>(const RaggedParams&, int, unsigned, hipStream_t);
+FA2_DECLARE_RAGGED(0, 16)
+FA2_DECLARE_RAGGED(0, 32)
+FA2_DECLARE_RAGGED(0, 64)
+FA2_DECLARE_RAGGED(0, 128)
+FA2_DECLARE_RAGGED(1, 16)
+FA2_DECLARE_RAGGED(1, 32)
+FA2_DECLARE_RAGGED(1, 64)
+FA2_DECLARE_RAGGED(1, 128)
+#undef FA2_DECLARE_RAGGED
+
+}  // namespace fa2

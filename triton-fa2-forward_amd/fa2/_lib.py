@@ -16,6 +16,28 @@ LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libfa2_fwd.
 
 # C-ABI symbols declared in include/fa2_fwd.h, with (restype, argtypes).
 _i32, _i64p, _vp = ctypes.c_int32, ctypes.POINTER(ctypes.c_int64), ctypes.c_void_p
+_i64x3 = ctypes.c_int64 * 3
+
+
+class Cache(ctypes.Structure):
+    """fa2_cache"""
+    _fields_ = [("k", _vp), ("v", _vp), ("k_scale", _vp), ("v_scale", _vp), ("k_stride", _i64x3),
+                ("v_stride", _i64x3), ("k_scale_stride", _i64x3), ("v_scale_stride", _i64x3), ("n_pages", _i32),
+                ("h_kv", _i32), ("page_size", _i32), ("head_dim", _i32), ("cache_dtype", _i32)]
+
+
+class Sequences(ctypes.Structure):
+    """fa2_sequences"""
+    _fields_ = [("cu", _vp), ("lens", _vp), ("table", _vp), ("table_stride", ctypes.c_int64), ("n_seq", _i32),
+                ("n_tokens", _i32), ("max_pages", _i32)]
+
+
+class Rotation(ctypes.Structure):
+    """fa2_rotation"""
+    _fields_ = [("freqs", _vp), ("half", _i32), ("interleaved", _i32), ("scale", ctypes.c_double)]
+
+
+_cachep, _seqp, _rotp = (ctypes.POINTER(t) for t in (Cache, Sequences, Rotation))
 SIGNATURES = {
     "fa2_attn_fwd": (ctypes.c_int, [_vp, _vp, _vp, _vp, _i64p, _i64p, _i64p, _i64p,
                                     _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32,
@@ -35,11 +57,21 @@ SIGNATURES = {
     "fa2_default_config": (ctypes.c_int, [_i32, ctypes.POINTER(_i32), ctypes.POINTER(_i32),
                                           ctypes.POINTER(_i32), ctypes.POINTER(_i32)]),
     "fa2_should_pack_gqa": (ctypes.c_int, [_i32, _i32, _i32]),
+    "fa2_rotary": (ctypes.c_int, [_vp, _vp, _i64p, _i64p, _vp, _i32, _i64p, _rotp, _i32, _i32, _i32, _i32, _i32,
+                                  _vp]),
+    "fa2_cache_write": (ctypes.c_int, [_cachep, _seqp, _vp, _vp, _i64p, _i64p, _vp, _vp, _i64p, _i64p, _i32, _rotp,
+                                       _i32, _vp]),
+    "fa2_cache_read": (ctypes.c_int, [_cachep, _seqp, _vp, _vp, _i64p, _i64p, _i32, _vp]),
+    "fa2_attn_packed": (ctypes.c_int, [_vp, _vp, _vp, _vp, _i64p, _i64p, _i64p, _i64p, _vp, _vp, _i32, _i32, _i32,
+                                       _i32, _i32, _i32, _i32, _i32, ctypes.c_float, _vp, _vp]),
+    "fa2_attn_paged": (ctypes.c_int, [_vp, _vp, _i64p, _i64p, _cachep, _seqp, _i32, _i32, _i32, ctypes.c_float,
+                                      _vp, _vp]),
     "fa2_last_error": (ctypes.c_char_p, []),
     "fa2_version": (ctypes.c_char_p, []),
 }
 
 DTYPE_CODE = {torch.float16: 0, torch.bfloat16: 1}
+CACHE_DTYPE_CODE = {**DTYPE_CODE, torch.float8_e4m3fn: 2}
 
 _LIB = None
 
@@ -90,7 +122,8 @@ _STRIDES = {}
 
 
 def _strides(t):
-    """The element strides as the C array the ABI takes. The stride of a size-1 dimension never
+    """The element strides as the C array the ABI takes (four; the entry points of packed rows and of the
+    cache read the first two or three). The stride of a size-1 dimension never
     enters an address; pass 0 so that only the strides the kernel actually steps by are checked
     against the 16-byte rule. The arrays are cached per (shape, strides): the library only reads
     them during the call, and building one costs more than the rest of a small call."""
@@ -171,3 +204,71 @@ def workspace_bytes_for(B, H_q, H_kv, N_q, N_kv, D, dtype, causal, num_splits):
 def num_splits(B, H_q, H_kv, N_q, N_kv, D, causal, block_m, block_n, num_cus):
     return int(lib().fa2_num_splits(B, H_q, H_kv, N_q, N_kv, D, int(bool(causal)), block_m,
                                     block_n, num_cus))
+
+
+# ---- serving: packed sequences, the paged cache, rotary positions
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _checked(rc, name):
+    if rc != 0:
+        raise RuntimeError(f"{name} failed ({rc}): {last_error()}")
+
+
+def cache_of(cache):
+    """The C description of a fa2.paged.KVCache that satisfies its checks."""
+    pages, h_kv, page_size, head_dim = cache.k.shape
+
+    def strides(t):
+        return _i64x3(*([0] * 3 if t is None else (0 if n == 1 else s for n, s in zip(t.shape[:3], t.stride()))))
+
+    return Cache(_ptr(cache.k), _ptr(cache.v), _ptr(cache.k_scale), _ptr(cache.v_scale), strides(cache.k),
+                 strides(cache.v), strides(cache.k_scale), strides(cache.v_scale), pages, h_kv, page_size,
+                 head_dim, CACHE_DTYPE_CODE[cache.k.dtype])
+
+
+def sequences_of(cu, lens, table, n_tokens):
+    """The C description of sequences over a cache (dense int32 tensors; table rows any distance apart)."""
+    return Sequences(_ptr(cu), _ptr(lens), _ptr(table), 0 if table.shape[0] == 1 else table.stride(0),
+                     lens.numel(), n_tokens, table.shape[1])
+
+
+def rotary(x, out, positions, rotation, stream):
+    """Call fa2_rotary on [B, H, N, D] tensors and positions [B, N]."""
+    B, H, N, D = x.shape
+    _checked(lib().fa2_rotary(x.data_ptr(), out.data_ptr(), _strides(x), _strides(out), positions.data_ptr(),
+                              positions.element_size(), (ctypes.c_int64 * 2)(*positions.stride()),
+                              ctypes.byref(rotation), B, H, N, D, DTYPE_CODE[x.dtype], stream), "fa2_rotary")
+
+
+def cache_write(cache, seq, k, v, q, q_out, rotation, stream):
+    """Call fa2_cache_write; q, q_out and rotation may be None."""
+    _checked(lib().fa2_cache_write(
+        ctypes.byref(cache), ctypes.byref(seq), k.data_ptr(), v.data_ptr(), _strides(k), _strides(v), _ptr(q),
+        _ptr(q_out), None if q is None else _strides(q), None if q is None else _strides(q_out),
+        0 if q is None else q.shape[1], None if rotation is None else ctypes.byref(rotation), DTYPE_CODE[k.dtype],
+        stream), "fa2_cache_write")
+
+
+def cache_read(cache, seq, k, v, stream):
+    """Call fa2_cache_read."""
+    _checked(lib().fa2_cache_read(ctypes.byref(cache), ctypes.byref(seq), k.data_ptr(), v.data_ptr(), _strides(k),
+                                  _strides(v), DTYPE_CODE[k.dtype], stream), "fa2_cache_read")
+
+
+def attn_packed(q, k, v, out, cu, cu_kv, causal, qk_scale, lse, stream):
+    """Call fa2_attn_packed; cu_kv and lse may be None."""
+    T, H_q, D = q.shape
+    _checked(lib().fa2_attn_packed(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _strides(q), _strides(k), _strides(v),
+        _strides(out), cu.data_ptr(), _ptr(cu_kv), cu.numel() - 1, T, k.shape[0], H_q, k.shape[1], D,
+        DTYPE_CODE[q.dtype], int(bool(causal)), qk_scale, _ptr(lse), stream), "fa2_attn_packed")
+
+
+def attn_paged(q, out, cache, seq, causal, qk_scale, lse, stream):
+    """Call fa2_attn_paged; lse may be None."""
+    _checked(lib().fa2_attn_paged(q.data_ptr(), out.data_ptr(), _strides(q), _strides(out), ctypes.byref(cache),
+                                  ctypes.byref(seq), q.shape[1], DTYPE_CODE[q.dtype], int(bool(causal)), qk_scale,
+                                  _ptr(lse), stream), "fa2_attn_paged")
