@@ -232,9 +232,9 @@ def write(cache, seq, k=P, dtype=1, q=None, q_out=None, rotation=None, h_q=4, ks
                                       None if rotation is None else ctypes.byref(rotation), dtype, None)
 
 
-def paged(cache, seq, q=P, dtype=1, h_q=4, scale=0.1, lse=None):
+def paged(cache, seq, q=P, dtype=1, h_q=4, scale=0.1, lse=None, ws=P, n_ws=1 << 40):
     s = strides(256, 64)
-    return _lib.lib().fa2_attn_paged(q, P, s, s, ctypes.byref(cache), ctypes.byref(seq), h_q, dtype, 1, scale, lse, None)
+    return _lib.lib().fa2_attn_paged(q, P, s, s, ctypes.byref(cache), ctypes.byref(seq), h_q, dtype, 1, scale, lse, ws, n_ws, None)
 
 
 @needs_lib
@@ -244,7 +244,8 @@ def paged(cache, seq, q=P, dtype=1, h_q=4, scale=0.1, lse=None):
     (dict(head_dim=48), -1), (dict(head_dim=16), -1), (dict(k=None), -1), (dict(v=P + 8), -2),
     (dict(k_stride=(2048, 1024, 60)), -2), (dict(v_stride=(-2048, 1024, 64)), -2), (dict(k_stride=(2048, 1024, 1 << 23)), -1),
     (dict(cache_dtype=2, k_scale=P, v_scale=P, k_stride=(2048, 1024, 72)), -2),
-    (dict(cache_dtype=2, k_scale=P, v_scale=P, k_scale_stride=(-1, 0, 0)), -1)])
+    (dict(cache_dtype=2, k_scale=P, v_scale=P, k_scale_stride=(-1, 0, 0)), -1),
+    (dict(cache_dtype=2, k_scale=P, v_scale=P, v_scale_stride=(32, 16, 1 << 23)), -1)])
 def test_c_cache_refusals(change, code):
     cache = c_cache(**change)
     s = strides(128, 64)
@@ -281,6 +282,14 @@ def test_c_call_refusals():
     assert paged(c_cache(), c_seq(), q=None) == -1
     assert paged(c_cache(), c_seq(), lse=P + 2) == -2
     assert paged(c_cache(), c_seq(n_tokens=1 << 30), h_q=8) == -1  # 2^32 rows of a KV head
+    need = _lib.paged_workspace_bytes(4, 2, 64, 3, 2, 256)
+    assert need > 0
+    assert paged(c_cache(), c_seq(), ws=None) == -1 and "workspace" in _lib.last_error()
+    assert paged(c_cache(), c_seq(), n_ws=need - 1) == -1 and str(need) in _lib.last_error()
+    assert paged(c_cache(), c_seq(), ws=P + 128) == -2
+    for sizes in ((3, 2, 64, 3, 2, 256), (4, 2, 48, 3, 2, 256), (4, 2, 64, 0, 2, 256), (4, 2, 64, 3, 0, 256), (4, 2, 64, 3, 2, 0)):
+        assert _lib.paged_workspace_bytes(*sizes) == 0
+    assert _lib.paged_workspace_bytes(32, 8, 128, 1 << 20, 4, 256) == 0  # row tiles enough: none are shared
     assert _lib.lib().fa2_cache_write(None, None, P, P, None, None, None, None, None, None, 0, None, 1, None) == -1
     # nothing to do
     assert write(c_cache(), c_seq(n_tokens=0)) == 0 and write(c_cache(), c_seq(n_seq=0, cu=None)) == 0

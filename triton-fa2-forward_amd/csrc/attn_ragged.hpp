@@ -6,62 +6,31 @@
 //   last key. A row that sees no key gets O = 0 and a log-sum-exp of -inf.
 //
 // All query heads of a KV head share a workgroup's rows: row r of a sequence is position r / group, head
-// r % group. Lengths are known on the device only, so the grid covers the most row tiles that n_tokens
-// rows in n_seq sequences can have, and a workgroup finds its own (sequence, tile) by a scan of cu, 64
-// sequences at a time; workgroups past the last tile exit.
+// r % group. Which rows and keys a workgroup takes: ragged_work.hpp.
 //
-// The tile arithmetic is attn_fwd_wavesplit.hpp's: 32 rows, S^T = K Q^T and O^T += V^T P^T with
-// v_mfma_f32_32x32x16, P in registers, online softmax in base 2 with a lazily moved reference. Here the
-// four waves of a workgroup take the key tiles of its 32 rows in turn, each through LDS buffers of its
-// own, and merge once in LDS.
+// The tile arithmetic is attn_fwd_kernel.hpp's: S^T = K Q^T and O^T += V^T P^T with v_mfma_f32_32x32x16, P
+// in registers, online softmax in base 2 with a lazily moved reference. Two forms:
+//   * GW = 4: 128 rows, 32 a wave, which walk tiles of 64 keys together (attn_fwd_kernel.hpp's one-tile
+//     loop: one barrier per tile, K two tiles and V one tile ahead). For prompts and chunks of them.
+//   * GW = 1: 32 rows, whose key tiles the four waves take in turn, each through LDS buffers of its own without
+//     a barrier, and merge once in LDS (attn_fwd_wavesplit.hpp). For single tokens and small grids.
+// K and V rows of 16 bits go from HBM to LDS directly; the rows of one load instruction lie in one page (the
+// host's rule on page sizes), so a load has one scalar resource, and the pages of the next 64 loads' worth of tiles
+// sit in a register, a lane each. e4m3 rows go through registers, converted to the 16-bit type on
+// their way into LDS (once per workgroup or wave, not once per operand read): from there on the sources are alike.
 #pragma once
 
 #include "attn_fwd_wavesplit.hpp"
-#include "serve_common.hpp"
-#include "serve_launch.hpp"
+#include "ragged_work.hpp"
 
 namespace fa2 {
 
-// Keys per tile of one wave
-constexpr int ragged_block_n(int head_dim) { return head_dim == 128 ? 32 : 64; }
-
-// Sum over the lanes before and at this one
-__device__ __forceinline__ int wave_scan(int x, int lane) {
-#pragma unroll
-  for (int off = 1; off < 64; off *= 2) {
-    const int y = __shfl_up(x, off, 64);
-    if (lane >= off) x += y;
-  }
-  return x;
+// Keys per tile
+constexpr int ragged_block_n(int head_dim, int row_waves) {
+  return row_waves == 4 ? (head_dim == 16 ? 128 : 64) : head_dim == 128 ? 32 : 64;
 }
 
-// The rank-th row tile (BM rows of a KV head's group) of the sequences in order, wave-uniform; seq < 0: none
-struct RowTile {
-  int seq, tile;
-};
-template <int BM>
-__device__ __forceinline__ RowTile find_row_tile(const int32_t* cu, int n_seq, int n_tokens, int group,
-                                                 int rank, int lane) {
-  int base = 0;
-  for (int s0 = 0; s0 < n_seq; s0 += 64) {
-    const int s = s0 + lane;
-    int tiles = 0;
-    if (s < n_seq) {
-      const int rows = row_bound(cu, s + 1, n_tokens) - row_bound(cu, s, n_tokens);
-      tiles = (max(rows, 0) * group + BM - 1) / BM;
-    }
-    const int upto = wave_scan(tiles, lane);
-    const uint64_t past = __builtin_amdgcn_ballot_w64(base + upto > rank);
-    if (past) {
-      const int l = __builtin_ctzll(past);
-      return RowTile{s0 + l, rank - base - __builtin_amdgcn_readlane(upto - tiles, l)};
-    }
-    base += __builtin_amdgcn_readlane(upto, 63);
-  }
-  return RowTile{-1, 0};
-}
-
-template <int DT, int D, int SRC>
+template <int DT, int D, int SRC, int GW>
 __global__ __launch_bounds__(256)
 __attribute__((amdgpu_waves_per_eu(2)))
 void attn_ragged_kernel(const RaggedParams p) {
@@ -69,8 +38,10 @@ void attn_ragged_kernel(const RaggedParams p) {
   constexpr bool kE4m3 = SRC == kSourceE4m3;
   constexpr bool kPages = SRC != kSourcePacked;
   constexpr int EB = kE4m3 ? 1 : 2;      // bytes of a cached element
-  constexpr int BN = ragged_block_n(D);
-  constexpr int KG = 4;                  // key groups: waves
+  constexpr int BN = ragged_block_n(D, GW);
+  constexpr int BM = 32 * GW;            // rows per workgroup
+  constexpr int KG = 4 / GW;             // key groups of GW waves
+  constexpr int BUFS = GW == 1 ? 1 : 2;  // K (and V) tiles in LDS per group
   constexpr int KS = D / 16;             // 16-dim k-steps of S^T = K Q^T
   constexpr int DB = (D + 31) / 32;      // 32-dim row blocks of O^T
   constexpr int NB = BN / 32;            // 32-key row blocks of S^T
@@ -78,167 +49,40 @@ void attn_ragged_kernel(const RaggedParams p) {
   constexpr int CPR = D / 8;             // 16-byte chunks per K / V row in LDS
   constexpr int TCH = BN * CPR;          // chunks per K (or V) tile
   constexpr int NI = TCH / 64 * EB / 2;  // 1 KiB loads per tile
+  constexpr int JW = (NI + GW - 1) / GW; // ... per wave
   constexpr int RPI = BN / NI;           // rows of one load (one page: the host's rule on page sizes)
+  constexpr int LPR = 64 / RPI;          // lanes per row of a load
   static_assert(NI >= 1 && BN % NI == 0, "a tile must be whole 1 KiB loads");
   constexpr int QPR = D / 4;             // 16-byte pieces of an fp32 output row
 
-  constexpr int kKvChunks = KG * 2 * TCH;
-  constexpr int kMergeChunks = KG * 32 * QPR;
+  constexpr int kKvChunks = KG * BUFS * 2 * TCH;
+  constexpr int kMergeChunks = KG > 1 ? BM * KG * QPR : 0;
   __shared__ u32x4 lds[kKvChunks > kMergeChunks ? kKvChunks : kMergeChunks];
-  __shared__ float sm[KG][32][3];  // m, l, exact l of every wave's rows
-  __shared__ int odd[32];          // rows whose sums are not finite
+  __shared__ float sm[KG][KG > 1 ? BM : 1][3];  // m, l, exact l of every group's rows
+  __shared__ int odd[KG > 1 ? BM : 1];          // rows whose sums are not finite
 
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lane = tid & 63;
   const int c = lane & 31;
   const int g = lane >> 5;
+  const int grp = wave / GW, gwave = wave % GW;
 
-  // ---- which head and row tile: a KV head stays on one XCD where the heads split evenly over them, so
-  // that its row tiles share K and V in one L2
-  const int xcds = 1 << p.xcd_shift;
   int hkv, rank;
-  if ((p.h_kv & (xcds - 1)) == 0) {
-    const int per = p.h_kv >> p.xcd_shift, slot = (int)blockIdx.x >> p.xcd_shift;
-    hkv = ((int)blockIdx.x & (xcds - 1)) * per + slot % per;
-    rank = slot / per;
-  } else {
-    hkv = (int)blockIdx.x % p.h_kv;
-    rank = (int)blockIdx.x / p.h_kv;
+  head_and_rank(p, (int)blockIdx.x, &hkv, &rank);
+  Cursor cur;
+  Share share = {0, 0, 0, 0};
+  if (p.shares > 0) {
+    share = find_share<BM, kPages>(p, rank, lane, &cur);
+    if (share.x >= share.end) return;
+  } else if (!find_tile<BM, kPages>(p, rank, lane, &cur)) {
+    return;
   }
-  const RowTile rt = find_row_tile<32>(p.seq.cu, p.seq.n_seq, p.seq.n_tokens, p.group, rank, lane);
-  if (rt.seq < 0) return;
-  const int t_first = row_bound(p.seq.cu, rt.seq, p.seq.n_tokens);
-  const int n_q = row_bound(p.seq.cu, rt.seq + 1, p.seq.n_tokens) - t_first;
-  int n_kv, kv_first = 0;
-  if constexpr (kPages) {
-    n_kv = (int)min((int64_t)max(p.seq.lens[rt.seq], 0), (int64_t)p.seq.max_pages << p.seq.page_shift);
-  } else {
-    kv_first = row_bound(p.cu_kv, rt.seq, p.kv_tokens);
-    n_kv = max(row_bound(p.cu_kv, rt.seq + 1, p.kv_tokens) - kv_first, 0);
-  }
-  const int rows = n_q * p.group;
-  const int row0 = rt.tile * 32;  // this workgroup's rows [row0, row_end)
-  const int row_end = min(row0 + 32, rows);
-  const int shift = n_kv - n_q;   // causal: position i sees keys up to i + shift
-
-  // ---- this lane's row; rows past the last repeat it and are never stored
-  const int r = min(row0 + c, rows - 1);
-  const int pos = r / p.group;
-  u32x4 qreg[KS];
-  {
-    const int head = hkv * p.group + (r - pos * p.group);
-    const uint16_t* qrow = p.q + (int64_t)(t_first + pos) * p.sqt + head * p.sqh + 8 * g;
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) qreg[ks] = *(const u32x4*)(qrow + 16 * ks);
-  }
-  // the last key of a position, the end of the keys that some row sees, and of those that every row sees
-  auto last_of = [&](int i) { return p.causal ? min(i + shift, n_kv - 1) : n_kv - 1; };
-  const int last_key = last_of(pos);
-  const int kv_end = max(last_of((row_end - 1) / p.group) + 1, 0);
-  const int full_end = max(last_of(row0 / p.group) + 1, 0);
-
-  // ---- this wave's tiles: wave, wave + KG, ...
-  const int n_tiles = (kv_end + BN - 1) / BN;
-  const int count = (n_tiles - wave + KG - 1) / KG;
-  auto key_of = [&](int i) { return (wave + i * KG) * BN; };  // first key of tile i
-
-  // ---- pages of the wave's tiles, a block of 64 table entries in a register: lane x holds the entry of
-  // tile x / per_tile, page x % per_tile of the tile. An entry that is no page of the cache reads page 0
-  // and makes the rows NaN.
-  const int page_shift = p.seq.page_shift;
-  const int tile_shift = kPages ? max(0, 31 - __builtin_clz(BN) - page_shift) : 0;  // log2 pages per tile
-  int entries = 0, bad = 0;
-  auto load_entries = [&](int i0) {
-    const int i = i0 + (lane >> tile_shift);
-    const int64_t n = (int64_t)(wave + (int64_t)i * KG) * BN + ((int64_t)(lane & ((1 << tile_shift) - 1)) << page_shift);
-    int e = 0;
-    if (i < count && n < kv_end) e = p.seq.table[rt.seq * p.seq.table_stride + (n >> page_shift)];
-    if ((unsigned)e >= (unsigned)p.seq.n_pages) {
-      bad = 1;
-      e = 0;
-    }
-    return e;
-  };
-  // the page of tile i's row x (wave-uniform)
-  auto page_of = [&](int i, int x) {
-    return __builtin_amdgcn_readlane(entries, ((i << tile_shift) & 63) + (x >> page_shift));
-  };
-
-  // ---- K/V rows -> LDS (bf16 / fp16, XOR-swizzled 16-byte chunks as in attn_fwd_kernel.hpp)
-  const CacheTensor* const tens[2] = {&p.kc, &p.vc};
-  uint32_t off[2][NI];  // this lane's byte offset inside load j
-#pragma unroll
-  for (int t = 0; t < 2; ++t)
-#pragma unroll
-    for (int j = 0; j < NI; ++j) {
-      if constexpr (kE4m3) {
-        off[t][j] = (uint32_t)((lane / (D / 16)) * tens[t]->token + (lane % (D / 16)) * 16);
-      } else {
-        const int row = lane / CPR, col = lane % CPR, in_tile = j * RPI + row;
-        const int key = t == 0 ? k_key<D>(pi_row(in_tile & 31) & 15) : v_key<D>(in_tile & 15);
-        off[t][j] = (uint32_t)(row * tens[t]->token + (col ^ key) * 8) * 2u;
-      }
-    }
-  // buffer resource of load j of tile i: the rows of it that lie before kv_end (others read as zeros)
-  auto rows_at = [&](int t, int i, int j) {
-    const int n0 = i < count ? key_of(i) + j * RPI : kv_end;
-    const int valid = min(kv_end - n0, RPI);
-    const CacheTensor& x = *tens[t];
-    const uint32_t bytes = valid > 0 ? ((uint32_t)(valid - 1) * (uint32_t)x.token + (uint32_t)D) * EB : 0u;
-    int64_t at = (int64_t)hkv * x.head;
-    if constexpr (kPages)
-      at += (int64_t)page_of(i, j * RPI) * x.page + (int64_t)(n0 & ((1 << page_shift) - 1)) * x.token;
-    else
-      at += (int64_t)(kv_first + n0) * x.token;
-    return make_desc(x.data + (valid > 0 ? at * EB : 0), bytes);
-  };
-  const FA2_LDS char* kbuf = (const FA2_LDS char*)(lds + wave * 2 * TCH);
-  const FA2_LDS char* vbuf = kbuf + TCH * 16;
-  auto issue = [&](int t, int i) {
-    const FA2_LDS char* buf = t == 0 ? kbuf : vbuf;
-#pragma unroll
-    for (int j = 0; j < NI; ++j) load_lds16(rows_at(t, i, j), off[t][j], lds_addr(buf + j * 1024));
-  };
-  // e4m3: through registers, converted on the way (16 values of one row a lane)
-  struct Raw {
-    u32x4 w[NI];
-    uint32_t scale[NI];
-  };
-  auto fetch = [&](int t, int i, Raw& raw) {
-    const CacheTensor& x = *tens[t];
-#pragma unroll
-    for (int j = 0; j < NI; ++j) {
-      const int n0 = i < count ? key_of(i) + j * RPI : kv_end;
-      const int row = lane / (D / 16);
-      const bool ok = n0 + row < kv_end;
-      raw.w[j] = u32x4{0u, 0u, 0u, 0u};
-      raw.scale[j] = 0u;
-      if (ok) {
-        const int64_t page = page_of(i, j * RPI);
-        const int in_page = (n0 & ((1 << page_shift) - 1)) + row;
-        raw.w[j] = *(const u32x4*)(x.data + page * x.page + hkv * x.head + (int64_t)in_page * x.token +
-                                   (lane % (D / 16)) * 16);
-        raw.scale[j] = x.scale[page * x.scale_page + hkv * x.scale_head + (int64_t)in_page * x.scale_token];
-      }
-    }
-  };
-  auto store = [&](int t, const Raw& raw) {
-    FA2_LDS char* buf = (FA2_LDS char*)(t == 0 ? kbuf : vbuf);
-#pragma unroll
-    for (int j = 0; j < NI; ++j) {
-      const int row = j * RPI + lane / (D / 16), chunk = lane % (D / 16) * 2;
-      const int key = t == 0 ? k_key<D>(pi_row(row & 31) & 15) : v_key<D>(row & 15);
-      const float scale = e8m0_to_f32(raw.scale[j]);
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const u32x2 lo = e4m3_to_16<DT>(raw.w[j][2 * h], scale), hi = e4m3_to_16<DT>(raw.w[j][2 * h + 1], scale);
-        *(u32x4 FA2_LDS*)(buf + (row * CPR + ((chunk + h) ^ key)) * 16) = u32x4{lo[0], lo[1], hi[0], hi[1]};
-      }
-    }
-  };
 
   // ---- LDS operand reads, as in attn_fwd_kernel.hpp
+  const FA2_LDS char* gbuf = (const FA2_LDS char*)(lds + grp * BUFS * 2 * TCH);
+  auto kbuf = [&](int i) { return gbuf + (BUFS == 1 ? 0 : (i & 1) * TCH * 16); };
+  auto vbuf = [&](int i) { return kbuf(i) + BUFS * TCH * 16; };
   const int kk = k_key<D>(c & 15);
   const int vj = (lane & 15) >> 2;
   const int vq = lane & 3;
@@ -247,6 +91,10 @@ void attn_ragged_kernel(const RaggedParams p) {
   uint32_t koffs[KS], voffs[2][DB];
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks) koffs[ks] = (uint32_t)((pi_row(c) * CPR + ((2 * ks + g) ^ kk)) * 16);
+  if constexpr (GW > 1) {
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(koffs[ks]));  // (kept whole: attn_fwd_kernel.hpp)
+  }
 #pragma unroll
   for (int rr = 0; rr < 2; ++rr)
 #pragma unroll
@@ -255,268 +103,682 @@ void attn_ragged_kernel(const RaggedParams p) {
       const int chunk = (4 * db + 2 * vdh + (vsig >> 1)) ^ v_key<D>(row);
       voffs[rr][db] = (uint32_t)(row * (D * 2) + chunk * 16 + (vsig & 1) * 8);
     }
-  auto k_operand = [&](int ks, int nb) { return *(const u32x4 FA2_LDS*)(kbuf + koffs[ks] + nb * 32 * CPR * 16); };
-  auto v_operand = [&](int t, int db) {
-    const u32x2 lo = lds_read_tr(vbuf + voffs[0][db] + t * 16 * D * 2);
-    const u32x2 hi = lds_read_tr(vbuf + voffs[1][db] + t * 16 * D * 2);
+  auto k_operand = [&](int i, int ks, int nb) {
+    return *(const u32x4 FA2_LDS*)(kbuf(i) + koffs[ks] + nb * 32 * CPR * 16);
+  };
+  auto v_operand = [&](int i, int t, int db) {
+    const u32x2 lo = lds_read_tr(vbuf(i) + voffs[0][db] + t * 16 * D * 2);
+    const u32x2 hi = lds_read_tr(vbuf(i) + voffs[1][db] + t * 16 * D * 2);
     return u32x4{lo[0], lo[1], hi[0], hi[1]};
   };
 
-  // ---- the online softmax of one tile, base 2, with a lazily moved reference (attn_fwd_wavesplit.hpp)
-  float m_i = -INFINITY, l_i = 0.f, l_exact = 0.f;
-  f32x16 acc[DB];
+  // ---- this head's K and V: where they start, the bytes between pages and between tokens (below 2^31: the
+  // host's limits), and this lane's offset from a tile's first row in load j of the tile
+  const int page_shift = p.seq.page_shift;
+  struct Source {
+    const char* data;
+    uint32_t page, token;
+  };
+  const Source ks = {p.kc.data + hkv * p.kc.head * EB, (uint32_t)p.kc.page * EB, (uint32_t)p.kc.token * EB};
+  const Source vs = {p.vc.data + hkv * p.vc.head * EB, (uint32_t)p.vc.page * EB, (uint32_t)p.vc.token * EB};
+  const Source kscale = {(const char*)p.kc.scale + hkv * p.kc.scale_head, (uint32_t)p.kc.scale_page, (uint32_t)p.kc.scale_token};
+  const Source vscale = {(const char*)p.vc.scale + hkv * p.vc.scale_head, (uint32_t)p.vc.scale_page, (uint32_t)p.vc.scale_token};
+  uint32_t koff[JW], voff[JW], kscale_off[JW], vscale_off[JW];
 #pragma unroll
-  for (int db = 0; db < DB; ++db) acc[db] = f32x16{};
+  for (int jj = 0; jj < JW; ++jj) {
+    const int row = (gwave + jj * GW) * RPI + lane / LPR, x = lane % LPR;
+    if constexpr (kE4m3) {
+      koff[jj] = (uint32_t)row * ks.token + x * 16;
+      voff[jj] = (uint32_t)row * vs.token + x * 16;
+      kscale_off[jj] = (uint32_t)row * kscale.token;
+      vscale_off[jj] = (uint32_t)row * vscale.token;
+    } else {
+      koff[jj] = (uint32_t)row * ks.token + (x ^ k_key<D>(pi_row(row & 31) & 15)) * 16;
+      voff[jj] = (uint32_t)row * vs.token + (x ^ v_key<D>(row & 15)) * 16;
+    }
+  }
+
   const float qk_scale = p.qk_scale;
   const bool want_exact = p.lse != nullptr;
-  auto softmax = [&](f32x16 (&s)[NB], u32x4 (&pb)[NT], int n0) {
-    if (n0 + BN > full_end) {
-      const int lim = last_key - n0 - 8 * g;
+
+  // ---- one piece: the cursor's row tile, its key tiles [part 0: all of them] `from` .. `to` of `of`
+  for (bool first_piece = true;; first_piece = false) {
+    const LaneSequence sq = sequence_at(cur.lanes, cur.l);
+    const int seq = cur.s0 + cur.l, n_kv = sq.n_kv;
+    const int rows = sq.n_q * p.group;
+    const int row0 = cur.tile * BM;       // this workgroup's rows [row0, row_end)
+    const int row_end = min(row0 + BM, rows);
+    const int shift = n_kv - sq.n_q;      // causal: position i sees keys up to i + shift
+    // the last key of a position, the end of the keys that some row sees, and of those that every row sees
+    auto last_of = [&](int i) { return p.causal ? min(i + shift, n_kv - 1) : n_kv - 1; };
+    const int see_end = max(last_of((row_end - 1) / p.group) + 1, 0);
+    const int full_end = max(last_of(row0 / p.group) + 1, 0);
+    const int all_tiles = (see_end + BN - 1) / BN;
+
+    int t_begin = 0, t_end = all_tiles;
+    bool starts = true, ends = true;  // whether the piece holds the tile's first and last keys
+    if (p.shares > 0) {
+      const int64_t length = lengths_of<BM>(p, sq.n_q, n_kv).of(cur.tile);
+      const int64_t out = min(length, share.in + (share.end - share.x));
+      starts = share.in == 0;
+      ends = out == length;
+      // a cut at x of the tile's length lies before key tile x * all_tiles / length: the shares on both
+      // sides of it compute the same
+      auto cut = [&](int64_t x) { return (int)((double)x * all_tiles / (double)length); };
+      if (!starts) t_begin = cut(share.in);
+      if (!ends) t_end = cut(out);
+      share.x += out - share.in;
+      share.in = 0;
+    }
+    const int kv_begin = t_begin * BN, kv_end = min(t_end * BN, see_end);
+    if (!first_piece) __syncthreads();  // the last piece's merge has left LDS
+
+    // ---- this lane's row; rows past the last repeat it and are never stored
+    const int wr = gwave * 32 + c;  // the row inside the workgroup
+    const int r = min(row0 + wr, rows - 1);
+    const int pos = r / p.group;
+    const int last_key = last_of(pos);
+    u32x4 qreg[KS];
+    {
+      const int head = hkv * p.group + (r - pos * p.group);
+      const uint16_t* qrow = p.q + (int64_t)(sq.first + pos) * p.sqt + head * p.sqh + 8 * g;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) qreg[ks] = *(const u32x4*)(qrow + 16 * ks);
+    }
+
+    // ---- this group's key tiles: grp, grp + KG, ... of the piece
+    const int n_tiles = t_end - t_begin;
+    const int count = (n_tiles - grp + KG - 1) / KG;
+    auto key_of = [&](int i) { return kv_begin + (grp + i * KG) * BN; };  // first key of tile i
+
+    // ---- pages: lane x of `pages` holds the page of tile x / per_tile of the current block of 64 / per_tile
+    // tiles, its page x % per_tile; `pages_next` those of the next block, on their way. An entry that
+    // is no page of the cache reads page 0 and makes the rows NaN.
+    constexpr int kLog2Bn = BN == 32 ? 5 : BN == 64 ? 6 : 7;
+    const int tile_shift = kPages ? max(0, kLog2Bn - page_shift) : 0;  // log2 pages per tile
+    const int block = 64 >> tile_shift;  // tiles of a block
+    int pages = 0, pages_next = 0, bad = 0;
+    auto load_pages = [&](int i0) {
+      const int i = i0 + (lane >> tile_shift);
+      const int64_t n = kv_begin + (int64_t)(grp + (int64_t)i * KG) * BN +
+                        ((int64_t)(lane & ((1 << tile_shift) - 1)) << page_shift);
+      int e = 0;
+      if (i < count && n < kv_end) e = p.seq.table[seq * p.seq.table_stride + (n >> page_shift)];
+      return e;
+    };
+    auto checked_pages = [&](int e) {
+      if ((unsigned)e >= (unsigned)p.seq.n_pages) {
+        bad = 1;
+        e = 0;
+      }
+      return e;
+    };
+    // Moves on to the block that holds tile i, when i is its first (i > 0, in order). The wait for the loads of
+    // the entries is here and nowhere else: the compiler does not count the asm loads around it.
+    auto turn_pages = [&](int i) {
+      if (kPages && (i & (block - 1)) == 0) {
+        asm volatile("" : "+v"(pages_next));
+        pages = checked_pages(pages_next);
+        pages_next = load_pages(i + block);
+      }
+    };
+    // the page of tile i's row x (wave-uniform)
+    auto page_of = [&](int i, int x) {
+      return __builtin_amdgcn_readlane(pages, ((i << tile_shift) & 63) + (x >> page_shift));
+    };
+
+    // ---- the memory of tile i's rows before kv_end (a load gives zeros past them), for load j: the tile's first
+    // row as if all of the tile lay in the page of load j's rows. One page for the whole tile where it holds
+    // the tile's keys.
+    const bool one_page = !kPages || page_shift >= kLog2Bn;
+    auto tile_bytes = [&](const Source& x, int i, int row_bytes) {
+      const int valid = max(min(kv_end - key_of(i), BN), 0);
+      return (uint32_t)max(valid * (int)x.token - ((int)x.token - row_bytes), 0);
+    };
+    auto tile_data = [&](const Source& x, int i, int j) {
+      const int n = key_of(i);
+      if constexpr (kPages) {
+        const int in_page = (n + j * RPI) & ((1 << page_shift) - 1);
+        return x.data + (uint64_t)(uint32_t)page_of(i, j * RPI) * x.page + (int64_t)(in_page - j * RPI) * x.token;
+      } else {
+        return x.data + (uint64_t)(uint32_t)(sq.kv_first + n) * x.token;
+      }
+    };
+    auto issue = [&](const Source& x, const uint32_t (&off)[JW], const FA2_LDS char* buf, int i) {
+      const uint32_t bytes = tile_bytes(x, i, D * 2);
+      u32x4 rsrc;
+      if (one_page) {
+        rsrc = make_desc(tile_data(x, i, 0), bytes);
+#pragma unroll
+        for (int jj = 0; jj < JW; ++jj) {
+          const int j = gwave + jj * GW;
+          if (NI % GW == 0 || j < NI) load_lds16_settled(rsrc, off[jj], lds_addr(buf + j * 1024));
+        }
+      } else {
+#pragma unroll
+        for (int jj = 0; jj < JW; ++jj) {
+          const int j = gwave + jj * GW;
+          if (NI % GW == 0 || j < NI) load_lds16_settled(make_desc(tile_data(x, i, j), bytes), off[jj], lds_addr(buf + j * 1024));
+        }
+      }
+    };
+    auto issue_k = [&](int i) { issue(ks, koff, kbuf(i), i); };
+    auto issue_v = [&](int i) { issue(vs, voff, vbuf(i), i); };
+
+    // ---- e4m3: 16 values of one row a lane, and the row's scale byte
+    struct Raw {
+      u32x4 w[JW];
+      uint32_t scale[JW];
+    };
+    auto fetch = [&](const Source& x, const Source& xs, const uint32_t (&off)[JW], const uint32_t (&soff)[JW], int i, Raw& raw) {
+      const uint32_t bytes = tile_bytes(x, i, D), scale_bytes = tile_bytes(xs, i, 1);
+#pragma unroll
+      for (int jj = 0; jj < JW; ++jj) {
+        const int j = gwave + jj * GW;
+        if (NI % GW == 0 || j < NI) {
+          raw.w[jj] = load_buffer16(buffer_of(tile_data(x, i, j), bytes), off[jj]);
+          raw.scale[jj] = load_buffer1(buffer_of(tile_data(xs, i, j), scale_bytes), soff[jj]);
+        }
+      }
+    };
+    auto fetch_k = [&](int i, Raw& raw) { fetch(ks, kscale, koff, kscale_off, i, raw); };
+    auto fetch_v = [&](int i, Raw& raw) { fetch(vs, vscale, voff, vscale_off, i, raw); };
+    auto store = [&](bool is_v, const FA2_LDS char* to, Raw& raw) {
+      FA2_LDS char* buf = (FA2_LDS char*)to;
+#pragma unroll
+      for (int jj = 0; jj < JW; ++jj) {
+        const int j = gwave + jj * GW;
+        if (NI % GW == 0 || j < NI) {
+          // nothing that uses what was loaded moves up across this point, and with it the wait for it
+          asm volatile("" : "+v"(raw.w[jj]), "+v"(raw.scale[jj]));
+          const int row = j * RPI + lane / LPR, chunk = lane % LPR * 2;
+          const int key = is_v ? v_key<D>(row & 15) : k_key<D>(pi_row(row & 31) & 15);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const u32x2 lo = e4m3_to_16<DT>(raw.w[jj][2 * h], raw.scale[jj]);
+            const u32x2 hi = e4m3_to_16<DT>(raw.w[jj][2 * h + 1], raw.scale[jj]);
+            *(u32x4 FA2_LDS*)(buf + (row * CPR + ((chunk + h) ^ key)) * 16) = u32x4{lo[0], lo[1], hi[0], hi[1]};
+          }
+        }
+      }
+    };
+
+    // ---- the online softmax of one tile, base 2, with a lazily moved reference (attn_fwd_wavesplit.hpp)
+    float m_i = -INFINITY, l_i = 0.f, l_exact = 0.f;
+    f32x16 acc[DB];
+#pragma unroll
+    for (int db = 0; db < DB; ++db) acc[db] = f32x16{};
+    auto softmax = [&](f32x16 (&s)[NB], u32x4 (&pb)[NT], int n0) {
+      if (n0 + BN > full_end) {
+        const int lim = last_key - n0 - 8 * g;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int x = 0; x < 16; ++x)
+            if (nb * 32 + 16 * (x / 8) + (x % 8) > lim) s[nb][x] = -INFINITY;
+      }
+      float mx = -INFINITY;
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) mx = fmaxf(mx, s[nb][x]);
+      mx = pair_max(mx) * qk_scale;
+      const bool grow = mx > m_i + kRescaleTau;
+      if (__builtin_amdgcn_ballot_w64(grow)) {
+        const float m_new = grow ? mx : m_i;
+        const float alpha = grow ? __builtin_amdgcn_exp2f(m_i - m_new) : 1.0f;
+        l_i *= alpha;
+        l_exact *= alpha;
+#pragma unroll
+        for (int db = 0; db < DB; ++db) acc[db] *= alpha;
+        m_i = m_new;
+      }
+      // a row that has seen no key in its tiles yet (reference -inf) gets weights 0, not NaN
+      const float m_ref = m_i == -INFINITY ? 0.f : m_i;
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
         for (int x = 0; x < 16; ++x)
-          if (nb * 32 + 16 * (x / 8) + (x % 8) > lim) s[nb][x] = -INFINITY;
-    }
-    float mx = -INFINITY;
+          s[nb][x] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[nb][x], qk_scale, -m_ref));
+      if (want_exact) l_exact += lane_sum(s);
+      float rs0 = 0.f, rs1 = 0.f;
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-      for (int x = 0; x < 16; ++x) mx = fmaxf(mx, s[nb][x]);
-    mx = pair_max(mx) * qk_scale;
-    const bool grow = mx > m_i + kRescaleTau;
-    if (__builtin_amdgcn_ballot_w64(grow)) {
-      const float m_new = grow ? mx : m_i;
-      const float alpha = grow ? __builtin_amdgcn_exp2f(m_i - m_new) : 1.0f;
-      l_i *= alpha;
-      l_exact *= alpha;
-#pragma unroll
-      for (int db = 0; db < DB; ++db) acc[db] *= alpha;
-      m_i = m_new;
-    }
-    // a row that has seen no key in this wave's tiles yet (reference -inf) gets weights 0, not NaN
-    const float m_ref = m_i == -INFINITY ? 0.f : m_i;
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-      for (int x = 0; x < 16; ++x)
-        s[nb][x] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[nb][x], qk_scale, -m_ref));
-    if (want_exact) l_exact += lane_sum(s);
-    float rs0 = 0.f, rs1 = 0.f;
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      const int nb = t >> 1, h = t & 1;
-      pb[t] = u32x4{E::pack2(s[nb][8 * h + 0], s[nb][8 * h + 1]), E::pack2(s[nb][8 * h + 2], s[nb][8 * h + 3]),
-                    E::pack2(s[nb][8 * h + 4], s[nb][8 * h + 5]), E::pack2(s[nb][8 * h + 6], s[nb][8 * h + 7])};
-      rs0 = E::sum2(pb[t][0], rs0);
-      rs1 = E::sum2(pb[t][1], rs1);
-      rs0 = E::sum2(pb[t][2], rs0);
-      rs1 = E::sum2(pb[t][3], rs1);
-    }
-    l_i += rs0 + rs1;
-  };
+      for (int t = 0; t < NT; ++t) {
+        const int nb = t >> 1, h = t & 1;
+        pb[t] = u32x4{E::pack2(s[nb][8 * h + 0], s[nb][8 * h + 1]), E::pack2(s[nb][8 * h + 2], s[nb][8 * h + 3]),
+                      E::pack2(s[nb][8 * h + 4], s[nb][8 * h + 5]), E::pack2(s[nb][8 * h + 6], s[nb][8 * h + 7])};
+        rs0 = E::sum2(pb[t][0], rs0);
+        rs1 = E::sum2(pb[t][1], rs1);
+        rs0 = E::sum2(pb[t][2], rs0);
+        rs1 = E::sum2(pb[t][3], rs1);
+      }
+      l_i += rs0 + rs1;
+    };
 
-  const int block = 64 >> tile_shift;  // tiles of one block of entries
-  if constexpr (kPages) entries = load_entries(0);
-  Raw kraw, vraw;
-  if constexpr (kE4m3) {
-    fetch(0, 0, kraw);
-    fetch(1, 0, vraw);
-  } else {
-    issue(0, 0);
-    issue(1, 0);
-    // Q is waited for here: the compiler does not count the asm loads, so its own wait for Q is for
-    // everything in flight, and inside the loop it would come every time
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qreg[ks]));
-  }
-  for (int i = 0; i < count; ++i) {
-    if constexpr (kE4m3) store(0, kraw);
-    else wait_vm_fence<NI>();  // K_i has landed; V_i may be in flight
-    u32x4 kop[KS][NB];
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb) kop[ks][nb] = k_operand(ks, nb);
-    if (kPages && ((i + 1) & (block - 1)) == 0) entries = load_entries(i + 1);
-    if constexpr (kE4m3) {
-      fetch(0, i + 1, kraw);
-    } else {
-      wait_lds_fence();  // the operands have left the buffer: refill it
-      issue(0, i + 1);
+    if constexpr (kPages) {
+      pages = checked_pages(load_pages(0));
+      pages_next = load_pages(block);
     }
-    f32x16 s[NB];
+    Raw kraw, vraw;
+    if constexpr (GW == 1) {
+      if constexpr (kE4m3) {
+        fetch_k(0, kraw);
+        fetch_v(0, vraw);
+      } else {
+        if (count > 0) {
+          issue_k(0);
+          issue_v(0);
+        }
+        // Q is waited for here: the compiler does not count the asm loads, so its own wait for Q is for
+        // everything in flight, and inside the loop it would come every time
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) s[nb] = f32x16{};
+        for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qreg[ks]));
+      }
+      for (int i = 0; i < count; ++i) {
+        if constexpr (kE4m3) store(false, kbuf(i), kraw);
+        else wait_vm_fence<NI>();  // K_i has landed; V_i may be in flight
+        u32x4 kop[KS][NB];
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
+        for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) s[nb] = E::mma(kop[ks][nb], qreg[ks], s[nb]);
-    u32x4 pb[NT];
-    softmax(s, pb, key_of(i));
-    if constexpr (kE4m3) store(1, vraw);
-    else wait_vm_fence<NI>();  // V_i has landed; K_{i+1} may be in flight
+          for (int nb = 0; nb < NB; ++nb) kop[ks][nb] = k_operand(i, ks, nb);
+        turn_pages(i + 1);
+        if constexpr (kE4m3) {
+          fetch_k(i + 1, kraw);
+        } else {
+          wait_lds_fence();  // the operands have left the buffer: refill it
+          if (i + 1 < count) issue_k(i + 1);
+        }
+        f32x16 s[NB];
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+        for (int nb = 0; nb < NB; ++nb) s[nb] = f32x16{};
 #pragma unroll
-      for (int db = 0; db < DB; ++db) acc[db] = E::mma(v_operand(t, db), pb[t], acc[db]);
-    if constexpr (kE4m3) {
-      fetch(1, i + 1, vraw);
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) s[nb] = E::mma(kop[ks][nb], qreg[ks], s[nb]);
+        u32x4 pb[NT];
+        softmax(s, pb, key_of(i));
+        if constexpr (kE4m3) store(true, vbuf(i), vraw);
+        else if (i + 1 < count) wait_vm_fence<NI>();  // V_i has landed; K_{i+1} may be in flight
+        else wait_vm_fence<0>();
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int db = 0; db < DB; ++db) acc[db] = E::mma(v_operand(i, t, db), pb[t], acc[db]);
+        if constexpr (kE4m3) {
+          fetch_v(i + 1, vraw);
+        } else {
+          wait_lds_fence();
+          if (i + 1 < count) issue_v(i + 1);
+        }
+      }
     } else {
-      wait_lds_fence();
-      issue(1, i + 1);
+      // attn_fwd_kernel.hpp's one-tile loop. 16-bit sources: K_{j+2} and V_{j+1} are issued after tile j's barrier
+      // and land before tile j + 1's. e4m3: K_{j+1} and V_j, fetched into registers one tile earlier, are
+      // converted and written before tile j's barrier; the next ones are fetched right after.
+      constexpr int LA_S = KS < 4 ? KS : 4;
+      constexpr int NPV = NT * DB;
+      constexpr int kLaV = D == 128 ? 2 : 4;
+      constexpr int LA_V = NPV < kLaV ? NPV : kLaV;
+      constexpr int NKP = LA_S * NB;
+      u32x4 kop[LA_S][NB];
+      if (n_tiles > 0) {
+        if constexpr (kE4m3) {
+          fetch_k(0, kraw);
+          store(false, kbuf(0), kraw);
+          fetch_k(1, kraw);
+          fetch_v(0, vraw);
+        } else {
+          issue_k(0);
+          issue_v(0);
+          if (n_tiles > 1) issue_k(1);
+          // K_0 has landed; V_0 and K_1 may be in flight (where every wave issues as many loads)
+          if (NI % GW != 0) wait_vm_fence<0>();
+          else if (n_tiles > 1) wait_vm_fence<2 * JW>();
+          else wait_vm_fence<JW>();
+        }
+        __syncthreads();
+#pragma unroll
+        for (int ks = 0; ks < LA_S; ++ks)
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb)
+            kop[ks][nb] = *(const volatile u32x4 FA2_LDS*)(kbuf(0) + koffs[ks] + nb * 32 * CPR * 16);
+      }
+      // Q is waited for here, on every path: the compiler does not count the asm loads (see above)
+#pragma unroll
+      for (int x = 0; x < KS; ++x) asm volatile("" : "+v"(qreg[x]));
+      // tiles that start past every row of the wave add exact zeros: their products are skipped
+      const int wave_last = __builtin_amdgcn_readlane(last_key, 31);  // rows grow with the lane
+      const int n_active = row0 + gwave * 32 >= row_end || wave_last < kv_begin
+                               ? 0 : min(n_tiles, (wave_last - kv_begin) / BN + 1);
+      auto turn_tile = [&](int j) {  // before tile j's barrier and after it: all that keeps the loads going
+        if constexpr (kE4m3) {
+          store(false, kbuf(j + 1), kraw);
+          store(true, vbuf(j), vraw);
+          fetch_v(j + 1, vraw);  // (j + 1's block of pages: K's have not moved on yet)
+          turn_pages(j + 2);
+          fetch_k(j + 2, kraw);
+          __syncthreads();
+        } else {
+          wait_vm_fence<0>();  // this wave's loads of V_j and K_{j+1} have landed
+          __syncthreads();     // ... every wave's; and every wave is done with K_j
+          if (j + 1 < n_tiles) issue_v(j + 1);  // (as above)
+          turn_pages(j + 2);
+          if (j + 2 < n_tiles) issue_k(j + 2);
+        }
+      };
+      for (int j = 0; j < n_active; ++j) {
+        __builtin_amdgcn_s_setprio(1);
+        f32x16 s[NB];
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) s[nb] = f32x16{};
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          const int slot = ks % LA_S;
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) s[nb] = E::mma(kop[slot][nb], qreg[ks], s[nb]);
+          if (ks + LA_S < KS) {
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) kop[slot][nb] = k_operand(j, ks + LA_S, nb);
+          }
+        }
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          __builtin_amdgcn_sched_group_barrier(0x008, NB, 0);
+          if (ks + LA_S < KS) __builtin_amdgcn_sched_group_barrier(0x100, NB, 0);
+        }
+        __builtin_amdgcn_s_setprio(0);
+        turn_tile(j);
+        u32x4 va[LA_V], pb[NT];
+#pragma unroll
+        for (int x = 0; x < LA_V; ++x) va[x] = v_operand(j, x / DB, x % DB);
+        softmax(s, pb, key_of(j));
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int x = 0; x < NPV; ++x) {
+          acc[x % DB] = E::mma(va[x % LA_V], pb[x / DB], acc[x % DB]);
+          if (x + LA_V < NPV) va[x % LA_V] = v_operand(j, (x + LA_V) / DB, (x + LA_V) % DB);
+          // K_{j+1}'s first operands (a harmless stale read after the last tile)
+#pragma unroll
+          for (int y = x * NKP / NPV; y < (x + 1) * NKP / NPV; ++y)
+            kop[y / NB][y % NB] = k_operand(j + 1, y / NB, y % NB);
+        }
+#pragma unroll
+        for (int x = 0; x < NPV; ++x) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          const int nreads = (x + LA_V < NPV ? 2 : 0) + ((x + 1) * NKP / NPV - x * NKP / NPV);
+#pragma unroll
+          for (int y = 0; y < nreads; ++y) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+      }
+      __builtin_amdgcn_s_setprio(0);
+      for (int j = n_active; j < n_tiles; ++j) turn_tile(j);
     }
-  }
 
-  // ---- merge the waves through LDS: O^T blocks as 16-byte pieces [wave][row][4 dims]
-  if (tid < 32) odd[tid] = 0;
-  if constexpr (!kE4m3) wait_vm_fence<0>();
-  __syncthreads();  // every wave is done with every K/V buffer
-  FA2_LDS f32x4* ob = (FA2_LDS f32x4*)lds;
-  auto piece = [&](int group, int row, int q) {
-    return (group * 32 + row) * QPR + (q ^ (row & (QPR < 8 ? QPR - 1 : 7)));
-  };
-  if (__builtin_amdgcn_ballot_w64(bad != 0)) m_i = __uint_as_float(0x7fc00000u);
-  {
+    // ---- the piece's results. A weight of zero times an infinite or NaN value is NaN, and such a value may
+    // lie in a key of a tile that the row does not see: rows whose sums are not finite are computed again, over the
+    // keys that they see alone.
+    if (__builtin_amdgcn_ballot_w64(bad != 0)) m_i = __uint_as_float(0x7fc00000u);
     const float l = pair_sum(l_i);
     const float lx = want_exact ? pair_sum(l_exact) : l;
-    // A weight of zero times an infinite or NaN value is NaN: such a value may lie in a key of the tile
-    // that the row does not see. Rows whose sums are not finite are computed again below, over the keys
-    // that they see alone.
     float test = 0.f;
 #pragma unroll
     for (int db = 0; db < DB; ++db)
 #pragma unroll
       for (int x = 0; x < 16; ++x) test = __builtin_fmaf(acc[db][x], 0.f, test);
-    if (row0 + c < row_end) {
-      if (test != 0.f) odd[c] = 1;
-#pragma unroll
-      for (int db = 0; db < DB; ++db)
-#pragma unroll
-        for (int h = 0; h < 4; ++h) {
-          const int q = 8 * db + 4 * (h >> 1) + 2 * g + (h & 1);  // dims 4 q .. 4 q + 3
-          if (q < QPR) {
-            f32x4 x;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = acc[db][4 * h + e];
-            ob[piece(wave, c, q)] = x;
-          }
+    const bool whole = starts && ends;
+    float* const part = whole ? nullptr : part_of<BM, D>(p, hkv, rank, starts ? 1 : 0);
+    // row x of the workgroup: its place in out, q and lse
+    struct RowPlace {
+      int64_t token;
+      int head, pos;
+    };
+    auto place = [&](int x) {
+      const int i = (row0 + x) / p.group;
+      return RowPlace{(int64_t)(sq.first + i), hkv * p.group + (row0 + x - i * p.group), i};
+    };
+    // m, l and exact l of row x, by one lane
+    auto put_sums = [&](int x, float m, float sum, float exact) {
+      if (part) {
+        *(f32x4*)(part + x * (D + 4) + D) = f32x4{m, sum, exact, 0.f};
+      } else if (p.lse) {
+        const RowPlace at = place(x);
+        p.lse[(int64_t)at.head * p.seq.n_tokens + at.token] = (m + log2f(exact)) * kLn2;
+      }
+    };
+    // One row again, by a wave: 64 keys at a time, one a lane; only keys that the row sees are read.
+    auto again = [&](int x, bool nan) {
+      const RowPlace at = place(x);
+      const int end = nan ? kv_begin : min(last_of(at.pos) + 1, kv_end);
+      const uint16_t* qrow = p.q + at.token * p.sqt + at.head * p.sqh;
+      int page = 0;
+      auto row_at = [&](const CacheTensor& y, int n) {
+        if constexpr (kPages) {
+          page = p.seq.table[seq * p.seq.table_stride + (n >> page_shift)];
+          if ((unsigned)page >= (unsigned)p.seq.n_pages) page = 0;
+          return y.data + (page * y.page + hkv * y.head + (int64_t)(n & ((1 << page_shift) - 1)) * y.token) * EB;
+        } else {
+          return y.data + ((int64_t)(sq.kv_first + n) * y.token + hkv * y.head) * EB;
         }
-      if (g == 0) {
-        sm[wave][c][0] = m_i;
-        sm[wave][c][1] = l;
-        sm[wave][c][2] = lx;
+      };
+      auto scale_at = [&](const CacheTensor& y, int n) {
+        if constexpr (kE4m3)
+          return e8m0_to_f32(y.scale[page * y.scale_page + hkv * y.scale_head +
+                                     (int64_t)(n & ((1 << page_shift) - 1)) * y.scale_token]);
+        else
+          return 1.0f;
+      };
+      auto value = [&](const char* row, float scale, int d) {
+        if constexpr (kE4m3) {
+          const auto v = __builtin_amdgcn_cvt_pk_f32_fp8((int)(uint32_t)(uint8_t)row[d], false);
+          return v[0] * scale;
+        } else {
+          return to_f32<DT>(((const uint16_t*)row)[d]);
+        }
+      };
+      bool no_lse = nan;  // (an infinite score has one, though the row has no weights)
+      float m = -INFINITY, sum = 0.f, o[(D + 63) / 64] = {};
+      for (int n0 = kv_begin; n0 < end; n0 += 64) {
+        const int n = n0 + lane;
+        float s = -INFINITY;
+        if (n < end) {
+          const char* krow = row_at(p.kc, n);
+          const float scale = scale_at(p.kc, n);
+          s = 0.f;
+          for (int d = 0; d < D; ++d) s = __builtin_fmaf(to_f32<DT>(qrow[d]), value(krow, scale, d), s);
+          s *= qk_scale;
+        }
+        no_lse |= __builtin_amdgcn_ballot_w64(s != s) != 0;
+        float m_new = s;  // fmaxf drops a NaN score here; its weight is NaN below
+#pragma unroll
+        for (int o2 = 32; o2 >= 1; o2 /= 2) m_new = fmaxf(m_new, __shfl_xor(m_new, o2, 64));
+        m_new = fmaxf(m, m_new);
+        const float m_ref = m_new == -INFINITY ? 0.f : m_new;
+        const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m_ref);
+        const float w = n < end ? __builtin_amdgcn_exp2f(s - m_ref) : 0.f;
+        m = m_new;
+        sum = sum * alpha + w;
+#pragma unroll
+        for (int y = 0; y < (D + 63) / 64; ++y) o[y] *= alpha;
+        for (int y = 0; y < min(end - n0, 64); ++y) {
+          const float wy = __shfl(w, y, 64);
+          const char* vrow = row_at(p.vc, n0 + y);
+          const float scale = scale_at(p.vc, n0 + y);
+#pragma unroll
+          for (int z = 0; z < (D + 63) / 64; ++z)
+            if (lane + 64 * z < D) o[z] = __builtin_fmaf(wy, value(vrow, scale, lane + 64 * z), o[z]);
+        }
+      }
+#pragma unroll
+      for (int o2 = 32; o2 >= 1; o2 /= 2) sum += __shfl_xor(sum, o2, 64);
+      if (no_lse) m = __uint_as_float(0x7fc00000u);
+      const float inv = last_of(at.pos) < 0 ? 0.f : 1.0f / sum;
+#pragma unroll
+      for (int y = 0; y < (D + 63) / 64; ++y)
+        if (lane + 64 * y < D) {
+          const float v = nan ? m : o[y];
+          if (part)
+            part[x * (D + 4) + lane + 64 * y] = v;
+          else
+            p.o[at.token * p.sot + at.head * p.soh + lane + 64 * y] =
+                (uint16_t)E::pack2(last_of(at.pos) < 0 ? 0.f : v * inv, 0.f);
+        }
+      // (an infinite score without a NaN one: the row's log-sum-exp is infinite too)
+      if (lane == 0) put_sums(x, m, sum, m == INFINITY ? 1.0f : sum);
+    };
+
+    if constexpr (KG == 1) {
+      const bool mine = row0 + wr < row_end;
+      uint64_t again_rows = __builtin_amdgcn_ballot_w64(mine && test != 0.f);
+      again_rows = (again_rows | (again_rows >> 32)) & 0xffffffffu;
+      if (mine && !((again_rows >> c) & 1)) {
+        const float inv = last_key < 0 ? 0.f : 1.0f / l;  // no key: 0
+        const RowPlace at = place(wr);
+        uint16_t* orow = p.o + at.token * p.sot + at.head * p.soh;
+        const float nan_or_0 = m_i != m_i ? m_i : 0.f;
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int d0 = 32 * db + 16 * h + 8 * g;
+            if (d0 < D) {
+              if (part) {
+                f32x4 lo, hi;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  lo[i] = acc[db][8 * h + i];
+                  hi[i] = acc[db][8 * h + 4 + i];
+                }
+                *(f32x4*)(part + wr * (D + 4) + d0) = lo;
+                *(f32x4*)(part + wr * (D + 4) + d0 + 4) = hi;
+              } else {
+                float y[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) y[i] = __builtin_fmaf(acc[db][8 * h + i], inv, nan_or_0);
+                *(u32x4*)(orow + d0) = u32x4{E::pack2(y[0], y[1]), E::pack2(y[2], y[3]), E::pack2(y[4], y[5]),
+                                             E::pack2(y[6], y[7])};
+              }
+            }
+          }
+        if (g == 0) put_sums(wr, m_i, l, lx);
+      }
+      for (uint64_t todo = again_rows; todo; todo &= todo - 1)
+        again(gwave * 32 + __builtin_ctzll(todo), m_i != m_i);
+    } else {
+      // ---- merge the groups through LDS: O^T blocks as 16-byte pieces [group][row][4 dims], then
+      // every thread folds the groups of its pieces
+      if (tid < BM) odd[tid] = 0;
+      if constexpr (!kE4m3) wait_vm_fence<0>();
+      __syncthreads();  // every wave is done with every K/V buffer
+      FA2_LDS f32x4* ob = (FA2_LDS f32x4*)lds;
+      auto piece = [&](int group, int row, int q) {
+        return (group * BM + row) * QPR + (q ^ (row & (QPR < 8 ? QPR - 1 : 7)));
+      };
+      if (row0 + wr < row_end) {
+        if (test != 0.f) odd[wr] = 1;
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+          for (int h = 0; h < 4; ++h) {
+            const int q = 8 * db + 4 * (h >> 1) + 2 * g + (h & 1);  // dims 4 q .. 4 q + 3
+            if (q < QPR) {
+              f32x4 x;
+#pragma unroll
+              for (int e = 0; e < 4; ++e) x[e] = acc[db][4 * h + e];
+              ob[piece(grp, wr, q)] = x;
+            }
+          }
+        if (g == 0) {
+          sm[grp][wr][0] = m_i;
+          sm[grp][wr][1] = l;
+          sm[grp][wr][2] = lx;
+        }
+      }
+      __syncthreads();
+      for (int t = tid; t < (row_end - row0) * QPR; t += 256) {
+        const int x = t / QPR, q = t % QPR;
+        if (odd[x]) continue;
+        float m = -INFINITY, ls = 0.f, lxs = 0.f;
+#pragma unroll
+        for (int y = 0; y < KG; ++y) m = fmaxf(m, sm[y][x][0]);
+        f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int y = 0; y < KG; ++y) {
+          const float mw = sm[y][x][0];
+          const float w = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - m);  // NaN: a bad page
+          ls = __builtin_fmaf(w, sm[y][x][1], ls);
+          lxs = __builtin_fmaf(w, sm[y][x][2], lxs);
+          const f32x4 v = ob[piece(y, x, q)];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(w, v[e], o[e]);
+        }
+        const RowPlace at = place(x);
+        if (part) {
+          *(f32x4*)(part + x * (D + 4) + 4 * q) = o;
+        } else {
+          const float inv = last_of(at.pos) < 0 ? 0.f : 1.0f / ls;  // no key: 0
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[e] *= inv;
+          *(u32x2*)(p.o + at.token * p.sot + at.head * p.soh + 4 * q) = u32x2{E::pack2(o[0], o[1]), E::pack2(o[2], o[3])};
+        }
+        if (q == 0) put_sums(x, m, ls, lxs);
+      }
+      for (int x = wave; x < row_end - row0; x += 4) {
+        if (!odd[x]) continue;
+        bool nan = false;
+#pragma unroll
+        for (int y = 0; y < KG; ++y) nan |= sm[y][x][0] != sm[y][x][0];
+        again(x, nan);
       }
     }
+    if (share.x >= share.end || !next_tile<BM, kPages>(p, lane, &cur)) return;
   }
-  __syncthreads();
-  for (int t = tid; t < (row_end - row0) * QPR; t += 256) {
-    const int wr = t / QPR, q = t % QPR;
-    if (odd[wr]) continue;
-    float m = -INFINITY, l = 0.f, lx = 0.f;
-    bool nan = false;
-#pragma unroll
-    for (int x = 0; x < KG; ++x) {
-      m = fmaxf(m, sm[x][wr][0]);
-      nan |= sm[x][wr][0] != sm[x][wr][0];
-    }
+}
+
+// Merges the pieces of the row tile that ends in share `rank` and starts in an earlier one: with M the largest of the
+// pieces' references m_i, O = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i, in the order of the shares.
+template <int DT, int D, bool PAGES, int GW>
+__global__ __launch_bounds__(256) void attn_ragged_combine_kernel(const RaggedParams p) {
+  using E = Elem<DT>;
+  constexpr int BM = 32 * GW, QPR = D / 4;
+  const int lane = threadIdx.x & 63;
+  int hkv, rank;
+  head_and_rank(p, (int)blockIdx.x, &hkv, &rank);
+  Cursor cur;
+  const Share share = find_share<BM, PAGES>(p, rank, lane, &cur);
+  if (share.x >= share.end || share.in == 0) return;
+  const LaneSequence sq = sequence_at(cur.lanes, cur.l);
+  const int64_t length = lengths_of<BM>(p, sq.n_q, sq.n_kv).of(cur.tile);
+  if (length - share.in > share.end - share.x) return;  // it ends in a later share
+  const int first = (int)((share.x - share.in) / share.size);
+  const int rows = sq.n_q * p.group, row0 = cur.tile * BM;
+  const int n = min(BM, rows - row0) * QPR;
+  for (int t = (int)threadIdx.x; t < n; t += 256) {
+    const int x = t / QPR, q = t % QPR;
+    float M = -INFINITY;
+    for (int i = first; i <= rank; ++i)
+      M = fmaxf(M, part_of<BM, D>(p, hkv, i, i == first)[x * (D + 4) + D]);
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int x = 0; x < KG; ++x) {
-      const float mw = sm[x][wr][0];
-      const float w = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - m);
-      l = __builtin_fmaf(w, sm[x][wr][1], l);
-      lx = __builtin_fmaf(w, sm[x][wr][2], lx);
-      const f32x4 v = ob[piece(x, wr, q)];
+    float l = 0.f, lx = 0.f;
+    bool nan = false;
+    for (int i = first; i <= rank; ++i) {
+      const float* part = part_of<BM, D>(p, hkv, i, i == first) + x * (D + 4);
+      const f32x4 sums = *(const f32x4*)(part + D), v = *(const f32x4*)(part + 4 * q);
+      const float w = sums[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sums[0] - M);
+      nan |= sums[0] != sums[0];
+      l = __builtin_fmaf(w, sums[1], l);
+      lx = __builtin_fmaf(w, sums[2], lx);
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(w, v[e], o[e]);
     }
-    if (nan) m = l = lx = __uint_as_float(0x7fc00000u);
-    const int opos = (row0 + wr) / p.group;
-    const int head = hkv * p.group + (row0 + wr - opos * p.group);
-    const float inv_l = last_of(opos) < 0 && !nan ? 0.f : 1.0f / l;  // no key: 0
-#pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] *= inv_l;
-    uint16_t* orow = p.o + (int64_t)(t_first + opos) * p.sot + head * p.soh + 4 * q;
-    *(u32x2*)orow = u32x2{E::pack2(o[0], o[1]), E::pack2(o[2], o[3])};
-    if (p.lse && q == 0) p.lse[(int64_t)head * p.seq.n_tokens + t_first + opos] = (m + log2f(lx)) * kLn2;
-  }
-
-  // ---- rows with sums that are not finite, a wave per row in turn: 64 keys at a time, one a lane
-  for (int wr = wave; wr < row_end - row0; wr += 4) {
-    if (!odd[wr]) continue;
-    const int opos = (row0 + wr) / p.group;
-    const int head = hkv * p.group + (row0 + wr - opos * p.group);
-    bool nan = false;
-#pragma unroll
-    for (int x = 0; x < KG; ++x) nan |= sm[x][wr][0] != sm[x][wr][0];
-    const int end = nan ? 0 : last_of(opos) + 1;
-    const uint16_t* qrow = p.q + (int64_t)(t_first + opos) * p.sqt + head * p.sqh;
-    int page = 0;
-    auto row_at = [&](const CacheTensor& x, int n) {
-      if constexpr (kPages) {
-        page = p.seq.table[rt.seq * p.seq.table_stride + (n >> page_shift)];
-        if ((unsigned)page >= (unsigned)p.seq.n_pages) page = 0;
-        return x.data + (page * x.page + hkv * x.head + (int64_t)(n & ((1 << page_shift) - 1)) * x.token) * EB;
-      } else {
-        return x.data + ((int64_t)(kv_first + n) * x.token + hkv * x.head) * EB;
-      }
-    };
-    auto scale_at = [&](const CacheTensor& x, int n) {
-      return e8m0_to_f32(x.scale[page * x.scale_page + hkv * x.scale_head +
-                                 (int64_t)(n & ((1 << page_shift) - 1)) * x.scale_token]);
-    };
-    auto value = [&](const char* row, float scale, int d) {
-      if constexpr (kE4m3) {
-        const auto v = __builtin_amdgcn_cvt_pk_f32_fp8((int)(uint32_t)(uint8_t)row[d], false);
-        return v[0] * scale;
-      } else {
-        return to_f32<DT>(((const uint16_t*)row)[d]);
-      }
-    };
-    bool no_lse = nan;  // (an infinite score has one, though the row has no weights)
-    float m = -INFINITY, l = 0.f, o[(D + 63) / 64] = {};
-    for (int n0 = 0; n0 < end; n0 += 64) {
-      const int n = n0 + lane;
-      float s = -INFINITY;
-      if (n < end) {
-        const char* krow = row_at(p.kc, n);
-        float scale = 1.f;
-        if constexpr (kE4m3) scale = scale_at(p.kc, n);
-        s = 0.f;
-        for (int d = 0; d < D; ++d) s = __builtin_fmaf(to_f32<DT>(qrow[d]), value(krow, scale, d), s);
-        s *= qk_scale;
-      }
-      no_lse |= __builtin_amdgcn_ballot_w64(s != s) != 0;
-      float m_new = s;  // fmaxf drops a NaN score here; its weight is NaN below
-#pragma unroll
-      for (int o2 = 32; o2 >= 1; o2 /= 2) m_new = fmaxf(m_new, __shfl_xor(m_new, o2, 64));
-      m_new = fmaxf(m, m_new);
-      const float m_ref = m_new == -INFINITY ? 0.f : m_new;
-      const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m_ref);
-      const float w = n < end ? __builtin_amdgcn_exp2f(s - m_ref) : 0.f;
-      m = m_new;
-      l = l * alpha + w;
-#pragma unroll
-      for (int x = 0; x < (D + 63) / 64; ++x) o[x] *= alpha;
-      for (int y = 0; y < min(end - n0, 64); ++y) {
-        const float wy = __shfl(w, y, 64);
-        const char* vrow = row_at(p.vc, n0 + y);
-        float scale = 1.f;
-        if constexpr (kE4m3) scale = scale_at(p.vc, n0 + y);
-#pragma unroll
-        for (int x = 0; x < (D + 63) / 64; ++x)
-          if (lane + 64 * x < D) o[x] = __builtin_fmaf(wy, value(vrow, scale, lane + 64 * x), o[x]);
-      }
-    }
-#pragma unroll
-    for (int o2 = 32; o2 >= 1; o2 /= 2) l += __shfl_xor(l, o2, 64);
-    uint16_t* orow = p.o + (int64_t)(t_first + opos) * p.sot + head * p.soh;
-#pragma unroll
-    for (int x = 0; x < (D + 63) / 64; ++x)
-      if (lane + 64 * x < D) orow[lane + 64 * x] = (uint16_t)E::pack2(nan ? l / l : end <= 0 ? 0.f : o[x] / l, 0.f);
-    if (p.lse && lane == 0)
-      p.lse[(int64_t)head * p.seq.n_tokens + t_first + opos] = no_lse ? l / l : m == INFINITY ? m : (m + log2f(l)) * kLn2;
+    const int pos = (row0 + x) / p.group, head = hkv * p.group + (row0 + x - pos * p.group);
+    const int64_t token = sq.first + pos;
+    const bool none = (p.causal ? min(pos + sq.n_kv - sq.n_q, sq.n_kv - 1) : sq.n_kv - 1) < 0;
+    const float inv = none ? 0.f : 1.0f / l;
+    *(u32x2*)(p.o + token * p.sot + head * p.soh + 4 * q) =
+        u32x2{E::pack2(o[0] * inv, o[1] * inv), E::pack2(o[2] * inv, o[3] * inv)};
+    if (p.lse && q == 0)  // (an infinite score has an infinite log-sum-exp, though the row has no weights)
+      p.lse[(int64_t)head * p.seq.n_tokens + token] = !nan && M == INFINITY ? M : (M + log2f(lx)) * kLn2;
   }
 }
 

@@ -4,21 +4,37 @@
 
 namespace fa2 {
 
-template <int DT, int D>
-int launch_ragged(const RaggedParams& p, int source, unsigned grid, hipStream_t s) {
-  switch (source) {
-    case kSourcePacked:
-      hipLaunchKernelGGL((attn_ragged_kernel<DT, D, kSourcePacked>), dim3(grid), dim3(256), 0, s, p);
-      break;
-    case kSourcePages:
-      hipLaunchKernelGGL((attn_ragged_kernel<DT, D, kSourcePages>), dim3(grid), dim3(256), 0, s, p);
-      break;
-    default:
-      hipLaunchKernelGGL((attn_ragged_kernel<DT, D, kSourceE4m3>), dim3(grid), dim3(256), 0, s, p);
+namespace {
+
+template <int SRC, int GW>
+int launch_form(const RaggedParams& p, unsigned grid, hipStream_t s) {
+  hipLaunchKernelGGL((attn_ragged_kernel<FA2_DT, FA2_D, SRC, GW>), dim3(grid), dim3(256), 0, s, p);
+  hipError_t e = hipGetLastError();
+  if constexpr (SRC != kSourcePacked) {
+    if (e == hipSuccess && p.shares > 0) {
+      hipLaunchKernelGGL((attn_ragged_combine_kernel<FA2_DT, FA2_D, true, GW>), dim3(grid), dim3(256), 0, s, p);
+      e = hipGetLastError();
+    }
   }
-  return (int)hipGetLastError();
+  return (int)e;
 }
 
-template int launch_ragged<FA2_DT, FA2_D>(const RaggedParams&, int, unsigned, hipStream_t);
+}  // namespace
+
+template <>
+int launch_ragged<FA2_DT, FA2_D>(const RaggedParams& p, int source, int row_waves, unsigned grid, hipStream_t s) {
+  if (row_waves == 1) {
+    switch (source) {
+      case kSourcePacked: return launch_form<kSourcePacked, 1>(p, grid, s);
+      case kSourcePages: return launch_form<kSourcePages, 1>(p, grid, s);
+      default: return launch_form<kSourceE4m3, 1>(p, grid, s);
+    }
+  }
+  switch (source) {
+    case kSourcePacked: return launch_form<kSourcePacked, 4>(p, grid, s);
+    case kSourcePages: return launch_form<kSourcePages, 4>(p, grid, s);
+    default: return launch_form<kSourceE4m3, 4>(p, grid, s);
+  }
+}
 
 }  // namespace fa2

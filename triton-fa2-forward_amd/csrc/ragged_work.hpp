@@ -1,0 +1,235 @@
+// ragged_work.hpp - which rows and keys a workgroup of the ragged attention kernel takes. Sequence lengths
+// are known on the device only, so every workgroup works this out from the index vectors: 64 sequences
+// at a time, one a lane, their lengths kept in registers for the next piece.
+//
+// A row tile is BM rows of one KV head's group of query heads of one sequence; every head has the same tiles.
+// Two ways to deal them out:
+//   * a workgroup per tile (as many workgroups as n_tokens rows in n_seq sequences can have tiles at most).
+//     With up to 64 sequences the tiles go by their index in their sequence, highest first: causal tiles
+//     of high index see the most keys, so the longest start first.
+//   * `shares` workgroups per head, each an equal share of the head's tiles laid end to end, a tile's length being
+//     its keys (an estimate, linear in the tile's index, so that a sequence's sum is a closed form; it only
+//     decides where the cuts lie). A share starts and ends inside tiles: a tile cut by a share's end leaves
+//     partial results (slot 1 of the share it starts in, slot 0 of the others), which the combine kernel merges. For
+//     few or uneven tiles, decoding above all, whatever the lengths are.
+#pragma once
+
+#include "serve_common.hpp"
+#include "serve_launch.hpp"
+
+namespace fa2 {
+
+// Keys that a tile costs beside its own: its rows' loads, its merge and stores.
+constexpr int kTileCost = 64;
+// Keys of the smallest share: four tiles of 64, or two of 32 for each of four waves.
+constexpr int kLeastShare = 256;
+
+// The sequence that this lane holds of a block of 64
+struct LaneSequence {
+  int first, n_q, n_kv, kv_first;
+};
+
+template <bool PAGES>
+__device__ __forceinline__ LaneSequence lane_sequence(const RaggedParams& p, int s) {
+  LaneSequence q = {0, 0, 0, 0};
+  if (s >= p.seq.n_seq) return q;
+  q.first = row_bound(p.seq.cu, s, p.seq.n_tokens);
+  q.n_q = max(row_bound(p.seq.cu, s + 1, p.seq.n_tokens) - q.first, 0);
+  if constexpr (PAGES) {
+    q.n_kv = (int)min((int64_t)max(p.seq.lens[s], 0), (int64_t)p.seq.max_pages << p.seq.page_shift);
+  } else {
+    q.kv_first = row_bound(p.cu_kv, s, p.kv_tokens);
+    q.n_kv = max(row_bound(p.cu_kv, s + 1, p.kv_tokens) - q.kv_first, 0);
+  }
+  return q;
+}
+
+// The block's lane l, wave-uniform
+__device__ __forceinline__ LaneSequence sequence_at(const LaneSequence& q, int l) {
+  return LaneSequence{__builtin_amdgcn_readlane(q.first, l), __builtin_amdgcn_readlane(q.n_q, l),
+                      __builtin_amdgcn_readlane(q.n_kv, l), __builtin_amdgcn_readlane(q.kv_first, l)};
+}
+
+template <int BM>
+__device__ __forceinline__ int row_tiles(int n_q, int group) {
+  return (n_q * group + BM - 1) / BM;
+}
+
+// The length of a sequence's tiles on the line that is shared out: tile t's is base + slope t.
+struct Lengths {
+  int64_t base, slope;
+  __device__ int64_t of(int64_t t) const { return base + slope * t; }
+  __device__ int64_t before(int64_t t) const { return t * base + slope * (t * (t - 1) / 2); }
+};
+template <int BM>
+__device__ __forceinline__ Lengths lengths_of(const RaggedParams& p, int n_q, int n_kv) {
+  if (!p.causal) return Lengths{(int64_t)n_kv + kTileCost, 0};
+  const int64_t slope = BM / p.group;
+  return Lengths{(int64_t)max(n_kv - n_q, 0) + slope + kTileCost, slope};
+}
+
+__device__ __forceinline__ int64_t wave_scan(int64_t x, int lane) {
+#pragma unroll
+  for (int off = 1; off < 64; off *= 2) {
+    const int64_t y = __shfl_up(x, off, 64);
+    if (lane >= off) x += y;
+  }
+  return x;
+}
+__device__ __forceinline__ int64_t readlane64(int64_t x, int l) {
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)x, l);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)((uint64_t)x >> 32), l);
+  return (int64_t)(((uint64_t)hi << 32) | lo);
+}
+
+// A place among the sequences: the block of 64 that starts at s0 is in `lanes`, the sequence is its lane l.
+struct Cursor {
+  int s0, l, tile;
+  LaneSequence lanes;
+};
+
+// The rank-th row tile; false: there are fewer.
+template <int BM, bool PAGES>
+__device__ __forceinline__ bool find_tile(const RaggedParams& p, int rank, int lane, Cursor* c) {
+  c->lanes = lane_sequence<PAGES>(p, lane);
+  if (p.seq.n_seq <= 64) {
+    // Tiles of index t and above, over all sequences: A(t) = sum_s max(tiles_s - t, 0). The rank-th tile in the
+    // order of falling t has the largest t with A(t) > rank; every lane tries a t of its own.
+    const int tiles = row_tiles<BM>(c->lanes.n_q, p.group);
+    int hi = 0;
+    for (int s = 0; s < p.seq.n_seq; ++s) hi = max(hi, __builtin_amdgcn_readlane(tiles, s));
+    auto above = [&](int t) {
+      int a = 0;
+      for (int s = 0; s < p.seq.n_seq; ++s) a += max(__builtin_amdgcn_readlane(tiles, s) - t, 0);
+      return a;
+    };
+    if (above(0) <= rank) return false;
+    int lo = 0;
+    while (hi - lo > 1) {
+      const int step = (hi - lo + 63) / 64;
+      const int t = lo + lane * step;
+      const uint64_t yes = __builtin_amdgcn_ballot_w64(t < hi && above(t) > rank);
+      lo += (__builtin_popcountll(yes) - 1) * step;
+      hi = min(lo + step, hi);
+    }
+    const int nth = rank - __builtin_amdgcn_readfirstlane(above(lo + 1));  // among the sequences with a tile lo
+    const uint64_t have = __builtin_amdgcn_ballot_w64(tiles > lo);
+    const int before = __builtin_popcountll(have & ((1ull << lane) - 1));
+    c->s0 = 0;
+    c->l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(((have >> lane) & 1) && before == nth));
+    c->tile = lo;
+    return true;
+  }
+  int64_t base = 0;
+  for (int s0 = 0; s0 < p.seq.n_seq; s0 += 64) {
+    if (s0) c->lanes = lane_sequence<PAGES>(p, s0 + lane);
+    const int64_t tiles = row_tiles<BM>(c->lanes.n_q, p.group);
+    const int64_t upto = base + wave_scan(tiles, lane);
+    const uint64_t past = __builtin_amdgcn_ballot_w64(upto > rank);
+    if (past) {
+      c->s0 = s0;
+      c->l = __builtin_ctzll(past);
+      c->tile = rank - (int)readlane64(upto - tiles, c->l);
+      return true;
+    }
+    base = readlane64(upto, 63);
+  }
+  return false;
+}
+
+// Share j: [x, end) of the line, the cursor at the tile that x lies in, `in` from its start; x >= end: nothing.
+struct Share {
+  int64_t x, end, in, size;
+};
+template <int BM, bool PAGES>
+__device__ __forceinline__ Share find_share(const RaggedParams& p, int j, int lane, Cursor* c) {
+  c->lanes = lane_sequence<PAGES>(p, lane);
+  auto length = [&]() {
+    return lengths_of<BM>(p, c->lanes.n_q, c->lanes.n_kv).before(row_tiles<BM>(c->lanes.n_q, p.group));
+  };
+  int64_t mine = length();
+  int64_t upto = wave_scan(mine, lane);
+  int64_t total = readlane64(upto, 63);
+  for (int s0 = 64; s0 < p.seq.n_seq; s0 += 64) {
+    c->lanes = lane_sequence<PAGES>(p, s0 + lane);
+    total += readlane64(wave_scan(length(), lane), 63);
+  }
+  Share w;
+  w.size = max((total + p.shares - 1) / p.shares, (int64_t)kLeastShare);
+  w.x = w.size * j;
+  w.end = min(w.x + w.size, total);
+  w.in = 0;
+  if (w.x >= w.end) return w;
+  int64_t base = 0;
+  c->s0 = 0;
+  if (p.seq.n_seq > 64) c->lanes = lane_sequence<PAGES>(p, lane);
+  while (base + readlane64(upto, 63) <= w.x) {  // (w.x < total: ends within the sequences)
+    base += readlane64(upto, 63);
+    c->s0 += 64;
+    if (c->s0 >= p.seq.n_seq) {  // only if the lengths changed since they were summed
+      w.end = w.x;
+      return w;
+    }
+    c->lanes = lane_sequence<PAGES>(p, c->s0 + lane);
+    mine = length();
+    upto = wave_scan(mine, lane);
+  }
+  c->l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(base + upto > w.x));
+  w.in = w.x - base - readlane64(upto - mine, c->l);
+  const LaneSequence q = sequence_at(c->lanes, c->l);
+  const Lengths len = lengths_of<BM>(p, q.n_q, q.n_kv);
+  int lo = 0, hi = row_tiles<BM>(q.n_q, p.group);  // the largest t with before(t) <= in
+  while (hi - lo > 1) {
+    const int t = (lo + hi) / 2;
+    if (len.before(t) <= w.in)
+      lo = t;
+    else
+      hi = t;
+  }
+  c->tile = lo;
+  w.in -= len.before(lo);
+  return w;
+}
+
+// The next tile after the cursor's; false: there is none.
+template <int BM, bool PAGES>
+__device__ __forceinline__ bool next_tile(const RaggedParams& p, int lane, Cursor* c) {
+  const LaneSequence q = sequence_at(c->lanes, c->l);
+  if (++c->tile < row_tiles<BM>(q.n_q, p.group)) return true;
+  c->tile = 0;
+  for (;;) {
+    const uint64_t have = __builtin_amdgcn_ballot_w64(c->lanes.n_q > 0 && lane > c->l);
+    if (have) {
+      c->l = __builtin_ctzll(have);
+      return true;
+    }
+    c->s0 += 64;
+    if (c->s0 >= p.seq.n_seq) return false;
+    c->l = -1;
+    c->lanes = lane_sequence<PAGES>(p, c->s0 + lane);
+  }
+}
+
+// The (KV head, rank) of a workgroup: a head stays on one XCD where the heads split evenly over them, and on a
+// fixed few where the XCDs split evenly over the heads, so that its tiles share K and V in an L2.
+__device__ __forceinline__ void head_and_rank(const RaggedParams& p, int block, int* head, int* rank) {
+  const int xcds = 1 << p.xcd_shift;
+  const int xcd = block & (xcds - 1), slot = block >> p.xcd_shift;
+  if ((p.h_kv & (xcds - 1)) == 0) {
+    const int per = p.h_kv >> p.xcd_shift;
+    *head = xcd * per + slot % per;
+    *rank = slot / per;
+  } else {
+    *head = block % p.h_kv;
+    *rank = block / p.h_kv;
+  }
+}
+
+// A share's partial results: slot 1 of the tile that it starts and does not finish, slot 0 of the one that
+// it starts in the middle of.
+template <int BM, int D>
+__device__ __forceinline__ float* part_of(const RaggedParams& p, int head, int share, int slot) {
+  return p.parts + (((int64_t)head * p.shares + share) * 2 + slot) * (BM * (D + 4));
+}
+
+}  // namespace fa2

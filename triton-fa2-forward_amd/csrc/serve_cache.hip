@@ -243,7 +243,7 @@ __global__ __launch_bounds__(256) void cache_read_kernel(const CacheParams p) {
       const char* src = cache_row(c, at, h, p.seq.page_shift, E4M3 ? 1 : 2);
       if constexpr (E4M3) {
         const u32x2 b = *(const u32x2*)(src + 8 * chunk);
-        const float scale = e8m0_to_f32(*scale_row(c, at, h, p.seq.page_shift));
+        const uint32_t scale = *scale_row(c, at, h, p.seq.page_shift);
         const u32x2 lo = e4m3_to_16<DT>(b[0], scale), hi = e4m3_to_16<DT>(b[1], scale);
         w = u32x4{lo[0], lo[1], hi[0], hi[1]};
       } else {

@@ -59,18 +59,48 @@ __device__ __forceinline__ Place find_place(const Sequences& q, int t, int lane)
   return p;
 }
 
+// load_lds16 (attn_fwd_common.hpp) behind five wait states. A vector instruction may have written the
+// resource's SGPRs right before (a readfirstlane, or the reload of a spilled SGPR), and a scalar one M0; the
+// hardware needs 5 and 1 wait states before a buffer load reads them, and the compiler, which inserts
+// those before its own loads, does not look into inline asm. Without them a load of a tile in several pages
+// ran with the resource of the load before it.
+__device__ __forceinline__ void load_lds16_settled(u32x4 desc, uint32_t voffset, uint32_t lds_base) {
+  asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
+               :
+               : "v"(voffset), "s"(desc), "{m0}"(lds_base)
+               : "memory");
+}
+
+// A buffer resource over [data, data + bytes) (wave-uniform), and loads through it: past it they give zeros.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const char* data, uint32_t bytes) {
+  const uint64_t a = reinterpret_cast<uint64_t>(data);
+  auto uniform = [](uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); };
+  const uint64_t base = (uint64_t)uniform((uint32_t)(a >> 32)) << 32 | uniform((uint32_t)a);
+  return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(base), 0, (int)uniform(bytes), 0x00020000);
+}
+__device__ __forceinline__ u32x4 load_buffer16(__amdgpu_buffer_rsrc_t rsrc, uint32_t offset) {
+  return __builtin_amdgcn_raw_buffer_load_b128(rsrc, (int)offset, 0, 0);
+}
+__device__ __forceinline__ uint32_t load_buffer1(__amdgpu_buffer_rsrc_t rsrc, uint32_t offset) {
+  return __builtin_amdgcn_raw_buffer_load_b8(rsrc, (int)offset, 0, 0);
+}
+
 // 2^(byte - 127) of an e8m0 scale byte (255: NaN)
 __device__ __forceinline__ float e8m0_to_f32(uint32_t b) {
   return __uint_as_float(b == 0 ? 0x00400000u : b == 255u ? 0x7fc00000u : b << 23);
 }
 
-// 4 e4m3 values of a word times scale, rounded to the 16-bit type (exactly, but where the product leaves
-// the type's range): two packed pairs.
+// 4 e4m3 values of a word times 2^(byte - 127), rounded to the 16-bit type (exactly, but where the product
+// leaves the type's range): two packed pairs. The instruction takes its scale from a float's exponent bits.
 template <int DT>
-__device__ __forceinline__ u32x2 e4m3_to_16(uint32_t w, float scale) {
-  const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false);
-  const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
-  return u32x2{Elem<DT>::pack2(lo[0] * scale, lo[1] * scale), Elem<DT>::pack2(hi[0] * scale, hi[1] * scale)};
+__device__ __forceinline__ u32x2 e4m3_to_16(uint32_t w, uint32_t scale_byte) {
+  const float scale = __uint_as_float(scale_byte << 23);
+  if constexpr (DT == 0)
+    return u32x2{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, false)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, true))};
+  else
+    return u32x2{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, false)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, true))};
 }
 
 }  // namespace fa2

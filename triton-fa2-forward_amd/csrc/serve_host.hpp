@@ -10,6 +10,10 @@ namespace {
 
 bool power_of_two(int64_t x) { return x > 0 && (x & (x - 1)) == 0; }
 
+// Longest sequence and most rows: positions stay 32-bit in the kernels with two rounds of four 128-key tiles of
+// headroom.
+constexpr int32_t kMaxKeys = 0x7fffffff - 2048;
+
 // `n` strides of a 16-bit tensor (or of e4m3 bytes: multiples of 16) and its pointer
 int check_rows(const char* what, const void* p, const int64_t* stride, int n, int multiple) {
   if (!p) return fail(FA2_EINVAL, "null pointer: %s", what);
@@ -64,18 +68,28 @@ int check_cache(const fa2_cache* c, const fa2_sequences* q, int32_t dtype, fa2::
   if (const int rc = check_rows("the cache's v", c->v, c->v_stride, 3, multiple)) return rc;
   if (c->k_stride[2] > kMaxRowStride || c->v_stride[2] > kMaxRowStride)
     return fail(FA2_EINVAL, "a cache's token stride above %lld elements is not supported", (long long)kMaxRowStride);
+  // the kernels add a page's bytes and a token's in 32 bits to a 64-bit base
+  const int64_t most = 0x7fffffffLL / (e4m3 ? 1 : 2);
+  for (const int64_t* s : {c->k_stride, c->v_stride})
+    if (s[0] > most || s[2] * c->page_size > most)
+      return fail(FA2_EINVAL, "a cache's pages must lie, and extend, less than 2^31 bytes apart");
   if (e4m3) {
     if (!c->k_scale || !c->v_scale) return fail(FA2_EINVAL, "an e4m3 cache needs k_scale and v_scale");
     for (int i = 0; i < 3; ++i)
       if (c->k_scale_stride[i] < 0 || c->v_scale_stride[i] < 0)
         return fail(FA2_EINVAL, "strides of the cache's scales must not be negative");
+    if (c->k_scale_stride[2] > kMaxRowStride || c->v_scale_stride[2] > kMaxRowStride)
+      return fail(FA2_EINVAL, "a scale's token stride above %lld is not supported", (long long)kMaxRowStride);
+    for (const int64_t* s : {c->k_scale_stride, c->v_scale_stride})
+      if (s[0] > most || s[2] * c->page_size > most)
+        return fail(FA2_EINVAL, "the scales of a cache's pages must lie, and extend, less than 2^31 bytes apart");
   }
   if (q->n_seq < 0 || q->n_tokens < 0 || q->max_pages < 0 || q->table_stride < 0)
     return fail(FA2_EINVAL, "bad sizes: n_seq=%d n_tokens=%d max_pages=%d table_stride=%lld", q->n_seq, q->n_tokens,
                 q->max_pages, (long long)q->table_stride);
-  if (q->n_tokens > kMaxSeq) return fail(FA2_EINVAL, "n_tokens must be at most %d", kMaxSeq);
-  if ((int64_t)q->max_pages * c->page_size > kMaxSeq)
-    return fail(FA2_EINVAL, "max_pages * page_size must be at most %d (32-bit key positions), got %lld", kMaxSeq,
+  if (q->n_tokens > kMaxKeys) return fail(FA2_EINVAL, "n_tokens must be at most %d", kMaxKeys);
+  if ((int64_t)q->max_pages * c->page_size > kMaxKeys)
+    return fail(FA2_EINVAL, "max_pages * page_size must be at most %d (32-bit key positions), got %lld", kMaxKeys,
                 (long long)q->max_pages * c->page_size);
   if (q->n_seq > 0 && q->n_tokens > 0 && (!q->cu || !q->lens || (q->max_pages > 0 && !q->table)))
     return fail(FA2_EINVAL, "null pointer: cu, lens or table");
@@ -102,37 +116,70 @@ unsigned cache_grid(fa2::CacheParams* p, int64_t rows_per_token, int32_t head_di
   return (unsigned)(((int64_t)p->seq.n_tokens + p->tokens_per_wg - 1) / p->tokens_per_wg);
 }
 
-// The heads, mask and scale of a ragged attention call, and its grid: the most row tiles of block_m rows
-// that n_tokens rows in n_seq sequences can have, for every KV head.
-int check_heads(int32_t h_q, int32_t h_kv, int32_t n_tokens, int32_t n_seq, float qk_scale, const float* lse,
-                int block_m, int64_t* grid) {
+// The form of a ragged attention call (attn_ragged.hpp, ragged_work.hpp), from what the host knows of it: the
+// rows and sequences, not the lengths.
+struct RaggedPlan {
+  int row_waves = 4;  // 32-row workgroups (1) or 128-row ones (4)
+  int shares = 0;     // workgroups per KV head that share its work; 0: one per row tile
+  int64_t grid = 0;
+  size_t workspace = 0;
+};
+RaggedPlan ragged_plan(bool paged, int32_t h_q, int32_t h_kv, int32_t head_dim, int32_t n_tokens, int32_t n_seq, int cus) {
+  RaggedPlan pl;
+  const int64_t rows = (int64_t)n_tokens * (h_q / h_kv);
+  auto tiles = [&](int64_t block_m) { return (rows + (int64_t)n_seq * (block_m - 1)) / block_m; };  // at most
+  if (paged)
+    pl.row_waves = rows <= (int64_t)32 * n_seq ? 1 : 4;
+  else
+    pl.row_waves = tiles(32) * h_kv <= 2 * (int64_t)cus ? 1 : 4;
+  const int64_t n = tiles(32 * pl.row_waves);
+  if (paged && n * h_kv < 8 * (int64_t)cus) {
+    pl.shares = std::max(1, 2 * cus / h_kv);
+    pl.workspace = (size_t)h_kv * pl.shares * 2 * 32 * pl.row_waves * (head_dim + 4) * sizeof(float);
+  }
+  pl.grid = (pl.shares ? pl.shares : n) * h_kv;
+  return pl;
+}
+
+// The heads and scale of a ragged attention call.
+int check_heads(int32_t h_q, int32_t h_kv, int32_t n_tokens, float qk_scale, const float* lse) {
   if (h_q <= 0 || h_kv <= 0) return fail(FA2_EINVAL, "bad sizes: h_q=%d h_kv=%d", h_q, h_kv);
   if (h_q % h_kv) return fail(FA2_EINVAL, "GQA needs H_q divisible by H_kv (%d %% %d)", h_q, h_kv);
   if (!(qk_scale > 0.f) || !std::isfinite(qk_scale))
     return fail(FA2_EINVAL, "qk_scale (sm_scale * log2 e) must be positive and finite, got %g", (double)qk_scale);
   if (reinterpret_cast<uintptr_t>(lse) & 3u) return fail(FA2_EALIGN, "lse must be 4-byte aligned");
   const int64_t rows = (int64_t)n_tokens * (h_q / h_kv);
-  if (rows > kMaxSeq) return fail(FA2_EINVAL, "n_tokens * (h_q / h_kv) must be at most %d, got %lld", kMaxSeq, (long long)rows);
-  const int64_t tiles = (rows + (int64_t)n_seq * (block_m - 1)) / block_m;
-  if (tiles > 0x7fffffffLL / h_kv)
-    return fail(FA2_EINVAL, "grid of %lld x %d workgroups is too large", (long long)tiles, h_kv);
-  *grid = tiles * h_kv;
+  if (rows > kMaxKeys) return fail(FA2_EINVAL, "n_tokens * (h_q / h_kv) must be at most %d, got %lld", kMaxKeys, (long long)rows);
   return FA2_OK;
 }
 
-int launch_ragged(int32_t dtype, int32_t head_dim, const fa2::RaggedParams& p, int source, int64_t grid, void* stream) {
-  const unsigned g = (unsigned)grid;
+// Launches a checked call whose heads, tensors and sequences are in p.
+int launch_ragged(int32_t dtype, int32_t head_dim, int32_t h_q, fa2::RaggedParams& p, int source, void* workspace,
+                  size_t workspace_bytes, void* stream) {
   const hipStream_t s = static_cast<hipStream_t>(stream);
+  const Topology topo = device_topology(stream_device(s));
+  const RaggedPlan pl = ragged_plan(source != fa2::kSourcePacked, h_q, p.h_kv, head_dim, p.seq.n_tokens, p.seq.n_seq, topo.cus);
+  if (pl.grid > 0x7fffffffLL) return fail(FA2_EINVAL, "grid of %lld workgroups is too large", (long long)pl.grid);
+  if (pl.workspace) {
+    if (!workspace || workspace_bytes < pl.workspace)
+      return fail(FA2_EINVAL, "the call needs a workspace of %zu bytes, got %zu", pl.workspace, workspace ? workspace_bytes : (size_t)0);
+    if (reinterpret_cast<uintptr_t>(workspace) & 255u) return fail(FA2_EALIGN, "the workspace must be 256-byte aligned");
+  }
+  p.group = h_q / p.h_kv;
+  p.xcd_shift = topo.xcd_shift;
+  p.shares = pl.shares;
+  p.parts = static_cast<float*>(workspace);
+  const unsigned g = (unsigned)pl.grid;
   int e;
   switch (dtype * 4 + dim_index(head_dim)) {
-    case 0: e = fa2::launch_ragged<0, 16>(p, source, g, s); break;
-    case 1: e = fa2::launch_ragged<0, 32>(p, source, g, s); break;
-    case 2: e = fa2::launch_ragged<0, 64>(p, source, g, s); break;
-    case 3: e = fa2::launch_ragged<0, 128>(p, source, g, s); break;
-    case 4: e = fa2::launch_ragged<1, 16>(p, source, g, s); break;
-    case 5: e = fa2::launch_ragged<1, 32>(p, source, g, s); break;
-    case 6: e = fa2::launch_ragged<1, 64>(p, source, g, s); break;
-    default: e = fa2::launch_ragged<1, 128>(p, source, g, s);
+    case 0: e = fa2::launch_ragged<0, 16>(p, source, pl.row_waves, g, s); break;
+    case 1: e = fa2::launch_ragged<0, 32>(p, source, pl.row_waves, g, s); break;
+    case 2: e = fa2::launch_ragged<0, 64>(p, source, pl.row_waves, g, s); break;
+    case 3: e = fa2::launch_ragged<0, 128>(p, source, pl.row_waves, g, s); break;
+    case 4: e = fa2::launch_ragged<1, 16>(p, source, pl.row_waves, g, s); break;
+    case 5: e = fa2::launch_ragged<1, 32>(p, source, pl.row_waves, g, s); break;
+    case 6: e = fa2::launch_ragged<1, 64>(p, source, pl.row_waves, g, s); break;
+    default: e = fa2::launch_ragged<1, 128>(p, source, pl.row_waves, g, s);
   }
   return launched(e, "attention");
 }
@@ -236,12 +283,11 @@ int fa2_attn_packed(const void* q, const void* k, const void* v, void* out, cons
   g_err[0] = '\0';
   fa2::RaggedParams p{};
   if (const int rc = check_type(head_dim, dtype)) return rc;
-  if (n_seq < 0 || n_tokens < 0 || kv_tokens < 0 || kv_tokens > kMaxSeq)
+  if (n_seq < 0 || n_tokens < 0 || kv_tokens < 0 || kv_tokens > kMaxKeys)
     return fail(FA2_EINVAL, "bad sizes: n_seq=%d n_tokens=%d kv_tokens=%d", n_seq, n_tokens, kv_tokens);
   if (!cu_kv && kv_tokens != n_tokens)
     return fail(FA2_EINVAL, "k and v of %d rows for q of %d need their own cu_kv", kv_tokens, n_tokens);
-  int64_t grid = 0;
-  if (const int rc = check_heads(h_q, h_kv, n_tokens, n_seq, qk_scale, lse, 32, &grid)) return rc;
+  if (const int rc = check_heads(h_q, h_kv, n_tokens, qk_scale, lse)) return rc;
   if (n_seq == 0 || n_tokens == 0) return FA2_OK;
   if (!cu) return fail(FA2_EINVAL, "null pointer: cu");
   if (const int rc = check_rows("q", q, q_stride, 2, 8)) return rc;
@@ -264,21 +310,19 @@ int fa2_attn_packed(const void* q, const void* k, const void* v, void* out, cons
   p.seq.n_tokens = n_tokens;
   p.cu_kv = cu_kv ? cu_kv : cu;
   p.kv_tokens = kv_tokens;
-  p.h_kv = h_kv; p.group = h_q / h_kv;
+  p.h_kv = h_kv;
   p.causal = causal != 0;
   p.qk_scale = qk_scale;
-  p.xcd_shift = device_topology(stream_device(static_cast<hipStream_t>(stream))).xcd_shift;
-  return launch_ragged(dtype, head_dim, p, fa2::kSourcePacked, grid, stream);
+  return launch_ragged(dtype, head_dim, h_q, p, fa2::kSourcePacked, nullptr, 0, stream);
 }
 
 int fa2_attn_paged(const void* q, void* out, const int64_t q_stride[2], const int64_t o_stride[2],
                    const fa2_cache* cache, const fa2_sequences* seq, int32_t h_q, int32_t dtype, int32_t causal,
-                   float qk_scale, float* lse, void* stream) {
+                   float qk_scale, float* lse, void* workspace, size_t workspace_bytes, void* stream) {
   g_err[0] = '\0';
   fa2::RaggedParams p{};
   if (const int rc = check_cache(cache, seq, dtype, &p.kc, &p.vc, &p.seq)) return rc;
-  int64_t grid = 0;
-  if (const int rc = check_heads(h_q, cache->h_kv, seq->n_tokens, seq->n_seq, qk_scale, lse, 32, &grid)) return rc;
+  if (const int rc = check_heads(h_q, cache->h_kv, seq->n_tokens, qk_scale, lse)) return rc;
   if (p.seq.n_seq == 0 || p.seq.n_tokens == 0) return FA2_OK;
   if (const int rc = check_rows("q", q, q_stride, 2, 8)) return rc;
   if (const int rc = check_rows("out", out, o_stride, 2, 8)) return rc;
@@ -287,12 +331,18 @@ int fa2_attn_paged(const void* q, void* out, const int64_t q_stride[2], const in
   p.lse = lse;
   p.sqt = q_stride[0]; p.sqh = q_stride[1];
   p.sot = o_stride[0]; p.soh = o_stride[1];
-  p.h_kv = cache->h_kv; p.group = h_q / cache->h_kv;
+  p.h_kv = cache->h_kv;
   p.causal = causal != 0;
   p.qk_scale = qk_scale;
-  p.xcd_shift = device_topology(stream_device(static_cast<hipStream_t>(stream))).xcd_shift;
-  return launch_ragged(dtype, cache->head_dim, p,
-                       cache->cache_dtype == FA2_DTYPE_E4M3 ? fa2::kSourceE4m3 : fa2::kSourcePages, grid, stream);
+  return launch_ragged(dtype, cache->head_dim, h_q, p,
+                       cache->cache_dtype == FA2_DTYPE_E4M3 ? fa2::kSourceE4m3 : fa2::kSourcePages, workspace,
+                       workspace_bytes, stream);
+}
+
+size_t fa2_paged_workspace_bytes(int32_t h_q, int32_t h_kv, int32_t head_dim, int32_t n_tokens, int32_t n_seq,
+                                 int32_t num_cus) {
+  if (h_q <= 0 || h_kv <= 0 || h_q % h_kv || dim_index(head_dim) < 0 || n_tokens <= 0 || n_seq <= 0 || num_cus <= 0) return 0;
+  return ragged_plan(true, h_q, h_kv, head_dim, n_tokens, n_seq, num_cus).workspace;
 }
 
 }  // extern "C"

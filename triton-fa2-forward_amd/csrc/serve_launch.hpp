@@ -17,11 +17,14 @@ int launch_cache(bool write, int dtype, int head_dim, bool e4m3, const CachePara
 // Where K and V of a ragged attention launch lie: packed rows, 16-bit pages, e4m3 pages.
 constexpr int kSourcePacked = 0, kSourcePages = 1, kSourceE4m3 = 2;
 
+// The ragged attention kernel with 32 * row_waves (1 or 4) rows per workgroup, and after it, with p.shares > 0,
+// the merge of the row tiles that its shares cut.
 template <int DT, int D>
-int launch_ragged(const RaggedParams& p, int source, unsigned grid, hipStream_t stream);
+int launch_ragged(const RaggedParams& p, int source, int row_waves, unsigned grid, hipStream_t stream);
 
 #define FA2_DECLARE_RAGGED(DT, D) \
-  extern template int launch_ragged<DT, D>(const RaggedParams&, int, unsigned, hipStream_t);
+  template <>                     \
+  int launch_ragged<DT, D>(const RaggedParams&, int, int, unsigned, hipStream_t);
 FA2_DECLARE_RAGGED(0, 16)
 FA2_DECLARE_RAGGED(0, 32)
 FA2_DECLARE_RAGGED(0, 64)

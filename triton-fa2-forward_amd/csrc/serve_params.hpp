@@ -78,6 +78,10 @@ struct RaggedParams {
   int32_t h_kv, group, causal;
   float qk_scale;
   int32_t xcd_shift;
+  // 0: a workgroup per row tile. Above: that many workgroups per KV head share its work evenly by
+  // cutting the row tiles' key ranges; the pieces of a cut row tile meet in `parts`.
+  int32_t shares;
+  float* parts;  // [h_kv * shares][2][block_m][head_dim + 4]: O, then m, l, exact l
 };
 
 }  // namespace fa2

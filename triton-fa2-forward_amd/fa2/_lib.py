@@ -65,7 +65,8 @@ SIGNATURES = {
     "fa2_attn_packed": (ctypes.c_int, [_vp, _vp, _vp, _vp, _i64p, _i64p, _i64p, _i64p, _vp, _vp, _i32, _i32, _i32,
                                        _i32, _i32, _i32, _i32, _i32, ctypes.c_float, _vp, _vp]),
     "fa2_attn_paged": (ctypes.c_int, [_vp, _vp, _i64p, _i64p, _cachep, _seqp, _i32, _i32, _i32, ctypes.c_float,
-                                      _vp, _vp]),
+                                      _vp, _vp, ctypes.c_size_t, _vp]),
+    "fa2_paged_workspace_bytes": (ctypes.c_size_t, [_i32] * 6),
     "fa2_last_error": (ctypes.c_char_p, []),
     "fa2_version": (ctypes.c_char_p, []),
 }
@@ -267,8 +268,13 @@ def attn_packed(q, k, v, out, cu, cu_kv, causal, qk_scale, lse, stream):
         DTYPE_CODE[q.dtype], int(bool(causal)), qk_scale, _ptr(lse), stream), "fa2_attn_packed")
 
 
-def attn_paged(q, out, cache, seq, causal, qk_scale, lse, stream):
-    """Call fa2_attn_paged; lse may be None."""
+def paged_workspace_bytes(H_q, H_kv, D, n_tokens, n_seq, num_cus):
+    return int(lib().fa2_paged_workspace_bytes(H_q, H_kv, D, n_tokens, n_seq, num_cus))
+
+
+def attn_paged(q, out, cache, seq, causal, qk_scale, lse, workspace, stream):
+    """Call fa2_attn_paged; lse and workspace (uint8) may be None."""
     _checked(lib().fa2_attn_paged(q.data_ptr(), out.data_ptr(), _strides(q), _strides(out), ctypes.byref(cache),
                                   ctypes.byref(seq), q.shape[1], DTYPE_CODE[q.dtype], int(bool(causal)), qk_scale,
-                                  _ptr(lse), stream), "fa2_attn_paged")
+                                  _ptr(lse), _ptr(workspace), 0 if workspace is None else workspace.numel(), stream),
+             "fa2_attn_paged")
