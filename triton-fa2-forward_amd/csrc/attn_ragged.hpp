@@ -74,7 +74,10 @@ void attn_ragged_kernel(const RaggedParams p) {
   Share share = {0, 0, 0, 0};
   if (p.shares > 0) {
     share = find_share<BM, kPages>(p, rank, lane, &cur);
-    if (share.x >= share.end) return;
+    if (share.x >= share.end) {
+      if (tid == 0) merge_of(p, hkv, rank)->first = -1;
+      return;
+    }
   } else if (!find_tile<BM, kPages>(p, rank, lane, &cur)) {
     return;
   }
@@ -167,6 +170,11 @@ void attn_ragged_kernel(const RaggedParams p) {
       auto cut = [&](int64_t x) { return (int)((double)x * all_tiles / (double)length); };
       if (!starts) t_begin = cut(share.in);
       if (!ends) t_end = cut(out);
+      if (first_piece && tid == 0) {  // what the merge of a tile that ends here needs to know
+        Merge m = {-1, row0, row_end - row0, sq.first, n_kv, shift};
+        if (!starts && ends) m.first = (int)((share.x - share.in) / share.size);
+        *merge_of(p, hkv, rank) = m;
+      }
       share.x += out - share.in;
       share.in = 0;
     }
@@ -736,44 +744,48 @@ void attn_ragged_kernel(const RaggedParams p) {
 }
 
 // Merges the pieces of the row tile that ends in share `rank` and starts in an earlier one: with M the largest of the
-// pieces' references m_i, O = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i, in the order of the shares.
-template <int DT, int D, bool PAGES, int GW>
+// pieces' references m_i, O = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i, in the order of the shares. 32 rows a
+// workgroup, 4 dims a thread; bound by the latency of the pieces' loads, so four pieces are loaded at once.
+template <int DT, int D, int GW>
 __global__ __launch_bounds__(256) void attn_ragged_combine_kernel(const RaggedParams p) {
   using E = Elem<DT>;
-  constexpr int BM = 32 * GW, QPR = D / 4;
-  const int lane = threadIdx.x & 63;
-  int hkv, rank;
-  head_and_rank(p, (int)blockIdx.x, &hkv, &rank);
-  Cursor cur;
-  const Share share = find_share<BM, PAGES>(p, rank, lane, &cur);
-  if (share.x >= share.end || share.in == 0) return;
-  const LaneSequence sq = sequence_at(cur.lanes, cur.l);
-  const int64_t length = lengths_of<BM>(p, sq.n_q, sq.n_kv).of(cur.tile);
-  if (length - share.in > share.end - share.x) return;  // it ends in a later share
-  const int first = (int)((share.x - share.in) / share.size);
-  const int rows = sq.n_q * p.group, row0 = cur.tile * BM;
-  const int n = min(BM, rows - row0) * QPR;
+  constexpr int BM = 32 * GW, QPR = D / 4, STEP = 4;
+  const int rank = (int)blockIdx.x / GW % p.shares, hkv = (int)blockIdx.x / GW / p.shares;
+  const Merge at = *merge_of(p, hkv, rank);
+  if (at.first < 0) return;
+  const int x0 = (int)blockIdx.x % GW * 32;
+  const int n = min(32, at.rows - x0) * QPR;
   for (int t = (int)threadIdx.x; t < n; t += 256) {
-    const int x = t / QPR, q = t % QPR;
-    float M = -INFINITY;
-    for (int i = first; i <= rank; ++i)
-      M = fmaxf(M, part_of<BM, D>(p, hkv, i, i == first)[x * (D + 4) + D]);
+    const int x = x0 + t / QPR, q = t % QPR;
+    float M = -INFINITY, l = 0.f, lx = 0.f;
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    float l = 0.f, lx = 0.f;
     bool nan = false;
-    for (int i = first; i <= rank; ++i) {
-      const float* part = part_of<BM, D>(p, hkv, i, i == first) + x * (D + 4);
-      const f32x4 sums = *(const f32x4*)(part + D), v = *(const f32x4*)(part + 4 * q);
-      const float w = sums[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sums[0] - M);
-      nan |= sums[0] != sums[0];
-      l = __builtin_fmaf(w, sums[1], l);
-      lx = __builtin_fmaf(w, sums[2], lx);
+    for (int i0 = at.first; i0 <= rank; i0 += STEP) {
+      f32x4 sums[STEP], v[STEP];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(w, v[e], o[e]);
+      for (int k = 0; k < STEP; ++k) {
+        const int i = min(i0 + k, rank);
+        const float* part = part_of<BM, D>(p, hkv, i, i == at.first) + x * (D + 4);
+        sums[k] = *(const f32x4*)(part + D);
+        v[k] = *(const f32x4*)(part + 4 * q);
+      }
+#pragma unroll
+      for (int k = 0; k < STEP; ++k) {
+        if (i0 + k > rank) break;
+        const float m = sums[k][0], M_new = fmaxf(M, m);
+        const float a = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - M_new);
+        const float w = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - M_new);
+        nan |= m != m;
+        M = M_new;
+        l = l * a + w * sums[k][1];
+        lx = lx * a + w * sums[k][2];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = o[e] * a + w * v[k][e];
+      }
     }
-    const int pos = (row0 + x) / p.group, head = hkv * p.group + (row0 + x - pos * p.group);
-    const int64_t token = sq.first + pos;
-    const bool none = (p.causal ? min(pos + sq.n_kv - sq.n_q, sq.n_kv - 1) : sq.n_kv - 1) < 0;
+    const int pos = (at.row0 + x) / p.group, head = hkv * p.group + (at.row0 + x - pos * p.group);
+    const int64_t token = at.token + pos;
+    const bool none = (p.causal ? min(pos + at.shift, at.n_kv - 1) : at.n_kv - 1) < 0;
     const float inv = none ? 0.f : 1.0f / l;
     *(u32x2*)(p.o + token * p.sot + head * p.soh + 4 * q) =
         u32x2{E::pack2(o[0] * inv, o[1] * inv), E::pack2(o[2] * inv, o[3] * inv)};

@@ -232,4 +232,15 @@ __device__ __forceinline__ float* part_of(const RaggedParams& p, int head, int s
   return p.parts + (((int64_t)head * p.shares + share) * 2 + slot) * (BM * (D + 4));
 }
 
+// What the merge of the tile that ends in a share needs: the share it starts in (-1: none ends here, or it lies in
+// this share alone), its first row in the sequence and its rows, the sequence's first token, its keys, and the shift of its
+// causal mask.
+struct alignas(16) Merge {
+  int first, row0, rows, token, n_kv, shift;
+};
+__device__ __forceinline__ Merge* merge_of(const RaggedParams& p, int head, int share) {
+  static_assert(sizeof(Merge) == kMergeBytes);
+  return static_cast<Merge*>(p.merges) + ((int64_t)head * p.shares + share);
+}
+
 }  // namespace fa2

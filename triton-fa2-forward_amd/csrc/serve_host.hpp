@@ -122,7 +122,7 @@ struct RaggedPlan {
   int row_waves = 4;  // 32-row workgroups (1) or 128-row ones (4)
   int shares = 0;     // workgroups per KV head that share its work; 0: one per row tile
   int64_t grid = 0;
-  size_t workspace = 0;
+  size_t parts = 0, workspace = 0;  // bytes of the partial results, and with what their merge needs to know
 };
 RaggedPlan ragged_plan(bool paged, int32_t h_q, int32_t h_kv, int32_t head_dim, int32_t n_tokens, int32_t n_seq, int cus) {
   RaggedPlan pl;
@@ -135,7 +135,8 @@ RaggedPlan ragged_plan(bool paged, int32_t h_q, int32_t h_kv, int32_t head_dim, 
   const int64_t n = tiles(32 * pl.row_waves);
   if (paged && n * h_kv < 8 * (int64_t)cus) {
     pl.shares = std::max(1, 2 * cus / h_kv);
-    pl.workspace = (size_t)h_kv * pl.shares * 2 * 32 * pl.row_waves * (head_dim + 4) * sizeof(float);
+    pl.parts = (size_t)h_kv * pl.shares * 2 * 32 * pl.row_waves * (head_dim + 4) * sizeof(float);  // (a multiple of 256)
+    pl.workspace = pl.parts + (size_t)h_kv * pl.shares * fa2::kMergeBytes;
   }
   pl.grid = (pl.shares ? pl.shares : n) * h_kv;
   return pl;
@@ -169,6 +170,7 @@ int launch_ragged(int32_t dtype, int32_t head_dim, int32_t h_q, fa2::RaggedParam
   p.xcd_shift = topo.xcd_shift;
   p.shares = pl.shares;
   p.parts = static_cast<float*>(workspace);
+  p.merges = static_cast<char*>(workspace) + pl.parts;
   const unsigned g = (unsigned)pl.grid;
   int e;
   switch (dtype * 4 + dim_index(head_dim)) {

@@ -64,6 +64,8 @@ struct CacheParams {
   RotaryPlan rot;
 };
 
+constexpr int kMergeBytes = 32;
+
 // Attention of packed rows. K and V are packed rows too (source 0), pages of 16-bit elements (1) or of
 // e4m3 (2).
 struct RaggedParams {
@@ -82,6 +84,7 @@ struct RaggedParams {
   // cutting the row tiles' key ranges; the pieces of a cut row tile meet in `parts`.
   int32_t shares;
   float* parts;  // [h_kv * shares][2][block_m][head_dim + 4]: O, then m, l, exact l
+  void* merges;  // [h_kv * shares] of kMergeBytes: the tile that ends in each share
 };
 
 }  // namespace fa2

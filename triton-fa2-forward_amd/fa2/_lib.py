@@ -101,15 +101,24 @@ def build_id():
                                              *sys.version_info[:2])
 
 
-def _load_fast_call():
-    """The native common call of attention() (csrc/fa2_torch.cpp), built beside the library; None where
-    it is missing or was built for another torch or Python: attention() then makes every call itself,
-    through ctypes."""
+def _load_native():
+    """The native common calls (csrc/fa2_torch.cpp), built beside the library; None where they are missing
+    or were built for another torch or Python: the Python functions then make every call themselves, through
+    ctypes."""
     try:
         from . import _torch_call
     except ImportError:
         return None
-    return _torch_call.call if getattr(_torch_call, "built_for", None) == build_id() else None
+    return _torch_call if getattr(_torch_call, "built_for", None) == build_id() else None
+
+
+native = _load_native()  # the serving operators' (fa2.rotary, fa2.packed, fa2.paged)
+
+
+def _load_fast_call():
+    """attention()'s native common call, or None."""
+    module = _load_native()
+    return None if module is None else module.call
 
 
 fast_call = _load_fast_call()

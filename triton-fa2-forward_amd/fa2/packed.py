@@ -64,6 +64,10 @@ def attention_packed(q, k, v, cu_seqlens, cu_seqlens_kv=None, *, causal=True, sm
         A row that sees no key gets 0, and a log-sum-exp of -inf.
     return_lse: also return the natural-log log-sum-exp of every row's scaled scores, fp32 [H_q, T].
     """
+    if _lib.native is not None:  # the common call, made natively; None: not one of those
+        result = _lib.native.attn_packed(q, k, v, cu_seqlens, cu_seqlens_kv, causal, sm_scale, return_lse, out)
+        if result is not None:
+            return result if out is None else (out, result[1]) if return_lse else out
     assert q.dim() == k.dim() == v.dim() == 3
     T, H_q, D = q.shape
     T_kv, H_kv, Dk = k.shape

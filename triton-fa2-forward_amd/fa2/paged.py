@@ -107,6 +107,11 @@ def cache_write(cache, k, v, block_table, cu_seqlens, seqlens, *, rotary=None, q
     Not written: tokens past the table or in a page outside the cache, and rows past the last
     sequence. Two tokens in one place are the caller's to avoid.
     """
+    if _lib.native is not None:  # the common call, made natively; None: not one of those
+        result = _lib.native.cache_write(*cache, block_table, cu_seqlens, seqlens, k, v,
+                                         *((None, False, 1.0) if rotary is None else rotary), q, q_out)
+        if result is not None:
+            return q_out if q is None or q_out is not None else result
     _check_cache(cache, k.dtype)
     _check_kv(cache, k, v)
     T, D = k.shape[0], k.shape[2]
@@ -145,6 +150,10 @@ def cache_read(cache, block_table, cu_seqlens, seqlens, n_tokens, *, dtype=None,
     if dtype is None:
         assert cache.k.dtype in _16BIT or out is not None, "an e4m3 cache needs the dtype to read it as"
         dtype = cache.k.dtype if out is None else out[0].dtype
+    if out is None and _lib.native is not None:  # the common call, made natively; None: not one of those
+        result = _lib.native.cache_read(*cache, block_table, cu_seqlens, seqlens, n_tokens, dtype)
+        if result is not None:
+            return result
     _check_cache(cache, dtype)
     if n_tokens < 0:
         raise ValueError(f"n_tokens must not be negative, got {n_tokens}")
@@ -177,6 +186,10 @@ def attention_paged(q, cache, block_table, cu_seqlens, seqlens, *, causal=True, 
     rows that see its tokens NaN.
     return_lse: also return the natural-log log-sum-exp of every row's scaled scores, fp32 [H_q, T].
     """
+    if _lib.native is not None:  # the common call, made natively; None: not one of those
+        result = _lib.native.attn_paged(*cache, block_table, cu_seqlens, seqlens, q, causal, sm_scale, return_lse, out)
+        if result is not None:
+            return result if out is None else (out, result[1]) if return_lse else out
     assert q.dim() == 3
     T, H_q, D = q.shape
     _check_cache(cache, q.dtype)

@@ -94,6 +94,10 @@ def rotary(x, positions, plan, *, out=None):
     positions: int32 or int64. Returns out, laid out like x; out=x rotates in place. A pair (a, b) at
     position p becomes scale * (a cos - b sin, b cos + a sin) of the angle p * freqs[i].
     """
+    if _lib.native is not None:  # the common call, made natively; None: not one of those
+        result = _lib.native.rotary(x, positions, *plan, out)
+        if result is not None:
+            return result if out is None else out
     assert x.dim() in (3, 4) and x.dtype in (torch.float16, torch.bfloat16)
     D = x.shape[-1]
     assert D in (16, 32, 64, 128), "head_dim must be a power of two in [16, 128]"
