@@ -63,6 +63,28 @@ def attention(q, k, v, causal, sm_scale=None):
     if causal:
         see = torch.arange(m, device=q.device) <= torch.arange(n, device=q.device)[:, None] + (m - n)
     some = see.any(1)
+    group = h_q // h_kv
+    for h in range(h_kv):  # the group of query heads of a KV head at once
+        heads = slice(h * group, (h + 1) * group)
+        qh, kt, vh = q[:, heads].double().reshape(n * group, D), k[:, h].double().t().contiguous(), v[:, h].double()
+        sees = see.repeat_interleave(group, 0)
+        any_ = some.repeat_interleave(group)
+        s = (qh @ kt * sm_scale).masked_fill(~sees, -math.inf)
+        w = torch.where(sees, torch.softmax(s, 1), 0.0)
+        fine = vh.isfinite().all(1)
+        o = w[:, fine] @ vh[fine]
+        for j in (~fine).nonzero()[:, 0].tolist():  # infinite and NaN values: only where they are seen
+            o += torch.where(sees[:, j, None], w[:, j, None] * vh[j], 0.0)
+        out[:, heads] = torch.where(any_[:, None], o, 0.0).view(n, group, D)
+        size[:, heads] = torch.where(any_[:, None], w[:, fine] @ vh[fine].abs(), 0.0).view(n, group, D)
+        lse[heads] = torch.where(any_, torch.logsumexp(s, 1), -math.inf).view(n, group).t()
+        score = (qh.abs() @ kt.abs()).masked_fill(~sees, 0.0).nan_to_num(0, 0, 0).amax(1) * sm_scale
+        big[:, heads, 0] = score.view(n, group)
+    return out, lse, size, big
+    see = torch.ones(n, m, dtype=torch.bool, device=q.device)
+    if causal:
+        see = torch.arange(m, device=q.device) <= torch.arange(n, device=q.device)[:, None] + (m - n)
+    some = see.any(1)
     for h in range(h_q):
         qh, kh, vh = q[:, h].double(), k[:, h // (h_q // h_kv)].double(), v[:, h // (h_q // h_kv)].double()
         s = (qh @ kh.t().contiguous() * sm_scale).masked_fill(~see, -math.inf)

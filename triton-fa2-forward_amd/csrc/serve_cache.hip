@@ -22,7 +22,8 @@ namespace fa2 {
 
 namespace {
 
-constexpr int kMaxTokensPerWg = 8;
+constexpr int kMaxTokensPerWg = 16;
+constexpr int kRowsAtOnce = 4;  // rows of a lane whose loads are in flight together
 constexpr int kMaxHalf = 64;  // head_dim 128, all of it rotated
 
 // cos and sin of 2 pi x for |x| <= 1/2 turns
@@ -43,22 +44,35 @@ __device__ __forceinline__ void fill_angles(double (*cs)[kMaxHalf][2], const Rot
   }
 }
 
-// The 8 values x[8 chunk ..] of a row, rotated (T: the type the products are formed in)
+// This lane's 8 values x[8 chunk ..] of a row, and with them the 8 that they are paired with where those lie in
+// another chunk of the row
+struct Chunks {
+  u32x4 own, other;
+};
+__device__ __forceinline__ Chunks load_chunks(const uint16_t* row, int chunk, int half, bool interleaved) {
+  Chunks x;
+  x.own = *(const u32x4*)(row + 8 * chunk);
+  x.other = u32x4{0u, 0u, 0u, 0u};
+  const int d0 = 8 * chunk;
+  if (d0 < 2 * half && !interleaved) x.other = *(const u32x4*)(row + (d0 >= half ? d0 - half : d0 + half));
+  return x;
+}
+
+// ... rotated (T: the type the products are formed in)
 template <int DT, class T>
-__device__ __forceinline__ void rotated8(const uint16_t* row, int chunk, const RotaryPlan& rot,
+__device__ __forceinline__ void rotated8(const Chunks& in, int chunk, int half, bool interleaved,
                                          const double (*cs)[2], T (&y)[8]) {
-  const u32x4 own = *(const u32x4*)(row + 8 * chunk);
   float x[8];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    x[2 * i] = to_f32<DT>((uint16_t)own[i]);
-    x[2 * i + 1] = to_f32<DT>((uint16_t)(own[i] >> 16));
+    x[2 * i] = to_f32<DT>((uint16_t)in.own[i]);
+    x[2 * i + 1] = to_f32<DT>((uint16_t)(in.own[i] >> 16));
   }
   const int d0 = 8 * chunk;
-  if (d0 >= 2 * rot.half) {
+  if (d0 >= 2 * half) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) y[i] = x[i];
-  } else if (rot.interleaved) {
+  } else if (interleaved) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const T c = (T)cs[d0 / 2 + i][0], s = (T)cs[d0 / 2 + i][1];
@@ -66,13 +80,12 @@ __device__ __forceinline__ void rotated8(const uint16_t* row, int chunk, const R
       y[2 * i + 1] = (T)x[2 * i + 1] * c + (T)x[2 * i] * s;
     }
   } else {
-    const bool second = d0 >= rot.half;
-    const int f0 = second ? d0 - rot.half : d0;
-    const u32x4 other = *(const u32x4*)(row + (second ? f0 : d0 + rot.half));
+    const bool second = d0 >= half;
+    const int f0 = second ? d0 - half : d0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const T c = (T)cs[f0 + i][0], s = (T)cs[f0 + i][1];
-      const T o = (T)to_f32<DT>((uint16_t)(other[i / 2] >> (16 * (i & 1))));
+      const T o = (T)to_f32<DT>((uint16_t)(in.other[i / 2] >> (16 * (i & 1))));
       y[i] = (T)x[i] * c + (second ? o * s : -(o * s));
     }
   }
@@ -107,21 +120,27 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryParams p) {
     const int t = r / p.heads, h = r - t * p.heads;
     const int64_t b = (t0 + t) / p.n, i = (t0 + t) - b * p.n;
     float y[8];
-    rotated8<DT>(p.x + b * p.sxb + h * p.sxh + i * p.sxn, chunk, p.rot, cs[t], y);
+    rotated8<DT>(load_chunks(p.x + b * p.sxb + h * p.sxh + i * p.sxn, chunk, p.rot.half, p.rot.interleaved), chunk,
+                 p.rot.half, p.rot.interleaved, cs[t], y);
     *(u32x4*)(p.out + b * p.sob + h * p.soh + i * p.son + 8 * chunk) = pack8<DT>(y);
   }
 }
 
 // ---- the cache -------------------------------------------------------------------------------
 
-__device__ __forceinline__ char* cache_row(const CacheTensor& c, const Place& p, int head, int page_shift,
-                                           int bytes) {
-  const int64_t at = p.page * c.page + head * c.head + (int64_t)(p.pos & ((1 << page_shift) - 1)) * c.token;
-  return c.data + at * bytes;
+// Where a row of K (or V) lies in the cache, in elements, and its scale byte. Both tensors' strides are scalars and
+// the choice between them is made value by value: a reference to one of them, chosen per lane, would
+// have every lane load the strides from the kernel's arguments.
+__device__ __forceinline__ int64_t pick(bool second, int64_t a, int64_t b) { return second ? b : a; }
+__device__ __forceinline__ char* cache_row(const CacheParams& p, bool v, const Place& at, int head, int bytes) {
+  const int64_t row = at.pos & ((1 << p.seq.page_shift) - 1);
+  return (v ? p.vc.data : p.kc.data) + bytes * (at.page * pick(v, p.kc.page, p.vc.page) + head * pick(v, p.kc.head, p.vc.head) +
+                                                row * pick(v, p.kc.token, p.vc.token));
 }
-__device__ __forceinline__ uint8_t* scale_row(const CacheTensor& c, const Place& p, int head, int page_shift) {
-  return c.scale + p.page * c.scale_page + head * c.scale_head +
-         (int64_t)(p.pos & ((1 << page_shift) - 1)) * c.scale_token;
+__device__ __forceinline__ uint8_t* scale_row(const CacheParams& p, bool v, const Place& at, int head) {
+  const int64_t row = at.pos & ((1 << p.seq.page_shift) - 1);
+  return (v ? p.vc.scale : p.kc.scale) + at.page * pick(v, p.kc.scale_page, p.vc.scale_page) +
+         head * pick(v, p.kc.scale_head, p.vc.scale_head) + row * pick(v, p.kc.scale_token, p.vc.scale_token);
 }
 
 // One row's 8 values of this lane as e4m3, with the row's scale byte (D / 8 lanes hold a row).
@@ -158,15 +177,6 @@ __device__ __forceinline__ u32x2 quantise8(const T (&y)[8], uint32_t* scale_byte
   return u32x2{w[0], w[1]};
 }
 
-// The places of the workgroup's tokens, a wave per token in turn
-__device__ __forceinline__ void fill_places(Place* places, const Sequences& q, int t0, int tokens) {
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  for (int t = wave; t < tokens; t += 4) {
-    const Place p = find_place(q, t0 + t, lane);
-    if (lane == 0) places[t] = p;
-  }
-}
-
 // Rows per token: K heads, V heads, then (q) query heads. K is rotated in float64: a rotated value next to
 // a border between two e4m3 values goes to the one that its exact value goes to.
 template <int DT, int D, bool E4M3>
@@ -176,82 +186,126 @@ __global__ __launch_bounds__(256) void cache_write_kernel(const CacheParams p) {
   __shared__ Place places[kMaxTokensPerWg];
   const int t0 = (int)blockIdx.x * p.tokens_per_wg;
   const int tokens = min(p.tokens_per_wg, p.seq.n_tokens - t0);
-  fill_places(places, p.seq, t0, tokens);
-  __syncthreads();
-  if (p.rot.half) {
-    fill_angles(cs, p.rot, tokens, [&](int t) -> int64_t { return places[t].pos; });
-    __syncthreads();
-  }
   const int chunk = threadIdx.x % LPR;
   const int per_token = 2 * p.h_kv + (p.q ? p.h_q : 0);
   const int rows = tokens * per_token;
-  RotaryPlan none = p.rot;
-  none.half = 0;
-  for (int r = threadIdx.x / LPR; r < rows; r += 256 / LPR) {
-    const int t = r / per_token, x = r - t * per_token;
-    const Place at = places[t];
-    if (at.seq < 0) continue;
-    const int64_t tok = t0 + t;
-    if (x >= 2 * p.h_kv) {
-      const int h = x - 2 * p.h_kv;
-      float y[8];
-      rotated8<DT>(p.q + tok * p.sqt + h * p.sqh, chunk, p.rot, cs[t], y);
-      *(u32x4*)(p.q_out + tok * p.sot + h * p.soh + 8 * chunk) = pack8<DT>(y);
-      continue;
+  const int half = p.rot.half;
+  const bool interleaved = p.rot.interleaved;
+  for (int base = 0; base < rows; base += kRowsAtOnce * (256 / LPR)) {
+    Chunks in[kRowsAtOnce];
+    int token[kRowsAtOnce], which[kRowsAtOnce];  // row `which` of the token's; -1: nothing to do
+#pragma unroll
+    for (int u = 0; u < kRowsAtOnce; ++u) {
+      const int r = base + u * (256 / LPR) + (int)threadIdx.x / LPR;
+      token[u] = r / per_token;
+      which[u] = r < rows ? r - token[u] * per_token : -1;
+      if (r >= rows) continue;
+      const int x = which[u];
+      const int64_t tok = t0 + token[u];
+      const bool is_q = x >= 2 * p.h_kv, is_v = !is_q && x >= p.h_kv;
+      const uint16_t* src = is_q ? p.q : is_v ? p.v : p.k;
+      const int64_t at = tok * (is_q ? p.sqt : is_v ? p.svt : p.skt) +
+                         (is_q ? x - 2 * p.h_kv : is_v ? x - p.h_kv : x) * (is_q ? p.sqh : is_v ? p.svh : p.skh);
+      in[u] = load_chunks(src + at, chunk, is_v ? 0 : half, interleaved);
     }
-    if (at.page < 0) continue;
-    const bool is_v = x >= p.h_kv;
-    const int h = is_v ? x - p.h_kv : x;
-    const uint16_t* src = is_v ? p.v + tok * p.svt + h * p.svh : p.k + tok * p.skt + h * p.skh;
-    const CacheTensor& c = is_v ? p.vc : p.kc;
-    char* dst = cache_row(c, at, h, p.seq.page_shift, E4M3 ? 1 : 2);
-    if constexpr (E4M3) {
-      double y[8];
-      rotated8<DT>(src, chunk, is_v ? none : p.rot, cs[t], y);
-      uint32_t byte;
-      const u32x2 w = quantise8<DT, D>(y, &byte);
-      *(u32x2*)(dst + 8 * chunk) = w;
-      if (chunk == 0) *scale_row(c, at, h, p.seq.page_shift) = (uint8_t)byte;
-    } else {
-      float y[8];
-      rotated8<DT>(src, chunk, is_v ? none : p.rot, cs[t], y);
-      *(u32x4*)(dst + 16 * chunk) = pack8<DT>(y);
+    if (base == 0) {  // while the first rows are on their way
+      LanePlace place;
+      int page = -1;
+      const bool looks_up = threadIdx.x < 64;
+      if (looks_up) {
+        place = find_positions(p.seq, t0, tokens, (int)threadIdx.x);
+        if ((int)threadIdx.x < tokens) places[threadIdx.x].pos = place.pos;
+        page = find_page(p.seq, place);  // on its way while the angles are computed
+      }
+      __syncthreads();
+      if (p.rot.half) fill_angles(cs, p.rot, tokens, [&](int t) -> int64_t { return places[t].pos; });
+      if (looks_up && (int)threadIdx.x < tokens) places[threadIdx.x].page = page;
+      __syncthreads();
+    }
+#pragma unroll
+    for (int u = 0; u < kRowsAtOnce; ++u) {
+      const int x = which[u];
+      if (x < 0) continue;
+      const Place at = places[token[u]];
+      if (at.pos < 0) continue;
+      const double(*angles)[2] = cs[token[u]];
+      if (x >= 2 * p.h_kv) {
+        float y[8];
+        rotated8<DT>(in[u], chunk, half, interleaved, angles, y);
+        *(u32x4*)(p.q_out + (int64_t)(t0 + token[u]) * p.sot + (x - 2 * p.h_kv) * p.soh + 8 * chunk) = pack8<DT>(y);
+        continue;
+      }
+      if (at.page < 0) continue;
+      const bool is_v = x >= p.h_kv;
+      const int h = is_v ? x - p.h_kv : x;
+      char* dst = cache_row(p, is_v, at, h, E4M3 ? 1 : 2);
+      if constexpr (E4M3) {
+        double y[8];
+        rotated8<DT>(in[u], chunk, is_v ? 0 : half, interleaved, angles, y);
+        uint32_t byte;
+        const u32x2 w = quantise8<DT, D>(y, &byte);
+        *(u32x2*)(dst + 8 * chunk) = w;
+        if (chunk == 0) *scale_row(p, is_v, at, h) = (uint8_t)byte;
+      } else {
+        float y[8];
+        rotated8<DT>(in[u], chunk, is_v ? 0 : half, interleaved, angles, y);
+        *(u32x4*)(dst + 16 * chunk) = pack8<DT>(y);
+      }
     }
   }
 }
 
+// 16 bytes of the cache a lane: 8 values, or 16 of e4m3
 template <int DT, int D, bool E4M3>
 __global__ __launch_bounds__(256) void cache_read_kernel(const CacheParams p) {
-  constexpr int LPR = D / 8;
+  constexpr int LPR = D / (E4M3 ? 16 : 8), STEP = 256 / LPR, ROWS = 8;
   __shared__ Place places[kMaxTokensPerWg];
   const int t0 = (int)blockIdx.x * p.tokens_per_wg;
   const int tokens = min(p.tokens_per_wg, p.seq.n_tokens - t0);
-  fill_places(places, p.seq, t0, tokens);
+  if (threadIdx.x < 64) {
+    const LanePlace place = find_positions(p.seq, t0, tokens, (int)threadIdx.x);
+    const int page = find_page(p.seq, place);
+    if ((int)threadIdx.x < tokens) places[threadIdx.x] = Place{place.pos, page};
+  }
   __syncthreads();
   const int chunk = threadIdx.x % LPR;
-  const int rows = tokens * 2 * p.h_kv;
-  for (int r = threadIdx.x / LPR; r < rows; r += 256 / LPR) {
-    const int t = r / (2 * p.h_kv), x = r - t * 2 * p.h_kv;
-    const Place at = places[t];
-    if (at.seq < 0) continue;
-    const int64_t tok = t0 + t;
-    const bool is_v = x >= p.h_kv;
-    const int h = is_v ? x - p.h_kv : x;
-    const CacheTensor& c = is_v ? p.vc : p.kc;
-    u32x4 w = {0u, 0u, 0u, 0u};
-    if (at.page >= 0) {
-      const char* src = cache_row(c, at, h, p.seq.page_shift, E4M3 ? 1 : 2);
+  const int per_token = 2 * p.h_kv;
+  const int rows = tokens * per_token;
+  for (int r0 = threadIdx.x / LPR; r0 < rows; r0 += ROWS * STEP) {
+    u32x4 w[ROWS];
+    uint32_t scale[ROWS];
+    uint16_t* dst[ROWS];
+#pragma unroll
+    for (int u = 0; u < ROWS; ++u) {
+      const int r = r0 + u * STEP;
+      dst[u] = nullptr;
+      w[u] = u32x4{0u, 0u, 0u, 0u};
+      scale[u] = 0u;
+      if (r >= rows) continue;
+      const int t = r / per_token, x = r - t * per_token;
+      const Place at = places[t];
+      if (at.pos < 0) continue;
+      const int64_t tok = t0 + t;
+      const bool is_v = x >= p.h_kv;
+      const int h = is_v ? x - p.h_kv : x;
+      dst[u] = is_v ? p.v + tok * p.svt + h * p.svh : p.k + tok * p.skt + h * p.skh;
+      if (at.page < 0) continue;
+      w[u] = *(const u32x4*)(cache_row(p, is_v, at, h, E4M3 ? 1 : 2) + 16 * chunk);
+      if constexpr (E4M3) scale[u] = *scale_row(p, is_v, at, h);
+    }
+#pragma unroll
+    for (int u = 0; u < ROWS; ++u) {
+      if (!dst[u]) continue;
       if constexpr (E4M3) {
-        const u32x2 b = *(const u32x2*)(src + 8 * chunk);
-        const uint32_t scale = *scale_row(c, at, h, p.seq.page_shift);
-        const u32x2 lo = e4m3_to_16<DT>(b[0], scale), hi = e4m3_to_16<DT>(b[1], scale);
-        w = u32x4{lo[0], lo[1], hi[0], hi[1]};
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const u32x2 lo = e4m3_to_16<DT>(w[u][2 * i], scale[u]), hi = e4m3_to_16<DT>(w[u][2 * i + 1], scale[u]);
+          *(u32x4*)(dst[u] + 16 * chunk + 8 * i) = u32x4{lo[0], lo[1], hi[0], hi[1]};
+        }
       } else {
-        w = *(const u32x4*)(src + 16 * chunk);
+        *(u32x4*)(dst[u] + 8 * chunk) = w[u];
       }
     }
-    uint16_t* dst = is_v ? p.v + tok * p.svt + h * p.svh : p.k + tok * p.skt + h * p.skh;
-    *(u32x4*)(dst + 8 * chunk) = w;
   }
 }
 
@@ -276,9 +330,9 @@ int launch_cache_d(bool write, bool e4m3, const CacheParams& p, unsigned grid, h
 
 }  // namespace
 
-int serve_tokens_per_wg(int lanes_per_token) {
+int serve_tokens_per_wg(int lanes_per_token, int64_t tokens, int64_t least_wgs) {
   int n = 1;
-  while (n < kMaxTokensPerWg && 2 * n * lanes_per_token <= 256) n *= 2;
+  while (n < kMaxTokensPerWg && (2 * n * lanes_per_token <= 256 || tokens >= 2 * n * least_wgs)) n *= 2;
   return n;
 }
 

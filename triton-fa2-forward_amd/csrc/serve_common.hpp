@@ -34,29 +34,47 @@ __device__ __forceinline__ int find_sequence(const int32_t* cu, int n_seq, int t
   return lo;
 }
 
-// A packed row's sequence and position in it; seq < 0: the row belongs to none, or its place is before
-// the sequence's start (more rows than tokens).
+// A packed row's position in its sequence and the page of the cache that holds it. pos < 0: the row belongs to no
+// sequence, or its place is before the sequence's start (more rows than tokens). page < 0: past the table, or not a
+// page of the cache.
 struct Place {
-  int seq;
   int pos;
-  int page;  // -1: past the table, or not a page of the cache
+  int page;
 };
-__device__ __forceinline__ Place find_place(const Sequences& q, int t, int lane) {
-  Place p = {-1, 0, -1};
-  if (t >= q.n_tokens) return p;
-  const int s = find_sequence(q.cu, q.n_seq, t, lane);
-  const int end = row_bound(q.cu, s + 1, q.n_tokens);
-  if (t < row_bound(q.cu, s, q.n_tokens) || t >= end) return p;
-  const int64_t pos = (int64_t)max(q.lens[s], 0) - (end - t);
-  if (pos < 0) return p;
-  p.seq = s;
-  p.pos = (int)pos;
-  const int slot = p.pos >> q.page_shift;
-  if (slot < q.max_pages) {
-    const int page = q.table[s * q.table_stride + slot];
-    if ((unsigned)page < (unsigned)q.n_pages) p.page = page;
+
+// The sequences and positions of rows t0 .. t0 + tokens - 1 (at most 64), a lane each, by one wave: the ends of 64
+// sequences are loaded at once (past 64 sequences, of those from the first row's on, which is looked up) and
+// compared with every row, and the lengths of all rows are loaded together: two loads in a row for a group of rows.
+struct LanePlace {
+  int seq, pos;  // pos < 0: none
+};
+__device__ __forceinline__ LanePlace find_positions(const Sequences& q, int t0, int tokens, int lane) {
+  const int first = q.n_seq <= 64 ? 0 : find_sequence(q.cu, q.n_seq, t0, lane);
+  const int end = first + lane < q.n_seq ? q.cu[first + lane + 1] : 0x7fffffff;
+  int seq = first;
+  for (int i = 0; i < tokens; ++i) {  // (scalar: a ballot per row)
+    const uint64_t before = __builtin_amdgcn_ballot_w64(end <= t0 + i);
+    int s = first + __builtin_popcountll(before);
+    // 64 sequences that end before the row: it lies past them all
+    if (s - first == 64 && q.n_seq > 64) s = find_sequence(q.cu, q.n_seq, t0 + i, lane);
+    if (lane == i) seq = s;
   }
+  LanePlace p = {seq, -1};
+  const int t = t0 + lane;
+  if (lane >= tokens || seq >= q.n_seq) return p;
+  const int length = max(q.lens[seq], 0);
+  const int upto = row_bound(q.cu, seq + 1, q.n_tokens);
+  if (t < row_bound(q.cu, seq, q.n_tokens) || t >= upto) return p;
+  const int64_t pos = (int64_t)length - (upto - t);
+  if (pos >= 0) p.pos = (int)pos;
   return p;
+}
+// The page of a lane's position, as Place's
+__device__ __forceinline__ int find_page(const Sequences& q, const LanePlace& p) {
+  const int slot = p.pos >> q.page_shift;
+  if (p.pos < 0 || slot >= q.max_pages) return -1;
+  const int page = q.table[p.seq * q.table_stride + slot];
+  return (unsigned)page < (unsigned)q.n_pages ? page : -1;
 }
 
 // load_lds16 (attn_fwd_common.hpp) behind five wait states. A vector instruction may have written the

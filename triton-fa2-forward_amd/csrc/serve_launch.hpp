@@ -7,8 +7,9 @@
 
 namespace fa2 {
 
-// Tokens of one workgroup of the rotary and cache kernels: as many as its 256 lanes take rows of at once.
-int serve_tokens_per_wg(int lanes_per_token);
+// Tokens of one workgroup of the rotary and cache kernels: as many as its 256 lanes take rows of at once, and more
+// while at least `least_wgs` workgroups are left.
+int serve_tokens_per_wg(int lanes_per_token, int64_t tokens, int64_t least_wgs);
 
 int launch_rotary(int dtype, int head_dim, const RotaryParams& p, unsigned grid, hipStream_t stream);
 int launch_cache(bool write, int dtype, int head_dim, bool e4m3, const CacheParams& p, unsigned grid,
