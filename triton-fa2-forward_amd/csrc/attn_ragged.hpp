@@ -33,8 +33,9 @@ constexpr int ragged_block_n(int head_dim, int row_waves) {
 template <int DT, int D, int SRC, int GW>
 __global__ __launch_bounds__(256)
 __attribute__((amdgpu_waves_per_eu(2)))
-void attn_ragged_kernel(const RaggedParams p) {
+void attn_ragged_kernel(const RaggedParams) {
   using E = Elem<DT>;
+  ParamsRef p = params_here();
   constexpr bool kE4m3 = SRC == kSourceE4m3;
   constexpr bool kPages = SRC != kSourcePacked;
   constexpr int EB = kE4m3 ? 1 : 2;      // bytes of a cached element
@@ -50,7 +51,9 @@ void attn_ragged_kernel(const RaggedParams p) {
   constexpr int TCH = BN * CPR;          // chunks per K (or V) tile
   constexpr int NI = TCH / 64 * EB / 2;  // 1 KiB loads per tile
   constexpr int JW = (NI + GW - 1) / GW; // ... per wave
-  constexpr int RPI = BN / NI;           // rows of one load (one page: the host's rule on page sizes)
+  constexpr int RPI = BN / NI;           // rows of one load
+  // rows of a page at least (one load's rows lie in one page: the host's rule on page sizes), and the loads of them
+  constexpr int SEG = RPI > 16 ? RPI : 16, LPS = SEG / RPI;
   constexpr int LPR = 64 / RPI;          // lanes per row of a load
   static_assert(NI >= 1 && BN % NI == 0, "a tile must be whole 1 KiB loads");
   constexpr int QPR = D / 4;             // 16-byte pieces of an fp32 output row
@@ -70,18 +73,6 @@ void attn_ragged_kernel(const RaggedParams p) {
 
   int hkv, rank;
   head_and_rank(p, (int)blockIdx.x, &hkv, &rank);
-  Cursor cur;
-  Share share = {0, 0, 0, 0};
-  if (p.shares > 0) {
-    share = find_share<BM, kPages>(p, rank, lane, &cur);
-    if (share.x >= share.end) {
-      if (tid == 0) merge_of(p, hkv, rank)->first = -1;
-      return;
-    }
-  } else if (!find_tile<BM, kPages>(p, rank, lane, &cur)) {
-    return;
-  }
-
   // ---- LDS operand reads, as in attn_fwd_kernel.hpp
   const FA2_LDS char* gbuf = (const FA2_LDS char*)(lds + grp * BUFS * 2 * TCH);
   auto kbuf = [&](int i) { return gbuf + (BUFS == 1 ? 0 : (i & 1) * TCH * 16); };
@@ -116,7 +107,7 @@ void attn_ragged_kernel(const RaggedParams p) {
   };
 
   // ---- this head's K and V: where they start, the bytes between pages and between tokens (below 2^31: the
-  // host's limits), and this lane's offset from a tile's first row in load j of the tile
+  // host's limits), and this lane's offset from a segment's first row in load u of the segment
   const int page_shift = p.seq.page_shift;
   struct Source {
     const char* data;
@@ -126,26 +117,39 @@ void attn_ragged_kernel(const RaggedParams p) {
   const Source vs = {p.vc.data + hkv * p.vc.head * EB, (uint32_t)p.vc.page * EB, (uint32_t)p.vc.token * EB};
   const Source kscale = {(const char*)p.kc.scale + hkv * p.kc.scale_head, (uint32_t)p.kc.scale_page, (uint32_t)p.kc.scale_token};
   const Source vscale = {(const char*)p.vc.scale + hkv * p.vc.scale_head, (uint32_t)p.vc.scale_page, (uint32_t)p.vc.scale_token};
-  uint32_t koff[JW], voff[JW], kscale_off[JW], vscale_off[JW];
+  uint32_t koff[LPS], voff[LPS], kscale_off[LPS], vscale_off[LPS];
 #pragma unroll
-  for (int jj = 0; jj < JW; ++jj) {
-    const int row = (gwave + jj * GW) * RPI + lane / LPR, x = lane % LPR;
+  for (int u = 0; u < LPS; ++u) {
+    const int row = u * RPI + lane / LPR, x = lane % LPR;  // (the swizzle keys repeat every 16 rows)
     if constexpr (kE4m3) {
-      koff[jj] = (uint32_t)row * ks.token + x * 16;
-      voff[jj] = (uint32_t)row * vs.token + x * 16;
-      kscale_off[jj] = (uint32_t)row * kscale.token;
-      vscale_off[jj] = (uint32_t)row * vscale.token;
+      koff[u] = (uint32_t)row * ks.token + x * 16;
+      voff[u] = (uint32_t)row * vs.token + x * 16;
+      kscale_off[u] = (uint32_t)row * kscale.token;
+      vscale_off[u] = (uint32_t)row * vscale.token;
     } else {
-      koff[jj] = (uint32_t)row * ks.token + (x ^ k_key<D>(pi_row(row & 31) & 15)) * 16;
-      voff[jj] = (uint32_t)row * vs.token + (x ^ v_key<D>(row & 15)) * 16;
+      koff[u] = (uint32_t)row * ks.token + (x ^ k_key<D>(pi_row(row & 31) & 15)) * 16;
+      voff[u] = (uint32_t)row * vs.token + (x ^ v_key<D>(row & 15)) * 16;
     }
   }
 
   const float qk_scale = p.qk_scale;
-  const bool want_exact = p.lse != nullptr;
+  const bool want_exact = p.lse != nullptr, causal = p.causal != 0, shared = p.shares > 0;
 
-  // ---- one piece: the cursor's row tile, its key tiles [part 0: all of them] `from` .. `to` of `of`
-  for (bool first_piece = true;; first_piece = false) {
+  // ---- the workgroup's work: the pieces of its share, or its one tile
+  Cursor cur;
+  Share share = {0, 0, 0, 0};
+  if (shared) {
+    share = find_share<BM, kPages>(p, rank, lane, &cur);
+    if (share.x >= share.end) {
+      if (tid == 0) merge_of(p, hkv, rank)->first = -1;
+      return;
+    }
+  } else if (!find_tile<BM, kPages>(p, rank, lane, &cur)) {
+    return;
+  }
+  bool fresh = true;  // LDS has not been used yet
+  for (bool first_piece = true, more = true; more; first_piece = false) {
+    ParamsRef p = params_here();
     const LaneSequence sq = sequence_at(cur.lanes, cur.l);
     const int seq = cur.s0 + cur.l, n_kv = sq.n_kv;
     const int rows = sq.n_q * p.group;
@@ -153,33 +157,39 @@ void attn_ragged_kernel(const RaggedParams p) {
     const int row_end = min(row0 + BM, rows);
     const int shift = n_kv - sq.n_q;      // causal: position i sees keys up to i + shift
     // the last key of a position, the end of the keys that some row sees, and of those that every row sees
-    auto last_of = [&](int i) { return p.causal ? min(i + shift, n_kv - 1) : n_kv - 1; };
+    auto last_of = [&](int i) { return causal ? min(i + shift, n_kv - 1) : n_kv - 1; };
     const int see_end = max(last_of((row_end - 1) / p.group) + 1, 0);
     const int full_end = max(last_of(row0 / p.group) + 1, 0);
     const int all_tiles = (see_end + BN - 1) / BN;
 
     int t_begin = 0, t_end = all_tiles;
-    bool starts = true, ends = true;  // whether the piece holds the tile's first and last keys
-    if (p.shares > 0) {
+    float* part = nullptr;  // where the piece's partial results go, if it is not the whole tile
+    if (shared) {
       const int64_t length = lengths_of<BM>(p, sq.n_q, n_kv).of(cur.tile);
       const int64_t out = min(length, share.in + (share.end - share.x));
-      starts = share.in == 0;
-      ends = out == length;
-      // a cut at x of the tile's length lies before key tile x * all_tiles / length: the shares on both
-      // sides of it compute the same
-      auto cut = [&](int64_t x) { return (int)((double)x * all_tiles / (double)length); };
-      if (!starts) t_begin = cut(share.in);
-      if (!ends) t_end = cut(out);
+      if (share.in > 0) t_begin = cut_at(share.in, length, all_tiles);
+      if (out < length) t_end = cut_at(out, length, all_tiles);
+      // nothing between the cuts (a tile that sees no key at all belongs to the share that it starts in)
+      const bool empty = all_tiles == 0 ? share.in > 0 : t_begin == t_end;
+      const bool whole = t_begin == 0 && t_end == all_tiles;
+      if (!whole) part = part_of<BM, D>(p, hkv, rank, share.in == 0);
       if (first_piece && tid == 0) {  // what the merge of a tile that ends here needs to know
         Merge m = {-1, row0, row_end - row0, sq.first, n_kv, shift};
-        if (!starts && ends) m.first = (int)((share.x - share.in) / share.size);
+        if (!empty && !whole && t_end == all_tiles) m.first = (int)((share.x - share.in) / share.size);
         *merge_of(p, hkv, rank) = m;
       }
+      const bool null_part = empty && !whole && tid < row_end - row0;
       share.x += out - share.in;
       share.in = 0;
+      if (empty) {
+        if (null_part) *(f32x4*)(part + part_sums<BM, D>(tid)) = f32x4{-INFINITY, 0.f, 0.f, 0.f};
+        more = share.x < share.end && next_tile<BM, kPages>(p, lane, &cur);
+        continue;
+      }
     }
     const int kv_begin = t_begin * BN, kv_end = min(t_end * BN, see_end);
-    if (!first_piece) __syncthreads();  // the last piece's merge has left LDS
+    if (!fresh) __syncthreads();  // the last piece's merge has left LDS
+    fresh = false;
 
     // ---- this lane's row; rows past the last repeat it and are never stored
     const int wr = gwave * 32 + c;  // the row inside the workgroup
@@ -207,6 +217,7 @@ void attn_ragged_kernel(const RaggedParams p) {
     const int block = 64 >> tile_shift;  // tiles of a block
     int pages = 0, pages_next = 0, bad = 0;
     auto load_pages = [&](int i0) {
+      ParamsRef p = params_here();
       const int i = i0 + (lane >> tile_shift);
       const int64_t n = kv_begin + (int64_t)(grp + (int64_t)i * KG) * BN +
                         ((int64_t)(lane & ((1 << tile_shift) - 1)) << page_shift);
@@ -215,7 +226,7 @@ void attn_ragged_kernel(const RaggedParams p) {
       return e;
     };
     auto checked_pages = [&](int e) {
-      if ((unsigned)e >= (unsigned)p.seq.n_pages) {
+      if ((unsigned)e >= (unsigned)params_here().seq.n_pages) {
         bad = 1;
         e = 0;
       }
@@ -235,39 +246,32 @@ void attn_ragged_kernel(const RaggedParams p) {
       return __builtin_amdgcn_readlane(pages, ((i << tile_shift) & 63) + (x >> page_shift));
     };
 
-    // ---- the memory of tile i's rows before kv_end (a load gives zeros past them), for load j: the tile's first
-    // row as if all of the tile lay in the page of load j's rows. One page for the whole tile where it holds
-    // the tile's keys.
-    const bool one_page = !kPages || page_shift >= kLog2Bn;
-    auto tile_bytes = [&](const Source& x, int i, int row_bytes) {
-      const int valid = max(min(kv_end - key_of(i), BN), 0);
+    // ---- a wave loads JW KiB of consecutive rows of a tile, from row gwave * JW * RPI on: segments of SEG rows, each in
+    // one page, with a buffer resource each. Rows from kv_end on read as zeros.
+    constexpr int NS = JW / LPS;
+    static_assert(JW % LPS == 0, "a wave loads whole segments");
+    const bool loads = NI % GW == 0 || gwave < NI;  // (tiles of fewer KiB than waves)
+    auto segment_row = [&](int s) { return gwave * JW * RPI + s * SEG; };
+    auto segment_data = [&](const Source& x, int i, int s) {
+      const int n = key_of(i) + segment_row(s);
+      if constexpr (kPages)
+        return x.data + (uint64_t)(uint32_t)page_of(i, segment_row(s)) * x.page +
+               (uint64_t)(uint32_t)(n & ((1 << page_shift) - 1)) * x.token;
+      else
+        return x.data + (uint64_t)(uint32_t)(sq.kv_first + n) * x.token;
+    };
+    auto segment_bytes = [&](const Source& x, int i, int s, int row_bytes) {
+      const int valid = max(min(kv_end - key_of(i) - segment_row(s), SEG), 0);
       return (uint32_t)max(valid * (int)x.token - ((int)x.token - row_bytes), 0);
     };
-    auto tile_data = [&](const Source& x, int i, int j) {
-      const int n = key_of(i);
-      if constexpr (kPages) {
-        const int in_page = (n + j * RPI) & ((1 << page_shift) - 1);
-        return x.data + (uint64_t)(uint32_t)page_of(i, j * RPI) * x.page + (int64_t)(in_page - j * RPI) * x.token;
-      } else {
-        return x.data + (uint64_t)(uint32_t)(sq.kv_first + n) * x.token;
-      }
-    };
-    auto issue = [&](const Source& x, const uint32_t (&off)[JW], const FA2_LDS char* buf, int i) {
-      const uint32_t bytes = tile_bytes(x, i, D * 2);
-      u32x4 rsrc;
-      if (one_page) {
-        rsrc = make_desc(tile_data(x, i, 0), bytes);
+    auto issue = [&](const Source& x, const uint32_t (&off)[LPS], const FA2_LDS char* buf, int i) {
+      if (!loads) return;
 #pragma unroll
-        for (int jj = 0; jj < JW; ++jj) {
-          const int j = gwave + jj * GW;
-          if (NI % GW == 0 || j < NI) load_lds16_settled(rsrc, off[jj], lds_addr(buf + j * 1024));
-        }
-      } else {
+      for (int s = 0; s < NS; ++s) {
+        const u32x4 rsrc = make_desc(segment_data(x, i, s), segment_bytes(x, i, s, D * 2));
 #pragma unroll
-        for (int jj = 0; jj < JW; ++jj) {
-          const int j = gwave + jj * GW;
-          if (NI % GW == 0 || j < NI) load_lds16_settled(make_desc(tile_data(x, i, j), bytes), off[jj], lds_addr(buf + j * 1024));
-        }
+        for (int u = 0; u < LPS; ++u)
+          load_lds16_settled(rsrc, off[u], lds_addr(buf + (gwave * JW + s * LPS + u) * 1024));
       }
     };
     auto issue_k = [&](int i) { issue(ks, koff, kbuf(i), i); };
@@ -278,14 +282,17 @@ void attn_ragged_kernel(const RaggedParams p) {
       u32x4 w[JW];
       uint32_t scale[JW];
     };
-    auto fetch = [&](const Source& x, const Source& xs, const uint32_t (&off)[JW], const uint32_t (&soff)[JW], int i, Raw& raw) {
-      const uint32_t bytes = tile_bytes(x, i, D), scale_bytes = tile_bytes(xs, i, 1);
+    auto fetch = [&](const Source& x, const Source& xs, const uint32_t (&off)[LPS], const uint32_t (&scale_off)[LPS], int i,
+                     Raw& raw) {
+      if (!loads) return;
 #pragma unroll
-      for (int jj = 0; jj < JW; ++jj) {
-        const int j = gwave + jj * GW;
-        if (NI % GW == 0 || j < NI) {
-          raw.w[jj] = load_buffer16(buffer_of(tile_data(x, i, j), bytes), off[jj]);
-          raw.scale[jj] = load_buffer1(buffer_of(tile_data(xs, i, j), scale_bytes), soff[jj]);
+      for (int s = 0; s < NS; ++s) {
+        const auto rsrc = buffer_of(segment_data(x, i, s), segment_bytes(x, i, s, D));
+        const auto scales = buffer_of(segment_data(xs, i, s), segment_bytes(xs, i, s, 1));
+#pragma unroll
+        for (int u = 0; u < LPS; ++u) {
+          raw.w[s * LPS + u] = load_buffer16(rsrc, off[u]);
+          raw.scale[s * LPS + u] = load_buffer1(scales, scale_off[u]);
         }
       }
     };
@@ -293,20 +300,18 @@ void attn_ragged_kernel(const RaggedParams p) {
     auto fetch_v = [&](int i, Raw& raw) { fetch(vs, vscale, voff, vscale_off, i, raw); };
     auto store = [&](bool is_v, const FA2_LDS char* to, Raw& raw) {
       FA2_LDS char* buf = (FA2_LDS char*)to;
+      if (!loads) return;
 #pragma unroll
       for (int jj = 0; jj < JW; ++jj) {
-        const int j = gwave + jj * GW;
-        if (NI % GW == 0 || j < NI) {
-          // nothing that uses what was loaded moves up across this point, and with it the wait for it
-          asm volatile("" : "+v"(raw.w[jj]), "+v"(raw.scale[jj]));
-          const int row = j * RPI + lane / LPR, chunk = lane % LPR * 2;
-          const int key = is_v ? v_key<D>(row & 15) : k_key<D>(pi_row(row & 31) & 15);
+        // nothing that uses what was loaded moves up across this point, and with it the wait for it
+        asm volatile("" : "+v"(raw.w[jj]), "+v"(raw.scale[jj]));
+        const int row = (gwave * JW + jj) * RPI + lane / LPR, chunk = lane % LPR * 2;
+        const int key = is_v ? v_key<D>(row & 15) : k_key<D>(pi_row(row & 31) & 15);
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const u32x2 lo = e4m3_to_16<DT>(raw.w[jj][2 * h], raw.scale[jj]);
-            const u32x2 hi = e4m3_to_16<DT>(raw.w[jj][2 * h + 1], raw.scale[jj]);
-            *(u32x4 FA2_LDS*)(buf + (row * CPR + ((chunk + h) ^ key)) * 16) = u32x4{lo[0], lo[1], hi[0], hi[1]};
-          }
+        for (int h = 0; h < 2; ++h) {
+          const u32x2 lo = e4m3_to_16<DT>(raw.w[jj][2 * h], raw.scale[jj]);
+          const u32x2 hi = e4m3_to_16<DT>(raw.w[jj][2 * h + 1], raw.scale[jj]);
+          *(u32x4 FA2_LDS*)(buf + (row * CPR + ((chunk + h) ^ key)) * 16) = u32x4{lo[0], lo[1], hi[0], hi[1]};
         }
       }
     };
@@ -534,42 +539,42 @@ void attn_ragged_kernel(const RaggedParams p) {
     for (int db = 0; db < DB; ++db)
 #pragma unroll
       for (int x = 0; x < 16; ++x) test = __builtin_fmaf(acc[db][x], 0.f, test);
-    const bool whole = starts && ends;
-    float* const part = whole ? nullptr : part_of<BM, D>(p, hkv, rank, starts ? 1 : 0);
     // row x of the workgroup: its place in out, q and lse
+    ParamsRef pe = params_here();
+    const int group = pe.group;
     struct RowPlace {
       int64_t token;
       int head, pos;
     };
     auto place = [&](int x) {
-      const int i = (row0 + x) / p.group;
-      return RowPlace{(int64_t)(sq.first + i), hkv * p.group + (row0 + x - i * p.group), i};
+      const int i = (row0 + x) / group;
+      return RowPlace{(int64_t)(sq.first + i), hkv * group + (row0 + x - i * group), i};
     };
     // m, l and exact l of row x, by one lane
     auto put_sums = [&](int x, float m, float sum, float exact) {
       if (part) {
-        *(f32x4*)(part + x * (D + 4) + D) = f32x4{m, sum, exact, 0.f};
-      } else if (p.lse) {
+        *(f32x4*)(part + part_sums<BM, D>(x)) = f32x4{m, sum, exact, 0.f};
+      } else if (pe.lse) {
         const RowPlace at = place(x);
-        p.lse[(int64_t)at.head * p.seq.n_tokens + at.token] = (m + log2f(exact)) * kLn2;
+        pe.lse[(int64_t)at.head * pe.seq.n_tokens + at.token] = (m + log2f(exact)) * kLn2;
       }
     };
     // One row again, by a wave: 64 keys at a time, one a lane; only keys that the row sees are read.
     auto again = [&](int x, bool nan) {
       const RowPlace at = place(x);
       const int end = nan ? kv_begin : min(last_of(at.pos) + 1, kv_end);
-      const uint16_t* qrow = p.q + at.token * p.sqt + at.head * p.sqh;
+      const uint16_t* qrow = pe.q + at.token * pe.sqt + at.head * pe.sqh;
       int page = 0;
-      auto row_at = [&](const CacheTensor& y, int n) {
+      auto row_at = [&](const auto& y, int n) {
         if constexpr (kPages) {
-          page = p.seq.table[seq * p.seq.table_stride + (n >> page_shift)];
-          if ((unsigned)page >= (unsigned)p.seq.n_pages) page = 0;
+          page = pe.seq.table[seq * pe.seq.table_stride + (n >> page_shift)];
+          if ((unsigned)page >= (unsigned)pe.seq.n_pages) page = 0;
           return y.data + (page * y.page + hkv * y.head + (int64_t)(n & ((1 << page_shift) - 1)) * y.token) * EB;
         } else {
           return y.data + ((int64_t)(sq.kv_first + n) * y.token + hkv * y.head) * EB;
         }
       };
-      auto scale_at = [&](const CacheTensor& y, int n) {
+      auto scale_at = [&](const auto& y, int n) {
         if constexpr (kE4m3)
           return e8m0_to_f32(y.scale[page * y.scale_page + hkv * y.scale_head +
                                      (int64_t)(n & ((1 << page_shift) - 1)) * y.scale_token]);
@@ -590,8 +595,8 @@ void attn_ragged_kernel(const RaggedParams p) {
         const int n = n0 + lane;
         float s = -INFINITY;
         if (n < end) {
-          const char* krow = row_at(p.kc, n);
-          const float scale = scale_at(p.kc, n);
+          const char* krow = row_at(pe.kc, n);
+          const float scale = scale_at(pe.kc, n);
           s = 0.f;
           for (int d = 0; d < D; ++d) s = __builtin_fmaf(to_f32<DT>(qrow[d]), value(krow, scale, d), s);
           s *= qk_scale;
@@ -610,8 +615,8 @@ void attn_ragged_kernel(const RaggedParams p) {
         for (int y = 0; y < (D + 63) / 64; ++y) o[y] *= alpha;
         for (int y = 0; y < min(end - n0, 64); ++y) {
           const float wy = __shfl(w, y, 64);
-          const char* vrow = row_at(p.vc, n0 + y);
-          const float scale = scale_at(p.vc, n0 + y);
+          const char* vrow = row_at(pe.vc, n0 + y);
+          const float scale = scale_at(pe.vc, n0 + y);
 #pragma unroll
           for (int z = 0; z < (D + 63) / 64; ++z)
             if (lane + 64 * z < D) o[z] = __builtin_fmaf(wy, value(vrow, scale, lane + 64 * z), o[z]);
@@ -626,9 +631,9 @@ void attn_ragged_kernel(const RaggedParams p) {
         if (lane + 64 * y < D) {
           const float v = nan ? m : o[y];
           if (part)
-            part[x * (D + 4) + lane + 64 * y] = v;
+            part[part_index<GW, D>(x, lane + 64 * y)] = v;
           else
-            p.o[at.token * p.sot + at.head * p.soh + lane + 64 * y] =
+            pe.o[at.token * pe.sot + at.head * pe.soh + lane + 64 * y] =
                 (uint16_t)E::pack2(last_of(at.pos) < 0 ? 0.f : v * inv, 0.f);
         }
       // (an infinite score without a NaN one: the row's log-sum-exp is infinite too)
@@ -642,7 +647,7 @@ void attn_ragged_kernel(const RaggedParams p) {
       if (mine && !((again_rows >> c) & 1)) {
         const float inv = last_key < 0 ? 0.f : 1.0f / l;  // no key: 0
         const RowPlace at = place(wr);
-        uint16_t* orow = p.o + at.token * p.sot + at.head * p.soh;
+        uint16_t* orow = pe.o + at.token * pe.sot + at.head * pe.soh;
         const float nan_or_0 = m_i != m_i ? m_i : 0.f;
 #pragma unroll
         for (int db = 0; db < DB; ++db)
@@ -657,8 +662,8 @@ void attn_ragged_kernel(const RaggedParams p) {
                   lo[i] = acc[db][8 * h + i];
                   hi[i] = acc[db][8 * h + 4 + i];
                 }
-                *(f32x4*)(part + wr * (D + 4) + d0) = lo;
-                *(f32x4*)(part + wr * (D + 4) + d0 + 4) = hi;
+                *(f32x4*)(part + part_index<GW, D>(wr, d0)) = lo;
+                *(f32x4*)(part + part_index<GW, D>(wr, d0 + 4)) = hi;
               } else {
                 float y[8];
 #pragma unroll
@@ -722,12 +727,12 @@ void attn_ragged_kernel(const RaggedParams p) {
         }
         const RowPlace at = place(x);
         if (part) {
-          *(f32x4*)(part + x * (D + 4) + 4 * q) = o;
+          *(f32x4*)(part + part_index<GW, D>(x, 4 * q)) = o;
         } else {
           const float inv = last_of(at.pos) < 0 ? 0.f : 1.0f / ls;  // no key: 0
 #pragma unroll
           for (int e = 0; e < 4; ++e) o[e] *= inv;
-          *(u32x2*)(p.o + at.token * p.sot + at.head * p.soh + 4 * q) = u32x2{E::pack2(o[0], o[1]), E::pack2(o[2], o[3])};
+          *(u32x2*)(pe.o + at.token * pe.sot + at.head * pe.soh + 4 * q) = u32x2{E::pack2(o[0], o[1]), E::pack2(o[2], o[3])};
         }
         if (q == 0) put_sums(x, m, ls, lxs);
       }
@@ -739,24 +744,30 @@ void attn_ragged_kernel(const RaggedParams p) {
         again(x, nan);
       }
     }
-    if (share.x >= share.end || !next_tile<BM, kPages>(p, lane, &cur)) return;
+    more = share.x < share.end && next_tile<BM, kPages>(params_here(), lane, &cur);
   }
 }
 
 // Merges the pieces of the row tile that ends in share `rank` and starts in an earlier one: with M the largest of the
 // pieces' references m_i, O = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i, in the order of the shares. 32 rows a
-// workgroup, 4 dims a thread; bound by the latency of the pieces' loads, so four pieces are loaded at once.
+// workgroup, 4 dims a thread; bound by the latency of the pieces' loads, so a thread has one item and loads several
+// pieces at once.
+constexpr int combine_threads(int head_dim) { return head_dim <= 32 ? 256 : 8 * head_dim; }
 template <int DT, int D, int GW>
-__global__ __launch_bounds__(256) void attn_ragged_combine_kernel(const RaggedParams p) {
+__global__ __launch_bounds__(combine_threads(D)) void attn_ragged_combine_kernel(const RaggedParams) {
   using E = Elem<DT>;
-  constexpr int BM = 32 * GW, QPR = D / 4, STEP = 4;
+  ParamsRef p = params_here();
+  constexpr int BM = 32 * GW, QPR = D / 4, STEP = 6;
   const int rank = (int)blockIdx.x / GW % p.shares, hkv = (int)blockIdx.x / GW / p.shares;
   const Merge at = *merge_of(p, hkv, rank);
   if (at.first < 0) return;
   const int x0 = (int)blockIdx.x % GW * 32;
-  const int n = min(32, at.rows - x0) * QPR;
-  for (int t = (int)threadIdx.x; t < n; t += 256) {
-    const int x = x0 + t / QPR, q = t % QPR;
+  const int n = (GW == 1 ? min(32, at.rows) : 32) * QPR;
+  for (int t = (int)threadIdx.x; t < n; t += combine_threads(D)) {
+    // 4 dims of a row a thread, in the order that the partial results lie in
+    const int x = x0 + (GW == 1 ? t / QPR : t & 31);
+    const int q = GW == 1 ? t % QPR : t / 128 * 4 + (t / 32 & 1) * 2 + (t / 64 & 1);
+    if (x >= at.rows) continue;
     float M = -INFINITY, l = 0.f, lx = 0.f;
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
     bool nan = false;
@@ -765,9 +776,9 @@ __global__ __launch_bounds__(256) void attn_ragged_combine_kernel(const RaggedPa
 #pragma unroll
       for (int k = 0; k < STEP; ++k) {
         const int i = min(i0 + k, rank);
-        const float* part = part_of<BM, D>(p, hkv, i, i == at.first) + x * (D + 4);
-        sums[k] = *(const f32x4*)(part + D);
-        v[k] = *(const f32x4*)(part + 4 * q);
+        const float* part = part_of<BM, D>(p, hkv, i, i == at.first);
+        sums[k] = *(const f32x4*)(part + part_sums<BM, D>(x));
+        v[k] = *(const f32x4*)(part + part_index<GW, D>(x, 4 * q));
       }
 #pragma unroll
       for (int k = 0; k < STEP; ++k) {
@@ -780,7 +791,7 @@ __global__ __launch_bounds__(256) void attn_ragged_combine_kernel(const RaggedPa
         l = l * a + w * sums[k][1];
         lx = lx * a + w * sums[k][2];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = o[e] * a + w * v[k][e];
+        for (int e = 0; e < 4; ++e) o[e] = o[e] * a + (m == -INFINITY ? 0.f : w * v[k][e]);  // (such a piece may be empty)
       }
     }
     const int pos = (at.row0 + x) / p.group, head = hkv * p.group + (at.row0 + x - pos * p.group);

@@ -12,7 +12,7 @@ int launch_form(const RaggedParams& p, unsigned grid, hipStream_t s) {
   hipError_t e = hipGetLastError();
   if constexpr (SRC != kSourcePacked) {
     if (e == hipSuccess && p.shares > 0) {
-      hipLaunchKernelGGL((attn_ragged_combine_kernel<FA2_DT, FA2_D, GW>), dim3(grid * GW), dim3(256), 0, s, p);
+      hipLaunchKernelGGL((attn_ragged_combine_kernel<FA2_DT, FA2_D, GW>), dim3(grid * GW), dim3(combine_threads(FA2_D)), 0, s, p);
       e = hipGetLastError();
     }
   }

@@ -19,6 +19,17 @@
 
 namespace fa2 {
 
+// The kernel's arguments, read where they lie. The compiler loads an argument once, at the kernel's start, and keeps it;
+// there are many here, most of them used before and after the tile loop only, and kept in spilled SGPRs they
+// cost the loop vector registers. Behind this point's opaque pointer they are loaded again.
+#define FA2_CONSTANT __attribute__((address_space(4)))
+using ParamsRef = const FA2_CONSTANT RaggedParams&;
+__device__ __forceinline__ ParamsRef params_here() {
+  auto p = (const FA2_CONSTANT RaggedParams*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *p;
+}
+
 // Keys that a tile costs beside its own: its rows' loads, its merge and stores.
 constexpr int kTileCost = 64;
 // Keys of the smallest share: four tiles of 64, or two of 32 for each of four waves.
@@ -30,7 +41,7 @@ struct LaneSequence {
 };
 
 template <bool PAGES>
-__device__ __forceinline__ LaneSequence lane_sequence(const RaggedParams& p, int s) {
+__device__ __forceinline__ LaneSequence lane_sequence(ParamsRef p, int s) {
   LaneSequence q = {0, 0, 0, 0};
   if (s >= p.seq.n_seq) return q;
   q.first = row_bound(p.seq.cu, s, p.seq.n_tokens);
@@ -62,7 +73,7 @@ struct Lengths {
   __device__ int64_t before(int64_t t) const { return t * base + slope * (t * (t - 1) / 2); }
 };
 template <int BM>
-__device__ __forceinline__ Lengths lengths_of(const RaggedParams& p, int n_q, int n_kv) {
+__device__ __forceinline__ Lengths lengths_of(ParamsRef p, int n_q, int n_kv) {
   if (!p.causal) return Lengths{(int64_t)n_kv + kTileCost, 0};
   const int64_t slope = BM / p.group;
   return Lengths{(int64_t)max(n_kv - n_q, 0) + slope + kTileCost, slope};
@@ -90,7 +101,7 @@ struct Cursor {
 
 // The rank-th row tile; false: there are fewer.
 template <int BM, bool PAGES>
-__device__ __forceinline__ bool find_tile(const RaggedParams& p, int rank, int lane, Cursor* c) {
+__device__ __forceinline__ bool find_tile(ParamsRef p, int rank, int lane, Cursor* c) {
   c->lanes = lane_sequence<PAGES>(p, lane);
   if (p.seq.n_seq <= 64) {
     // Tiles of index t and above, over all sequences: A(t) = sum_s max(tiles_s - t, 0). The rank-th tile in the
@@ -137,16 +148,17 @@ __device__ __forceinline__ bool find_tile(const RaggedParams& p, int rank, int l
   return false;
 }
 
-// Share j: [x, end) of the line, the cursor at the tile that x lies in, `in` from its start; x >= end: nothing.
+// Share j: [x, end) of the line, the cursor at the tile that x lies in, `in` from its start; x >= end: nothing. 
 struct Share {
   int64_t x, end, in, size;
 };
 template <int BM, bool PAGES>
-__device__ __forceinline__ Share find_share(const RaggedParams& p, int j, int lane, Cursor* c) {
-  c->lanes = lane_sequence<PAGES>(p, lane);
+__device__ __forceinline__ Share find_share(ParamsRef p, int j, int lane, Cursor* c) {
   auto length = [&]() {
     return lengths_of<BM>(p, c->lanes.n_q, c->lanes.n_kv).before(row_tiles<BM>(c->lanes.n_q, p.group));
   };
+  c->lanes = lane_sequence<PAGES>(p, lane);
+  c->s0 = 0;
   int64_t mine = length();
   int64_t upto = wave_scan(mine, lane);
   int64_t total = readlane64(upto, 63);
@@ -155,13 +167,13 @@ __device__ __forceinline__ Share find_share(const RaggedParams& p, int j, int la
     total += readlane64(wave_scan(length(), lane), 63);
   }
   Share w;
-  w.size = max((total + p.shares - 1) / p.shares, (int64_t)kLeastShare);
+  // (the same for every workgroup; how it is rounded does not matter, as long as shares * size reaches the total)
+  w.size = max((int64_t)((double)total * p.per_share) + 1, (int64_t)kLeastShare);
   w.x = w.size * j;
   w.end = min(w.x + w.size, total);
   w.in = 0;
   if (w.x >= w.end) return w;
   int64_t base = 0;
-  c->s0 = 0;
   if (p.seq.n_seq > 64) c->lanes = lane_sequence<PAGES>(p, lane);
   while (base + readlane64(upto, 63) <= w.x) {  // (w.x < total: ends within the sequences)
     base += readlane64(upto, 63);
@@ -191,20 +203,29 @@ __device__ __forceinline__ Share find_share(const RaggedParams& p, int j, int la
   return w;
 }
 
-// The next tile after the cursor's; false: there is none.
+// A cut at x of a tile's length, in its key tiles: the shares on both sides of it compute the same. A cut within the
+// tile's first or last key tile is moved to its end, as a piece costs more than a key tile (its prologue,
+// epilogue and merge).
+__device__ __forceinline__ int cut_at(int64_t x, int64_t length, int key_tiles) {
+  const int t = (int)((double)x * key_tiles / (double)length);
+  return t <= 1 ? 0 : t >= key_tiles - 1 ? key_tiles : t;
+}
+
+// The next tile after the cursor's on the line; false: there is none.
 template <int BM, bool PAGES>
-__device__ __forceinline__ bool next_tile(const RaggedParams& p, int lane, Cursor* c) {
+__device__ __forceinline__ bool next_tile(ParamsRef p, int lane, Cursor* c) {
   const LaneSequence q = sequence_at(c->lanes, c->l);
   if (++c->tile < row_tiles<BM>(q.n_q, p.group)) return true;
   c->tile = 0;
   for (;;) {
-    const uint64_t have = __builtin_amdgcn_ballot_w64(c->lanes.n_q > 0 && lane > c->l);
+    const uint64_t have =
+        __builtin_amdgcn_ballot_w64(row_tiles<BM>(c->lanes.n_q, p.group) > 0 && lane > c->l);
     if (have) {
       c->l = __builtin_ctzll(have);
       return true;
     }
+    if (c->s0 + 64 >= p.seq.n_seq) return false;
     c->s0 += 64;
-    if (c->s0 >= p.seq.n_seq) return false;
     c->l = -1;
     c->lanes = lane_sequence<PAGES>(p, c->s0 + lane);
   }
@@ -212,7 +233,7 @@ __device__ __forceinline__ bool next_tile(const RaggedParams& p, int lane, Curso
 
 // The (KV head, rank) of a workgroup: a head stays on one XCD where the heads split evenly over them, and on a
 // fixed few where the XCDs split evenly over the heads, so that its tiles share K and V in an L2.
-__device__ __forceinline__ void head_and_rank(const RaggedParams& p, int block, int* head, int* rank) {
+__device__ __forceinline__ void head_and_rank(ParamsRef p, int block, int* head, int* rank) {
   const int xcds = 1 << p.xcd_shift;
   const int xcd = block & (xcds - 1), slot = block >> p.xcd_shift;
   if ((p.h_kv & (xcds - 1)) == 0) {
@@ -225,11 +246,25 @@ __device__ __forceinline__ void head_and_rank(const RaggedParams& p, int block, 
   }
 }
 
-// A share's partial results: slot 1 of the tile that it starts and does not finish, slot 0 of the one that
-// it starts in the middle of.
+// A share's partial results: slot 1 of the tile that starts in it, slot 0 of the one that it goes on with.
 template <int BM, int D>
-__device__ __forceinline__ float* part_of(const RaggedParams& p, int head, int share, int slot) {
+__device__ __forceinline__ float* part_of(ParamsRef p, int head, int share, int slot) {
   return p.parts + (((int64_t)head * p.shares + share) * 2 + slot) * (BM * (D + 4));
+}
+
+// Where element (row x, dim d) of a partial result lies. 128-row tiles keep the accumulators' layout, four dims a lane
+// and 64 lanes side by side, so that a wave's stores and loads are whole KiB; 32-row tiles, merged through LDS
+// before, rows of dims. m, l and exact l of every row follow.
+template <int GW, int D>
+__device__ __forceinline__ int part_index(int x, int d) {
+  if constexpr (GW == 1) return x * D + d;
+  const int c = x & 31, db = d / 32, h = d / 16 & 1, g = d / 8 & 1, half = d / 4 & 1;
+  return (x / 32) * 32 * D + ((2 * db + h) * 2 + half) * 256 + (32 * g + c) * 4 + (d & 3);
+}
+
+template <int BM, int D>
+__device__ __forceinline__ int part_sums(int x) {
+  return BM * D + x * 4;
 }
 
 // What the merge of the tile that ends in a share needs: the share it starts in (-1: none ends here, or it lies in
@@ -238,9 +273,9 @@ __device__ __forceinline__ float* part_of(const RaggedParams& p, int head, int s
 struct alignas(16) Merge {
   int first, row0, rows, token, n_kv, shift;
 };
-__device__ __forceinline__ Merge* merge_of(const RaggedParams& p, int head, int share) {
+__device__ __forceinline__ Merge* merge_of(ParamsRef p, int head, int share) {
   static_assert(sizeof(Merge) == kMergeBytes);
-  return static_cast<Merge*>(p.merges) + ((int64_t)head * p.shares + share);
+  return static_cast<Merge*>(p.merges) + (int64_t)head * p.shares + share;
 }
 
 }  // namespace fa2

@@ -173,6 +173,7 @@ int launch_ragged(int32_t dtype, int32_t head_dim, int32_t h_q, fa2::RaggedParam
   p.group = h_q / p.h_kv;
   p.xcd_shift = topo.xcd_shift;
   p.shares = pl.shares;
+  p.per_share = pl.shares ? 1.0 / pl.shares : 0.0;
   p.parts = static_cast<float*>(workspace);
   p.merges = static_cast<char*>(workspace) + pl.parts;
   const unsigned g = (unsigned)pl.grid;

@@ -83,6 +83,7 @@ struct RaggedParams {
   // 0: a workgroup per row tile. Above: that many workgroups per KV head share its work evenly by
   // cutting the row tiles' key ranges; the pieces of a cut row tile meet in `parts`.
   int32_t shares;
+  double per_share;  // 1 / shares
   float* parts;  // [h_kv * shares][2][block_m][head_dim + 4]: O, then m, l, exact l
   void* merges;  // [h_kv * shares] of kMergeBytes: the tile that ends in each share
 };
