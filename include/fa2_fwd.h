@@ -351,8 +351,8 @@ FA2_API int fa2_attn_paged(const void* q, void* out, const int64_t q_stride[2], 
 
 /* fa2_paged_workspace_bytes - what fa2_attn_paged needs on a GPU of num_cus CUs. Host policy only: it does
  * not depend on the lengths. */
-FA2_API size_t fa2_paged_workspace_bytes(int32_t h_q, int32_t h_kv, int32_t head_dim, int32_t n_tokens,
-                                         int32_t n_seq, int32_t num_cus);
+FA2_API size_t fa2_paged_workspace_bytes(int32_t h_q, int32_t h_kv, int32_t head_dim, int32_t cache_dtype,
+                                         int32_t n_tokens, int32_t n_seq, int32_t num_cus);
 
 /* Thread-local description of the last failure in this thread ("" if none). */
 FA2_API const char* fa2_last_error(void);

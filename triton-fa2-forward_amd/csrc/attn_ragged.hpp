@@ -30,9 +30,10 @@ constexpr int ragged_block_n(int head_dim, int row_waves) {
   return row_waves == 4 ? (head_dim == 16 ? 128 : 64) : head_dim == 128 ? 32 : 64;
 }
 
-template <int DT, int D, int SRC, int GW>
+// LSE: with 128 rows, whether p.lse is set (a branch on it inside the tile loop would cost 10% without it being taken).
+template <int DT, int D, int SRC, int GW, bool LSE>
 __global__ __launch_bounds__(256)
-__attribute__((amdgpu_waves_per_eu(2)))
+__attribute__((amdgpu_waves_per_eu(ragged_waves(D, SRC, GW))))
 void attn_ragged_kernel(const RaggedParams) {
   using E = Elem<DT>;
   ParamsRef p = params_here();
@@ -133,7 +134,7 @@ void attn_ragged_kernel(const RaggedParams) {
   }
 
   const float qk_scale = p.qk_scale;
-  const bool want_exact = p.lse != nullptr, causal = p.causal != 0, shared = p.shares > 0;
+  const bool want_exact = GW == 1 ? p.lse != nullptr : LSE, causal = p.causal != 0, shared = kPages && p.shares > 0;
 
   // ---- the workgroup's work: the pieces of its share, or its one tile
   Cursor cur;
@@ -744,7 +745,7 @@ void attn_ragged_kernel(const RaggedParams) {
         again(x, nan);
       }
     }
-    more = share.x < share.end && next_tile<BM, kPages>(params_here(), lane, &cur);
+    more = shared && share.x < share.end && next_tile<BM, kPages>(params_here(), lane, &cur);
   }
 }
 

@@ -8,7 +8,10 @@ namespace {
 
 template <int SRC, int GW>
 int launch_form(const RaggedParams& p, unsigned grid, hipStream_t s) {
-  hipLaunchKernelGGL((attn_ragged_kernel<FA2_DT, FA2_D, SRC, GW>), dim3(grid), dim3(256), 0, s, p);
+  if (GW > 1 && p.lse)
+    hipLaunchKernelGGL((attn_ragged_kernel<FA2_DT, FA2_D, SRC, GW, (GW > 1)>), dim3(grid), dim3(256), 0, s, p);
+  else
+    hipLaunchKernelGGL((attn_ragged_kernel<FA2_DT, FA2_D, SRC, GW, false>), dim3(grid), dim3(256), 0, s, p);
   hipError_t e = hipGetLastError();
   if constexpr (SRC != kSourcePacked) {
     if (e == hipSuccess && p.shares > 0) {

@@ -128,8 +128,9 @@ struct RaggedPlan {
   int64_t grid = 0;
   size_t parts = 0, workspace = 0;  // bytes of the partial results, and with what their merge needs to know
 };
-RaggedPlan ragged_plan(bool paged, int32_t h_q, int32_t h_kv, int32_t head_dim, int32_t n_tokens, int32_t n_seq, int cus) {
+RaggedPlan ragged_plan(int source, int32_t h_q, int32_t h_kv, int32_t head_dim, int32_t n_tokens, int32_t n_seq, int cus) {
   RaggedPlan pl;
+  const bool paged = source != fa2::kSourcePacked;
   const int64_t rows = (int64_t)n_tokens * (h_q / h_kv);
   auto tiles = [&](int64_t block_m) { return (rows + (int64_t)n_seq * (block_m - 1)) / block_m; };  // at most
   if (paged)
@@ -138,7 +139,7 @@ RaggedPlan ragged_plan(bool paged, int32_t h_q, int32_t h_kv, int32_t head_dim, 
     pl.row_waves = tiles(32) * h_kv <= 2 * (int64_t)cus ? 1 : 4;
   const int64_t n = tiles(32 * pl.row_waves);
   if (paged && n * h_kv < 8 * (int64_t)cus) {
-    pl.shares = std::max(1, 2 * cus / h_kv);
+    pl.shares = std::max(1, fa2::ragged_waves(head_dim, source, pl.row_waves) * cus / h_kv);
     pl.parts = (size_t)h_kv * pl.shares * 2 * 32 * pl.row_waves * (head_dim + 4) * sizeof(float);  // (a multiple of 256)
     pl.workspace = pl.parts + (size_t)h_kv * pl.shares * fa2::kMergeBytes;
   }
@@ -163,7 +164,7 @@ int launch_ragged(int32_t dtype, int32_t head_dim, int32_t h_q, fa2::RaggedParam
                   size_t workspace_bytes, void* stream) {
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const Topology topo = device_topology(stream_device(s));
-  const RaggedPlan pl = ragged_plan(source != fa2::kSourcePacked, h_q, p.h_kv, head_dim, p.seq.n_tokens, p.seq.n_seq, topo.cus);
+  const RaggedPlan pl = ragged_plan(source, h_q, p.h_kv, head_dim, p.seq.n_tokens, p.seq.n_seq, topo.cus);
   if (pl.grid > 0x7fffffffLL) return fail(FA2_EINVAL, "grid of %lld workgroups is too large", (long long)pl.grid);
   if (pl.workspace) {
     if (!workspace || workspace_bytes < pl.workspace)
@@ -346,10 +347,11 @@ int fa2_attn_paged(const void* q, void* out, const int64_t q_stride[2], const in
                        workspace_bytes, stream);
 }
 
-size_t fa2_paged_workspace_bytes(int32_t h_q, int32_t h_kv, int32_t head_dim, int32_t n_tokens, int32_t n_seq,
-                                 int32_t num_cus) {
+size_t fa2_paged_workspace_bytes(int32_t h_q, int32_t h_kv, int32_t head_dim, int32_t cache_dtype, int32_t n_tokens,
+                                 int32_t n_seq, int32_t num_cus) {
+  const int source = cache_dtype == FA2_DTYPE_E4M3 ? fa2::kSourceE4m3 : fa2::kSourcePages;
   if (h_q <= 0 || h_kv <= 0 || h_q % h_kv || dim_index(head_dim) < 0 || n_tokens <= 0 || n_seq <= 0 || num_cus <= 0) return 0;
-  return ragged_plan(true, h_q, h_kv, head_dim, n_tokens, n_seq, num_cus).workspace;
+  return ragged_plan(source, h_q, h_kv, head_dim, n_tokens, n_seq, num_cus).workspace;
 }
 
 }  // extern "C"

@@ -18,6 +18,13 @@ int launch_cache(bool write, int dtype, int head_dim, bool e4m3, const CachePara
 // Where K and V of a ragged attention launch lie: packed rows, 16-bit pages, e4m3 pages.
 constexpr int kSourcePacked = 0, kSourcePages = 1, kSourceE4m3 = 2;
 
+// Its workgroups per CU (waves per SIMD), by registers: packed rows keep nothing from tile to tile (128 VGPRs at
+// head_dim 64). Measured at head_dim 64 on MI355X: packed prompts of 3k to 8k, 2 / 3 / 4 a CU 394 / 390 / 384 us; a chunk of
+// 2000 over 8k keys, 16-bit pages 170 / 165 / 223 (spilled), e4m3 pages 193 / 195 / 359.
+constexpr int ragged_waves(int head_dim, int source, int row_waves) {
+  return row_waves == 1 || head_dim == 128 || source == kSourceE4m3 ? 2 : source == kSourcePages ? 3 : 4;
+}
+
 // The ragged attention kernel with 32 * row_waves (1 or 4) rows per workgroup, and after it, with p.shares > 0,
 // the merge of the row tiles that its shares cut.
 template <int DT, int D>

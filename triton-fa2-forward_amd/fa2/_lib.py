@@ -66,7 +66,7 @@ SIGNATURES = {
                                        _i32, _i32, _i32, _i32, _i32, ctypes.c_float, _vp, _vp]),
     "fa2_attn_paged": (ctypes.c_int, [_vp, _vp, _i64p, _i64p, _cachep, _seqp, _i32, _i32, _i32, ctypes.c_float,
                                       _vp, _vp, ctypes.c_size_t, _vp]),
-    "fa2_paged_workspace_bytes": (ctypes.c_size_t, [_i32] * 6),
+    "fa2_paged_workspace_bytes": (ctypes.c_size_t, [_i32] * 7),
     "fa2_last_error": (ctypes.c_char_p, []),
     "fa2_version": (ctypes.c_char_p, []),
 }
@@ -277,8 +277,8 @@ def attn_packed(q, k, v, out, cu, cu_kv, causal, qk_scale, lse, stream):
         DTYPE_CODE[q.dtype], int(bool(causal)), qk_scale, _ptr(lse), stream), "fa2_attn_packed")
 
 
-def paged_workspace_bytes(H_q, H_kv, D, n_tokens, n_seq, num_cus):
-    return int(lib().fa2_paged_workspace_bytes(H_q, H_kv, D, n_tokens, n_seq, num_cus))
+def paged_workspace_bytes(H_q, H_kv, D, cache_dtype, n_tokens, n_seq, num_cus):
+    return int(lib().fa2_paged_workspace_bytes(H_q, H_kv, D, CACHE_DTYPE_CODE[cache_dtype], n_tokens, n_seq, num_cus))
 
 
 def attn_paged(q, out, cache, seq, causal, qk_scale, lse, workspace, stream):

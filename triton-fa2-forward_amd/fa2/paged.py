@@ -203,7 +203,7 @@ def attention_paged(q, cache, block_table, cu_seqlens, seqlens, *, causal=True, 
     lse = torch.empty((H_q, T), dtype=torch.float32, device=q.device) if return_lse else None
     c, s, alive = _step(cache, block_table, cu_seqlens, seqlens, T)
     if out.numel():
-        n = _lib.paged_workspace_bytes(H_q, H_kv, D, T, seqlens.numel(), _cu_count(q.device))
+        n = _lib.paged_workspace_bytes(H_q, H_kv, D, cache.k.dtype, T, seqlens.numel(), _cu_count(q.device))
         ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
         with torch.cuda.device(q.device):
             _lib.attn_paged(_rows(q), o_, c, s, causal, qk_scale, lse, ws,
