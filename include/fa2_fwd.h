@@ -339,7 +339,7 @@ FA2_API int fa2_attn_packed(const void* q, const void* k, const void* v, void* o
  * fa2_attn_paged - attention of every sequence's packed rows over its lens[s] tokens in the cache (their own k
  * and v written there first: fa2_cache_write), masks and lse as in fa2_attn_packed. dtype is q's and out's type, and
  * a 16-bit cache's; e4m3 values are read in that type. A page outside the cache makes the rows that
- * see its tokens NaN.
+ * see its tokens NaN, and may make other rows of its sequence NaN.
  *   workspace  device memory, 256-byte aligned, of at least fa2_paged_workspace_bytes(...) bytes (may be NULL
  *              where that is 0), owned by the caller and untouched until the launch has run: the partial
  *              results of sequences whose tokens several workgroups share.
@@ -349,10 +349,10 @@ FA2_API int fa2_attn_paged(const void* q, void* out, const int64_t q_stride[2], 
                            int32_t causal, float qk_scale, float* lse, void* workspace,
                            size_t workspace_bytes, void* stream);
 
-/* fa2_paged_workspace_bytes - what fa2_attn_paged needs on a GPU of num_cus CUs. Host policy only: it does
- * not depend on the lengths. */
+/* fa2_paged_workspace_bytes - what fa2_attn_paged needs on a GPU of num_cus CUs for a table of max_keys =
+ * max_pages * page_size tokens. Host policy only: it does not depend on the lengths. */
 FA2_API size_t fa2_paged_workspace_bytes(int32_t h_q, int32_t h_kv, int32_t head_dim, int32_t cache_dtype,
-                                         int32_t n_tokens, int32_t n_seq, int32_t num_cus);
+                                         int32_t n_tokens, int32_t n_seq, int64_t max_keys, int32_t num_cus);
 
 /* Thread-local description of the last failure in this thread ("" if none). */
 FA2_API const char* fa2_last_error(void);

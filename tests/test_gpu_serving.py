@@ -348,7 +348,15 @@ def test_packed_indices_that_do_not_ascend():
 # ------------------------------------------------------------------------------------------
 
 PAGED = [([1], [1]), ([1] * 5, [1, 33, 64, 700, 129]), ([4, 0, 1, 40, 129], [4, 50, 1000, 41, 129]),
-         ([3, 5, 2], [1, 0, 2]), ([1] * 66, [2 + 5 * i for i in range(66)])]
+         ([3, 5, 2], [1, 0, 2]), ([1] * 66, [2 + 5 * i for i in range(66)]),
+         ([40] * 70, [20 + 7 * i for i in range(70)])]
+
+
+def widened(table, page_size, keys=1600):
+    """The table with entries behind the last pages for sequences of `keys` tokens: workgroups share the work of calls
+    whose sequences may be long"""
+    more = max(-(-keys // page_size) - table.shape[1], 0)
+    return torch.cat([table, torch.full((table.shape[0], more), -1, dtype=torch.int32, device=table.device)], 1)
 
 
 def check_paged(q, cache, pages, cu, lens, causal, dtype, out, lse, sm_scale=None):
@@ -373,18 +381,20 @@ def test_paged(dtype, e4m3, D, page_size, h_q, h_kv):
                     bytes_of(t)[page, :, row] = 0x7f if e4m3 else math.nan
         T = sum(new) + 2
         q, out = randn((T, h_q, D), dtype, 30 + seed), torch.full((T, h_q, D), 7.0, dtype=dtype, device="cuda")
-        for causal in (True, False):
-            got, lse = attention_paged(q, cache, pages.table, cu, seqlens, causal=causal, return_lse=True, out=out)
+        for causal, table in ((c, t) for t in (pages.table, widened(pages.table, page_size)) for c in (True, False)):
+            got, lse = attention_paged(q, cache, table, cu, seqlens, causal=causal, return_lse=True, out=out.fill_(7.0))
             assert got is out and (out[-2:] == 7.0).all()
             check_paged(q, cache, pages, cu, lens, causal, dtype, out, lse)
-            assert torch.equal(attention_paged(q, cache, pages.table, cu, seqlens, causal=causal)[:-2], out[:-2])
+            assert torch.equal(attention_paged(q, cache, table, cu, seqlens, causal=causal)[:-2], out[:-2])
 
 
 @pytest.mark.parametrize("e4m3", [False, True])
-@pytest.mark.parametrize("new,lens", [([1, 1], [9000, 20]), ([300, 1, 1, 64], [5000, 3000, 1, 2100]), ([600], [4321])])
-def test_paged_long(e4m3, new, lens):
+@pytest.mark.parametrize("dtype,D,page_size", [(torch.bfloat16, 128, 32), (torch.float16, 64, 16), (torch.bfloat16, 32, 64),
+                                               (torch.float16, 16, 128)])
+@pytest.mark.parametrize("new,lens", [([1, 1], [9000, 20]), ([300, 1, 1, 64], [5000, 3000, 1, 2100]), ([600], [4321]),
+                                      ([200, 0, 1, 700], [100, 50, 6000, 350]), ([30] * 66 + [400], [40] * 66 + [5000])])
+def test_paged_long(e4m3, dtype, D, page_size, new, lens):
     from fa2.paged import attention_paged
-    D, page_size, dtype = 128, 32, torch.bfloat16
     pages, cu, seqlens = step_of(new, lens, page_size)
     cache = make_cache(pages.n_pages, 2, page_size, D, dtype, e4m3)
     q = randn((sum(new), 8, D), dtype, 3)
@@ -393,7 +403,8 @@ def test_paged_long(e4m3, new, lens):
         check_paged(q, cache, pages, cu, lens, causal, dtype, out, lse, 0.2)
 
 
-def test_paged_page_outside_the_cache():
+@pytest.mark.parametrize("wide", [False, True])
+def test_paged_page_outside_the_cache(wide):
     """A table entry that is no page makes the rows that see its tokens NaN, and leaves the others; one behind the last
     token is never read."""
     from fa2.paged import attention_paged
@@ -403,10 +414,11 @@ def test_paged_page_outside_the_cache():
         pages, cu, seqlens = step_of(new, lens, page_size)
         cache = make_cache(pages.n_pages, 2, page_size, D, dtype, e4m3)
         q = randn((32, 4, D), dtype, 3)
-        want = attention_paged(q, cache, pages.table, cu, seqlens)
+        whole = pages.table if not wide else widened(pages.table, page_size)
+        want = attention_paged(q, cache, whole, cu, seqlens)
         assert want.isfinite().all()
         for bad in (-1, pages.n_pages, 1 << 30, -2 ** 31):
-            table = pages.table.clone()
+            table = whole.clone()
             table[0, 3] = table[1, 12] = bad  # tokens 48 .. 63, and 192 .. 199 (rows 22 and on see them)
             out, lse = attention_paged(q, cache, table, cu, seqlens, return_lse=True)
             assert out[0].isnan().all() and lse[:, 0].isnan().all()
@@ -493,7 +505,8 @@ def test_chunks_and_steps_as_one_prompt(e4m3):
             assert (other.double() - dense.double()).abs().max() <= 8 * u * v_[r].abs().max()
 
 
-def test_graph_follows_lengths():
+@pytest.mark.parametrize("columns", [40, 120])  # (of 16 tokens: a workgroup per row tile, or equal shares)
+def test_graph_follows_lengths(columns):
     """A step captured once and replayed with other lengths, tables and values, a padded batch among them: rows behind the
     last sequence keep what they held."""
     from fa2.paged import KVCache, attention_paged, cache_write
@@ -502,7 +515,7 @@ def test_graph_follows_lengths():
     q, k, v = (torch.zeros(T, h, D, dtype=dtype, device="cuda") for h in (h_q, h_kv, h_kv))
     cu = torch.zeros(S + 1, dtype=torch.int32, device="cuda")
     seqlens = torch.zeros(S, dtype=torch.int32, device="cuda")
-    table = torch.zeros(S, 40, dtype=torch.int32, device="cuda")
+    table = torch.zeros(S, columns, dtype=torch.int32, device="cuda")
     out, q_out = torch.zeros_like(q), torch.zeros_like(q)
     caches = [KVCache.empty(300, h_kv, page_size, D, t) for t in (dtype, torch.float8_e4m3fn)]
 
@@ -523,7 +536,7 @@ def test_graph_follows_lengths():
                 t.copy_(randn((T, h, D), dtype, seed))
             pages = oracle.Pages(lens, page_size, n_pages=300, seed=seed, device="cuda")
             table.fill_(-1)
-            table[:, :pages.table.shape[1]] = pages.table[:, :40]
+            table[:, :pages.table.shape[1]] = pages.table[:, :columns]
             cu.copy_(cumulative(new)), seqlens.copy_(torch.tensor(lens, dtype=torch.int32))
             start = [t if t is None else t.clone() for t in cache]
             out.fill_(7.0), q_out.fill_(5.0)

@@ -282,14 +282,16 @@ def test_c_call_refusals():
     assert paged(c_cache(), c_seq(), q=None) == -1
     assert paged(c_cache(), c_seq(), lse=P + 2) == -2
     assert paged(c_cache(), c_seq(n_tokens=1 << 30), h_q=8) == -1  # 2^32 rows of a KV head
-    need = _lib.paged_workspace_bytes(4, 2, 64, torch.bfloat16, 3, 2, 256)
+    need = _lib.paged_workspace_bytes(4, 2, 64, torch.bfloat16, 3, 2, 4096, 256)
     assert need > 0
-    assert paged(c_cache(), c_seq(), ws=None) == -1 and "workspace" in _lib.last_error()
-    assert paged(c_cache(), c_seq(), n_ws=need - 1) == -1 and str(need) in _lib.last_error()
-    assert paged(c_cache(), c_seq(), ws=P + 128) == -2
+    long = c_seq(max_pages=256, table_stride=256)  # (the two pages of c_seq() need none)
+    assert paged(c_cache(), long, ws=None) == -1 and "workspace" in _lib.last_error()
+    assert paged(c_cache(), long, n_ws=need - 1) == -1 and str(need) in _lib.last_error()
+    assert paged(c_cache(), long, ws=P + 128) == -2
     for h_q, D, n, n_seq, cus in ((3, 64, 3, 2, 256), (4, 48, 3, 2, 256), (4, 64, 0, 2, 256), (4, 64, 3, 0, 256), (4, 64, 3, 2, 0)):
-        assert _lib.paged_workspace_bytes(h_q, 2, D, torch.bfloat16, n, n_seq, cus) == 0
-    assert _lib.paged_workspace_bytes(32, 8, 128, torch.float8_e4m3fn, 1 << 20, 4, 256) == 0  # row tiles enough: none are shared
+        assert _lib.paged_workspace_bytes(h_q, 2, D, torch.bfloat16, n, n_seq, 4096, cus) == 0
+    assert _lib.paged_workspace_bytes(4, 2, 64, torch.bfloat16, 3, 2, 1536, 256) == 0  # no sequence is long enough
+    assert _lib.paged_workspace_bytes(32, 8, 128, torch.float8_e4m3fn, 1 << 20, 4, 1 << 20, 256) == 0  # row tiles enough: none are shared
     assert _lib.lib().fa2_cache_write(None, None, P, P, None, None, None, None, None, None, 0, None, 1, None) == -1
     # nothing to do
     assert write(c_cache(), c_seq(n_tokens=0)) == 0 and write(c_cache(), c_seq(n_seq=0, cu=None)) == 0

@@ -500,7 +500,8 @@ PyObject* attn_paged(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   if (scale == 0.f || cus < 1 || !row_strides(*q, 8, qs) || !out_of(args[11], *q, &out, os)) Py_RETURN_NONE;
   const int32_t T = (int32_t)q->size(0), hq = (int32_t)q->size(1);
   if (want_lse) lse = at::empty({hq, T}, q->options().dtype(at::kFloat));
-  const size_t n_ws = fa2_paged_workspace_bytes(hq, c.h_kv, c.head_dim, c.cache_dtype, T, s.n_seq, cus);
+  const size_t n_ws = fa2_paged_workspace_bytes(hq, c.h_kv, c.head_dim, c.cache_dtype, T, s.n_seq,
+                                                (int64_t)s.max_pages * c.page_size, cus);
   if (n_ws) ws = at::empty({(int64_t)n_ws}, q->options().dtype(at::kByte));
   void* stream = c10::hip::getCurrentHIPStream(device.index()).stream();
   const void* qp = q->data_ptr();

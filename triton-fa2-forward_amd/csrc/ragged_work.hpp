@@ -11,7 +11,8 @@
 //     its keys (an estimate, linear in the tile's index, so that a sequence's sum is a closed form; it only
 //     decides where the cuts lie). A share starts and ends inside tiles: a tile cut by a share's end leaves
 //     partial results (slot 1 of the share it starts in, slot 0 of the others), which the combine kernel merges. For
-//     few or uneven tiles, decoding above all, whatever the lengths are.
+//     few or uneven tiles, decoding above all, whatever the lengths are. Where a tile per workgroup would take no
+//     longer after all (whole_tiles), that is what the workgroups do.
 #pragma once
 
 #include "serve_common.hpp"
@@ -30,8 +31,13 @@ __device__ __forceinline__ ParamsRef params_here() {
   return *p;
 }
 
-// Keys that a tile costs beside its own: its rows' loads, its merge and stores.
-constexpr int kTileCost = 64;
+// Keys that a tile costs beside its own: its rows' loads, its merge and stores. Measured on MI355X, in keys of cost
+// 64 / 128 / 256 / 384: 4 prompts of 2000 in 128-row tiles (a share of short tiles alone holds many of them)
+// 201 / 185 / 164 / 166 us; steps of 64 sequences of 1000 keys in 32-row tiles 46.5 / 47.8 / 48.0 / 49.0.
+template <int BM>
+constexpr int kTileCost = BM == 32 ? 64 : 256;
+// ... and what sharing the tiles out costs a 128-row workgroup: more pieces, the partial results, their merge
+constexpr int kShareCost = 640;
 // Keys of the smallest share: four tiles of 64, or two of 32 for each of four waves.
 constexpr int kLeastShare = 256;
 
@@ -74,9 +80,9 @@ struct Lengths {
 };
 template <int BM>
 __device__ __forceinline__ Lengths lengths_of(ParamsRef p, int n_q, int n_kv) {
-  if (!p.causal) return Lengths{(int64_t)n_kv + kTileCost, 0};
+  if (!p.causal) return Lengths{(int64_t)n_kv + kTileCost<BM>, 0};
   const int64_t slope = BM / p.group;
-  return Lengths{(int64_t)max(n_kv - n_q, 0) + slope + kTileCost, slope};
+  return Lengths{(int64_t)max(n_kv - n_q, 0) + slope + kTileCost<BM>, slope};
 }
 
 __device__ __forceinline__ int64_t wave_scan(int64_t x, int lane) {
@@ -148,7 +154,23 @@ __device__ __forceinline__ bool find_tile(ParamsRef p, int rank, int lane, Curso
   return false;
 }
 
-// Share j: [x, end) of the line, the cursor at the tile that x lies in, `in` from its start; x >= end: nothing. 
+__device__ __forceinline__ int64_t wave_max(int64_t x) {
+#pragma unroll
+  for (int off = 32; off >= 1; off /= 2) x = max(x, (int64_t)__shfl_xor(x, off, 64));
+  return x;
+}
+
+// Whether a tile per workgroup takes no longer than equal shares, as estimated: as many tiles as workgroups at most, whose
+// longest costs no more than a share and what sharing costs. With one workgroup a CU, half of those that
+// fit, a key takes 5/8 of the time. Measured on MI355X (32 / 8 heads of 128), whole tiles and shares: 4 prompts of 500
+// 25 and 41 us; a chunk of 500 behind 500 33 and 40, behind 2k 62 and 53; 4 of 500 behind 4k 146 and 161.
+__device__ __forceinline__ bool whole_tiles(ParamsRef p, int64_t tiles, int64_t total, int64_t longest) {
+  if (tiles > p.shares) return false;
+  return (2 * tiles <= p.shares ? 5 * longest / 8 : longest) <= (int64_t)((double)total * p.per_share) + kShareCost;
+}
+
+// Share j: [x, end) of the line, the cursor at the tile that x lies in, `in` from its start; x >= end: nothing.
+// With whole_tiles, the j-th tile.
 struct Share {
   int64_t x, end, in, size;
 };
@@ -172,6 +194,19 @@ __device__ __forceinline__ Share find_share(ParamsRef p, int j, int lane, Cursor
   w.x = w.size * j;
   w.end = min(w.x + w.size, total);
   w.in = 0;
+  if (BM != 32 && p.seq.n_seq <= 64) {
+    const Lengths len = lengths_of<BM>(p, c->lanes.n_q, c->lanes.n_kv);
+    const int64_t tiles = row_tiles<BM>(c->lanes.n_q, p.group), tiles_upto = wave_scan(tiles, lane);
+    if (whole_tiles(p, readlane64(tiles_upto, 63), total, wave_max(tiles > 0 ? len.of(tiles - 1) : 0))) {
+      const uint64_t past = __builtin_amdgcn_ballot_w64(tiles_upto > j);
+      w.end = w.x;
+      if (!past) return w;
+      c->l = __builtin_ctzll(past);
+      c->tile = j - (int)readlane64(tiles_upto - tiles, c->l);
+      w.end += readlane64(len.of(c->tile), c->l);
+      return w;
+    }
+  }
   if (w.x >= w.end) return w;
   int64_t base = 0;
   if (p.seq.n_seq > 64) c->lanes = lane_sequence<PAGES>(p, lane);

@@ -121,14 +121,27 @@ unsigned cache_grid(fa2::CacheParams* p, int64_t rows_per_token, int32_t head_di
 }
 
 // The form of a ragged attention call (attn_ragged.hpp, ragged_work.hpp), from what the host knows of it: the
-// rows and sequences, not the lengths.
+// rows, the sequences and a bound on their keys, not the lengths. Measured on MI355X, us:
+//   * packed rows: 32-row workgroups up to two tiles a CU, of sequences long enough that four waves have keys to take in
+//     turn. 16 heads of 64, one sequence, 32 and 128 rows: 120 keys 7.0 and 6.5, 250 7.3 and 8.2, 1000 (512
+//     tiles) 12.1 and 18.1, 4000 (2000 tiles) 78 and 63; 4 x 250 of 32 / 8 heads of 128 (1024 tiles) 21.5 and 11.8.
+//   * pages: 32-row workgroups for up to 32 rows a sequence on average. 16 sequences behind 4k, 32 / 8 heads of 128, rows a
+//     sequence: 16 50 and 66, 32 55 and 69, 64 60 and 71 - but 24 steps beside a chunk of 700 rows (35 on average)
+//     75 and 66, and beside one of 3500 153 and 117.
+//   * shares, or a workgroup a row tile: a tile each above 8 a CU, as then they even out (4 prompts of 4000, 500 and 611),
+//     and where no sequence can have more keys than a share saves: 4 prompts of 500 21 and 41, of 1000 46 and 71; of 2000 148 and 164; steps of 8
+//     sequences of 300 10 and 17, of 1000 16 and 19, of 2000 24 and 23; uneven ones of up to 1000, 64 and 256 of
+//     them, 33 and 33, 102 and 99.
+constexpr int64_t kShortKeys = 1536;
 struct RaggedPlan {
   int row_waves = 4;  // 32-row workgroups (1) or 128-row ones (4)
   int shares = 0;     // workgroups per KV head that share its work; 0: one per row tile
   int64_t grid = 0;
   size_t parts = 0, workspace = 0;  // bytes of the partial results, and with what their merge needs to know
 };
-RaggedPlan ragged_plan(int source, int32_t h_q, int32_t h_kv, int32_t head_dim, int32_t n_tokens, int32_t n_seq, int cus) {
+// keys: of packed rows, all of them; of pages, the most that a sequence can have
+RaggedPlan ragged_plan(int source, int32_t h_q, int32_t h_kv, int32_t head_dim, int32_t n_tokens, int32_t n_seq, int64_t keys,
+                       int cus) {
   RaggedPlan pl;
   const bool paged = source != fa2::kSourcePacked;
   const int64_t rows = (int64_t)n_tokens * (h_q / h_kv);
@@ -136,9 +149,9 @@ RaggedPlan ragged_plan(int source, int32_t h_q, int32_t h_kv, int32_t head_dim, 
   if (paged)
     pl.row_waves = rows <= (int64_t)32 * n_seq ? 1 : 4;
   else
-    pl.row_waves = tiles(32) * h_kv <= 2 * (int64_t)cus ? 1 : 4;
+    pl.row_waves = tiles(32) * h_kv <= 2 * (int64_t)cus && keys >= (int64_t)192 * n_seq ? 1 : 4;
   const int64_t n = tiles(32 * pl.row_waves);
-  if (paged && n * h_kv < 8 * (int64_t)cus) {
+  if (paged && n * h_kv < 8 * (int64_t)cus && keys > kShortKeys) {
     pl.shares = std::max(1, fa2::ragged_waves(head_dim, source, pl.row_waves) * cus / h_kv);
     pl.parts = (size_t)h_kv * pl.shares * 2 * 32 * pl.row_waves * (head_dim + 4) * sizeof(float);  // (a multiple of 256)
     pl.workspace = pl.parts + (size_t)h_kv * pl.shares * fa2::kMergeBytes;
@@ -160,11 +173,11 @@ int check_heads(int32_t h_q, int32_t h_kv, int32_t n_tokens, float qk_scale, con
 }
 
 // Launches a checked call whose heads, tensors and sequences are in p.
-int launch_ragged(int32_t dtype, int32_t head_dim, int32_t h_q, fa2::RaggedParams& p, int source, void* workspace,
+int launch_ragged(int32_t dtype, int32_t head_dim, int32_t h_q, fa2::RaggedParams& p, int source, int64_t keys, void* workspace,
                   size_t workspace_bytes, void* stream) {
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const Topology topo = device_topology(stream_device(s));
-  const RaggedPlan pl = ragged_plan(source, h_q, p.h_kv, head_dim, p.seq.n_tokens, p.seq.n_seq, topo.cus);
+  const RaggedPlan pl = ragged_plan(source, h_q, p.h_kv, head_dim, p.seq.n_tokens, p.seq.n_seq, keys, topo.cus);
   if (pl.grid > 0x7fffffffLL) return fail(FA2_EINVAL, "grid of %lld workgroups is too large", (long long)pl.grid);
   if (pl.workspace) {
     if (!workspace || workspace_bytes < pl.workspace)
@@ -321,7 +334,7 @@ int fa2_attn_packed(const void* q, const void* k, const void* v, void* out, cons
   p.h_kv = h_kv;
   p.causal = causal != 0;
   p.qk_scale = qk_scale;
-  return launch_ragged(dtype, head_dim, h_q, p, fa2::kSourcePacked, nullptr, 0, stream);
+  return launch_ragged(dtype, head_dim, h_q, p, fa2::kSourcePacked, kv_tokens, nullptr, 0, stream);
 }
 
 int fa2_attn_paged(const void* q, void* out, const int64_t q_stride[2], const int64_t o_stride[2],
@@ -343,15 +356,15 @@ int fa2_attn_paged(const void* q, void* out, const int64_t q_stride[2], const in
   p.causal = causal != 0;
   p.qk_scale = qk_scale;
   return launch_ragged(dtype, cache->head_dim, h_q, p,
-                       cache->cache_dtype == FA2_DTYPE_E4M3 ? fa2::kSourceE4m3 : fa2::kSourcePages, workspace,
-                       workspace_bytes, stream);
+                       cache->cache_dtype == FA2_DTYPE_E4M3 ? fa2::kSourceE4m3 : fa2::kSourcePages,
+                       (int64_t)p.seq.max_pages << p.seq.page_shift, workspace, workspace_bytes, stream);
 }
 
 size_t fa2_paged_workspace_bytes(int32_t h_q, int32_t h_kv, int32_t head_dim, int32_t cache_dtype, int32_t n_tokens,
-                                 int32_t n_seq, int32_t num_cus) {
+                                 int32_t n_seq, int64_t max_keys, int32_t num_cus) {
   const int source = cache_dtype == FA2_DTYPE_E4M3 ? fa2::kSourceE4m3 : fa2::kSourcePages;
   if (h_q <= 0 || h_kv <= 0 || h_q % h_kv || dim_index(head_dim) < 0 || n_tokens <= 0 || n_seq <= 0 || num_cus <= 0) return 0;
-  return ragged_plan(source, h_q, h_kv, head_dim, n_tokens, n_seq, num_cus).workspace;
+  return ragged_plan(source, h_q, h_kv, head_dim, n_tokens, n_seq, max_keys, num_cus).workspace;
 }
 
 }  // extern "C"

@@ -15,7 +15,7 @@ import torch  # noqa: F401  (must be loaded before the HIP library, see above)
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libfa2_fwd.so")
 
 # C-ABI symbols declared in include/fa2_fwd.h, with (restype, argtypes).
-_i32, _i64p, _vp = ctypes.c_int32, ctypes.POINTER(ctypes.c_int64), ctypes.c_void_p
+_i32, _i64, _i64p, _vp = ctypes.c_int32, ctypes.c_int64, ctypes.POINTER(ctypes.c_int64), ctypes.c_void_p
 _i64x3 = ctypes.c_int64 * 3
 
 
@@ -66,7 +66,7 @@ SIGNATURES = {
                                        _i32, _i32, _i32, _i32, _i32, ctypes.c_float, _vp, _vp]),
     "fa2_attn_paged": (ctypes.c_int, [_vp, _vp, _i64p, _i64p, _cachep, _seqp, _i32, _i32, _i32, ctypes.c_float,
                                       _vp, _vp, ctypes.c_size_t, _vp]),
-    "fa2_paged_workspace_bytes": (ctypes.c_size_t, [_i32] * 7),
+    "fa2_paged_workspace_bytes": (ctypes.c_size_t, [_i32] * 6 + [_i64, _i32]),
     "fa2_last_error": (ctypes.c_char_p, []),
     "fa2_version": (ctypes.c_char_p, []),
 }
@@ -277,8 +277,9 @@ def attn_packed(q, k, v, out, cu, cu_kv, causal, qk_scale, lse, stream):
         DTYPE_CODE[q.dtype], int(bool(causal)), qk_scale, _ptr(lse), stream), "fa2_attn_packed")
 
 
-def paged_workspace_bytes(H_q, H_kv, D, cache_dtype, n_tokens, n_seq, num_cus):
-    return int(lib().fa2_paged_workspace_bytes(H_q, H_kv, D, CACHE_DTYPE_CODE[cache_dtype], n_tokens, n_seq, num_cus))
+def paged_workspace_bytes(H_q, H_kv, D, cache_dtype, n_tokens, n_seq, max_keys, num_cus):
+    return int(lib().fa2_paged_workspace_bytes(H_q, H_kv, D, CACHE_DTYPE_CODE[cache_dtype], n_tokens, n_seq, max_keys,
+                                               num_cus))
 
 
 def attn_paged(q, out, cache, seq, causal, qk_scale, lse, workspace, stream):

@@ -183,7 +183,7 @@ def attention_paged(q, cache, block_table, cu_seqlens, seqlens, *, causal=True, 
     cache's type, or fp16 or bf16 with an e4m3 cache. causal: the sequence's last new token sees all of its tokens, the one before it
     all but the last. A row that sees no key gets 0, and a log-sum-exp of -inf; rows past the last sequence
     are left as they are in out (undefined in a new one). A page outside the cache makes the
-    rows that see its tokens NaN.
+    rows that see its tokens NaN, and may make other rows of its sequence NaN.
     return_lse: also return the natural-log log-sum-exp of every row's scaled scores, fp32 [H_q, T].
     """
     if _lib.native is not None:  # the common call, made natively; None: not one of those
@@ -203,7 +203,8 @@ def attention_paged(q, cache, block_table, cu_seqlens, seqlens, *, causal=True, 
     lse = torch.empty((H_q, T), dtype=torch.float32, device=q.device) if return_lse else None
     c, s, alive = _step(cache, block_table, cu_seqlens, seqlens, T)
     if out.numel():
-        n = _lib.paged_workspace_bytes(H_q, H_kv, D, cache.k.dtype, T, seqlens.numel(), _cu_count(q.device))
+        n = _lib.paged_workspace_bytes(H_q, H_kv, D, cache.k.dtype, T, seqlens.numel(),
+                                       block_table.shape[1] * cache.k.shape[2], _cu_count(q.device))
         ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
         with torch.cuda.device(q.device):
             _lib.attn_paged(_rows(q), o_, c, s, causal, qk_scale, lse, ws,
