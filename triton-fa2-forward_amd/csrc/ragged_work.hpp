@@ -157,7 +157,7 @@ __device__ __forceinline__ bool find_tile(ParamsRef p, int rank, int lane, Curso
 __device__ __forceinline__ int64_t wave_max(int64_t x) {
 #pragma unroll
   for (int off = 32; off >= 1; off /= 2) x = max(x, (int64_t)__shfl_xor(x, off, 64));
-  return x;
+  return readlane64(x, 0);  // (a scalar: what is chosen by it stays one too)
 }
 
 // Whether a tile per workgroup takes no longer than equal shares, as estimated: as many tiles as workgroups at most, whose
