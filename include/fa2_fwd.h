@@ -240,7 +240,8 @@ FA2_API int fa2_should_pack_gqa(int32_t n_q, int32_t group, int32_t block_m);
  * device by the launch itself: nothing is copied to the host, a captured launch follows what they hold at
  * each replay, and no value of theirs makes a launch read or write outside the tensors.
  * Strides are element strides with a unit head_dim stride; 16-bit pointers are 16-byte aligned and their
- * strides non-negative multiples of 8 elements, K and V rows at most 2^22 elements apart.
+ * strides non-negative multiples of 8 elements, K and V rows at most 2^22 elements apart. What a call writes
+ * has no stride of 0 over more than one row; out of attention and rotary may be q and x.
  */
 
 /* Element type of a cache that holds e4m3 (OCP, no infinities), with a scale byte per row. */

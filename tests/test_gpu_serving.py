@@ -348,8 +348,8 @@ def test_packed_indices_that_do_not_ascend():
 # ------------------------------------------------------------------------------------------
 
 PAGED = [([1], [1]), ([1] * 5, [1, 33, 64, 700, 129]), ([4, 0, 1, 40, 129], [4, 50, 1000, 41, 129]),
-         ([3, 5, 2], [1, 0, 2]), ([1] * 66, [2 + 5 * i for i in range(66)]),
-         ([40] * 70, [20 + 7 * i for i in range(70)])]
+         ([3, 5, 2], [1, 0, 2])]
+MANY = [([1] * 66, [2 + 5 * i for i in range(66)]), ([40] * 70, [20 + 7 * i for i in range(70)])]
 
 
 def widened(table, page_size, keys=1600):
@@ -370,8 +370,19 @@ def check_paged(q, cache, pages, cu, lens, causal, dtype, out, lse, sm_scale=Non
 @pytest.mark.parametrize("D,page_size", [(16, 64), (32, 32), (64, 16), (64, 128), (128, 16), (128, 64)])
 @pytest.mark.parametrize("h_q,h_kv", [(2, 2), (8, 2), (7, 1), (16, 8)])
 def test_paged(dtype, e4m3, D, page_size, h_q, h_kv):
+    check_paged_calls(PAGED, dtype, e4m3, D, page_size, h_q, h_kv)
+
+
+@pytest.mark.parametrize("dtype,e4m3,D,page_size,h_q,h_kv", [(torch.float16, False, 64, 16, 8, 2), (torch.bfloat16, True, 128, 64, 2, 2),
+                                                             (torch.bfloat16, False, 16, 32, 7, 1)])
+def test_paged_many_sequences(dtype, e4m3, D, page_size, h_q, h_kv):
+    """More than 64: a workgroup looks for its rows 64 sequences at a time"""
+    check_paged_calls(MANY, dtype, e4m3, D, page_size, h_q, h_kv)
+
+
+def check_paged_calls(steps, dtype, e4m3, D, page_size, h_q, h_kv):
     from fa2.paged import attention_paged
-    for seed, (new, lens) in enumerate(PAGED):
+    for seed, (new, lens) in enumerate(steps):
         pages, cu, seqlens = step_of(new, lens, page_size, seed)
         cache = make_cache(pages.n_pages, h_kv, page_size, D, dtype, e4m3, seed, ("hnd", "nhd")[seed % 2])
         for s, n in enumerate(lens):  # rows behind a sequence's last token hold NaN
@@ -581,3 +592,142 @@ def test_streams_at_once():
     for i, w in enumerate(want):
         for g in got[i]:
             assert torch.equal(g[0], w[0]) and torch.equal(g[1], w[1])
+
+
+def calls_of_each(seed=0, dtype=torch.bfloat16, e4m3=True):
+    """Every operator's call on tensors of its own, as functions of `out` (a tensor to write, or None)"""
+    from fa2.packed import attention_packed
+    from fa2.paged import attention_paged, cache_read, cache_write
+    from fa2.rotary import rotary
+    D, page_size, new, lens = 64, 64, [3, 0, 40, 1], [30, 5, 900, 1]
+    pages, cu, seqlens = step_of(new, lens, page_size, seed)
+    table = widened(pages.table, page_size)
+    cache = make_cache(pages.n_pages, 2, page_size, D, dtype, e4m3, seed)
+    T = sum(new)
+    q, k, v = (randn((T, h, D), dtype, seed + i) for i, h in enumerate((8, 2, 2)))
+    positions = torch.arange(T, device="cuda")
+    return {"rotary": lambda out=None: rotary(q, positions, plan_of(32, True, 0.5), out=out),
+            "cache_write": lambda out=None: cache_write(cache, k, v, table, cu, seqlens, rotary=plan_of(64), q=q, q_out=out),
+            "cache_read": lambda out=None: cache_read(cache, table, cu, seqlens, T, dtype=dtype,
+                                                      out=None if out is None else (out[:, :2], k.clone()))[0],
+            "packed": lambda out=None: attention_packed(q, k, v, cu, out=out),
+            "packed lse": lambda out=None: attention_packed(q, k, v, cu, causal=False, sm_scale=0.3, return_lse=True, out=out)[1],
+            "paged": lambda out=None: attention_paged(q, cache, table, cu, seqlens, out=out),
+            "paged lse": lambda out=None: attention_paged(q, cache, table, cu, seqlens, return_lse=True, out=out)[1]}
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+def test_both_ways_to_the_kernels(e4m3, monkeypatch):
+    """The native calls and the ones through ctypes launch the same."""
+    from fa2 import _lib
+    assert _lib.native is not None
+    native = {name: call() for name, call in calls_of_each(e4m3=e4m3).items()}
+    monkeypatch.setattr(_lib, "native", None)
+    for name, call in calls_of_each(e4m3=e4m3).items():
+        assert torch.equal(call(), native[name]), name
+
+
+@pytest.mark.parametrize("layout", ["dense", "odd storage", "every other value", "other order"])
+def test_out_of_any_layout(layout):
+    """An out that the kernels cannot address is written through a copy; what lies between its values stays."""
+    for name, call in calls_of_each().items():
+        want = call()
+        if name.endswith("lse"):
+            continue
+        shape = (44, 8, 64)
+        if layout == "dense":
+            store = torch.full(shape, 3.0, dtype=torch.bfloat16, device="cuda")
+            out = store
+        elif layout == "odd storage":
+            store = torch.full((44 * 8 * 64 + 1,), 3.0, dtype=torch.bfloat16, device="cuda")
+            out = store[1:].view(shape)
+        elif layout == "every other value":
+            store = torch.full((44, 8, 128), 3.0, dtype=torch.bfloat16, device="cuda")
+            out = store[..., ::2]
+        else:
+            store = torch.full((8, 44, 64), 3.0, dtype=torch.bfloat16, device="cuda")
+            out = store.transpose(0, 1)
+        got = call(out)
+        assert torch.equal(got, want), name
+        assert torch.equal(out[:, :want.shape[1]], want), name
+        if layout == "every other value":
+            assert (store[..., 1::2] == 3.0).all(), name
+
+
+def test_out_in_place_and_broadcast():
+    """out may be the call's own q; a broadcast one is refused."""
+    from fa2.packed import attention_packed
+    from fa2.paged import attention_paged, cache_read, cache_write
+    from fa2.rotary import rotary
+    for new, lens in (([1] * 6, [700, 3, 64, 1, 2000, 90]), ([300, 1, 70], [2500, 800, 70])):
+        pages, cu, seqlens = step_of(new, lens, 32)
+        for D, e4m3 in ((64, False), (128, True)):
+            cache = make_cache(pages.n_pages, 2, 32, D, torch.float16, e4m3)
+            T = sum(new)
+            q, k = randn((T, 8, D), torch.float16, 5), randn((T, 2, D), torch.float16, 6)
+            for call in (lambda q, out: attention_paged(q, cache, pages.table, cu, seqlens, out=out),
+                         lambda q, out: attention_packed(q, k, k, cu, out=out),
+                         lambda q, out: rotary(q, torch.arange(T, device="cuda"), plan_of(D), out=out)):
+                want = call(q, None)
+                x = q.clone()
+                assert torch.equal(call(x, x), want)
+                with pytest.raises(RuntimeError, match="stride of 0"):
+                    call(q, x[:, :1].expand(T, 8, D))
+            with pytest.raises(RuntimeError, match="stride of 0"):
+                cache_write(cache._replace(k=cache.k[:1].expand_as(cache.k)), k, k, pages.table, cu, seqlens)
+            with pytest.raises(RuntimeError, match="stride of 0"):
+                cache_read(cache, pages.table, cu, seqlens, T, out=(k, k[:1].expand(T, 2, D)))
+            # reading from heads that share their rows is fine
+            one = cache._replace(**{n: t[:, :1].expand(t.shape) for n, t in zip(cache._fields, cache) if t is not None})
+            apart = cache._replace(**{n: bytes_of(t).contiguous().view(t.dtype) for n, t in zip(one._fields, one) if t is not None})
+            assert torch.equal(attention_paged(q, one, pages.table, cu, seqlens),
+                               attention_paged(q, apart, pages.table, cu, seqlens))
+
+
+def test_tables_without_columns():
+    """No sequence has a token in the cache: rows get 0, nothing is written, zeros are read."""
+    from fa2.paged import attention_paged, cache_read, cache_write
+    cache = make_cache(2, 2, 16, 64, torch.float16, False)
+    before = [bytes_of(t).clone() for t in (cache.k, cache.v)]
+    cu, table = cumulative([3, 1]), torch.zeros(2, 0, dtype=torch.int32, device="cuda")
+    seqlens = torch.tensor([3, 9], dtype=torch.int32, device="cuda")
+    q, k = randn((4, 4, 64), torch.float16, 1), randn((4, 2, 64), torch.float16, 2)
+    out, lse = attention_paged(q, cache, table, cu, seqlens, return_lse=True)
+    assert (out == 0).all() and (lse == -math.inf).all()
+    cache_write(cache, k, k, table, cu, seqlens)
+    assert all(torch.equal(bytes_of(t), b) for t, b in zip((cache.k, cache.v), before))
+    assert all((t == 0).all() for t in cache_read(cache, table, cu, seqlens, 4))
+
+
+def test_two_graphs_of_one_pool():
+    """Two captured steps that share a memory pool, replayed in turn with other lengths and eager calls between."""
+    from fa2.paged import attention_paged
+    D, dtype, page_size = 128, torch.float16, 32
+    jobs = []
+    stream, pool = torch.cuda.Stream(), None
+    for i, new in enumerate(([1] * 8, [90, 1, 200, 1])):
+        most = [2000 + 100 * j for j in range(len(new))]
+        pages, cu, _ = step_of(new, most, page_size, seed=i)
+        cache = make_cache(pages.n_pages, 2, page_size, D, dtype, i == 1, i)
+        seqlens = torch.tensor(most, dtype=torch.int32, device="cuda")
+        q = randn((sum(new), 8, D), dtype, i)
+        out = torch.zeros_like(q)
+
+        def call(q=q, cache=cache, table=pages.table, cu=cu, seqlens=seqlens, out=None):
+            return attention_paged(q, cache, table, cu, seqlens, out=out)
+        call()
+        torch.cuda.synchronize()
+        stream.wait_stream(torch.cuda.current_stream())
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.stream(stream), torch.cuda.graph(graph, pool=pool, stream=stream):
+            call(out=out)
+        pool = graph.pool()
+        jobs.append((graph, call, seqlens, most, out))
+    torch.cuda.synchronize()
+    for round_ in range(4):
+        for graph, call, seqlens, most, out in jobs:
+            seqlens.copy_(torch.tensor([max(n - 631 * round_ * (j % 3), 300) for j, n in enumerate(most)], dtype=torch.int32))
+            out.fill_(9.0)
+            graph.replay()
+            assert torch.equal(out, call())
+    torch.cuda.synchronize()

@@ -293,6 +293,19 @@ def test_c_call_refusals():
     assert _lib.paged_workspace_bytes(4, 2, 64, torch.bfloat16, 3, 2, 1536, 256) == 0  # no sequence is long enough
     assert _lib.paged_workspace_bytes(32, 8, 128, torch.float8_e4m3fn, 1 << 20, 4, 1 << 20, 256) == 0  # row tiles enough: none are shared
     assert _lib.lib().fa2_cache_write(None, None, P, P, None, None, None, None, None, None, 0, None, 1, None) == -1
+    # rows that are written have places of their own
+    for stride in ((0, 1024, 64), (2048, 0, 64), (2048, 1024, 0)):
+        assert write(c_cache(v_stride=stride), c_seq()) == -1 and "stride of 0" in _lib.last_error()
+    e4m3 = dict(cache_dtype=2, k_scale=P, v_scale=P, v_scale_stride=(32, 16, 1))
+    assert write(c_cache(**e4m3), c_seq()) == -1 and "stride of 0" in _lib.last_error()
+    s, one = strides(256, 64), strides(0, 64)
+    assert _lib.lib().fa2_cache_read(ctypes.byref(c_cache()), ctypes.byref(c_seq()), P, P, s, one, 1, None) == -1
+    assert _lib.lib().fa2_attn_paged(P, P, s, one, ctypes.byref(c_cache()), ctypes.byref(c_seq()), 4, 1, 1, 0.1, None, None,
+                                     0, None) == -1 and "stride of 0" in _lib.last_error()
+    assert _lib.lib().fa2_attn_packed(P, P, P, P, s, s, s, one, P, None, 2, 3, 3, 4, 4, 64, 1, 1, 0.1, None, None) == -1
+    three = strides(768, 64, 0)
+    assert _lib.lib().fa2_rotary(P, P, strides(768, 64, 256), three, P, 4, strides(0, 1), ctypes.byref(rot), 1, 4, 3, 64, 1,
+                                 None) == -1 and "stride of 0" in _lib.last_error()
     # nothing to do
     assert write(c_cache(), c_seq(n_tokens=0)) == 0 and write(c_cache(), c_seq(n_seq=0, cu=None)) == 0
     assert paged(c_cache(), c_seq(n_tokens=0)) == 0 and _lib.last_error() == ""

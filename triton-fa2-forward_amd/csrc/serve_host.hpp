@@ -3,6 +3,9 @@
 // shares; everything here has internal linkage.
 #pragma once
 
+#include <initializer_list>
+#include <utility>
+
 #include "attn_fwd_host.hpp"
 #include "serve_launch.hpp"
 
@@ -23,6 +26,13 @@ int check_rows(const char* what, const void* p, const int64_t* stride, int n, in
     if (stride[i] < 0 || stride[i] % multiple)
       return fail(FA2_EALIGN, "strides of %s must be non-negative multiples of %d elements (%lld)", what,
                   multiple, (long long)stride[i]);
+  return FA2_OK;
+}
+
+// What is written has a place of its own for every row: no stride of zero over several
+int check_written(const char* what, std::initializer_list<std::pair<int64_t, int64_t>> count_and_stride) {
+  for (const auto& [count, stride] : count_and_stride)
+    if (count > 1 && stride == 0) return fail(FA2_EINVAL, "%s is written: it cannot have a stride of 0", what);
   return FA2_OK;
 }
 
@@ -224,6 +234,7 @@ int fa2_rotary(const void* x, void* out, const int64_t x_stride[3], const int64_
   if (batch == 0 || heads == 0 || n == 0) return FA2_OK;
   if (const int rc = check_rows("x", x, x_stride, 3, 8)) return rc;
   if (const int rc = check_rows("out", out, o_stride, 3, 8)) return rc;
+  if (const int rc = check_written("out", {{batch, o_stride[0]}, {heads, o_stride[1]}, {n, o_stride[2]}})) return rc;
   if (!positions || !p_stride) return fail(FA2_EINVAL, "null pointer: positions");
   if (reinterpret_cast<uintptr_t>(positions) % (unsigned)position_bytes)
     return fail(FA2_EALIGN, "positions must be aligned to their size");
@@ -254,11 +265,16 @@ int fa2_cache_write(const fa2_cache* cache, const fa2_sequences* seq, const void
   if (q && h_q < 1) return fail(FA2_EINVAL, "bad sizes: h_q=%d", h_q);
   if (cache->h_kv > (1 << 24) || h_q > (1 << 24)) return fail(FA2_EINVAL, "at most 2^24 heads");
   if (p.seq.n_seq == 0 || p.seq.n_tokens == 0) return FA2_OK;
+  for (const int64_t* s : {cache->k_stride, cache->v_stride, p.kc.scale ? cache->k_scale_stride : cache->k_stride,
+                           p.kc.scale ? cache->v_scale_stride : cache->v_stride})
+    if (const int rc = check_written("the cache", {{cache->n_pages, s[0]}, {cache->h_kv, s[1]}, {cache->page_size, s[2]}}))
+      return rc;
   if (const int rc = check_rows("k", k, k_stride, 2, 8)) return rc;
   if (const int rc = check_rows("v", v, v_stride, 2, 8)) return rc;
   if (q) {
     if (const int rc = check_rows("q", q, q_stride, 2, 8)) return rc;
     if (const int rc = check_rows("q_out", q_out, qo_stride, 2, 8)) return rc;
+    if (const int rc = check_written("q_out", {{p.seq.n_tokens, qo_stride[0]}, {h_q, qo_stride[1]}})) return rc;
     p.q = static_cast<const uint16_t*>(q);
     p.q_out = static_cast<uint16_t*>(q_out);
     p.sqt = q_stride[0]; p.sqh = q_stride[1];
@@ -285,6 +301,8 @@ int fa2_cache_read(const fa2_cache* cache, const fa2_sequences* seq, void* k, vo
   if (p.seq.n_seq == 0 || p.seq.n_tokens == 0) return FA2_OK;
   if (const int rc = check_rows("k", k, k_stride, 2, 8)) return rc;
   if (const int rc = check_rows("v", v, v_stride, 2, 8)) return rc;
+  for (const int64_t* s : {k_stride, v_stride})
+    if (const int rc = check_written("k and v", {{p.seq.n_tokens, s[0]}, {cache->h_kv, s[1]}})) return rc;
   p.k = static_cast<uint16_t*>(k);
   p.v = static_cast<uint16_t*>(v);
   p.skt = k_stride[0]; p.skh = k_stride[1];
@@ -313,6 +331,7 @@ int fa2_attn_packed(const void* q, const void* k, const void* v, void* out, cons
   if (!cu) return fail(FA2_EINVAL, "null pointer: cu");
   if (const int rc = check_rows("q", q, q_stride, 2, 8)) return rc;
   if (const int rc = check_rows("out", out, o_stride, 2, 8)) return rc;
+  if (const int rc = check_written("out", {{n_tokens, o_stride[0]}, {h_q, o_stride[1]}})) return rc;
   if (const int rc = check_rows("k", k, k_stride, 2, 8)) return rc;
   if (const int rc = check_rows("v", v, v_stride, 2, 8)) return rc;
   if (k_stride[0] > kMaxRowStride || v_stride[0] > kMaxRowStride)
@@ -347,6 +366,7 @@ int fa2_attn_paged(const void* q, void* out, const int64_t q_stride[2], const in
   if (p.seq.n_seq == 0 || p.seq.n_tokens == 0) return FA2_OK;
   if (const int rc = check_rows("q", q, q_stride, 2, 8)) return rc;
   if (const int rc = check_rows("out", out, o_stride, 2, 8)) return rc;
+  if (const int rc = check_written("out", {{p.seq.n_tokens, o_stride[0]}, {h_q, o_stride[1]}})) return rc;
   p.q = static_cast<const uint16_t*>(q);
   p.o = static_cast<uint16_t*>(out);
   p.lse = lse;

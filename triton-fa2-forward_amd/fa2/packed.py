@@ -63,6 +63,7 @@ def attention_packed(q, k, v, cu_seqlens, cu_seqlens_kv=None, *, causal=True, sm
     causal: row i of a sequence sees its keys up to i + n_kv - n_q (with one cu_seqlens: up to its own).
         A row that sees no key gets 0, and a log-sum-exp of -inf.
     return_lse: also return the natural-log log-sum-exp of every row's scaled scores, fp32 [H_q, T].
+    out: of q's shape and type, in any layout without shared elements; q itself is allowed.
     """
     if _lib.native is not None:  # the common call, made natively; None: not one of those
         result = _lib.native.attn_packed(q, k, v, cu_seqlens, cu_seqlens_kv, causal, sm_scale, return_lse, out)

@@ -185,6 +185,7 @@ def attention_paged(q, cache, block_table, cu_seqlens, seqlens, *, causal=True, 
     are left as they are in out (undefined in a new one). A page outside the cache makes the
     rows that see its tokens NaN, and may make other rows of its sequence NaN.
     return_lse: also return the natural-log log-sum-exp of every row's scaled scores, fp32 [H_q, T].
+    out: of q's shape and type, in any layout without shared elements; q itself is allowed.
     """
     if _lib.native is not None:  # the common call, made natively; None: not one of those
         result = _lib.native.attn_paged(*cache, block_table, cu_seqlens, seqlens, q, causal, sm_scale, return_lse, out)
