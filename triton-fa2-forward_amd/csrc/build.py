@@ -174,8 +174,7 @@ def build(jobs=8, verbose=False):
                           f"-DFA2_DT={dt}", f"-DFA2_D={d}", "-c",
                           os.path.join(CSRC, "attn_fwd_inst.hip"), "-o", obj])
             obj = os.path.join(OBJ_DIR, f"attn_ragged_dt{dt}_d{d}.o")
-            serve_units.append([cc, *common_flags(), "-Rpass-analysis=kernel-resource-usage",
-                                f"-DFA2_DT={dt}", f"-DFA2_D={d}", "-c",
+            serve_units.append([cc, *common_flags(), f"-DFA2_DT={dt}", f"-DFA2_D={d}", "-c",
                                 os.path.join(CSRC, "attn_ragged_inst.hip"), "-o", obj])
             obj = os.path.join(OBJ_DIR, f"attn_fwd_ablate_dt{dt}_d{d}.o")
             ablate_units.append([cc, *common_flags(), f"-DFA2_DT={dt}", f"-DFA2_D={d}", "-c",

@@ -12,7 +12,10 @@
 // is that of the row's finite values), and at the largest exponent of the row's type the largest
 // magnitude is 240 instead of 448, so that no stored value is past the type's own range.
 //
-// All of it is bound by HBM: 16 bytes per lane and load, a row's D / 8 lanes side by side.
+// All of it is bound by HBM, and small calls by the chain of lookups (sequence, length, page), which a group of
+// tokens makes together: 16 bytes per lane and load, a row's D / 8 lanes side by side. Measured on MI355X (kernel alone):
+// rotary of 16384 x 32 heads of 128 41 us, 6.5 TB/s, of 16 tokens 4.1; a write of 5096 tokens of 28 + 2 x 4 heads of 64 with
+// their rotation 16.4 us, 2.9 TB/s, of 64 tokens into e4m3 6.2; a read of 57071 tokens of 2 x 8 e4m3 heads of 128 71 us, 5 TB/s.
 #include <hip/hip_runtime.h>
 
 #include "serve_common.hpp"
