@@ -266,9 +266,10 @@ def test_packed(dtype, D, h_q, h_kv, causal):
 
 @pytest.mark.parametrize("causal", [True, False])
 @pytest.mark.parametrize("D", [64, 128])
-def test_packed_long(causal, D):
+@pytest.mark.parametrize("lens", [[2500, 1, 777, 1300], [300, 0, 1, 700, 129, 128, 0, 511, 90, 0], [7 * i % 400 for i in range(64)],
+                                  [200 + i for i in range(20)] * 4], ids=len)
+def test_packed_long(causal, D, lens):
     from fa2.packed import attention_packed
-    lens = [2500, 1, 777, 1300]
     T, cu = sum(lens), cumulative(lens)
     q, k, v = (randn((T, h, D), torch.bfloat16, i) for i, h in enumerate((8, 2, 2)))
     out, lse = attention_packed(q, k, v, cu, causal=causal, return_lse=True)
