@@ -18,6 +18,8 @@
 // their rotation 16.4 us, 2.9 TB/s, of 64 tokens into e4m3 6.2; a read of 57071 tokens of 2 x 8 e4m3 heads of 128 71 us, 5 TB/s.
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "serve_common.hpp"
 #include "serve_launch.hpp"
 
@@ -27,23 +29,26 @@ namespace {
 
 constexpr int kMaxTokensPerWg = 16;
 constexpr int kRowsAtOnce = 4;  // rows of a lane whose loads are in flight together
+// Scale bytes that a workgroup of several tokens keeps until its end, to store those of a head and page side by side.
+// Measured on MI355X: 16000 tokens of 2 x 8 heads of 128, keys rotated: 56 us a byte a store, 48 gathered.
+constexpr int kScalesAtOnce = 1024;
 constexpr int kMaxHalf = 64;  // head_dim 128, all of it rotated
 
 // cos and sin of 2 pi x for |x| <= 1/2 turns
 __device__ __forceinline__ void sincos_turns(double x, double* s, double* c) { sincospi(2.0 * x, s, c); }
 
-// cos and sin (times scale) of every pair's angle at the workgroup's tokens, into cs[token][pair][2]
-template <class Position>
-__device__ __forceinline__ void fill_angles(double (*cs)[kMaxHalf][2], const RotaryPlan& rot, int tokens,
-                                            Position&& position) {
+// cos and sin (times scale) of every pair's angle at the workgroup's tokens, formed in float64, into cs[token][pair][2] of
+// type A: float, rounded once, or double where the products are formed in float64.
+template <class A, class Position>
+__device__ __forceinline__ void fill_angles(A (*cs)[kMaxHalf][2], const RotaryPlan& rot, int tokens, Position&& position) {
   const int n = tokens * rot.half;
   for (int i = threadIdx.x; i < n; i += 256) {
     const int t = i / rot.half, f = i - t * rot.half;
     const double turns = (double)position(t) * rot.freqs[f] * 0.15915494309189533577;  // 1 / (2 pi)
     double s, c;
     sincos_turns(turns - rint(turns), &s, &c);
-    cs[t][f][0] = c * rot.scale;
-    cs[t][f][1] = s * rot.scale;
+    cs[t][f][0] = (A)(c * rot.scale);
+    cs[t][f][1] = (A)(s * rot.scale);
   }
 }
 
@@ -61,10 +66,10 @@ __device__ __forceinline__ Chunks load_chunks(const uint16_t* row, int chunk, in
   return x;
 }
 
-// ... rotated (T: the type the products are formed in)
-template <int DT, class T>
+// ... rotated (T: the type the products and sums are formed in, rounded to float once)
+template <int DT, class T, class A>
 __device__ __forceinline__ void rotated8(const Chunks& in, int chunk, int half, bool interleaved,
-                                         const double (*cs)[2], T (&y)[8]) {
+                                         const A (*cs)[2], float (&y)[8]) {
   float x[8];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -79,8 +84,8 @@ __device__ __forceinline__ void rotated8(const Chunks& in, int chunk, int half, 
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const T c = (T)cs[d0 / 2 + i][0], s = (T)cs[d0 / 2 + i][1];
-      y[2 * i] = (T)x[2 * i] * c - (T)x[2 * i + 1] * s;
-      y[2 * i + 1] = (T)x[2 * i + 1] * c + (T)x[2 * i] * s;
+      y[2 * i] = (float)((T)x[2 * i] * c - (T)x[2 * i + 1] * s);
+      y[2 * i + 1] = (float)((T)x[2 * i + 1] * c + (T)x[2 * i] * s);
     }
   } else {
     const bool second = d0 >= half;
@@ -89,16 +94,16 @@ __device__ __forceinline__ void rotated8(const Chunks& in, int chunk, int half, 
     for (int i = 0; i < 8; ++i) {
       const T c = (T)cs[f0 + i][0], s = (T)cs[f0 + i][1];
       const T o = (T)to_f32<DT>((uint16_t)(in.other[i / 2] >> (16 * (i & 1))));
-      y[i] = (T)x[i] * c + (second ? o * s : -(o * s));
+      y[i] = (float)((T)x[i] * c + (second ? o * s : -(o * s)));
     }
   }
 }
 
-template <int DT, class T>
-__device__ __forceinline__ u32x4 pack8(const T (&y)[8]) {
+template <int DT>
+__device__ __forceinline__ u32x4 pack8(const float (&y)[8]) {
   u32x4 r;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) r[i] = Elem<DT>::pack2((float)y[2 * i], (float)y[2 * i + 1]);
+  for (int i = 0; i < 4; ++i) r[i] = Elem<DT>::pack2(y[2 * i], y[2 * i + 1]);
   return r;
 }
 
@@ -107,7 +112,7 @@ __device__ __forceinline__ u32x4 pack8(const T (&y)[8]) {
 template <int DT, int D>
 __global__ __launch_bounds__(256) void rotary_kernel(const RotaryParams p) {
   constexpr int LPR = D / 8;  // lanes per row
-  __shared__ double cs[kMaxTokensPerWg][kMaxHalf][2];
+  __shared__ float cs[kMaxTokensPerWg][kMaxHalf][2];
   const int64_t total = (int64_t)p.batch * p.n;
   const int64_t t0 = (int64_t)blockIdx.x * p.tokens_per_wg;
   const int tokens = (int)min((int64_t)p.tokens_per_wg, total - t0);
@@ -123,7 +128,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryParams p) {
     const int t = r / p.heads, h = r - t * p.heads;
     const int64_t b = (t0 + t) / p.n, i = (t0 + t) - b * p.n;
     float y[8];
-    rotated8<DT>(load_chunks(p.x + b * p.sxb + h * p.sxh + i * p.sxn, chunk, p.rot.half, p.rot.interleaved), chunk,
+    rotated8<DT, float>(load_chunks(p.x + b * p.sxb + h * p.sxh + i * p.sxn, chunk, p.rot.half, p.rot.interleaved), chunk,
                  p.rot.half, p.rot.interleaved, cs[t], y);
     *(u32x4*)(p.out + b * p.sob + h * p.soh + i * p.son + 8 * chunk) = pack8<DT>(y);
   }
@@ -147,12 +152,12 @@ __device__ __forceinline__ uint8_t* scale_row(const CacheParams& p, bool v, cons
 }
 
 // One row's 8 values of this lane as e4m3, with the row's scale byte (D / 8 lanes hold a row).
-template <int DT, int D, class T>
-__device__ __forceinline__ u32x2 quantise8(const T (&y)[8], uint32_t* scale_byte) {
+template <int DT, int D>
+__device__ __forceinline__ u32x2 quantise8(const float (&y)[8], uint32_t* scale_byte) {
   float top = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float a = fabsf((float)y[i]);
+    const float a = fabsf(y[i]);
     top = a < INFINITY ? fmaxf(top, a) : top;  // finite values only (false for NaN)
   }
 #pragma unroll
@@ -164,14 +169,14 @@ __device__ __forceinline__ u32x2 quantise8(const T (&y)[8], uint32_t* scale_byte
   e = min(max(e, -126), kLargest);
   const float limit = e == kLargest ? 240.f : 448.f;
   *scale_byte = (uint32_t)(e + 127);
-  const T inv = (T)__uint_as_float((uint32_t)(127 - e) << 23);
+  const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
   uint32_t w[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     float z[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float x = (float)(y[4 * h + i] * inv);
+      const float x = y[4 * h + i] * inv;
       z[i] = fabsf(x) < INFINITY ? fminf(fmaxf(x, -limit), limit) : __uint_as_float(0x7fc00000u);
     }
     int r = __builtin_amdgcn_cvt_pk_fp8_f32(z[0], z[1], 0, false);
@@ -180,15 +185,20 @@ __device__ __forceinline__ u32x2 quantise8(const T (&y)[8], uint32_t* scale_byte
   return u32x2{w[0], w[1]};
 }
 
-// Rows per token: K heads, V heads, then (q) query heads. K is rotated in float64: a rotated value next to
-// a border between two e4m3 values goes to the one that its exact value goes to.
+// Rows per token: K heads, V heads, then (q) query heads. K of an e4m3 cache is rotated in float64 and rounded to float
+// once: products in float would take more of the values next to a border between two e4m3 values across it.
+// Scaling by a power of two adds no rounding. (V and what is not rotated in float: rows in float64 throughout took
+// 136 us where 125 are enough, 16000 tokens of 32 + 2 x 8 heads of 128.)
 template <int DT, int D, bool E4M3>
 __global__ __launch_bounds__(256) void cache_write_kernel(const CacheParams p) {
   constexpr int LPR = D / 8;
-  __shared__ double cs[kMaxTokensPerWg][kMaxHalf][2];
+  using Angle = std::conditional_t<E4M3, double, float>;
+  __shared__ Angle cs[kMaxTokensPerWg][kMaxHalf][2];
   __shared__ Place places[kMaxTokensPerWg];
+  __shared__ uint8_t scales[E4M3 ? kScalesAtOnce : 1];  // [K and V heads][tokens]
   const int t0 = (int)blockIdx.x * p.tokens_per_wg;
   const int tokens = min(p.tokens_per_wg, p.seq.n_tokens - t0);
+  const bool gather = E4M3 && tokens > 1 && (int64_t)tokens * 2 * p.h_kv <= kScalesAtOnce;
   const int chunk = threadIdx.x % LPR;
   const int per_token = 2 * p.h_kv + (p.q ? p.h_q : 0);
   const int rows = tokens * per_token;
@@ -231,10 +241,10 @@ __global__ __launch_bounds__(256) void cache_write_kernel(const CacheParams p) {
       if (x < 0) continue;
       const Place at = places[token[u]];
       if (at.pos < 0) continue;
-      const double(*angles)[2] = cs[token[u]];
+      const Angle(*angles)[2] = cs[token[u]];
       if (x >= 2 * p.h_kv) {
         float y[8];
-        rotated8<DT>(in[u], chunk, half, interleaved, angles, y);
+        rotated8<DT, float>(in[u], chunk, half, interleaved, angles, y);
         *(u32x4*)(p.q_out + (int64_t)(t0 + token[u]) * p.sot + (x - 2 * p.h_kv) * p.soh + 8 * chunk) = pack8<DT>(y);
         continue;
       }
@@ -243,17 +253,35 @@ __global__ __launch_bounds__(256) void cache_write_kernel(const CacheParams p) {
       const int h = is_v ? x - p.h_kv : x;
       char* dst = cache_row(p, is_v, at, h, E4M3 ? 1 : 2);
       if constexpr (E4M3) {
-        double y[8];
-        rotated8<DT>(in[u], chunk, is_v ? 0 : half, interleaved, angles, y);
+        float y[8];
+        if (is_v || half == 0)
+          rotated8<DT, float>(in[u], chunk, 0, interleaved, angles, y);
+        else
+          rotated8<DT, double>(in[u], chunk, half, interleaved, angles, y);
         uint32_t byte;
         const u32x2 w = quantise8<DT, D>(y, &byte);
         *(u32x2*)(dst + 8 * chunk) = w;
-        if (chunk == 0) *scale_row(p, is_v, at, h) = (uint8_t)byte;
+        if (chunk == 0) {
+          if (gather)
+            scales[x * tokens + token[u]] = (uint8_t)byte;
+          else
+            *scale_row(p, is_v, at, h) = (uint8_t)byte;
+        }
       } else {
         float y[8];
-        rotated8<DT>(in[u], chunk, is_v ? 0 : half, interleaved, angles, y);
+        rotated8<DT, float>(in[u], chunk, is_v ? 0 : half, interleaved, angles, y);
         *(u32x4*)(dst + 16 * chunk) = pack8<DT>(y);
       }
+    }
+  }
+  if constexpr (E4M3) {
+    if (!gather) return;
+    __syncthreads();
+    for (int i = threadIdx.x; i < tokens * 2 * p.h_kv; i += 256) {
+      const int x = i / tokens;
+      const Place at = places[i - x * tokens];
+      const bool is_v = x >= p.h_kv;
+      if (at.pos >= 0 && at.page >= 0) *scale_row(p, is_v, at, is_v ? x - p.h_kv : x) = scales[i];
     }
   }
 }
