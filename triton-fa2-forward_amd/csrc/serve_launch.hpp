@@ -20,9 +20,12 @@ constexpr int kSourcePacked = 0, kSourcePages = 1, kSourceE4m3 = 2;
 
 // Its workgroups per CU (waves per SIMD), by registers: packed rows keep nothing from tile to tile (128 VGPRs at
 // head_dim 64). Measured at head_dim 64 on MI355X: packed prompts of 3k to 8k, 2 / 3 / 4 a CU 394 / 390 / 384 us; a chunk of
-// 2000 over 8k keys, 16-bit pages 170 / 165 / 223 (spilled), e4m3 pages 193 / 195 / 359.
+// 2000 over 8k keys, 16-bit pages 170 / 165 / 223 (spilled), e4m3 pages 193 / 195 / 359. 32-row workgroups keep 32 KiB of LDS up
+// to head_dim 32 and 64 above: steps of 195 e4m3 sequences of up to 8000, 8 heads of 32, 123 / 104 / 121 us; of 97
+// 16-bit ones 84 / 90 / 93, of 195 with heads of 16 95 / 88 / 91.
 constexpr int ragged_waves(int head_dim, int source, int row_waves) {
-  return row_waves == 1 || head_dim == 128 || source == kSourceE4m3 ? 2 : source == kSourcePages ? 3 : 4;
+  if (row_waves == 1) return head_dim <= 32 ? 3 : 2;
+  return head_dim == 128 || source == kSourceE4m3 ? 2 : source == kSourcePages ? 3 : 4;
 }
 
 // The ragged attention kernel with 32 * row_waves (1 or 4) rows per workgroup, and after it, with p.shares > 0,
