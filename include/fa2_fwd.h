@@ -267,7 +267,8 @@ typedef struct fa2_cache {
 /*
  * Sequences over a paged cache, all device pointers: lens[s] tokens of sequence s are in the cache, the
  * sequence's packed rows being the last of them; token p lies in page table[s * table_stride + p / page_size]
- * at row p % page_size. max_pages: entries per row of the table.
+ * at row p % page_size. max_pages: entries per row of the table (attention takes a sequence of more tokens than
+ * they hold as one of max_pages * page_size).
  */
 typedef struct fa2_sequences {
   const int32_t* cu;

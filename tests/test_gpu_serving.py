@@ -700,6 +700,20 @@ def test_tables_without_columns():
     assert all((t == 0).all() for t in cache_read(cache, table, cu, seqlens, 4))
 
 
+def test_lengths_past_the_table():
+    from fa2.paged import attention_paged
+    for most, new in ((128, [1, 5]), (2048, [1, 300])):
+        pages, cu, seqlens = step_of(new, [most, 60 + new[1]], 32)
+        table = pages.table[:, :most // 32].contiguous()
+        for e4m3 in (False, True):
+            cache = make_cache(pages.n_pages, 2, 32, 64, torch.bfloat16, e4m3)
+            q = randn((sum(new), 8, 64), torch.bfloat16, 1)
+            long = torch.tensor([2 ** 31 - 1, 60 + new[1]], dtype=torch.int32, device="cuda")
+            for causal in (True, False):
+                assert torch.equal(attention_paged(q, cache, table, cu, long, causal=causal),
+                                   attention_paged(q, cache, table, cu, seqlens, causal=causal))
+
+
 def test_two_graphs_of_one_pool():
     """Two captured steps that share a memory pool, replayed in turn with other lengths and eager calls between."""
     from fa2.paged import attention_paged
