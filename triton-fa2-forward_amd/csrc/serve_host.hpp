@@ -126,7 +126,8 @@ int launched(int e, const char* what) {
 // 3567 110, 69 and 76 us. The rotary kernel has no such lookup, and takes as few tokens as fill its lanes.
 constexpr int64_t kWriteWgs = 1024, kReadWgs = 4096, kRotaryWgs = int64_t(1) << 40;
 unsigned cache_grid(fa2::CacheParams* p, int64_t rows_per_token, int32_t head_dim, int64_t least_wgs) {
-  p->tokens_per_wg = fa2::serve_tokens_per_wg((int)std::min<int64_t>(rows_per_token * (head_dim / 8), 256), p->seq.n_tokens, least_wgs);
+  p->tokens_per_wg = fa2::serve_tokens_per_wg((int)std::min<int64_t>(rows_per_token * (head_dim / 8), 256),
+                                              p->seq.n_tokens, least_wgs);
   return (unsigned)(((int64_t)p->seq.n_tokens + p->tokens_per_wg - 1) / p->tokens_per_wg);
 }
 
@@ -150,8 +151,8 @@ struct RaggedPlan {
   size_t parts = 0, workspace = 0;  // bytes of the partial results, and with what their merge needs to know
 };
 // keys: of packed rows, all of them; of pages, the most that a sequence can have
-RaggedPlan ragged_plan(int source, int32_t h_q, int32_t h_kv, int32_t head_dim, int32_t n_tokens, int32_t n_seq, int64_t keys,
-                       int cus) {
+RaggedPlan ragged_plan(int source, int32_t h_q, int32_t h_kv, int32_t head_dim, int32_t n_tokens, int32_t n_seq,
+                       int64_t keys, int cus) {
   RaggedPlan pl;
   const bool paged = source != fa2::kSourcePacked;
   const int64_t rows = (int64_t)n_tokens * (h_q / h_kv);
@@ -163,7 +164,8 @@ RaggedPlan ragged_plan(int source, int32_t h_q, int32_t h_kv, int32_t head_dim, 
   const int64_t n = tiles(32 * pl.row_waves);
   if (paged && n * h_kv < 8 * (int64_t)cus && keys > kShortKeys) {
     pl.shares = std::max(1, fa2::ragged_waves(head_dim, source, pl.row_waves) * cus / h_kv);
-    pl.parts = (size_t)h_kv * pl.shares * 2 * 32 * pl.row_waves * (head_dim + 4) * sizeof(float);  // (a multiple of 256)
+    // (a multiple of 256)
+    pl.parts = (size_t)h_kv * pl.shares * 2 * 32 * pl.row_waves * (head_dim + 4) * sizeof(float);
     pl.workspace = pl.parts + (size_t)h_kv * pl.shares * fa2::kMergeBytes;
   }
   pl.grid = (pl.shares ? pl.shares : n) * h_kv;
@@ -191,7 +193,8 @@ int launch_ragged(int32_t dtype, int32_t head_dim, int32_t h_q, fa2::RaggedParam
   if (pl.grid > 0x7fffffffLL) return fail(FA2_EINVAL, "grid of %lld workgroups is too large", (long long)pl.grid);
   if (pl.workspace) {
     if (!workspace || workspace_bytes < pl.workspace)
-      return fail(FA2_EINVAL, "the call needs a workspace of %zu bytes, got %zu", pl.workspace, workspace ? workspace_bytes : (size_t)0);
+      return fail(FA2_EINVAL, "the call needs a workspace of %zu bytes, got %zu", pl.workspace,
+                  workspace ? workspace_bytes : (size_t)0);
     if (reinterpret_cast<uintptr_t>(workspace) & 255u) return fail(FA2_EALIGN, "the workspace must be 256-byte aligned");
   }
   p.group = h_q / p.h_kv;
@@ -247,7 +250,8 @@ int fa2_rotary(const void* x, void* out, const int64_t x_stride[3], const int64_
   p.spb = p_stride[0]; p.spn = p_stride[1];
   p.batch = batch; p.heads = heads; p.n = n;
   if (heads > (1 << 24)) return fail(FA2_EINVAL, "at most 2^24 heads, got %d", heads);
-  p.tokens_per_wg = fa2::serve_tokens_per_wg((int)std::min<int64_t>((int64_t)heads * (head_dim / 8), 256), (int64_t)batch * n, kRotaryWgs);
+  p.tokens_per_wg = fa2::serve_tokens_per_wg((int)std::min<int64_t>((int64_t)heads * (head_dim / 8), 256),
+                                             (int64_t)batch * n, kRotaryWgs);
   const int64_t grid = ((int64_t)batch * n + p.tokens_per_wg - 1) / p.tokens_per_wg;
   if (grid > 0x7fffffffLL) return fail(FA2_EINVAL, "grid of %lld workgroups is too large", (long long)grid);
   return launched(fa2::launch_rotary(dtype, head_dim, p, (unsigned)grid, static_cast<hipStream_t>(stream)), "rotary");

@@ -180,10 +180,11 @@ def attention_paged(q, cache, block_table, cu_seqlens, seqlens, *, causal=True, 
 
     block_table, cu_seqlens and seqlens as in cache_write, which has put the new tokens' own k and v there; one
     new token per sequence is a decoding step, a part of a prompt a chunk, and both may be in one call. q is of the
-    cache's type, or fp16 or bf16 with an e4m3 cache. causal: the sequence's last new token sees all of its tokens, the one before it
-    all but the last. A sequence of more tokens than its row of the table holds counts as one of as many. A row that sees no key gets 0, and a log-sum-exp of -inf; rows past the last sequence
-    are left as they are in out (undefined in a new one). A page outside the cache makes the
-    rows that see its tokens NaN, and may make other rows of its sequence NaN.
+    cache's type, or fp16 or bf16 with an e4m3 cache. causal: the sequence's last new token sees all of its tokens,
+    the one before it all but the last. A row that sees no key gets 0, and a log-sum-exp of -inf; rows past the last
+    sequence are left as they are in out (undefined in a new one). A sequence of more tokens than its row of the
+    table holds counts as one of as many. A page outside the cache makes the rows that see its tokens NaN, and may
+    make other rows of its sequence NaN.
     return_lse: also return the natural-log log-sum-exp of every row's scaled scores, fp32 [H_q, T].
     out: of q's shape and type, in any layout without shared elements; q itself is allowed.
     """
