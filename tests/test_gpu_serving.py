@@ -403,7 +403,7 @@ def check_paged_calls(steps, dtype, e4m3, D, page_size, h_q, h_kv):
 @pytest.mark.parametrize("e4m3", [False, True])
 @pytest.mark.parametrize("dtype,D,page_size", [(torch.bfloat16, 128, 32), (torch.float16, 64, 16), (torch.bfloat16, 32, 64),
                                                (torch.float16, 16, 128)])
-@pytest.mark.parametrize("new,lens", [([1, 1], [9000, 20]), ([300, 1, 1, 64], [5000, 3000, 1, 2100]), ([600], [4321]),
+@pytest.mark.parametrize("new,lens", [([1, 1], [9000, 20]), ([1], [30000]), ([3], [12345]), ([300, 1, 1, 64], [5000, 3000, 1, 2100]), ([600], [4321]),
                                       ([200, 0, 1, 700], [100, 50, 6000, 350]), ([30] * 66 + [400], [40] * 66 + [5000])])
 def test_paged_long(e4m3, dtype, D, page_size, new, lens):
     from fa2.paged import attention_paged
