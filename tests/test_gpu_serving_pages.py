@@ -1,0 +1,52 @@
+"""GPU tests of table entries that are no page of the cache, wherever they lie among the workgroups that share a sequence's
+keys.
+"""
+
+import pytest
+import torch
+
+from oracle import serving as oracle
+from serving_check import cumulative, make_cache, randn
+
+pytestmark = pytest.mark.gpu
+
+
+# (new tokens, tokens in the cache) of the sequences: steps of one token (32-row workgroups) and a chunk beside steps (128-row
+# ones), over keys that several workgroups share; and steps and chunks that nobody shares, as their table is narrow
+CALLS = {"shared steps": ([1, 1, 1], [4000, 2500, 3333]), "shared chunk": ([300, 1, 40], [3000, 2500, 2000]),
+         "steps": ([1, 1, 4], [1500, 700, 600]), "chunk": ([300, 1, 40], [1500, 700, 600])}
+
+
+def call_of(name, page_size, D, dtype, e4m3, h_q=8, h_kv=2, seed=0):
+    new, lens = CALLS[name]
+    pages = oracle.Pages(lens, page_size, seed=seed, device="cuda")
+    pages.table = pages.table[:, :-(-max(lens) // page_size)].contiguous()
+    cache = make_cache(pages.n_pages, h_kv, page_size, D, dtype, e4m3, seed)
+    q = randn((sum(new), h_q, D), dtype, 30 + seed)
+    return new, lens, pages, cache, q, cumulative(new), torch.tensor(lens, dtype=torch.int32, device="cuda")
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("D,page_size", [(128, 128), (64, 256), (32, 64), (128, 16)])
+@pytest.mark.parametrize("call", CALLS)
+def test_rows_that_see_an_entry_that_is_no_page_are_nan(call, D, page_size, e4m3):
+    """One such entry, at every place of a sequence's table in turn, and runs of them up to a whole row: the rows that see its
+    tokens are NaN, their log-sum-exp too, and the other sequences as they were. A page of 128 tokens of head_dim 128 is a
+    tile for each of the four waves that take tiles in turn, so that none of them has a sum to show for its keys."""
+    from fa2.paged import attention_paged
+    new, lens, pages, cache, q, cu, seqlens = call_of(call, page_size, D, torch.bfloat16, e4m3)
+    want, want_lse = attention_paged(q, cache, pages.table, cu, seqlens, return_lse=True)
+    assert want.isfinite().all() and want_lse.isfinite().all()
+    s, first = 0, cu.tolist()
+    need = -(-lens[s] // page_size)
+    runs = [(i, i + 1) for i in range(0, need, max(1, need // 24))] + [(need // 3, need), (0, need), (need // 4, need // 2)]
+    for a, b in runs:
+        table = pages.table.clone()
+        table[s, a:b] = -1
+        out, lse = attention_paged(q, cache, table, cu, seqlens, return_lse=True)
+        # row i of the sequence sees its tokens up to lens - new + i
+        sees = [first[s] + i for i in range(new[s]) if lens[s] - new[s] + i >= a * page_size]
+        assert out[sees].isnan().all() and lse[:, sees].isnan().all(), (a, b)
+        assert torch.equal(attention_paged(q, cache, table, cu, seqlens)[sees].isnan(), out[sees].isnan())
+        others = [t for t in range(q.shape[0]) if not first[s] <= t < first[s + 1]]
+        assert torch.equal(out[others], want[others]) and torch.equal(lse[:, others], want_lse[:, others]), (a, b)

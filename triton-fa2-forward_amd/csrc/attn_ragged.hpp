@@ -726,13 +726,17 @@ void attn_ragged_kernel(const RaggedParams) {
         const int x = t / QPR, q = t % QPR;
         if (odd[x]) continue;
         float m = -INFINITY, ls = 0.f, lxs = 0.f;
+        bool nan = false;  // a group's reference: a bad page
 #pragma unroll
-        for (int y = 0; y < KG; ++y) m = fmaxf(m, sm[y][x][0]);
+        for (int y = 0; y < KG; ++y) {
+          nan |= sm[y][x][0] != sm[y][x][0];
+          m = fmaxf(m, sm[y][x][0]);
+        }
         f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int y = 0; y < KG; ++y) {
           const float mw = sm[y][x][0];
-          const float w = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - m);  // NaN: a bad page
+          const float w = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - m);  // (NaN stays NaN)
           ls = __builtin_fmaf(w, sm[y][x][1], ls);
           lxs = __builtin_fmaf(w, sm[y][x][2], lxs);
           const f32x4 v = ob[piece(y, x, q)];
@@ -748,7 +752,8 @@ void attn_ragged_kernel(const RaggedParams) {
           for (int e = 0; e < 4; ++e) o[e] *= inv;
           *(u32x2*)(pe.o + at.token * pe.sot + at.head * pe.soh + 4 * q) = u32x2{E::pack2(o[0], o[1]), E::pack2(o[2], o[3])};
         }
-        if (q == 0) put_sums(x, m, ls, lxs);
+        // (fmaxf has dropped a NaN reference, and a piece whose groups all met bad pages would pass for one without keys)
+        if (q == 0) put_sums(x, nan ? __uint_as_float(0x7fc00000u) : m, ls, lxs);
       }
       for (int x = wave; x < row_end - row0; x += 4) {
         if (!odd[x]) continue;
