@@ -1,12 +1,12 @@
-"""GPU tests of table entries that are no page of the cache, wherever they lie among the workgroups that share a sequence's
-keys.
+"""GPU tests of what a paged cache may hold beside ordinary tokens: table entries that are no page, wherever they lie among the
+workgroups that share a sequence's keys, and infinite and NaN values in keys that rows see.
 """
 
 import pytest
 import torch
 
 from oracle import serving as oracle
-from serving_check import cumulative, make_cache, randn
+from serving_check import CACHES, bytes_of, cached, check_attention, cumulative, make_cache, randn
 
 pytestmark = pytest.mark.gpu
 
@@ -50,3 +50,43 @@ def test_rows_that_see_an_entry_that_is_no_page_are_nan(call, D, page_size, e4m3
         assert torch.equal(attention_paged(q, cache, table, cu, seqlens)[sees].isnan(), out[sees].isnan())
         others = [t for t in range(q.shape[0]) if not first[s] <= t < first[s + 1]]
         assert torch.equal(out[others], want[others]) and torch.equal(lse[:, others], want_lse[:, others]), (a, b)
+
+
+BAD = {"inf": float("inf"), "-inf": float("-inf"), "nan": float("nan")}
+
+
+@pytest.mark.parametrize("dtype,D,page_size", [(torch.float16, 64, 16), (torch.bfloat16, 128, 64), (torch.float16, 128, 16),
+                                               (torch.bfloat16, 16, 64), (torch.float16, 32, 128)])
+@pytest.mark.parametrize("cache_type", CACHES)
+@pytest.mark.parametrize("call", CALLS)
+def test_values_that_are_not_finite(call, cache_type, dtype, D, page_size):
+    """An infinite or NaN value or key of a cached token (e4m3: NaN, and a scale that is none) reaches the rows that see it, and
+    no other: at the first token, within a tile, at the last token that every row sees and at the last one, which only the
+    last row does."""
+    from fa2.paged import attention_paged
+    e4m3 = cache_type == "e4m3"
+    new, lens, pages, cache, q, cu, seqlens = call_of(call, page_size, D, dtype, e4m3)
+    q = torch.where(q == 0, torch.ones_like(q), q)
+    s = 0
+    for which in ("k", "v"):
+        for at in (0, lens[s] // 2 + 5, lens[s] - new[s], lens[s] - 1):
+            page, row = (x.item() for x in pages.at(s, torch.tensor(at, device="cuda")))
+            for name in (("nan", "scale") if e4m3 else BAD):
+                one = cache._replace(**{which: cache._asdict()[which].clone()})
+                if name == "scale":  # e8m0 has NaN too
+                    scale = getattr(cache, which + "_scale").view(torch.uint8).clone()
+                    scale[page, 1, row] = 255
+                    one = one._replace(**{which + "_scale": scale.view(torch.float8_e8m0fnu)})
+                else:
+                    bytes_of(getattr(one, which))[page, 1, row, D // 2] = 0x7f if e4m3 else BAD[name]
+                for causal in (True, False):
+                    out, lse = attention_paged(q, one, pages.table, cu, seqlens, causal=causal, return_lse=True)
+
+                    def values(part, n):
+                        x = cached(one, part, *pages.at(n, torch.arange(lens[n], device="cuda"))).to(dtype).double()
+                        if name == "scale" and part == which and n == s:
+                            x[at, 1] = float("nan")
+                        return x
+                    check_attention(out, lse, q, lambda n: values("k", n), lambda n: values("v", n), cu, causal, dtype)
+                    assert torch.equal(attention_paged(q, one, pages.table, cu, seqlens, causal=causal).nan_to_num(5.0),
+                                       out.nan_to_num(5.0))
