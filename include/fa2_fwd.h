@@ -327,7 +327,8 @@ FA2_API int fa2_cache_read(const fa2_cache* cache, const fa2_sequences* seq, voi
  * fa2_attn_packed - attention within each of n_seq packed sequences: q and out [n_tokens, h_q, head_dim], k
  * and v [kv_tokens, h_kv, head_dim], strides [token, head]. cu_kv gives the sequences of k and v (NULL: cu,
  * and kv_tokens == n_tokens). causal: aligned at the end, the sequence's last row sees its last key, row i
- * keys up to i + n_kv - n_q. A row that sees no key gets 0 and a log-sum-exp of -inf.
+ * keys up to i + n_kv - n_q. A row that sees no key gets 0 and a log-sum-exp of -inf; with kv_tokens 0, k and v
+ * are not looked at (and may be NULL).
  * lse: NULL, or float[h_q * n_tokens], natural logarithm, row h * n_tokens + t.
  */
 FA2_API int fa2_attn_packed(const void* q, const void* k, const void* v, void* out,

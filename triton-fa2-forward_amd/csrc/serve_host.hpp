@@ -336,19 +336,21 @@ int fa2_attn_packed(const void* q, const void* k, const void* v, void* out, cons
   if (const int rc = check_rows("q", q, q_stride, 2, 8)) return rc;
   if (const int rc = check_rows("out", out, o_stride, 2, 8)) return rc;
   if (const int rc = check_written("out", {{n_tokens, o_stride[0]}, {h_q, o_stride[1]}})) return rc;
-  if (const int rc = check_rows("k", k, k_stride, 2, 8)) return rc;
-  if (const int rc = check_rows("v", v, v_stride, 2, 8)) return rc;
-  if (k_stride[0] > kMaxRowStride || v_stride[0] > kMaxRowStride)
-    return fail(FA2_EINVAL, "a k/v row stride above %lld elements is not supported", (long long)kMaxRowStride);
+  if (kv_tokens > 0) {  // (tensors of no rows may have no memory, and nothing of them is read)
+    if (const int rc = check_rows("k", k, k_stride, 2, 8)) return rc;
+    if (const int rc = check_rows("v", v, v_stride, 2, 8)) return rc;
+    if (k_stride[0] > kMaxRowStride || v_stride[0] > kMaxRowStride)
+      return fail(FA2_EINVAL, "a k/v row stride above %lld elements is not supported", (long long)kMaxRowStride);
+    p.kc.data = static_cast<char*>(const_cast<void*>(k));
+    p.kc.token = k_stride[0]; p.kc.head = k_stride[1];
+    p.vc.data = static_cast<char*>(const_cast<void*>(v));
+    p.vc.token = v_stride[0]; p.vc.head = v_stride[1];
+  }
   p.q = static_cast<const uint16_t*>(q);
   p.o = static_cast<uint16_t*>(out);
   p.lse = lse;
   p.sqt = q_stride[0]; p.sqh = q_stride[1];
   p.sot = o_stride[0]; p.soh = o_stride[1];
-  p.kc.data = static_cast<char*>(const_cast<void*>(k));
-  p.kc.token = k_stride[0]; p.kc.head = k_stride[1];
-  p.vc.data = static_cast<char*>(const_cast<void*>(v));
-  p.vc.token = v_stride[0]; p.vc.head = v_stride[1];
   p.seq.cu = cu;
   p.seq.n_seq = n_seq;
   p.seq.n_tokens = n_tokens;
