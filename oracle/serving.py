@@ -53,7 +53,7 @@ def attention(q, k, v, causal, sm_scale=None):
     n, h_q, D = q.shape
     m, h_kv = k.shape[:2]
     sm_scale = D ** -0.5 if sm_scale is None else sm_scale
-    out, size = torch.zeros(n, h_q, D, dtype=torch.float64, device=q.device), None
+    out = torch.zeros(n, h_q, D, dtype=torch.float64, device=q.device)
     size = torch.zeros_like(out)
     lse = torch.full((h_q, n), -math.inf, dtype=torch.float64, device=q.device)
     big = torch.zeros(n, h_q, 1, dtype=torch.float64, device=q.device)
@@ -80,22 +80,6 @@ def attention(q, k, v, causal, sm_scale=None):
         lse[heads] = torch.where(any_, torch.logsumexp(s, 1), -math.inf).view(n, group).t()
         score = (qh.abs() @ kt.abs()).masked_fill(~sees, 0.0).nan_to_num(0, 0, 0).amax(1) * sm_scale
         big[:, heads, 0] = score.view(n, group)
-    return out, lse, size, big
-    see = torch.ones(n, m, dtype=torch.bool, device=q.device)
-    if causal:
-        see = torch.arange(m, device=q.device) <= torch.arange(n, device=q.device)[:, None] + (m - n)
-    some = see.any(1)
-    for h in range(h_q):
-        qh, kh, vh = q[:, h].double(), k[:, h // (h_q // h_kv)].double(), v[:, h // (h_q // h_kv)].double()
-        s = (qh @ kh.t().contiguous() * sm_scale).masked_fill(~see, -math.inf)
-        w = torch.softmax(s[some], 1)
-        fine = vh.isfinite().all(1)
-        out[some, h] = torch.where(see[some], w, 0.0)[:, fine] @ vh[fine]
-        for j in (~fine).nonzero()[:, 0].tolist():  # infinite and NaN values: only where they are seen
-            out[some, h] += torch.where(see[some, j, None], w[:, j, None] * vh[j], 0.0)
-        size[some, h] = torch.where(see[some], w, 0.0)[:, fine] @ vh[fine].abs()
-        lse[h, some] = torch.logsumexp(s[some], 1)
-        big[:, h, 0] = (qh.abs() @ kh.abs().t().contiguous()).masked_fill(~see, 0.0).nan_to_num(0, 0, 0).amax(1) * sm_scale
     return out, lse, size, big
 
 
