@@ -222,6 +222,13 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
+def _int32(**sizes):
+    """Sizes as the C ABI takes them: a larger one would lose its upper bits on the way there."""
+    for name, n in sizes.items():
+        if not 0 <= n < 1 << 31:
+            raise ValueError(f"{name} must be below 2^31, got {n}")
+
+
 def _checked(rc, name):
     if rc != 0:
         raise RuntimeError(f"{name} failed ({rc}): {last_error()}")
@@ -230,6 +237,7 @@ def _checked(rc, name):
 def cache_of(cache):
     """The C description of a fa2.paged.KVCache that satisfies its checks."""
     pages, h_kv, page_size, head_dim = cache.k.shape
+    _int32(pages=pages, H_kv=h_kv, page_size=page_size)
 
     def strides(t):
         return _i64x3(*([0] * 3 if t is None else (0 if n == 1 else s for n, s in zip(t.shape[:3], t.stride()))))
@@ -241,6 +249,7 @@ def cache_of(cache):
 
 def sequences_of(cu, lens, table, n_tokens):
     """The C description of sequences over a cache (dense int32 tensors; table rows any distance apart)."""
+    _int32(sequences=lens.numel(), tokens=n_tokens, table_columns=table.shape[1])
     return Sequences(_ptr(cu), _ptr(lens), _ptr(table), 0 if table.shape[0] == 1 else table.stride(0),
                      lens.numel(), n_tokens, table.shape[1])
 
@@ -248,6 +257,7 @@ def sequences_of(cu, lens, table, n_tokens):
 def rotary(x, out, positions, rotation, stream):
     """Call fa2_rotary on [B, H, N, D] tensors and positions [B, N]."""
     B, H, N, D = x.shape
+    _int32(B=B, H=H, N=N)
     _checked(lib().fa2_rotary(x.data_ptr(), out.data_ptr(), _strides(x), _strides(out), positions.data_ptr(),
                               positions.element_size(), (ctypes.c_int64 * 2)(*positions.stride()),
                               ctypes.byref(rotation), B, H, N, D, DTYPE_CODE[x.dtype], stream), "fa2_rotary")
@@ -255,6 +265,7 @@ def rotary(x, out, positions, rotation, stream):
 
 def cache_write(cache, seq, k, v, q, q_out, rotation, stream):
     """Call fa2_cache_write; q, q_out and rotation may be None."""
+    _int32(H_q=0 if q is None else q.shape[1])
     _checked(lib().fa2_cache_write(
         ctypes.byref(cache), ctypes.byref(seq), k.data_ptr(), v.data_ptr(), _strides(k), _strides(v), _ptr(q),
         _ptr(q_out), None if q is None else _strides(q), None if q is None else _strides(q_out),
@@ -271,6 +282,7 @@ def cache_read(cache, seq, k, v, stream):
 def attn_packed(q, k, v, out, cu, cu_kv, causal, qk_scale, lse, stream):
     """Call fa2_attn_packed; cu_kv and lse may be None."""
     T, H_q, D = q.shape
+    _int32(T=T, H_q=H_q, T_kv=k.shape[0], H_kv=k.shape[1], sequences=cu.numel() - 1)
     _checked(lib().fa2_attn_packed(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _strides(q), _strides(k), _strides(v),
         _strides(out), cu.data_ptr(), _ptr(cu_kv), cu.numel() - 1, T, k.shape[0], H_q, k.shape[1], D,
@@ -284,6 +296,7 @@ def paged_workspace_bytes(H_q, H_kv, D, cache_dtype, n_tokens, n_seq, max_keys, 
 
 def attn_paged(q, out, cache, seq, causal, qk_scale, lse, workspace, stream):
     """Call fa2_attn_paged; lse and workspace (uint8) may be None."""
+    _int32(H_q=q.shape[1])
     _checked(lib().fa2_attn_paged(q.data_ptr(), out.data_ptr(), _strides(q), _strides(out), ctypes.byref(cache),
                                   ctypes.byref(seq), q.shape[1], DTYPE_CODE[q.dtype], int(bool(causal)), qk_scale,
                                   _ptr(lse), _ptr(workspace), 0 if workspace is None else workspace.numel(), stream),
