@@ -96,15 +96,24 @@ _KERNELS = {
         r"^_ZN3fa222attn_wave_split_kernelILi(\d)ELi(\d+)ELi(\d)ELi(\d+)ELb([01])ELi(\d+)EEEv"),
     "attn_wide_kernel": re.compile(r"^_ZN3fa216attn_wide_kernelILi(\d)ELi(\d+)ELb([01])EEEv"),
 }
+# ... and the serving kernels', with their names there
+_SERVING_KERNELS = {
+    "attn_ragged_kernel": (re.compile(r"attn_ragged_kernelILi(\d)ELi(\d+)ELi(\d)ELi(\d)ELb([01])EEEv"),
+                           ("source", "row_waves", "lse")),
+    "attn_ragged_combine_kernel": (re.compile(r"attn_ragged_combine_kernelILi(\d)ELi(\d+)ELi(\d)EEEv"), ("row_waves",)),
+    "rotary_kernel": (re.compile(r"rotary_kernelILi(\d)ELi(\d+)EEEv"), ()),
+    "cache_write_kernel": (re.compile(r"cache_write_kernelILi(\d)ELi(\d+)ELb([01])EEEv"), ("e4m3",)),
+    "cache_read_kernel": (re.compile(r"cache_read_kernelILi(\d)ELi(\d+)ELb([01])EEEv"), ("e4m3",)),
+}
 
 
-def parse_resources(stderr):
-    """kernel-resource-usage remarks -> {mangled name: {field: int}} for the attention kernels."""
+def parse_resources(stderr, known=lambda name: any(k.match(name) for k in _KERNELS.values())):
+    """kernel-resource-usage remarks -> {mangled name: {field: int}} for the attention kernels (or the `known` ones)."""
     out, cur = {}, None
     for m in _REMARK.finditer(stderr):
         key, val = m.group(1), m.group(2)
         if key == "Function Name":
-            cur = out.setdefault(val, {}) if any(k.match(val) for k in _KERNELS.values()) else None
+            cur = out.setdefault(val, {}) if known(val) else None
         elif cur is not None:
             cur[_FIELDS[key]] = int(val)
     return out
@@ -123,6 +132,15 @@ def describe_instance(name):
         waves, rows = (nw, 32 * nw) if kernel == "attn_fwd_kernel" else (4, 32 * nw)
     return {"kernel": kernel, "dtype": ("fp16", "bf16")[dt], "head_dim": d, "waves": waves, "block_m": rows,
             "block_n": bn, "causal": bool(causal), "variant": variant}
+
+
+def describe_serving(name):
+    """The template arguments of a serving kernel's mangled name (None: another kernel)."""
+    for kernel, (pattern, fields) in _SERVING_KERNELS.items():
+        if m := pattern.search(name):
+            dt, d, *rest = (int(x) for x in m.groups())
+            return {"kernel": kernel, "dtype": ("fp16", "bf16")[dt], "head_dim": d, **dict(zip(fields, rest))}
+    return None
 
 
 VARIANTS_DIR = os.path.join(PKG, "variants")
@@ -174,13 +192,13 @@ def build(jobs=8, verbose=False):
                           f"-DFA2_DT={dt}", f"-DFA2_D={d}", "-c",
                           os.path.join(CSRC, "attn_fwd_inst.hip"), "-o", obj])
             obj = os.path.join(OBJ_DIR, f"attn_ragged_dt{dt}_d{d}.o")
-            serve_units.append([cc, *common_flags(), f"-DFA2_DT={dt}", f"-DFA2_D={d}", "-c",
-                                os.path.join(CSRC, "attn_ragged_inst.hip"), "-o", obj])
+            serve_units.append([cc, *common_flags(), "-Rpass-analysis=kernel-resource-usage", f"-DFA2_DT={dt}",
+                                f"-DFA2_D={d}", "-c", os.path.join(CSRC, "attn_ragged_inst.hip"), "-o", obj])
             obj = os.path.join(OBJ_DIR, f"attn_fwd_ablate_dt{dt}_d{d}.o")
             ablate_units.append([cc, *common_flags(), f"-DFA2_DT={dt}", f"-DFA2_D={d}", "-c",
                                  os.path.join(CSRC, "attn_fwd_ablate_inst.hip"), "-o", obj])
-    serve_units.append([cc, *common_flags(), "-c", os.path.join(CSRC, "serve_cache.hip"),
-                        "-o", os.path.join(OBJ_DIR, "serve_cache.o")])
+    serve_units.append([cc, *common_flags(), "-Rpass-analysis=kernel-resource-usage", "-c",
+                        os.path.join(CSRC, "serve_cache.hip"), "-o", os.path.join(OBJ_DIR, "serve_cache.o")])
     shared = []
     for name in ("attn_fwd_wavesplit", "attn_fwd_combine", "attn_key_norm"):
         remarks = ["-Rpass-analysis=kernel-resource-usage"] if name == "attn_fwd_wavesplit" else []
@@ -210,9 +228,14 @@ def build(jobs=8, verbose=False):
     for err in errs[:len(units) + 1]:  # ... and the wave-split unit, the first shared one
         for name, fields in parse_resources(err).items():
             resources[name] = {**describe_instance(name), **fields}
+    serving = {}
+    for cmd, err in zip(everything, errs):
+        if cmd in serve_units:
+            for name, fields in parse_resources(err, describe_serving).items():
+                serving[name] = {**describe_serving(name), **fields}
     with open(RESOURCES_PATH + ".tmp", "w") as f:
         json.dump({"arch": ARCH, "source": "hipcc -Rpass-analysis=kernel-resource-usage",
-                   "kernels": dict(sorted(resources.items()))}, f, indent=1)
+                   "kernels": dict(sorted(resources.items())), "serving": dict(sorted(serving.items()))}, f, indent=1)
     os.replace(RESOURCES_PATH + ".tmp", RESOURCES_PATH)
 
     def link(objs, path):
