@@ -22,11 +22,12 @@
 // What bounds it, and what it measured on MI355X (kernel alone, its merge apart):
 //   * prompts: the instructions of a tile, one wave's products beside another's softmax. 8 packed sequences of up to 2048,
 //     32 / 8 heads of 128, bf16 causal: 114 us, 850 TFLOP/s, matrix cores 40% busy, 7.5 vector instructions a
-//     product; 4 of up to 8192, 16 heads of 64, fp16, with the log-sum-exp: 229 us, 800 TFLOP/s, 12.9.
-//   * chunks: the same, at 2 workgroups a CU by their registers. 2 e4m3 chunks of up to 2048 behind 12k and 32k: 950 to 990
-//     TFLOP/s. One of 500 beside 24 steps of up to 8k: 88 us and 12 of merge.
-//   * steps: reading K and V. 16 of up to 4095 tokens, 32 / 8 heads of 128, bf16, pages of 16: 27.5 us, 4.8 TB/s, and 4.5 of
-//     merge; 64 of up to 16000, e4m3: 200 us, 5.3 TB/s.
+//     product; 4 of up to 8192, 16 heads of 64, fp16, with the log-sum-exp: 232 us, 790 TFLOP/s, 12.9.
+//   * chunks: the same, at 2 workgroups a CU by their registers, which e4m3 at head_dim 128 does not get by with (18 or 19
+//     spilled, 7 of them with 32 rows). 2 e4m3 chunks of up to 2048 behind 12k and 32k: 1218 us, 930 TFLOP/s, and 17 of merge.
+//     One of 500 beside 24 steps of up to 8k: 88 us and 12 of merge.
+//   * steps: reading K and V. 16 of up to 4095 tokens, 32 / 8 heads of 128, bf16, pages of 16: 28 us, 4.7 TB/s, and 4.5 of
+//     merge; 64 of up to 16000, e4m3: 198 us, 5.3 TB/s.
 // Tried and dropped: writing e4m3's converted pairs in an order without bank conflicts (10% of the cycles have one; the
 // selects cost more: 1060 -> 1105 us); sequences of few rows as a line of shares apart (114 -> 122 us), and weighted
 // 1/2 or 2 in the one line (121 -> 140, 125).
@@ -330,7 +331,10 @@ void attn_ragged_kernel(const RaggedParams) {
       }
     };
 
-    // ---- the online softmax of one tile, base 2, with a lazily moved reference (attn_fwd_wavesplit.hpp)
+    // ---- the online softmax of one tile, base 2, with a lazily moved reference (attn_fwd_wavesplit.hpp). The weights are
+    // rounded to the 16-bit type, as the matrix instruction takes them, and the sum that the row is divided by is of the
+    // rounded ones, so that a row's weights still add up to one; the log-sum-exp is of the sum in float. Against weights in float
+    // the error of a row grows by 1.1 to 1.4 times (it is rounded to the same type at the end).
     float m_i = -INFINITY, l_i = 0.f, l_exact = 0.f;
     f32x16 acc[DB];
 #pragma unroll

@@ -8,8 +8,8 @@
 //     Up to 8 sequences' tiles go by their index in their sequence, highest first: causal tiles of high index see the most
 //     keys, so the longest start first. More sequences go one after the other, each from its highest tile down: its tiles
 //     share its K and V in an L2, and the search is shorter. Measured on MI355X, by index and by sequence: 4 of up to
-//     8192, 16 heads of 64, 293 and 331 us; 8 of up to 2048, 32 / 8 heads of 128, 149 and 150; 16 of 512 82 and 65; 64 of
-//     128 75 and 42, of 1024 937 and 766.
+//     8192, 16 heads of 64 with the log-sum-exp, 231 and 256 us; 8 of up to 2048, 32 / 8 heads of 128, 116 and 115 to 119;
+//     16 of 512 78 and 65; 64 of 128 77 and 46, of 1024 1012 and 689.
 //   * `shares` workgroups per head, each an equal share of the head's tiles laid end to end, a tile's length being
 //     its keys (an estimate, linear in the tile's index, so that a sequence's sum is a closed form; it only
 //     decides where the cuts lie). A share starts and ends inside tiles: a tile cut by a share's end leaves

@@ -12,10 +12,13 @@
 // is that of the row's finite values), and at the largest exponent of the row's type the largest
 // magnitude is 240 instead of 448, so that no stored value is past the type's own range.
 //
-// All of it is bound by HBM, and small calls by the chain of lookups (sequence, length, page), which a group of
-// tokens makes together: 16 bytes per lane and load, a row's D / 8 lanes side by side. Measured on MI355X (kernel alone):
-// rotary of 16384 x 32 heads of 128 41 us, 6.5 TB/s, of 16 tokens 4.1; a write of 5096 tokens of 28 + 2 x 4 heads of 64 with
-// their rotation 16.4 us, 2.9 TB/s, of 64 tokens into e4m3 6.2; a read of 57071 tokens of 2 x 8 e4m3 heads of 128 71 us, 5 TB/s.
+// Rotating and reading are bound by HBM, and small calls by the chain of lookups (sequence, length, page), which a group of
+// tokens makes together: 16 bytes per lane and load, a row's D / 8 lanes side by side. Writes wait for that chain and the
+// angles with few waves in flight, and for a last pass over the rows that may hold few of them (4 tokens of 36 rows: 128 and
+// 16). Measured on MI355X (kernel alone): rotary of 16384 x 32 heads of 128 40 us, 6.7 TB/s, of 16 tokens 3.8; a write of 5096
+// tokens of 28 + 2 x 4 heads of 64 with their rotation 16 us, 3.0 TB/s (1.5 waves a SIMD on average), of 64 tokens into
+// e4m3 5.9, of 16000 tokens of 2 x 8 heads of 128 into e4m3 52 us, 1.9 TB/s (2.7 waves a SIMD; LDS busy 15% of the cycles, bank
+// conflicts of the float64 angles 8%); a read of 57071 tokens of 2 x 8 e4m3 heads of 128 71 us, 5 TB/s.
 #include <hip/hip_runtime.h>
 
 #include <type_traits>

@@ -121,9 +121,9 @@ int launched(int e, const char* what) {
 }
 
 // Workgroups that the tokens of a call are gathered into at least, as a group of tokens shares the lookup of their places
-// (three loads in a row). Measured on MI355X: a write of 5096 tokens of 28 + 2 x 4 heads of 64 in 5096, 2548 and
-// 1274 workgroups 18.8, 16.3 and 14.7 us; a read of 57071 tokens of 2 x 8 e4m3 heads of 128 in 57071, 7134 and
-// 3567 110, 69 and 76 us. The rotary kernel has no such lookup, and takes as few tokens as fill its lanes.
+// (three loads in a row). Measured on MI355X (kernel alone): a write of 5096 tokens of 28 + 2 x 4 heads of 64 in 5096, 2548 and
+// 1274 workgroups 20.0, 16.8 and 16.4 us; a read of 57071 tokens of 2 x 8 e4m3 heads of 128 in 57071, 7134 and
+// 3567 112, 73 and 81 us. The rotary kernel has no such lookup, and takes as few tokens as fill its lanes.
 constexpr int64_t kWriteWgs = 1024, kReadWgs = 4096, kRotaryWgs = int64_t(1) << 40;
 unsigned cache_grid(fa2::CacheParams* p, int64_t rows_per_token, int32_t head_dim, int64_t least_wgs) {
   p->tokens_per_wg = fa2::serve_tokens_per_wg((int)std::min<int64_t>(rows_per_token * (head_dim / 8), 256),

@@ -5,12 +5,16 @@ bench/profile_target.py).
     python triton-fa2-forward_amd/profile_target.py --config C3 --launches 3 --copy-mib 1024
     python triton-fa2-forward_amd/profile_target.py --pack-short 1 --launches 20
     python triton-fa2-forward_amd/profile_target.py --shape X:16:32:8:1:4096:128:0:fp16 --launches 200
+    python triton-fa2-forward_amd/profile_target.py --operators paged-step-4k,packed-short --launches 6
 
 --pack-short N_Q runs the reference's few-queries shape instead (bench.py --pack-short: fp16,
 B 16, H 32/8, N_kv 4096, D 128, non-causal, default path: packed, automatic split-KV).
 
 --shape X:B:Hq:Hkv:Nq:Nkv:D:causal:dtype[:lse] runs any other call of attention() on N(0, 1) inputs,
 with the log-sum-exp where it ends in lse.
+
+--operators NAME,... (or all) runs the serving operators' measured cases of these names (perf/operators.py), one after the
+other.
 
 --lib PATH runs another build of the product library (csrc/build.py --variant) through the same
 call attention() makes (ab.py's), for the counters of an A/B.
@@ -29,6 +33,24 @@ sys.path.insert(0, HERE)
 sys.path.insert(0, os.path.dirname(HERE))
 
 
+def run_operators(names, launches):
+    import torch
+
+    import perf.operators as operators
+
+    operators.own = True
+    cases = [c for c in operators.listed() if names is None or c["name"] in names]
+    if len(cases) != len(names or cases):
+        raise SystemExit(f"profile_target: no such case among {names}")
+    for case in cases:
+        print(f"profile_target: {case['name']}, {launches} launches", flush=True)
+        state = operators.prepare(case, 1)
+        for _ in range(launches):
+            operators.run(state)
+        torch.cuda.synchronize()
+    print("profile_target: done", flush=True)
+
+
 def main():
     ap = argparse.ArgumentParser()
     ap.add_argument("--config", default="C3")
@@ -38,10 +60,14 @@ def main():
     ap.add_argument("--block-n", type=int, default=None)
     ap.add_argument("--pack-short", type=int, default=None, metavar="N_Q")
     ap.add_argument("--shape", default=None, help="X:B:Hq:Hkv:Nq:Nkv:D:causal:dtype[:lse]")
+    ap.add_argument("--operators", default=None, metavar="NAME,...", help="cases of perf/operators.py, or all")
     ap.add_argument("--lib", default=None, help="another build of libfa2_fwd.so (ab.py's call)")
     args = ap.parse_args()
 
     import torch
+
+    if args.operators:
+        return run_operators(None if args.operators == "all" else args.operators.split(","), args.launches)
 
     import bench
     from fa2.kernel import attention
