@@ -235,13 +235,14 @@ FA2_API int fa2_should_pack_gqa(int32_t n_q, int32_t group, int32_t block_m);
  * reference (its README.md:308-315 lists variable lengths and decoding as out of scope).
  *
  * Rows of several sequences lie back to back: sequence s owns rows cu[s] .. cu[s + 1] - 1 of a packed
- * tensor [n_tokens, heads, head_dim] (cu: int32, n_seq + 1 ascending entries on the device; rows past
- * cu[n_seq] belong to none and are left as they are). Lengths, page tables and positions are read on the
- * device by the launch itself: nothing is copied to the host, a captured launch follows what they hold at
- * each replay, and no value of theirs makes a launch read or write outside the tensors.
+ * tensor [n_tokens, heads, head_dim] (cu: int32, n_seq + 1 ascending entries on the device; rows before
+ * cu[0] and from cu[n_seq] on belong to none and are left as they are). Lengths, page tables and positions
+ * are read on the device by the launch itself: nothing is copied to the host, a captured launch follows what
+ * they hold at each replay, and no value of theirs makes a launch read or write outside the tensors.
  * Strides are element strides with a unit head_dim stride; 16-bit pointers are 16-byte aligned and their
  * strides non-negative multiples of 8 elements, K and V rows at most 2^22 elements apart. What a call writes
- * has no stride of 0 over more than one row; out of attention and rotary may be q and x.
+ * has no stride of 0 over more than one row and overlaps nothing that the call reads, but out of attention
+ * and rotary may be q and x, and q_out q.
  */
 
 /* Element type of a cache that holds e4m3 (OCP, no infinities), with a scale byte per row. */
@@ -251,8 +252,9 @@ FA2_API int fa2_should_pack_gqa(int32_t n_q, int32_t group, int32_t block_m);
  * A paged cache: k and v [n_pages, h_kv, page_size, head_dim], strides [page, head, token]. cache_dtype is
  * FA2_DTYPE_F16, FA2_DTYPE_BF16 or FA2_DTYPE_E4M3; with e4m3, strides are multiples of 16 bytes and
  * k_scale and v_scale [n_pages, h_kv, page_size] hold a byte e per row, whose values are e4m3 * 2^(e - 127)
- * (e8m0). page_size is a power of two of at least 16, and a page holds at least 1 KiB of each head's
- * rows (so head_dim 16 takes pages of 32 tokens, or 64 in e4m3, and head_dim 32 pages of 32 in e4m3).
+ * (e8m0). page_size is a power of two from 16 to 2^20, and a page holds at least 1 KiB of each head's
+ * rows (so head_dim 16 takes pages of 32 tokens, or 64 in e4m3, and head_dim 32 pages of 32 in e4m3); a page
+ * extends over less than 2^31 bytes and lies less than that from the next.
  */
 typedef struct fa2_cache {
   void* k;
@@ -268,7 +270,7 @@ typedef struct fa2_cache {
  * Sequences over a paged cache, all device pointers: lens[s] tokens of sequence s are in the cache, the
  * sequence's packed rows being the last of them; token p lies in page table[s * table_stride + p / page_size]
  * at row p % page_size. max_pages: entries per row of the table (attention takes a sequence of more tokens than
- * they hold as one of max_pages * page_size).
+ * they hold as one of max_pages * page_size, which is at most 2^31 - 2049).
  */
 typedef struct fa2_sequences {
   const int32_t* cu;

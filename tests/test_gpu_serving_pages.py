@@ -1,5 +1,5 @@
 """GPU tests of what a paged cache may hold beside ordinary tokens: table entries that are no page, wherever they lie among the
-workgroups that share a sequence's keys, and infinite and NaN values in keys that rows see.
+workgroups that share a sequence's keys, and infinite and NaN values in keys that rows see; and of rows that belong to no sequence.
 """
 
 import pytest
@@ -90,3 +90,48 @@ def test_values_that_are_not_finite(call, cache_type, dtype, D, page_size):
                     check_attention(out, lse, q, lambda n: values("k", n), lambda n: values("v", n), cu, causal, dtype)
                     assert torch.equal(attention_paged(q, one, pages.table, cu, seqlens, causal=causal).nan_to_num(5.0),
                                        out.nan_to_num(5.0))
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("n_seq,group", [(5, 40), (64, 2), (65, 1), (200, 3)])
+def test_rows_of_no_sequence(n_seq, group, e4m3):
+    """Rows before the first sequence and behind the last, and rows before their sequence's start, stay as they are in every
+    operator's output; sequences without rows lie between the others, more than 64 of them side by side among 200."""
+    from fa2.packed import attention_packed
+    from fa2.paged import attention_paged, cache_read, cache_write
+    from fa2.rotary import rotary, rotary_plan
+    D, page_size, h_kv, dtype, first = 64, 32, 2, torch.bfloat16, 37
+    new = [3 + s % 5 if s in (1, 2, n_seq // 2, n_seq - 1) else 0 for s in range(n_seq)]
+    lens = [n - 2 if s == 2 else n + 11 * (s % 7) for s, n in enumerate(new)]  # sequence 2: two rows before its start
+    pages = oracle.Pages(lens, page_size, device="cuda")
+    cache = make_cache(pages.n_pages, h_kv, page_size, D, dtype, e4m3)
+    cu, seqlens = cumulative(new) + first, torch.tensor(lens, dtype=torch.int32, device="cuda")
+    at, T = cu.tolist(), first + sum(new) + 9
+    q, k, v = (randn((T, h, D), dtype, i) for i, h in enumerate((h_kv * group, h_kv, h_kv)))
+    position = torch.full((T,), -1, device="cuda")
+    for s, n in enumerate(new):
+        position[at[s]:at[s + 1]] = torch.arange(lens[s] - n, lens[s], device="cuda")
+    placed = position >= 0
+    plan = rotary_plan(D)
+    q_out, k_out, v_out, out = (torch.full_like(t, 7.0) for t in (q, k, v, q))
+    cache_write(cache, k, v, pages.table, cu, seqlens, rotary=plan, q=q, q_out=q_out)
+    cache_read(cache, pages.table, cu, seqlens, T, out=(k_out, v_out))
+    assert torch.equal(q_out[placed], rotary(q, position, plan)[placed])
+    if not e4m3:
+        assert torch.equal(k_out[placed], rotary(k, position, plan)[placed]) and torch.equal(v_out[placed], v[placed])
+    for t in (q_out, k_out, v_out):
+        assert (t[~placed] == 7.0).all()
+
+    def rows_of_none(t):
+        return torch.cat([t[:first], t[at[-1]:]])
+    for causal in (True, False):
+        _, lse = attention_paged(q, cache, pages.table, cu, seqlens, causal=causal, return_lse=True, out=out.fill_(7.0))
+        assert (rows_of_none(out) == 7.0).all()
+
+        def of(which):
+            return lambda s: cached(cache, which, *pages.at(s, torch.arange(lens[s], device="cuda"))).to(dtype).double()
+        check_attention(out, lse, q, of("k"), of("v"), cu, causal, dtype)
+        _, lse = attention_packed(q, k, v, cu, causal=causal, return_lse=True, out=out.fill_(7.0))
+        assert (rows_of_none(out) == 7.0).all()
+        check_attention(out, lse, q, lambda s: k[at[s]:at[s + 1]].double(), lambda s: v[at[s]:at[s + 1]].double(), cu, causal,
+                        dtype)

@@ -58,12 +58,13 @@ def attention_packed(q, k, v, cu_seqlens, cu_seqlens_kv=None, *, causal=True, sm
     q: [T, H_q, D]; k, v: [T_kv, H_kv, D], fp16 or bf16, D in (16, 32, 64, 128), H_q % H_kv == 0; returns out
     [T, H_q, D], laid out like q.
     cu_seqlens: int32 [S + 1] on the GPU, ascending: sequence s owns rows cu_seqlens[s] .. cu_seqlens[s + 1] - 1 of
-        q, and of k and v unless cu_seqlens_kv gives theirs. Rows past the last sequence are left as they
-        are in out (undefined in a new one).
+        q, and of k and v unless cu_seqlens_kv gives theirs. Rows of no sequence are left as they are in
+        out (undefined in a new one).
     causal: row i of a sequence sees its keys up to i + n_kv - n_q (with one cu_seqlens: up to its own).
         A row that sees no key gets 0, and a log-sum-exp of -inf.
     return_lse: also return the natural-log log-sum-exp of every row's scaled scores, fp32 [H_q, T].
-    out: of q's shape and type, in any layout without shared elements; q itself is allowed.
+    out: of q's shape and type, in any layout without shared elements; q itself is allowed, and no other memory that
+        the call reads.
     """
     if _lib.native is not None:  # the common call, made natively; None: not one of those
         result = _lib.native.attn_packed(q, k, v, cu_seqlens, cu_seqlens_kv, causal, sm_scale, return_lse, out)

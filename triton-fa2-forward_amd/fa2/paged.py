@@ -26,8 +26,8 @@ _16BIT = (torch.float16, torch.bfloat16)
 class KVCache(NamedTuple):
     """k, v: [pages, H_kv, page_size, D], fp16, bf16 or float8_e4m3fn, any strides with a unit one for D (a
     [pages, page_size, H_kv, D] storage by transpose(1, 2)); k_scale, v_scale: float8_e8m0fnu
-    [pages, H_kv, page_size] with e4m3, else None. page_size: a power of two of at least 16, and at least 1 KiB
-    of a head's rows."""
+    [pages, H_kv, page_size] with e4m3, else None. page_size: a power of two from 16 to 2^20, and at least 1 KiB
+    of a head's rows. A page extends over less than 2^31 bytes, and lies less than that from the next."""
     k: torch.Tensor
     v: torch.Tensor
     k_scale: Optional[torch.Tensor] = None
@@ -104,8 +104,9 @@ def cache_write(cache, k, v, block_table, cu_seqlens, seqlens, *, rotary=None, q
         into q_out (a new tensor; q_out=q rotates in place), which is returned.
     An e4m3 cache rounds each token and head once, against its own power-of-two scale (the least that holds its
     largest finite value); what is not finite becomes NaN.
-    Not written: tokens past the table or in a page outside the cache, and rows past the last
-    sequence. Two tokens in one place are the caller's to avoid.
+    Not written: tokens past the table or in a page outside the cache, rows of no sequence, and rows before their
+    sequence's start (where it has more rows than tokens in the cache); q_out is left as it is at the last two (undefined
+    in a new one). Two tokens in one place are the caller's to avoid.
     """
     if _lib.native is not None:  # the common call, made natively; None: not one of those
         result = _lib.native.cache_write(*cache, block_table, cu_seqlens, seqlens, k, v,
@@ -144,8 +145,8 @@ def cache_read(cache, block_table, cu_seqlens, seqlens, n_tokens, *, dtype=None,
     Takes the tokens that cache_write would write for the same block_table, cu_seqlens and seqlens; whole
     sequences with cu_seqlens the running sum of seqlens. n_tokens: rows of the result (cu_seqlens[-1], which is not
     copied to the host to find out). dtype: fp16 or bf16, for an e4m3 cache (a 16-bit one gives its own).
-    Tokens past the table or in a page outside the cache read as zeros; rows past the last sequence are
-    left as they are in out=(k, v) (undefined in new ones).
+    Tokens past the table or in a page outside the cache read as zeros; rows of no sequence or before their
+    sequence's start are left as they are in out=(k, v) (undefined in new ones).
     """
     if dtype is None:
         assert cache.k.dtype in _16BIT or out is not None, "an e4m3 cache needs the dtype to read it as"
@@ -186,7 +187,8 @@ def attention_paged(q, cache, block_table, cu_seqlens, seqlens, *, causal=True, 
     table holds counts as one of as many. A page outside the cache makes the rows that see its tokens NaN, and may
     make other rows of its sequence NaN.
     return_lse: also return the natural-log log-sum-exp of every row's scaled scores, fp32 [H_q, T].
-    out: of q's shape and type, in any layout without shared elements; q itself is allowed.
+    out: of q's shape and type, in any layout without shared elements; q itself is allowed, and no other memory that
+        the call reads.
     """
     if _lib.native is not None:  # the common call, made natively; None: not one of those
         result = _lib.native.attn_paged(*cache, block_table, cu_seqlens, seqlens, q, causal, sm_scale, return_lse, out)
