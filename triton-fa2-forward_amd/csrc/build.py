@@ -25,7 +25,8 @@ FA2_TAIL_PRIVATE_PCT. It never replaces the product library.
 Both libraries are built with hidden visibility, so each exports exactly the functions its
 header declares (FA2_API). The compiler's resource report for every kernel instance (VGPRs,
 AGPRs, SGPRs, spills, LDS, occupancy; -Rpass-analysis=kernel-resource-usage) is saved to
-triton-fa2-forward_amd/fa2/kernel_resources.json, which sweep.py prints beside its timings.
+triton-fa2-forward_amd/fa2/kernel_resources.json: the attention kernels' under "kernels", which sweep.py prints beside its
+timings, the serving kernels' under "serving".
 """
 
 import argparse
