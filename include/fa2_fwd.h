@@ -359,6 +359,100 @@ FA2_API int fa2_attn_paged(const void* q, void* out, const int64_t q_stride[2], 
 FA2_API size_t fa2_paged_workspace_bytes(int32_t h_q, int32_t h_kv, int32_t head_dim, int32_t cache_dtype,
                                          int32_t n_tokens, int32_t n_seq, int64_t max_keys, int32_t num_cus);
 
+/*
+ * ---- A step beyond that: windows, common prefixes, normalised rotations of several axes, pages from lengths.
+ *
+ * fa2_attn_packed_window and fa2_attn_paged_window - fa2_attn_packed and fa2_attn_paged with the causal mask and a
+ * window: a row whose last key is n sees keys n - window + 1 .. n, and the sequence's first `sinks` (window >= 1,
+ * sinks >= 0). Keys of no row's window are not read, and entries of the table whose pages no row of the call sees are not
+ * looked at: such pages may belong to others.
+ */
+FA2_API int fa2_attn_packed_window(const void* q, const void* k, const void* v, void* out,
+                                   const int64_t q_stride[2], const int64_t k_stride[2],
+                                   const int64_t v_stride[2], const int64_t o_stride[2],
+                                   const int32_t* cu, const int32_t* cu_kv, int32_t n_seq, int32_t n_tokens,
+                                   int32_t kv_tokens, int32_t h_q, int32_t h_kv, int32_t head_dim, int32_t dtype,
+                                   int32_t window, int32_t sinks, float qk_scale, float* lse, void* stream);
+FA2_API int fa2_attn_paged_window(const void* q, void* out, const int64_t q_stride[2], const int64_t o_stride[2],
+                                  const fa2_cache* cache, const fa2_sequences* seq, int32_t h_q, int32_t dtype,
+                                  int32_t window, int32_t sinks, float qk_scale, float* lse, void* workspace,
+                                  size_t workspace_bytes, void* stream);
+FA2_API size_t fa2_paged_window_workspace_bytes(int32_t h_q, int32_t h_kv, int32_t head_dim, int32_t cache_dtype,
+                                                int32_t n_tokens, int32_t n_seq, int64_t max_keys, int32_t window,
+                                                int32_t sinks, int32_t num_cus);
+
+/*
+ * fa2_attn_paged_shared - fa2_attn_paged where the sequences' first shared[0] tokens (device int32) are the same and lie in
+ * the same pages: those are read once for all rows, from the row of the table of the first sequence that has rows. Of
+ * shared[0], as much counts as whole pages hold and as lies before every sequence's own rows; the tokens behind that
+ * are read from every sequence's own row of the table. The workspace must hold fa2_paged_shared_workspace_bytes(...).
+ */
+FA2_API int fa2_attn_paged_shared(const void* q, void* out, const int64_t q_stride[2], const int64_t o_stride[2],
+                                  const fa2_cache* cache, const fa2_sequences* seq, const int32_t* shared,
+                                  int32_t h_q, int32_t dtype, int32_t causal, float qk_scale, float* lse,
+                                  void* workspace, size_t workspace_bytes, void* stream);
+FA2_API size_t fa2_paged_shared_workspace_bytes(int32_t h_q, int32_t h_kv, int32_t head_dim, int32_t cache_dtype,
+                                                int32_t n_tokens, int32_t n_seq, int64_t max_keys, int32_t num_cus);
+
+/*
+ * What rows of q and k are turned by: every head x of q first becomes x / sqrt(mean x^2 + q_eps) * q_weight (device
+ * float[head_dim]; NULL: it stays), k likewise, and then pair i is rotated by freqs[i] times the position on axis axes[i]
+ * (device int32[half], 0 .. n_axes - 1, others count as the nearest; NULL: all on axis 0, n_axes 1). Squares and their sum
+ * are formed in float64.
+ */
+typedef struct fa2_turn {
+  fa2_rotation rotation;
+  const int32_t* axes;
+  const float* q_weight;
+  const float* k_weight;
+  double q_eps, k_eps;
+  int32_t n_axes;
+} fa2_turn;
+
+/*
+ * fa2_rotary_qk - q and k turned, in one launch. q and q_out [batch, h_q, n, head_dim], k and k_out of h_k heads, strides
+ * [b, h, n]; q_out may be q and k_out k, in the same layout; h_q or h_k may be 0. positions: int32 or int64, strides [axis, b, n].
+ */
+FA2_API int fa2_rotary_qk(const void* q, const void* k, void* q_out, void* k_out, const int64_t q_stride[3],
+                          const int64_t k_stride[3], const int64_t qo_stride[3], const int64_t ko_stride[3],
+                          const void* positions, int32_t position_bytes, const int64_t p_stride[3],
+                          const fa2_turn* turn, int32_t batch, int32_t h_q, int32_t h_k, int32_t n,
+                          int32_t head_dim, int32_t dtype, void* stream);
+
+/*
+ * fa2_cache_write_turned - fa2_cache_write with k turned before it is written, and q. positions: strides [axis, token], or NULL:
+ * each row's position in its sequence (of one axis).
+ */
+FA2_API int fa2_cache_write_turned(const fa2_cache* cache, const fa2_sequences* seq, const void* k, const void* v,
+                                   const int64_t k_stride[2], const int64_t v_stride[2], const void* q, void* q_out,
+                                   const int64_t q_stride[2], const int64_t qo_stride[2], int32_t h_q,
+                                   const void* positions, int32_t position_bytes, const int64_t p_stride[2],
+                                   const fa2_turn* turn, int32_t dtype, void* stream);
+
+/*
+ * fa2_pages_extend - the pages of new_tokens[s] more tokens of every sequence of lens[s] (negative ones count as 0).
+ * free_pages[0 .. count[0]) are free, of n_pages. Needs are counted in the order of the sequences; with N in all,
+ * the i-th gets free_pages[max(count - N, 0) + i], or -1 where that is not free; the page is entered into its place of the
+ * table [n_seq, max_pages] (tokens past the row need none). Writes count_out[0], what is left of the free ones; lens_out
+ * [n_seq], the lengths with the new tokens; cu_out [n_seq + 1], the new tokens' first rows; and for every row t below
+ * n_tokens its position in its sequence and its slot, page * page_size + place in the page (-1: no page), both -1 for
+ * rows of no sequence. Sums past 2^31 - 1 are written as that. What is written overlaps nothing that is read (the new entries
+ * of the table apart).
+ */
+FA2_API int fa2_pages_extend(const int32_t* free_pages, int32_t n_pages, const int32_t* count, int32_t* count_out,
+                             int32_t* table, int64_t table_stride, int32_t n_seq, int32_t max_pages,
+                             int32_t page_size, const int32_t* lens, const int32_t* new_tokens, int32_t* lens_out,
+                             int32_t* cu_out, int32_t* positions, int64_t* slots, int32_t n_tokens, void* stream);
+
+/*
+ * fa2_pages_release - entries first[s] .. last[s] - 1 of every sequence's row of the table go on top of the free pages,
+ * in the order of the sequences and entries; entries that are no page (not in 0 .. n_pages - 1) are left out, and what
+ * the n_pages places do not hold is dropped. count_out[0]: the free pages then. workspace: int32[n_seq + 1].
+ */
+FA2_API int fa2_pages_release(int32_t* free_pages, int32_t n_pages, const int32_t* count, int32_t* count_out,
+                              const int32_t* table, int64_t table_stride, int32_t n_seq, int32_t max_pages,
+                              const int32_t* first, const int32_t* last, int32_t* workspace, void* stream);
+
 /* Thread-local description of the last failure in this thread ("" if none). */
 FA2_API const char* fa2_last_error(void);
 

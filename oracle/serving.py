@@ -46,8 +46,9 @@ def to_e4m3(x, dtype):
     return torch.where(x.isfinite(), y, torch.full_like(y, math.nan)), e[..., 0]
 
 
-def attention(q, k, v, causal, sm_scale=None):
-    """One sequence: q [n, H_q, D] over k, v [m, H_kv, D], the causal mask aligned at the end. Float64 out
+def attention(q, k, v, causal, sm_scale=None, window=None, sinks=0):
+    """One sequence: q [n, H_q, D] over k, v [m, H_kv, D], the causal mask aligned at the end; of a window, a row sees the
+    `window` newest keys up to its last and the first `sinks`. Float64 out
     [n, H_q, D], lse [H_q, n], and for the bounds: the weights' sum of |v|, [n, H_q, D], and the largest sum of
     |q_d k_d| * sm_scale of a row, [n, H_q, 1]. Values of keys that a row does not see do not enter its result."""
     n, h_q, D = q.shape
@@ -62,6 +63,10 @@ def attention(q, k, v, causal, sm_scale=None):
     see = torch.ones(n, m, dtype=torch.bool, device=q.device)
     if causal:
         see = torch.arange(m, device=q.device) <= torch.arange(n, device=q.device)[:, None] + (m - n)
+    if window is not None:
+        last = torch.arange(n, device=q.device)[:, None] + (m - n)
+        key = torch.arange(m, device=q.device)
+        see &= (key > last - window) | (key < sinks)
     some = see.any(1)
     group = h_q // h_kv
     for h in range(h_kv):  # the group of query heads of a KV head at once

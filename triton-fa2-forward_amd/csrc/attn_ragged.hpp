@@ -43,9 +43,30 @@ constexpr int ragged_block_n(int head_dim, int row_waves) {
   return row_waves == 4 ? (head_dim == 16 ? 128 : 64) : head_dim == 128 ? 32 : 64;
 }
 
+// A row's results over the keys before a common prefix's end, kept in float beside each other: O, then m, l and exact l
+template <int D>
+__device__ __forceinline__ float* prefix_row(ParamsRef p, int64_t token, int head) {
+  return p.prefix + (token * (p.h_kv * p.group) + head) * (D + 4);
+}
+// Joined with the results (m, l, exact l) over the row's own keys: O = own * O_own + prefix * O_prefix. A NaN reference
+// makes the row NaN.
+struct Joined {
+  float own, prefix, lse;
+  __device__ Joined(float m, float l, float exact, const f32x4& of_prefix, bool no_key) {
+    const float M = fmaxf(m, of_prefix[0]);
+    const float a = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - M);
+    const float b = of_prefix[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(of_prefix[0] - M);
+    const float inv = no_key ? 0.f : 1.0f / (a * l + b * of_prefix[1]);
+    own = a * inv;
+    prefix = b * inv;
+    const bool nan = m != m || of_prefix[0] != of_prefix[0];
+    lse = !nan && M == INFINITY ? M : ((nan ? m + of_prefix[0] : M) + log2f(a * exact + b * of_prefix[2])) * kLn2;
+  }
+};
+
 // LSE: with 128 rows, whether p.lse is set: known to the compiler, the sums it needs mix with the rest of the tile's
 // instructions, and cost nothing where they are not asked for.
-template <int DT, int D, int SRC, int GW, bool LSE>
+template <int DT, int D, int SRC, int GW, bool LSE, int MODE>
 __global__ __launch_bounds__(256)
 __attribute__((amdgpu_waves_per_eu(ragged_waves(D, SRC, GW))))
 void attn_ragged_kernel(const RaggedParams) {
@@ -53,6 +74,7 @@ void attn_ragged_kernel(const RaggedParams) {
   ParamsRef p = params_here();
   constexpr bool kE4m3 = SRC == kSourceE4m3;
   constexpr bool kPages = SRC != kSourcePacked;
+  constexpr bool kWindow = MODE == kModeWindow, kPrefix = MODE == kModePrefix, kOwn = MODE == kModeOwn;
   constexpr int EB = kE4m3 ? 1 : 2;      // bytes of a cached element
   constexpr int BN = ragged_block_n(D, GW);
   constexpr int BM = 32 * GW;            // rows per workgroup
@@ -148,25 +170,27 @@ void attn_ragged_kernel(const RaggedParams) {
   }
 
   const float qk_scale = p.qk_scale;
-  const bool want_exact = GW == 1 ? p.lse != nullptr : LSE, causal = p.causal != 0, shared = kPages && p.shares > 0;
+  const bool want_exact = GW == 1 ? p.lse != nullptr : LSE, causal = !kPrefix && p.causal != 0,
+             shared = kPages && p.shares > 0;
 
   // ---- the workgroup's work: the pieces of its share, or its one tile
   Cursor cur;
+  if constexpr (kPrefix || kOwn) cur.prefix = common_prefix(p, lane);
   Share share = {0, 0, 0, 0};
   if (shared) {
-    share = find_share<BM, kPages>(p, rank, lane, &cur);
+    share = find_share<BM, kPages, MODE>(p, rank, lane, &cur);
     if (share.x >= share.end) {
       if (tid == 0) merge_of(p, hkv, rank)->first = -1;
       return;
     }
-  } else if (!find_tile<BM, kPages>(p, rank, lane, &cur)) {
+  } else if (!find_tile<BM, kPages, MODE>(p, rank, lane, &cur)) {
     return;
   }
   bool fresh = true;  // LDS has not been used yet
   for (bool first_piece = true, more = true; more; first_piece = false) {
     ParamsRef p = params_here();
     const LaneSequence sq = sequence_at(cur.lanes, cur.l);
-    const int seq = cur.s0 + cur.l, n_kv = sq.n_kv;
+    const int seq = kPrefix ? cur.prefix.row : cur.s0 + cur.l, n_kv = sq.n_kv;
     const int rows = sq.n_q * p.group;
     const int row0 = cur.tile * BM;       // this workgroup's rows [row0, row_end)
     const int row_end = min(row0 + BM, rows);
@@ -175,12 +199,20 @@ void attn_ragged_kernel(const RaggedParams) {
     auto last_of = [&](int i) { return causal ? min(i + shift, n_kv - 1) : n_kv - 1; };
     const int see_end = max(last_of((row_end - 1) / p.group) + 1, 0);
     const int full_end = max(last_of(row0 / p.group) + 1, 0);
-    const int all_tiles = (see_end + BN - 1) / BN;
+    // A window: the first key of a position (beside the sinks), the least and the largest of the tile's, and the key
+    // tiles between the sinks' and the window's, which are skipped. Key tiles are counted without those.
+    auto first_of = [&](int i) { return kWindow ? max(last_of(i) - p.window + 1, 0) : 0; };
+    const int sinks = kWindow ? p.sinks : 0;
+    const int see_begin = first_of(row0 / p.group), first_end = first_of((row_end - 1) / p.group);
+    const int sink_tiles = kWindow ? (min(sinks, see_end) + BN - 1) / BN : 0;
+    const int skip = kWindow ? max(see_begin / BN - sink_tiles, 0) : 0;
+    auto tile_key = [&](int t) { return (kWindow && t >= sink_tiles ? t + skip : t) * BN; };
+    const int all_tiles = (see_end + BN - 1) / BN - skip;
 
     int t_begin = 0, t_end = all_tiles;
     float* part = nullptr;  // where the piece's partial results go, if it is not the whole tile
     if (shared) {
-      const int64_t length = lengths_of<BM>(p, sq.n_q, n_kv).of(cur.tile);
+      const int64_t length = lengths_of<BM, MODE>(p, sq.n_q, n_kv).of(cur.tile);
       const int64_t out = min(length, share.in + (share.end - share.x));
       if (share.in > 0) t_begin = cut_at(share.in, length, all_tiles);
       if (out < length) t_end = cut_at(out, length, all_tiles);
@@ -198,11 +230,11 @@ void attn_ragged_kernel(const RaggedParams) {
       share.in = 0;
       if (empty) {
         if (null_part) *(f32x4*)(part + part_sums<BM, D>(tid)) = f32x4{-INFINITY, 0.f, 0.f, 0.f};
-        more = share.x < share.end && next_tile<BM, kPages>(p, lane, &cur);
+        more = share.x < share.end && next_tile<BM, kPages, MODE>(p, lane, &cur);
         continue;
       }
     }
-    const int kv_begin = t_begin * BN, kv_end = min(t_end * BN, see_end);
+    const int kv_begin = tile_key(t_begin), kv_end = min(kWindow ? tile_key(t_end - 1) + BN : t_end * BN, see_end);
     if (!fresh) __syncthreads();  // the last piece's merge has left LDS
     fresh = false;
 
@@ -210,7 +242,7 @@ void attn_ragged_kernel(const RaggedParams) {
     const int wr = gwave * 32 + c;  // the row inside the workgroup
     const int r = min(row0 + wr, rows - 1);
     const int pos = r / p.group;
-    const int last_key = last_of(pos);
+    const int last_key = last_of(pos), first_key = first_of(pos);
     u32x4 qreg[KS];
     {
       const int head = hkv * p.group + (r - pos * p.group);
@@ -222,7 +254,12 @@ void attn_ragged_kernel(const RaggedParams) {
     // ---- this group's key tiles: grp, grp + KG, ... of the piece
     const int n_tiles = t_end - t_begin;
     const int count = (n_tiles - grp + KG - 1) / KG;
-    auto key_of = [&](int i) { return kv_begin + (grp + i * KG) * BN; };  // first key of tile i
+    auto key_of = [&](int i) {  // first key of tile i
+      if constexpr (kWindow) return tile_key(t_begin + grp + i * KG);
+      return kv_begin + (grp + i * KG) * BN;
+    };
+    // whether no row sees any of `keys` keys from n on, those up to kv_end all being seen but for the window
+    auto hidden = [&](int n, int keys) { return kWindow && n >= sinks && n + keys <= see_begin; };
 
     // ---- pages: lane x of `pages` holds the page of tile x / per_tile of the current block of 64 / per_tile
     // tiles, its page x % per_tile; `pages_next` those of the next block, on their way. An entry that
@@ -230,14 +267,21 @@ void attn_ragged_kernel(const RaggedParams) {
     constexpr int kLog2Bn = BN == 32 ? 5 : BN == 64 ? 6 : 7;
     const int tile_shift = kPages ? max(0, kLog2Bn - page_shift) : 0;  // log2 pages per tile
     const int block = 64 >> tile_shift;  // tiles of a block
+    const int64_t first_token = kOwn ? sq.kv_first : 0;  // (whole pages)
     int pages = 0, pages_next = 0, bad = 0;
     auto load_pages = [&](int i0) {
       ParamsRef p = params_here();
       const int i = i0 + (lane >> tile_shift);
-      const int64_t n = kv_begin + (int64_t)(grp + (int64_t)i * KG) * BN +
-                        ((int64_t)(lane & ((1 << tile_shift) - 1)) << page_shift);
+      int64_t n;
+      if constexpr (kWindow)
+        n = tile_key(t_begin + grp + min(i, count) * KG);
+      else
+        n = kv_begin + (int64_t)(grp + (int64_t)i * KG) * BN;
+      n += (int64_t)(lane & ((1 << tile_shift) - 1)) << page_shift;
       int e = 0;
-      if (i < count && n < kv_end) e = p.seq.table[seq * p.seq.table_stride + (n >> page_shift)];
+      // (a page that no row sees may be none of the cache any more: its entry is not looked at, and nothing of it loaded)
+      if (i < count && n < kv_end && !hidden((int)(n >> page_shift << page_shift), 1 << page_shift))
+        e = p.seq.table[seq * p.seq.table_stride + ((n + first_token) >> page_shift)];
       return e;
     };
     auto checked_pages = [&](int e) {
@@ -276,7 +320,8 @@ void attn_ragged_kernel(const RaggedParams) {
         return x.data + (uint64_t)(uint32_t)(sq.kv_first + n) * x.token;
     };
     auto segment_bytes = [&](const Source& x, int i, int s, int row_bytes) {
-      const int valid = max(min(kv_end - key_of(i) - segment_row(s), SEG), 0);
+      const int n = key_of(i) + segment_row(s);
+      const int valid = hidden(n, SEG) ? 0 : max(min(kv_end - n, SEG), 0);
       return (uint32_t)max(valid * (int)x.token - ((int)x.token - row_bytes), 0);
     };
     auto issue = [&](const Source& x, const uint32_t (&off)[LPS], const FA2_LDS char* buf, int i) {
@@ -347,6 +392,16 @@ void attn_ragged_kernel(const RaggedParams) {
 #pragma unroll
           for (int x = 0; x < 16; ++x)
             if (nb * 32 + 16 * (x / 8) + (x % 8) > lim) s[nb][x] = -INFINITY;
+      }
+      if (kWindow && n0 < first_end && n0 + BN > sinks) {
+        const int lim = first_key - n0 - 8 * g, open = sinks - n0 - 8 * g;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int x = 0; x < 16; ++x) {
+            const int n = nb * 32 + 16 * (x / 8) + (x % 8);
+            if (n < lim && n >= open) s[nb][x] = -INFINITY;
+          }
       }
       float mx = -INFINITY;
 #pragma unroll
@@ -480,8 +535,14 @@ void attn_ragged_kernel(const RaggedParams) {
       for (int x = 0; x < KS; ++x) asm volatile("" : "+v"(qreg[x]));
       // tiles that start past every row of the wave add exact zeros: their products are skipped
       const int wave_last = __builtin_amdgcn_readlane(last_key, 31);  // rows grow with the lane
-      const int n_active = row0 + gwave * 32 >= row_end || wave_last < kv_begin
-                               ? 0 : min(n_tiles, (wave_last - kv_begin) / BN + 1);
+      int n_active = 0;
+      if constexpr (kWindow) {
+        const int upto = wave_last < 0 ? 0 : wave_last / BN + 1;  // key tiles that start up to wave_last
+        if (row0 + gwave * 32 < row_end)
+          n_active = min(n_tiles, max((upto > sink_tiles ? max(upto - skip, sink_tiles) : upto) - t_begin, 0));
+      } else if (!(row0 + gwave * 32 >= row_end || wave_last < kv_begin)) {
+        n_active = min(n_tiles, (wave_last - kv_begin) / BN + 1);
+      }
       auto turn_tile = [&](int j) {  // before tile j's barrier and after it: all that keeps the loads going
         if constexpr (kE4m3) {
           store(false, kbuf(j + 1), kraw);
@@ -572,6 +633,15 @@ void attn_ragged_kernel(const RaggedParams) {
     auto put_sums = [&](int x, float m, float sum, float exact) {
       if (part) {
         *(f32x4*)(part + part_sums<BM, D>(x)) = f32x4{m, sum, exact, 0.f};
+      } else if (kPrefix) {
+        const RowPlace at = place(x);
+        *(f32x4*)(prefix_row<D>(pe, at.token, at.head) + D) = f32x4{m, sum, exact, 0.f};
+      } else if (kOwn) {
+        if (pe.lse) {
+          const RowPlace at = place(x);
+          const Joined j(m, sum, exact, *(const f32x4*)(prefix_row<D>(pe, at.token, at.head) + D), last_of(at.pos) < 0);
+          pe.lse[(int64_t)at.head * pe.seq.n_tokens + at.token] = j.lse;
+        }
       } else if (pe.lse) {
         const RowPlace at = place(x);
         pe.lse[(int64_t)at.head * pe.seq.n_tokens + at.token] = (m + log2f(exact)) * kLn2;
@@ -585,7 +655,7 @@ void attn_ragged_kernel(const RaggedParams) {
       int page = 0;
       auto row_at = [&](const auto& y, int n) {
         if constexpr (kPages) {
-          page = pe.seq.table[seq * pe.seq.table_stride + (n >> page_shift)];
+          page = pe.seq.table[seq * pe.seq.table_stride + ((n + first_token) >> page_shift)];
           if ((unsigned)page >= (unsigned)pe.seq.n_pages) page = 0;
           return y.data + (page * y.page + hkv * y.head + (int64_t)(n & ((1 << page_shift) - 1)) * y.token) * EB;
         } else {
@@ -609,10 +679,13 @@ void attn_ragged_kernel(const RaggedParams) {
       };
       bool no_lse = nan;  // (an infinite score has one, though the row has no weights)
       float m = -INFINITY, sum = 0.f, o[(D + 63) / 64] = {};
+      const int from = first_of(at.pos);
+      auto sees = [&](int n) { return n < end && (!kWindow || n >= from || n < sinks); };
       for (int n0 = kv_begin; n0 < end; n0 += 64) {
+        if (kWindow && n0 >= sinks && n0 + 64 <= from) n0 = from;
         const int n = n0 + lane;
         float s = -INFINITY;
-        if (n < end) {
+        if (sees(n)) {
           const char* krow = row_at(pe.kc, n);
           const float scale = scale_at(pe.kc, n);
           s = 0.f;
@@ -626,12 +699,15 @@ void attn_ragged_kernel(const RaggedParams) {
         m_new = fmaxf(m, m_new);
         const float m_ref = m_new == -INFINITY ? 0.f : m_new;
         const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m_ref);
-        const float w = n < end ? __builtin_amdgcn_exp2f(s - m_ref) : 0.f;
+        const float w = sees(n) ? __builtin_amdgcn_exp2f(s - m_ref) : 0.f;
         m = m_new;
         sum = sum * alpha + w;
 #pragma unroll
         for (int y = 0; y < (D + 63) / 64; ++y) o[y] *= alpha;
         for (int y = 0; y < min(end - n0, 64); ++y) {
+          if constexpr (kWindow) {
+            if (!sees(n0 + y)) continue;
+          }
           const float wy = __shfl(w, y, 64);
           const char* vrow = row_at(pe.vc, n0 + y);
           const float scale = scale_at(pe.vc, n0 + y);
@@ -644,12 +720,19 @@ void attn_ragged_kernel(const RaggedParams) {
       for (int o2 = 32; o2 >= 1; o2 /= 2) sum += __shfl_xor(sum, o2, 64);
       if (no_lse) m = __uint_as_float(0x7fc00000u);
       const float inv = last_of(at.pos) < 0 ? 0.f : 1.0f / sum;
+      const float* before = kPrefix || kOwn ? prefix_row<D>(pe, at.token, at.head) : nullptr;
+      const Joined j(m, sum, sum, kOwn && !part ? *(const f32x4*)(before + D) : f32x4{-INFINITY, 0.f, 0.f, 0.f}, last_of(at.pos) < 0);
 #pragma unroll
       for (int y = 0; y < (D + 63) / 64; ++y)
         if (lane + 64 * y < D) {
           const float v = nan ? m : o[y];
           if (part)
             part[part_index<GW, D>(x, lane + 64 * y)] = v;
+          else if (kPrefix)
+            const_cast<float*>(before)[lane + 64 * y] = v;
+          else if (kOwn)
+            pe.o[at.token * pe.sot + at.head * pe.soh + lane + 64 * y] =
+                (uint16_t)E::pack2(last_of(at.pos) < 0 ? 0.f : v * j.own + before[lane + 64 * y] * j.prefix, 0.f);
           else
             pe.o[at.token * pe.sot + at.head * pe.soh + lane + 64 * y] =
                 (uint16_t)E::pack2(last_of(at.pos) < 0 ? 0.f : v * inv, 0.f);
@@ -667,21 +750,32 @@ void attn_ragged_kernel(const RaggedParams) {
         const RowPlace at = place(wr);
         uint16_t* orow = pe.o + at.token * pe.sot + at.head * pe.soh;
         const float nan_or_0 = m_i != m_i ? m_i : 0.f;
+        float* before = kPrefix || kOwn ? prefix_row<D>(pe, at.token, at.head) : nullptr;
+        const Joined j(m_i, l, l, kOwn && !part ? *(const f32x4*)(before + D) : f32x4{-INFINITY, 0.f, 0.f, 0.f}, last_key < 0);
 #pragma unroll
         for (int db = 0; db < DB; ++db)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const int d0 = 32 * db + 16 * h + 8 * g;
             if (d0 < D) {
-              if (part) {
+              if (part || kPrefix) {
                 f32x4 lo, hi;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                   lo[i] = acc[db][8 * h + i];
                   hi[i] = acc[db][8 * h + 4 + i];
                 }
-                *(f32x4*)(part + part_index<GW, D>(wr, d0)) = lo;
-                *(f32x4*)(part + part_index<GW, D>(wr, d0 + 4)) = hi;
+                float* to = kPrefix && !part ? before + d0 : part + part_index<GW, D>(wr, d0);
+                *(f32x4*)to = lo;
+                *(f32x4*)(kPrefix && !part ? to + 4 : part + part_index<GW, D>(wr, d0 + 4)) = hi;
+              } else if (kOwn) {
+                float y[8];
+                const f32x4 lo = *(const f32x4*)(before + d0), hi = *(const f32x4*)(before + d0 + 4);
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                  y[i] = __builtin_fmaf(acc[db][8 * h + i], j.own, (i < 4 ? lo[i] : hi[i - 4]) * j.prefix) + nan_or_0;
+                *(u32x4*)(orow + d0) = u32x4{E::pack2(y[0], y[1]), E::pack2(y[2], y[3]), E::pack2(y[4], y[5]),
+                                             E::pack2(y[6], y[7])};
               } else {
                 float y[8];
 #pragma unroll
@@ -748,8 +842,18 @@ void attn_ragged_kernel(const RaggedParams) {
           for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(w, v[e], o[e]);
         }
         const RowPlace at = place(x);
+        const float m_nan = nan ? __uint_as_float(0x7fc00000u) : m;
         if (part) {
           *(f32x4*)(part + part_index<GW, D>(x, 4 * q)) = o;
+        } else if (kPrefix) {
+          *(f32x4*)(prefix_row<D>(pe, at.token, at.head) + 4 * q) = o;
+        } else if (kOwn) {
+          const float* before = prefix_row<D>(pe, at.token, at.head);
+          const Joined j(m_nan, ls, lxs, *(const f32x4*)(before + D), last_of(at.pos) < 0);
+          const f32x4 v = *(const f32x4*)(before + 4 * q);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(o[e], j.own, v[e] * j.prefix);
+          *(u32x2*)(pe.o + at.token * pe.sot + at.head * pe.soh + 4 * q) = u32x2{E::pack2(o[0], o[1]), E::pack2(o[2], o[3])};
         } else {
           const float inv = last_of(at.pos) < 0 ? 0.f : 1.0f / ls;  // no key: 0
 #pragma unroll
@@ -757,7 +861,7 @@ void attn_ragged_kernel(const RaggedParams) {
           *(u32x2*)(pe.o + at.token * pe.sot + at.head * pe.soh + 4 * q) = u32x2{E::pack2(o[0], o[1]), E::pack2(o[2], o[3])};
         }
         // (fmaxf has dropped a NaN reference, and a piece whose groups all met bad pages would pass for one without keys)
-        if (q == 0) put_sums(x, nan ? __uint_as_float(0x7fc00000u) : m, ls, lxs);
+        if (q == 0) put_sums(x, m_nan, ls, lxs);
       }
       for (int x = wave; x < row_end - row0; x += 4) {
         if (!odd[x]) continue;
@@ -767,7 +871,7 @@ void attn_ragged_kernel(const RaggedParams) {
         again(x, nan);
       }
     }
-    more = shared && share.x < share.end && next_tile<BM, kPages>(params_here(), lane, &cur);
+    more = shared && share.x < share.end && next_tile<BM, kPages, MODE>(params_here(), lane, &cur);
   }
 }
 
@@ -794,7 +898,7 @@ struct Merged {
     for (int e = 0; e < 4; ++e) o[e] = o[e] * a + (none ? 0.f : w * v[e]);
   }
 };
-template <int DT, int D, int GW>
+template <int DT, int D, int GW, int MODE>
 __global__ __launch_bounds__(combine_threads(D)) void attn_ragged_combine_kernel(const RaggedParams) {
   using E = Elem<DT>;
   ParamsRef p = params_here();
@@ -844,7 +948,24 @@ __global__ __launch_bounds__(combine_threads(D)) void attn_ragged_combine_kernel
   if (way > 0 || x >= at.rows) return;
   const int pos = (at.row0 + x) / p.group, head = hkv * p.group + (at.row0 + x - pos * p.group);
   const int64_t token = at.token + pos;
+  if constexpr (MODE == kModePrefix) {
+    float* row = prefix_row<D>(p, token, head);
+    *(f32x4*)(row + 4 * q) = r.o;
+    if (q == 0) *(f32x4*)(row + D) = f32x4{r.nan ? __uint_as_float(0x7fc00000u) : r.M, r.l, r.lx, 0.f};
+    return;
+  }
   const bool none = (p.causal ? min(pos + at.shift, at.n_kv - 1) : at.n_kv - 1) < 0;
+  if constexpr (MODE == kModeOwn) {
+    const float* before = prefix_row<D>(p, token, head);
+    const Joined j(r.nan ? __uint_as_float(0x7fc00000u) : r.M, r.l, r.lx, *(const f32x4*)(before + D), none);
+    const f32x4 v = *(const f32x4*)(before + 4 * q);
+    f32x4 o;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(r.o[e], j.own, v[e] * j.prefix);
+    *(u32x2*)(p.o + token * p.sot + head * p.soh + 4 * q) = u32x2{E::pack2(o[0], o[1]), E::pack2(o[2], o[3])};
+    if (p.lse && q == 0) p.lse[(int64_t)head * p.seq.n_tokens + token] = j.lse;
+    return;
+  }
   const float inv = none ? 0.f : 1.0f / r.l;
   *(u32x2*)(p.o + token * p.sot + head * p.soh + 4 * q) =
       u32x2{E::pack2(r.o[0] * inv, r.o[1] * inv), E::pack2(r.o[2] * inv, r.o[3] * inv)};

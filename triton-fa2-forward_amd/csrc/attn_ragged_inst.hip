@@ -1,21 +1,24 @@
-// attn_ragged_inst.hip - the ragged attention kernel's instances of one (dtype, head_dim) pair, compiled
-// once per pair (FA2_DT, FA2_D).
+// attn_ragged_inst.hip - the ragged attention kernel's instances of one (dtype, head_dim) pair and one choice of keys, compiled
+// once for each (FA2_DT, FA2_D, FA2_MODE).
 #include "attn_ragged.hpp"
 
 namespace fa2 {
 
 namespace {
 
+// (a window's pieces merge as all keys' do)
+constexpr int kCombineMode = FA2_MODE == kModeWindow ? kModeAll : FA2_MODE;
+
 template <int SRC, int GW>
 int launch_form(const RaggedParams& p, unsigned grid, hipStream_t s) {
   if (GW > 1 && p.lse)
-    hipLaunchKernelGGL((attn_ragged_kernel<FA2_DT, FA2_D, SRC, GW, (GW > 1)>), dim3(grid), dim3(256), 0, s, p);
+    hipLaunchKernelGGL((attn_ragged_kernel<FA2_DT, FA2_D, SRC, GW, (GW > 1), FA2_MODE>), dim3(grid), dim3(256), 0, s, p);
   else
-    hipLaunchKernelGGL((attn_ragged_kernel<FA2_DT, FA2_D, SRC, GW, false>), dim3(grid), dim3(256), 0, s, p);
+    hipLaunchKernelGGL((attn_ragged_kernel<FA2_DT, FA2_D, SRC, GW, false, FA2_MODE>), dim3(grid), dim3(256), 0, s, p);
   hipError_t e = hipGetLastError();
   if constexpr (SRC != kSourcePacked) {
     if (e == hipSuccess && p.shares > 0) {
-      hipLaunchKernelGGL((attn_ragged_combine_kernel<FA2_DT, FA2_D, GW>), dim3(grid * GW), dim3(combine_threads(FA2_D)), 0, s, p);
+      hipLaunchKernelGGL((attn_ragged_combine_kernel<FA2_DT, FA2_D, GW, kCombineMode>), dim3(grid * GW), dim3(combine_threads(FA2_D)), 0, s, p);
       e = hipGetLastError();
     }
   }
@@ -25,16 +28,17 @@ int launch_form(const RaggedParams& p, unsigned grid, hipStream_t s) {
 }  // namespace
 
 template <>
-int launch_ragged<FA2_DT, FA2_D>(const RaggedParams& p, int source, int row_waves, unsigned grid, hipStream_t s) {
+int launch_ragged<FA2_DT, FA2_D, FA2_MODE>(const RaggedParams& p, int source, int row_waves, unsigned grid, hipStream_t s) {
+  constexpr int kNoPages = FA2_MODE == kModeAll || FA2_MODE == kModeWindow ? kSourcePacked : kSourcePages;  // (pages only)
   if (row_waves == 1) {
     switch (source) {
-      case kSourcePacked: return launch_form<kSourcePacked, 1>(p, grid, s);
+      case kSourcePacked: return launch_form<kNoPages, 1>(p, grid, s);
       case kSourcePages: return launch_form<kSourcePages, 1>(p, grid, s);
       default: return launch_form<kSourceE4m3, 1>(p, grid, s);
     }
   }
   switch (source) {
-    case kSourcePacked: return launch_form<kSourcePacked, 4>(p, grid, s);
+    case kSourcePacked: return launch_form<kNoPages, 4>(p, grid, s);
     case kSourcePages: return launch_form<kSourcePages, 4>(p, grid, s);
     default: return launch_form<kSourceE4m3, 4>(p, grid, s);
   }

@@ -3,9 +3,9 @@ measurement library libfa2_ablate.so beside it.
 
     python triton-fa2-forward_amd/csrc/build.py [-j 8] [--verbose]
 
-Compiles attn_fwd_inst.hip and attn_ragged_inst.hip once per (dtype, head_dim) pair plus the split-KV
-combine pass (attn_fwd_combine.hip), the key-norm pass (attn_key_norm.hip), the rotary and cache kernels
-(serve_cache.hip) and the C-ABI file fa2_fwd.hip,
+Compiles attn_fwd_inst.hip once per (dtype, head_dim) pair and attn_ragged_inst.hip once per pair and choice of keys, plus
+the split-KV combine pass (attn_fwd_combine.hip), the key-norm pass (attn_key_norm.hip), the rotary and cache kernels
+(serve_cache.hip, serve_turn.hip), the page kernels (serve_pages.hip) and the C-ABI file fa2_fwd.hip,
 in parallel, with hipcc for gfx950 only, and links them into
 triton-fa2-forward_amd/fa2/libfa2_fwd.so next to the Python front end that loads it. Beside it goes
 fa2/_torch_call.so, the front end's native common call (fa2_torch.cpp, against the installed torch). Then builds
@@ -26,7 +26,7 @@ Both libraries are built with hidden visibility, so each exports exactly the fun
 header declares (FA2_API). The compiler's resource report for every kernel instance (VGPRs,
 AGPRs, SGPRs, spills, LDS, occupancy; -Rpass-analysis=kernel-resource-usage) is saved to
 triton-fa2-forward_amd/fa2/kernel_resources.json: the attention kernels' under "kernels", which sweep.py prints beside its
-timings, the serving kernels' under "serving".
+timings, the serving kernels' under "serving", those of windows, common prefixes, normalised rotations and pages under "step".
 """
 
 import argparse
@@ -52,6 +52,8 @@ CAPI_DIR = os.path.join(ROOT, "tests", "capi")
 ARCH = "gfx950"
 DTYPES = (0, 1)            # 0 = fp16, 1 = bf16
 HEAD_DIMS = (16, 32, 64, 128)
+RAGGED_MODES = (0, 1, 2, 3)  # csrc/serve_params.hpp: all keys, a window's, a common prefix's, those behind it
+SERVE_UNITS = ("serve_cache", "serve_turn", "serve_pages")
 
 
 def hipcc():
@@ -99,12 +101,24 @@ _KERNELS = {
 }
 # ... and the serving kernels', with their names there
 _SERVING_KERNELS = {
-    "attn_ragged_kernel": (re.compile(r"attn_ragged_kernelILi(\d)ELi(\d+)ELi(\d)ELi(\d)ELb([01])EEEv"),
+    "attn_ragged_kernel": (re.compile(r"attn_ragged_kernelILi(\d)ELi(\d+)ELi(\d)ELi(\d)ELb([01])ELi0EEEv"),
                            ("source", "row_waves", "lse")),
-    "attn_ragged_combine_kernel": (re.compile(r"attn_ragged_combine_kernelILi(\d)ELi(\d+)ELi(\d)EEEv"), ("row_waves",)),
+    "attn_ragged_combine_kernel": (re.compile(r"attn_ragged_combine_kernelILi(\d)ELi(\d+)ELi(\d)ELi0EEEv"), ("row_waves",)),
     "rotary_kernel": (re.compile(r"rotary_kernelILi(\d)ELi(\d+)EEEv"), ()),
-    "cache_write_kernel": (re.compile(r"cache_write_kernelILi(\d)ELi(\d+)ELb([01])EEEv"), ("e4m3",)),
+    "cache_write_kernel": (re.compile(r"cache_write_kernelILi(\d)ELi(\d+)ELb([01])ENS_11CacheParamsEEEv"), ("e4m3",)),
     "cache_read_kernel": (re.compile(r"cache_read_kernelILi(\d)ELi(\d+)ELb([01])EEEv"), ("e4m3",)),
+}
+# ... and those of a step beyond that (windows, common prefixes, normalised rotations, pages)
+_STEP_KERNELS = {
+    "attn_ragged_kernel": (re.compile(r"attn_ragged_kernelILi(\d)ELi(\d+)ELi(\d)ELi(\d)ELb([01])ELi([123])EEEv"),
+                           ("source", "row_waves", "lse", "mode")),
+    "attn_ragged_combine_kernel": (re.compile(r"attn_ragged_combine_kernelILi(\d)ELi(\d+)ELi(\d)ELi([123])EEEv"),
+                                   ("row_waves", "mode")),
+    "rotary_qk_kernel": (re.compile(r"rotary_qk_kernelILi(\d)ELi(\d+)EEEv"), ()),
+    "cache_write_kernel": (re.compile(r"cache_write_kernelILi(\d)ELi(\d+)ELb([01])ENS_15CacheTurnParamsEEEv"), ("e4m3",)),
+    "pages_extend_kernel": (re.compile(r"pages_extend_kernelENS"), ()),
+    "pages_count_kernel": (re.compile(r"pages_count_kernelENS"), ()),
+    "pages_release_kernel": (re.compile(r"pages_release_kernelENS"), ()),
 }
 
 
@@ -135,13 +149,19 @@ def describe_instance(name):
             "block_n": bn, "causal": bool(causal), "variant": variant}
 
 
-def describe_serving(name):
+def describe_serving(name, kernels=_SERVING_KERNELS):
     """The template arguments of a serving kernel's mangled name (None: another kernel)."""
-    for kernel, (pattern, fields) in _SERVING_KERNELS.items():
+    for kernel, (pattern, fields) in kernels.items():
         if m := pattern.search(name):
+            if not m.groups():
+                return {"kernel": kernel}
             dt, d, *rest = (int(x) for x in m.groups())
             return {"kernel": kernel, "dtype": ("fp16", "bf16")[dt], "head_dim": d, **dict(zip(fields, rest))}
     return None
+
+
+def describe_step(name):
+    return describe_serving(name, _STEP_KERNELS)
 
 
 VARIANTS_DIR = os.path.join(PKG, "variants")
@@ -164,10 +184,11 @@ def build_variant(name, defines, jobs=8, verbose=False):
             cmds.append([cc, *flags, f"-DFA2_DT={dt}", f"-DFA2_D={d}", "-c",
                          os.path.join(CSRC, "attn_fwd_inst.hip"), "-o",
                          os.path.join(obj_dir, f"attn_fwd_dt{dt}_d{d}.o")])
-            cmds.append([cc, *flags, f"-DFA2_DT={dt}", f"-DFA2_D={d}", "-c",
-                         os.path.join(CSRC, "attn_ragged_inst.hip"), "-o",
-                         os.path.join(obj_dir, f"attn_ragged_dt{dt}_d{d}.o")])
-    for name_ in ("attn_fwd_combine", "attn_fwd_wavesplit", "attn_key_norm", "serve_cache", "fa2_fwd", "fa2_scratch"):
+            for mode in RAGGED_MODES:
+                cmds.append([cc, *flags, f"-DFA2_DT={dt}", f"-DFA2_D={d}", f"-DFA2_MODE={mode}", "-c",
+                             os.path.join(CSRC, "attn_ragged_inst.hip"), "-o",
+                             os.path.join(obj_dir, f"attn_ragged_dt{dt}_d{d}_m{mode}.o")])
+    for name_ in ("attn_fwd_combine", "attn_fwd_wavesplit", "attn_key_norm", *SERVE_UNITS, "fa2_fwd", "fa2_scratch"):
         cmds.append([cc, *flags, "-c", os.path.join(CSRC, name_ + ".hip"), "-o",
                      os.path.join(obj_dir, name_ + ".o")])
     with ThreadPoolExecutor(max_workers=max(1, jobs)) as ex:
@@ -192,14 +213,17 @@ def build(jobs=8, verbose=False):
             units.append([cc, *common_flags(), "-Rpass-analysis=kernel-resource-usage",
                           f"-DFA2_DT={dt}", f"-DFA2_D={d}", "-c",
                           os.path.join(CSRC, "attn_fwd_inst.hip"), "-o", obj])
-            obj = os.path.join(OBJ_DIR, f"attn_ragged_dt{dt}_d{d}.o")
-            serve_units.append([cc, *common_flags(), "-Rpass-analysis=kernel-resource-usage", f"-DFA2_DT={dt}",
-                                f"-DFA2_D={d}", "-c", os.path.join(CSRC, "attn_ragged_inst.hip"), "-o", obj])
+            for mode in RAGGED_MODES:
+                obj = os.path.join(OBJ_DIR, f"attn_ragged_dt{dt}_d{d}_m{mode}.o")
+                serve_units.append([cc, *common_flags(), "-Rpass-analysis=kernel-resource-usage", f"-DFA2_DT={dt}",
+                                    f"-DFA2_D={d}", f"-DFA2_MODE={mode}", "-c",
+                                    os.path.join(CSRC, "attn_ragged_inst.hip"), "-o", obj])
             obj = os.path.join(OBJ_DIR, f"attn_fwd_ablate_dt{dt}_d{d}.o")
             ablate_units.append([cc, *common_flags(), f"-DFA2_DT={dt}", f"-DFA2_D={d}", "-c",
                                  os.path.join(CSRC, "attn_fwd_ablate_inst.hip"), "-o", obj])
-    serve_units.append([cc, *common_flags(), "-Rpass-analysis=kernel-resource-usage", "-c",
-                        os.path.join(CSRC, "serve_cache.hip"), "-o", os.path.join(OBJ_DIR, "serve_cache.o")])
+    for name in SERVE_UNITS:
+        serve_units.append([cc, *common_flags(), "-Rpass-analysis=kernel-resource-usage", "-c",
+                            os.path.join(CSRC, name + ".hip"), "-o", os.path.join(OBJ_DIR, name + ".o")])
     shared = []
     for name in ("attn_fwd_wavesplit", "attn_fwd_combine", "attn_key_norm"):
         remarks = ["-Rpass-analysis=kernel-resource-usage"] if name == "attn_fwd_wavesplit" else []
@@ -229,14 +253,16 @@ def build(jobs=8, verbose=False):
     for err in errs[:len(units) + 1]:  # ... and the wave-split unit, the first shared one
         for name, fields in parse_resources(err).items():
             resources[name] = {**describe_instance(name), **fields}
-    serving = {}
+    serving, step = {}, {}
     for cmd, err in zip(everything, errs):
         if cmd in serve_units:
-            for name, fields in parse_resources(err, describe_serving).items():
-                serving[name] = {**describe_serving(name), **fields}
+            for found, describe in ((serving, describe_serving), (step, describe_step)):
+                for name, fields in parse_resources(err, describe).items():
+                    found[name] = {**describe(name), **fields}
     with open(RESOURCES_PATH + ".tmp", "w") as f:
         json.dump({"arch": ARCH, "source": "hipcc -Rpass-analysis=kernel-resource-usage",
-                   "kernels": dict(sorted(resources.items())), "serving": dict(sorted(serving.items()))}, f, indent=1)
+                   "kernels": dict(sorted(resources.items())), "serving": dict(sorted(serving.items())),
+                   "step": dict(sorted(step.items()))}, f, indent=1)
     os.replace(RESOURCES_PATH + ".tmp", RESOURCES_PATH)
 
     def link(objs, path):

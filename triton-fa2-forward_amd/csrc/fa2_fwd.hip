@@ -8,7 +8,7 @@
 #include <hip/hip_runtime.h>
 
 #include "attn_fwd_host.hpp"
-#include "serve_host.hpp"
+#include "serve_step_host.hpp"
 
 namespace {
 

@@ -1,5 +1,5 @@
 // fa2_torch.cpp - fa2/_torch_call.so: the common calls of fa2.kernel.attention and of the serving operators
-// (fa2.rotary, fa2.packed, fa2.paged), made natively.
+// (fa2.rotary, fa2.packed, fa2.paged, fa2.pages), made natively.
 //
 // attention()'s checks, policy, allocations and launch took 11-17 us per call in Python and ctypes
 // (a causal call of B1 H4 N256 D64 11.2 us, a split-KV one 16.5), more than the kernels of a short
@@ -362,11 +362,97 @@ PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   END_HANDLE_TH_ERRORS
 }
 
-// cache_write(k_cache, v_cache, k_scale, v_scale, table, cu, lens, k, v, freqs, interleaved, scale, q, q_out) -> q_out, or
-// True without q
-PyObject* cache_write(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+// A HeadNorm's weight and eps at args[0] and args[1] (None: no norm)
+bool norm_of(PyObject* const* args, int64_t head_dim, c10::Device device, const float** weight, double* eps) {
+  *weight = nullptr;
+  *eps = 0.0;
+  if (args[0] == Py_None) return true;
+  const at::Tensor* w = dense_of(args[0], 1, at::kFloat, device);
+  if (!w || w->size(0) != head_dim || !PyFloat_CheckExact(args[1])) return false;
+  *weight = (const float*)w->data_ptr();
+  *eps = PyFloat_AS_DOUBLE(args[1]);
+  return true;
+}
+
+// A plan's axes (None: one) and the positions of n tokens (of `batch` of them each), as the kernels take them
+bool axes_of(PyObject* axes, PyObject* positions, int64_t batch, int64_t n, c10::Device device, fa2_turn* t, const void** p,
+             int32_t* bytes, int64_t (&stride)[3]) {
+  t->axes = nullptr;
+  t->n_axes = 1;
+  const bool several = axes != Py_None;
+  if (several) {
+    const at::Tensor* a = dense_of(axes, 1, at::kInt, device);
+    if (!a || a->size(0) != t->rotation.half) return false;
+    t->axes = (const int32_t*)a->data_ptr();
+  }
+  if (!THPVariable_CheckExact(positions)) return false;
+  const at::Tensor& x = THPVariable_Unpack(positions);
+  const at::ScalarType type = x.defined() ? x.scalar_type() : at::kFloat;
+  if (type != at::kInt && type != at::kLong) return false;
+  const int64_t dim = x.dim() - several;  // of one axis
+  if (dim != 1 && (dim != 2 || batch == 0)) return false;
+  const at::Tensor* at = tensor_of(positions, x.dim(), type, device);
+  if (!at || at->size(x.dim() - 1) != n || (dim == 2 && at->size(several) != batch) || (several && at->size(0) < 1)) return false;
+  if (several) t->n_axes = (int32_t)at->size(0);
+  stride[0] = several ? at->stride(0) : 0;
+  stride[1] = dim == 2 ? at->stride(several) : 0;
+  stride[2] = at->stride(x.dim() - 1);
+  *p = at->data_ptr();
+  *bytes = type == at::kLong ? 8 : 4;
+  return true;
+}
+
+// rotary_qk(q, k, positions, freqs, interleaved, scale, axes, q_weight, q_eps, k_weight, k_eps, q_out, k_out) ->
+// (q_out, k_out); k may be None, and so is its result then
+PyObject* rotary_qk(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   HANDLE_TH_ERRORS
-  if (!arguments("cache_write", n_args, 14)) return nullptr;
+  if (!arguments("rotary_qk", n_args, 13)) return nullptr;
+  at::ScalarType type;
+  c10::Device device(c10::kCPU);
+  if (!rows_type(args[0], &type, &device)) Py_RETURN_NONE;
+  const bool packed = THPVariable_Unpack(args[0]).dim() == 3, has_k = args[1] != Py_None;
+  const at::Tensor* q = tensor_of(args[0], packed ? 3 : 4, type, device);
+  const at::Tensor* k = has_k ? tensor_of(args[1], packed ? 3 : 4, type, device) : nullptr;
+  if (!q || q->numel() == 0 || (has_k && (!k || k->numel() == 0)) || (!has_k && (args[9] != Py_None || args[12] != Py_None)))
+    Py_RETURN_NONE;
+  const int64_t B = packed ? 1 : q->size(0), N = packed ? q->size(0) : q->size(2), D = q->size(packed ? 2 : 3);
+  if (has_k && ((packed ? k->size(0) : k->size(2)) != N || (!packed && k->size(0) != B) || k->size(packed ? 2 : 3) != D))
+    Py_RETURN_NONE;
+  fa2_turn turn;
+  const void* pp;
+  int32_t bytes;
+  int64_t ps[3], t[4][3], s[4][3] = {};
+  at::Tensor q_out, k_out;
+  if (!rotation_of(args[3], args[4], args[5], device, &turn.rotation) ||
+      !axes_of(args[6], args[2], packed ? 0 : B, N, device, &turn, &pp, &bytes, ps) ||
+      !norm_of(args + 7, D, device, &turn.q_weight, &turn.q_eps) || !norm_of(args + 9, D, device, &turn.k_weight, &turn.k_eps) ||
+      !row_strides(*q, 8, t[0]) || !out_of(args[11], *q, &q_out, t[2]) ||
+      (has_k && (!row_strides(*k, 8, t[1]) || !out_of(args[12], *k, &k_out, t[3]))))
+    Py_RETURN_NONE;
+  for (int x = 0; x < 4; ++x)
+    for (int i = 0; i < 3 && (has_k || x % 2 == 0); ++i)  // [b, h, n] of a packed [n, h]
+      s[x][i] = !packed ? t[x][i] : i == 0 ? 0 : i == 1 ? t[x][1] : t[x][0];
+  void* stream = c10::hip::getCurrentHIPStream(device.index()).stream();
+  const void *qp = q->data_ptr(), *kp = has_k ? k->data_ptr() : nullptr;
+  void *qo = q_out.data_ptr(), *ko = has_k ? k_out.data_ptr() : nullptr;
+  const int32_t hq = (int32_t)q->size(1), hk = has_k ? (int32_t)k->size(1) : 0;
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = fa2_rotary_qk(qp, kp, qo, ko, s[0], s[1], s[2], s[3], pp, bytes, ps, &turn, (int32_t)B, hq, hk, (int32_t)N, (int32_t)D,
+                     code_of(type), stream);
+  Py_END_ALLOW_THREADS
+  if (rc != FA2_OK) Py_RETURN_NONE;
+  if (has_k) return pair_of(std::move(q_out), std::move(k_out));
+  PyObject* o = THPVariable_Wrap(std::move(q_out));
+  PyObject* both = o ? PyTuple_Pack(2, o, Py_None) : nullptr;
+  Py_XDECREF(o);
+  return both;
+  END_HANDLE_TH_ERRORS
+}
+
+// cache_write(k_cache, v_cache, k_scale, v_scale, table, cu, lens, k, v, freqs, interleaved, scale, axes, q, q_out) -> q_out, or
+// True without q; cache_write_turned with q_weight, q_eps, k_weight, k_eps and positions (or None) behind them
+PyObject* write_any(PyObject* const* args, bool turned) {
   at::ScalarType type;
   c10::Device device(c10::kCPU);
   if (!rows_type(args[7], &type, &device)) Py_RETURN_NONE;
@@ -376,32 +462,136 @@ PyObject* cache_write(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   if (!k || !v || k->sizes() != v->sizes() || k->numel() == 0 ||
       !cache_and_sequences(args, type, device, k->size(0), &c, &s) || k->size(1) != c.h_kv || k->size(2) != c.head_dim)
     Py_RETURN_NONE;
-  int64_t ks[2], vs[2], qs[2], os[2];
-  fa2_rotation rot;
-  const bool turn = args[9] != Py_None, has_q = args[12] != Py_None;
+  int64_t ks[2], vs[2], qs[2], os[2], ps[3] = {};
+  fa2_turn turn;
+  const void* pp = nullptr;
+  int32_t bytes = 0;
+  const bool turn_k = args[9] != Py_None, has_q = args[13] != Py_None;
   const at::Tensor* q = nullptr;
   at::Tensor out;
   if (!row_strides(*k, 8, ks) || !row_strides(*v, 8, vs) ||
-      (turn && !rotation_of(args[9], args[10], args[11], device, &rot)) || (has_q && !turn) ||
-      (!has_q && args[13] != Py_None))
+      (turn_k && !rotation_of(args[9], args[10], args[11], device, &turn.rotation)) || (has_q && !turn_k) ||
+      (!has_q && args[14] != Py_None))
     Py_RETURN_NONE;
+  if (turned) {
+    turn.axes = nullptr;
+    turn.n_axes = 1;
+    if (!turn_k || (!has_q && args[15] != Py_None) || !norm_of(args + 15, c.head_dim, device, &turn.q_weight, &turn.q_eps) ||
+        !norm_of(args + 17, c.head_dim, device, &turn.k_weight, &turn.k_eps) ||
+        (args[19] != Py_None ? !axes_of(args[12], args[19], 0, k->size(0), device, &turn, &pp, &bytes, ps)
+                             : args[12] != Py_None))
+      Py_RETURN_NONE;
+  }
   if (has_q) {
-    q = tensor_of(args[12], 3, type, device);
+    q = tensor_of(args[13], 3, type, device);
     if (!q || q->size(0) != k->size(0) || q->size(2) != k->size(2) || q->size(1) < 1 || !row_strides(*q, 8, qs) ||
-        !out_of(args[13], *q, &out, os))
+        !out_of(args[14], *q, &out, os))
       Py_RETURN_NONE;
   }
   void* stream = c10::hip::getCurrentHIPStream(device.index()).stream();
   const void *kp = k->data_ptr(), *vp = v->data_ptr(), *qp = has_q ? q->data_ptr() : nullptr;
   void* op = has_q ? out.data_ptr() : nullptr;
   const int32_t hq = has_q ? (int32_t)q->size(1) : 0;
+  const int64_t p2[2] = {ps[0], ps[2]};
   int rc;
   Py_BEGIN_ALLOW_THREADS
-  rc = fa2_cache_write(&c, &s, kp, vp, ks, vs, qp, op, qs, os, hq, turn ? &rot : nullptr, code_of(type), stream);
+  if (turned)
+    rc = fa2_cache_write_turned(&c, &s, kp, vp, ks, vs, qp, op, qs, os, hq, pp, bytes, p2, &turn, code_of(type), stream);
+  else
+    rc = fa2_cache_write(&c, &s, kp, vp, ks, vs, qp, op, qs, os, hq, turn_k ? &turn.rotation : nullptr, code_of(type), stream);
   Py_END_ALLOW_THREADS
   if (rc != FA2_OK) Py_RETURN_NONE;
   if (!has_q) Py_RETURN_TRUE;
   return THPVariable_Wrap(std::move(out));
+}
+PyObject* cache_write(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  return arguments("cache_write", n_args, 15) ? write_any(args, false) : nullptr;
+  END_HANDLE_TH_ERRORS
+}
+PyObject* cache_write_turned(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  return arguments("cache_write_turned", n_args, 20) ? write_any(args, true) : nullptr;
+  END_HANDLE_TH_ERRORS
+}
+
+// A pool's free and count at args[0] and args[1], the table at args[2], two int32 [S] at args[3] and args[4]: plain, dense
+// (the table in its rows) and on the current device
+struct Pages {
+  const at::Tensor *free, *count, *table, *a, *b;
+  int64_t table_stride;
+};
+bool pages_of(PyObject* const* args, Pages* p) {
+  if (!THPVariable_CheckExact(args[0]) || c10::impl::dispatch_mode_enabled() || at::impl::torch_function_mode_enabled()) return false;
+  const at::Tensor& f = THPVariable_Unpack(args[0]);
+  if (!f.defined() || !f.is_cuda() || f.device().index() != c10::hip::current_device()) return false;
+  p->free = dense_of(args[0], 1, at::kInt, f.device());
+  p->count = dense_of(args[1], 1, at::kInt, f.device());
+  p->table = tensor_of(args[2], 2, at::kInt, f.device());
+  p->a = dense_of(args[3], 1, at::kInt, f.device());
+  p->b = dense_of(args[4], 1, at::kInt, f.device());
+  if (!p->free || !p->count || !p->table || !p->a || !p->b || p->count->numel() != 1) return false;
+  const int64_t S = p->table->size(0), P = p->table->size(1);
+  p->table_stride = S == 1 ? 0 : p->table->stride(0);
+  return S > 0 && p->a->size(0) == S && p->b->size(0) == S && (P <= 1 || p->table->stride(1) == 1) &&
+         (S == 1 || P == 0 || p->table_stride >= P);
+}
+
+// pages_extend(free, count, table, lens, new, page_size, n_tokens) -> (count, cu, lens, positions, slots)
+PyObject* pages_extend(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  if (!arguments("pages_extend", n_args, 7)) return nullptr;
+  Pages p;
+  if (!pages_of(args, &p) || !PyLong_CheckExact(args[5]) || !PyLong_CheckExact(args[6])) Py_RETURN_NONE;
+  int overflow = 0, overflow2 = 0;
+  const long long page = PyLong_AsLongLongAndOverflow(args[5], &overflow), n = PyLong_AsLongLongAndOverflow(args[6], &overflow2);
+  if (overflow || overflow2 || page < 1 || page > INT32_MAX || n < 0 || n > INT32_MAX) Py_RETURN_NONE;
+  const int64_t S = p.table->size(0);
+  const auto options = p.free->options();
+  at::Tensor out[5] = {at::empty({1}, options), at::empty({S + 1}, options), at::empty({S}, options), at::empty({n}, options),
+                       at::empty({n}, options.dtype(at::kLong))};
+  void* stream = c10::hip::getCurrentHIPStream(p.free->device().index()).stream();
+  int32_t* to[4];
+  for (int i = 0; i < 4; ++i) to[i] = (int32_t*)out[i].data_ptr();
+  int64_t* slots = (int64_t*)out[4].data_ptr();
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = fa2_pages_extend((const int32_t*)p.free->data_ptr(), (int32_t)p.free->size(0), (const int32_t*)p.count->data_ptr(), to[0],
+                        (int32_t*)p.table->data_ptr(), p.table_stride, (int32_t)S, (int32_t)p.table->size(1), (int32_t)page,
+                        (const int32_t*)p.a->data_ptr(), (const int32_t*)p.b->data_ptr(), to[2], to[1], to[3], slots, (int32_t)n,
+                        stream);
+  Py_END_ALLOW_THREADS
+  if (rc != FA2_OK) Py_RETURN_NONE;
+  PyObject* all = PyTuple_New(5);
+  for (int i = 0; all && i < 5; ++i) {
+    PyObject* o = THPVariable_Wrap(std::move(out[i]));
+    if (o)
+      PyTuple_SET_ITEM(all, i, o);
+    else
+      Py_CLEAR(all);
+  }
+  return all;
+  END_HANDLE_TH_ERRORS
+}
+
+// pages_release(free, count, table, first, last) -> count
+PyObject* pages_release(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  if (!arguments("pages_release", n_args, 5)) return nullptr;
+  Pages p;
+  if (!pages_of(args, &p)) Py_RETURN_NONE;
+  const int64_t S = p.table->size(0);
+  at::Tensor count = at::empty({1}, p.free->options()), counts = at::empty({S + 1}, p.free->options());
+  void* stream = c10::hip::getCurrentHIPStream(p.free->device().index()).stream();
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = fa2_pages_release((int32_t*)p.free->data_ptr(), (int32_t)p.free->size(0), (const int32_t*)p.count->data_ptr(),
+                         (int32_t*)count.data_ptr(), (const int32_t*)p.table->data_ptr(), p.table_stride, (int32_t)S,
+                         (int32_t)p.table->size(1), (const int32_t*)p.a->data_ptr(), (const int32_t*)p.b->data_ptr(),
+                         (int32_t*)counts.data_ptr(), stream);
+  Py_END_ALLOW_THREADS
+  if (rc != FA2_OK) Py_RETURN_NONE;
+  return THPVariable_Wrap(std::move(count));
   END_HANDLE_TH_ERRORS
 }
 
@@ -438,10 +628,26 @@ PyObject* cache_read(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   END_HANDLE_TH_ERRORS
 }
 
-// attn_packed(q, k, v, cu, cu_kv, causal, sm_scale, return_lse, out)
+// window (None: all keys) and sinks at args[0] and args[1], as the C ABI takes them: *window 0 without one
+bool window_of(PyObject* const* args, int causal, int32_t* window, int32_t* sinks) {
+  if (!PyLong_CheckExact(args[1])) return false;
+  int overflow = 0;
+  const long long s = PyLong_AsLongLongAndOverflow(args[1], &overflow);
+  if (overflow || s < 0) return false;
+  *window = *sinks = 0;
+  if (args[0] == Py_None) return s == 0;
+  if (!PyLong_CheckExact(args[0]) || !causal) return false;
+  const long long w = PyLong_AsLongLongAndOverflow(args[0], &overflow);
+  if (overflow || w < 1) return false;
+  *window = (int32_t)(w < INT32_MAX ? w : INT32_MAX);
+  *sinks = (int32_t)(s < INT32_MAX ? s : INT32_MAX);
+  return true;
+}
+
+// attn_packed(q, k, v, cu, cu_kv, causal, sm_scale, return_lse, out, window, sinks)
 PyObject* attn_packed(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   HANDLE_TH_ERRORS
-  if (!arguments("attn_packed", n_args, 9)) return nullptr;
+  if (!arguments("attn_packed", n_args, 11)) return nullptr;
   at::ScalarType type;
   c10::Device device(c10::kCPU);
   if (!rows_type(args[0], &type, &device)) Py_RETURN_NONE;
@@ -456,8 +662,9 @@ PyObject* attn_packed(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
     Py_RETURN_NONE;
   const float scale = qk_scale_of(args[6], q->size(2));
   int64_t qs[2], ks[2], vs[2], os[2];
+  int32_t window, sinks;
   at::Tensor out, lse;
-  if (scale == 0.f || !row_strides(*q, 8, qs) || !row_strides(*k, 8, ks) || !row_strides(*v, 8, vs) ||
+  if (scale == 0.f || !window_of(args + 9, causal, &window, &sinks) || !row_strides(*q, 8, qs) || !row_strides(*k, 8, ks) || !row_strides(*v, 8, vs) ||
       !out_of(args[8], *q, &out, os))
     Py_RETURN_NONE;
   const int32_t T = (int32_t)q->size(0), hq = (int32_t)q->size(1), hkv = (int32_t)k->size(1);
@@ -470,18 +677,23 @@ PyObject* attn_packed(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   const int32_t n_seq = (int32_t)cu->size(0) - 1, T_kv = (int32_t)k->size(0), D = (int32_t)q->size(2);
   int rc;
   Py_BEGIN_ALLOW_THREADS
-  rc = fa2_attn_packed(qp, kp, vp, op, qs, ks, vs, os, cp, ckp, n_seq, T, T_kv, hq, hkv, D, code_of(type), causal, scale,
-                       lp, stream);
+  if (window)
+    rc = fa2_attn_packed_window(qp, kp, vp, op, qs, ks, vs, os, cp, ckp, n_seq, T, T_kv, hq, hkv, D, code_of(type), window,
+                                sinks, scale, lp, stream);
+  else
+    rc = fa2_attn_packed(qp, kp, vp, op, qs, ks, vs, os, cp, ckp, n_seq, T, T_kv, hq, hkv, D, code_of(type), causal, scale,
+                         lp, stream);
   Py_END_ALLOW_THREADS
   if (rc != FA2_OK) Py_RETURN_NONE;
   return want_lse ? pair_of(std::move(out), std::move(lse)) : THPVariable_Wrap(std::move(out));
   END_HANDLE_TH_ERRORS
 }
 
-// attn_paged(k_cache, v_cache, k_scale, v_scale, table, cu, lens, q, causal, sm_scale, return_lse, out)
+// attn_paged(k_cache, v_cache, k_scale, v_scale, table, cu, lens, q, causal, sm_scale, return_lse, out, window, sinks,
+// shared)
 PyObject* attn_paged(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   HANDLE_TH_ERRORS
-  if (!arguments("attn_paged", n_args, 12)) return nullptr;
+  if (!arguments("attn_paged", n_args, 15)) return nullptr;
   at::ScalarType type;
   c10::Device device(c10::kCPU);
   if (!rows_type(args[7], &type, &device)) Py_RETURN_NONE;
@@ -496,21 +708,34 @@ PyObject* attn_paged(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   const float scale = qk_scale_of(args[9], q->size(2));
   const int cus = cu_count(device.index());
   int64_t qs[2], os[2];
+  int32_t window, sinks;
   at::Tensor out, lse, ws;
+  const at::Tensor* shared = args[14] == Py_None ? nullptr : dense_of(args[14], 1, at::kInt, device);
+  if (!window_of(args + 12, causal, &window, &sinks) || (args[14] != Py_None && (!shared || shared->numel() != 1 || window)))
+    Py_RETURN_NONE;
   if (scale == 0.f || cus < 1 || !row_strides(*q, 8, qs) || !out_of(args[11], *q, &out, os)) Py_RETURN_NONE;
   const int32_t T = (int32_t)q->size(0), hq = (int32_t)q->size(1);
   if (want_lse) lse = at::empty({hq, T}, q->options().dtype(at::kFloat));
-  const size_t n_ws = fa2_paged_workspace_bytes(hq, c.h_kv, c.head_dim, c.cache_dtype, T, s.n_seq,
-                                                (int64_t)s.max_pages * c.page_size, cus);
+  const int64_t keys = (int64_t)s.max_pages * c.page_size;
+  const size_t n_ws =
+      shared   ? fa2_paged_shared_workspace_bytes(hq, c.h_kv, c.head_dim, c.cache_dtype, T, s.n_seq, keys, cus)
+      : window ? fa2_paged_window_workspace_bytes(hq, c.h_kv, c.head_dim, c.cache_dtype, T, s.n_seq, keys, window, sinks, cus)
+               : fa2_paged_workspace_bytes(hq, c.h_kv, c.head_dim, c.cache_dtype, T, s.n_seq, keys, cus);
   if (n_ws) ws = at::empty({(int64_t)n_ws}, q->options().dtype(at::kByte));
   void* stream = c10::hip::getCurrentHIPStream(device.index()).stream();
   const void* qp = q->data_ptr();
   void* op = out.data_ptr();
   float* lp = want_lse ? static_cast<float*>(lse.data_ptr()) : nullptr;
   void* wp = n_ws ? ws.data_ptr() : nullptr;
+  const int32_t* sp = shared ? (const int32_t*)shared->data_ptr() : nullptr;
   int rc;
   Py_BEGIN_ALLOW_THREADS
-  rc = fa2_attn_paged(qp, op, qs, os, &c, &s, hq, code_of(type), causal, scale, lp, wp, n_ws, stream);
+  if (shared)
+    rc = fa2_attn_paged_shared(qp, op, qs, os, &c, &s, sp, hq, code_of(type), causal, scale, lp, wp, n_ws, stream);
+  else if (window)
+    rc = fa2_attn_paged_window(qp, op, qs, os, &c, &s, hq, code_of(type), window, sinks, scale, lp, wp, n_ws, stream);
+  else
+    rc = fa2_attn_paged(qp, op, qs, os, &c, &s, hq, code_of(type), causal, scale, lp, wp, n_ws, stream);
   Py_END_ALLOW_THREADS
   if (rc != FA2_OK) Py_RETURN_NONE;
   return want_lse ? pair_of(std::move(out), std::move(lse)) : THPVariable_Wrap(std::move(out));
@@ -521,6 +746,7 @@ PyObject* attn_paged(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, "its Python function's call, or None"}
 PyMethodDef methods[] = {
     FA2_FAST(rotary), FA2_FAST(cache_write), FA2_FAST(cache_read), FA2_FAST(attn_packed), FA2_FAST(attn_paged),
+    FA2_FAST(rotary_qk), FA2_FAST(cache_write_turned), FA2_FAST(pages_extend), FA2_FAST(pages_release),
     {"call", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(call)), METH_FASTCALL,
      "call(q, k, v, causal, sm_scale, return_lse) -> attention()'s result, or None"},
     {"policy", policy, METH_VARARGS,

@@ -52,14 +52,57 @@ struct LaneSequence {
   int first, n_q, n_kv, kv_first;
 };
 
-template <bool PAGES>
-__device__ __forceinline__ LaneSequence lane_sequence(ParamsRef p, int s) {
+// The leading tokens that all sequences with new tokens have in common, and of whose rows of the table they are read. At
+// most p.shared says, whole pages, and none that is a row's own or behind it: every row of the call sees them all.
+// Everyone who asks gets the same answer, so that the two passes over the keys agree.
+struct Prefix {
+  int tokens, row;
+};
+__device__ __forceinline__ Prefix common_prefix(ParamsRef p, int lane) {
+  const int64_t most = (int64_t)p.seq.max_pages << p.seq.page_shift;
+  int tokens = min((int64_t)max(p.shared[0], 0), most), row = p.seq.n_seq;
+  for (int s0 = 0; s0 < p.seq.n_seq; s0 += 64) {
+    const int s = s0 + lane;
+    if (s >= p.seq.n_seq) continue;
+    const int n_q = row_bound(p.seq.cu, s + 1, p.seq.n_tokens) - row_bound(p.seq.cu, s, p.seq.n_tokens);
+    if (n_q <= 0) continue;
+    tokens = min(tokens, max((int)min((int64_t)p.seq.lens[s], most) - n_q, 0));
+    row = min(row, s);
+  }
+#pragma unroll
+  for (int off = 32; off >= 1; off /= 2) {
+    tokens = min(tokens, __shfl_xor(tokens, off, 64));
+    row = min(row, __shfl_xor(row, off, 64));
+  }
+  tokens = __builtin_amdgcn_readfirstlane(tokens) & ~((1 << p.seq.page_shift) - 1);
+  row = __builtin_amdgcn_readfirstlane(row);
+  return row == p.seq.n_seq ? Prefix{0, 0} : Prefix{tokens, row};
+}
+
+// Sequences whose tiles are dealt out
+template <int MODE>
+__device__ __forceinline__ int sequences(ParamsRef p) {
+  return MODE == kModePrefix ? min(p.seq.n_seq, 1) : p.seq.n_seq;
+}
+
+// kv_first: the first key's row in k and v, or, behind a common prefix, its position in the sequence
+template <bool PAGES, int MODE>
+__device__ __forceinline__ LaneSequence lane_sequence(ParamsRef p, int s, const Prefix& prefix) {
   LaneSequence q = {0, 0, 0, 0};
-  if (s >= p.seq.n_seq) return q;
+  if (s >= sequences<MODE>(p)) return q;
   q.first = row_bound(p.seq.cu, s, p.seq.n_tokens);
+  if constexpr (MODE == kModePrefix) {
+    q.n_q = max(row_bound(p.seq.cu, p.seq.n_seq, p.seq.n_tokens) - q.first, 0);
+    q.n_kv = prefix.tokens;
+    return q;
+  }
   q.n_q = max(row_bound(p.seq.cu, s + 1, p.seq.n_tokens) - q.first, 0);
   if constexpr (PAGES) {
     q.n_kv = (int)min((int64_t)max(p.seq.lens[s], 0), (int64_t)p.seq.max_pages << p.seq.page_shift);
+    if constexpr (MODE == kModeOwn) {
+      q.kv_first = prefix.tokens;
+      q.n_kv = max(q.n_kv - prefix.tokens, 0);
+    }
   } else {
     q.kv_first = row_bound(p.cu_kv, s, p.kv_tokens);
     q.n_kv = max(row_bound(p.cu_kv, s + 1, p.kv_tokens) - q.kv_first, 0);
@@ -84,11 +127,27 @@ struct Lengths {
   __device__ int64_t of(int64_t t) const { return base + slope * t; }
   __device__ int64_t before(int64_t t) const { return t * base + slope * (t * (t - 1) / 2); }
 };
-template <int BM>
-__device__ __forceinline__ Lengths lengths_of(ParamsRef p, int n_q, int n_kv) {
-  if (!p.causal) return Lengths{(int64_t)n_kv + kTileCost<BM>, 0};
-  const int64_t slope = BM / p.group;
-  return Lengths{(int64_t)max(n_kv - n_q, 0) + slope + kTileCost<BM>, slope};
+// ... of a window, at most `cap`, which tiles reach from `full` on.
+struct WindowLengths {
+  int64_t base, slope, cap, full;
+  __device__ int64_t of(int64_t t) const { return min(base + slope * t, cap); }
+  __device__ int64_t before(int64_t t) const {
+    const int64_t u = min(t, full);
+    return u * base + slope * (u * (u - 1) / 2) + (t - u) * cap;
+  }
+};
+template <int BM, int MODE>
+__device__ __forceinline__ auto lengths_of(ParamsRef p, int n_q, int n_kv) {
+  if constexpr (MODE == kModeWindow) {
+    const int64_t slope = BM / p.group, base = (int64_t)max(n_kv - n_q, 0) + slope + kTileCost<BM>;
+    const int64_t cap = (int64_t)p.window + p.sinks + slope + kTileCost<BM>;
+    const int64_t full = base >= cap ? 0 : slope == 0 ? (int64_t)1 << 31 : (cap - base + slope - 1) / slope;
+    return WindowLengths{base, slope, cap, full};
+  } else {
+    if (MODE == kModePrefix || !p.causal) return Lengths{(int64_t)n_kv + kTileCost<BM>, 0};
+    const int64_t slope = BM / p.group;
+    return Lengths{(int64_t)max(n_kv - n_q, 0) + slope + kTileCost<BM>, slope};
+  }
 }
 
 __device__ __forceinline__ int64_t wave_scan(int64_t x, int lane) {
@@ -109,21 +168,22 @@ __device__ __forceinline__ int64_t readlane64(int64_t x, int l) {
 struct Cursor {
   int s0, l, tile;
   LaneSequence lanes;
+  Prefix prefix;
 };
 
 // The rank-th row tile; false: there are fewer.
-template <int BM, bool PAGES>
+template <int BM, bool PAGES, int MODE>
 __device__ __forceinline__ bool find_tile(ParamsRef p, int rank, int lane, Cursor* c) {
-  c->lanes = lane_sequence<PAGES>(p, lane);
-  if (p.seq.n_seq <= kFewSequences) {
+  c->lanes = lane_sequence<PAGES, MODE>(p, lane, c->prefix);
+  if (sequences<MODE>(p) <= kFewSequences) {
     // Tiles of index t and above, over all sequences: A(t) = sum_s max(tiles_s - t, 0). The rank-th tile in the
     // order of falling t has the largest t with A(t) > rank; every lane tries a t of its own.
     const int tiles = row_tiles<BM>(c->lanes.n_q, p.group);
     int hi = 0;
-    for (int s = 0; s < p.seq.n_seq; ++s) hi = max(hi, __builtin_amdgcn_readlane(tiles, s));
+    for (int s = 0; s < sequences<MODE>(p); ++s) hi = max(hi, __builtin_amdgcn_readlane(tiles, s));
     auto above = [&](int t) {
       int a = 0;
-      for (int s = 0; s < p.seq.n_seq; ++s) a += max(__builtin_amdgcn_readlane(tiles, s) - t, 0);
+      for (int s = 0; s < sequences<MODE>(p); ++s) a += max(__builtin_amdgcn_readlane(tiles, s) - t, 0);
       return a;
     };
     if (above(0) <= rank) return false;
@@ -144,8 +204,8 @@ __device__ __forceinline__ bool find_tile(ParamsRef p, int rank, int lane, Curso
     return true;
   }
   int64_t base = 0;
-  for (int s0 = 0; s0 < p.seq.n_seq; s0 += 64) {
-    if (s0) c->lanes = lane_sequence<PAGES>(p, s0 + lane);
+  for (int s0 = 0; s0 < sequences<MODE>(p); s0 += 64) {
+    if (s0) c->lanes = lane_sequence<PAGES, MODE>(p, s0 + lane, c->prefix);
     const int64_t tiles = row_tiles<BM>(c->lanes.n_q, p.group);
     const int64_t upto = base + wave_scan(tiles, lane);
     const uint64_t past = __builtin_amdgcn_ballot_w64(upto > rank);
@@ -180,18 +240,18 @@ __device__ __forceinline__ bool whole_tiles(ParamsRef p, int64_t tiles, int64_t 
 struct Share {
   int64_t x, end, in, size;
 };
-template <int BM, bool PAGES>
+template <int BM, bool PAGES, int MODE>
 __device__ __forceinline__ Share find_share(ParamsRef p, int j, int lane, Cursor* c) {
   auto length = [&]() {
-    return lengths_of<BM>(p, c->lanes.n_q, c->lanes.n_kv).before(row_tiles<BM>(c->lanes.n_q, p.group));
+    return lengths_of<BM, MODE>(p, c->lanes.n_q, c->lanes.n_kv).before(row_tiles<BM>(c->lanes.n_q, p.group));
   };
-  c->lanes = lane_sequence<PAGES>(p, lane);
+  c->lanes = lane_sequence<PAGES, MODE>(p, lane, c->prefix);
   c->s0 = 0;
   int64_t mine = length();
   int64_t upto = wave_scan(mine, lane);
   int64_t total = readlane64(upto, 63);
-  for (int s0 = 64; s0 < p.seq.n_seq; s0 += 64) {
-    c->lanes = lane_sequence<PAGES>(p, s0 + lane);
+  for (int s0 = 64; s0 < sequences<MODE>(p); s0 += 64) {
+    c->lanes = lane_sequence<PAGES, MODE>(p, s0 + lane, c->prefix);
     total += readlane64(wave_scan(length(), lane), 63);
   }
   Share w;
@@ -200,8 +260,8 @@ __device__ __forceinline__ Share find_share(ParamsRef p, int j, int lane, Cursor
   w.x = w.size * j;
   w.end = min(w.x + w.size, total);
   w.in = 0;
-  if (BM != 32 && p.seq.n_seq <= 64) {
-    const Lengths len = lengths_of<BM>(p, c->lanes.n_q, c->lanes.n_kv);
+  if (BM != 32 && sequences<MODE>(p) <= 64) {
+    const auto len = lengths_of<BM, MODE>(p, c->lanes.n_q, c->lanes.n_kv);
     const int64_t tiles = row_tiles<BM>(c->lanes.n_q, p.group), tiles_upto = wave_scan(tiles, lane);
     if (whole_tiles(p, readlane64(tiles_upto, 63), total, wave_max(tiles > 0 ? len.of(tiles - 1) : 0))) {
       const uint64_t past = __builtin_amdgcn_ballot_w64(tiles_upto > j);
@@ -215,22 +275,22 @@ __device__ __forceinline__ Share find_share(ParamsRef p, int j, int lane, Cursor
   }
   if (w.x >= w.end) return w;
   int64_t base = 0;
-  if (p.seq.n_seq > 64) c->lanes = lane_sequence<PAGES>(p, lane);
+  if (sequences<MODE>(p) > 64) c->lanes = lane_sequence<PAGES, MODE>(p, lane, c->prefix);
   while (base + readlane64(upto, 63) <= w.x) {  // (w.x < total: ends within the sequences)
     base += readlane64(upto, 63);
     c->s0 += 64;
-    if (c->s0 >= p.seq.n_seq) {  // only if the lengths changed since they were summed
+    if (c->s0 >= sequences<MODE>(p)) {  // only if the lengths changed since they were summed
       w.end = w.x;
       return w;
     }
-    c->lanes = lane_sequence<PAGES>(p, c->s0 + lane);
+    c->lanes = lane_sequence<PAGES, MODE>(p, c->s0 + lane, c->prefix);
     mine = length();
     upto = wave_scan(mine, lane);
   }
   c->l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(base + upto > w.x));
   w.in = w.x - base - readlane64(upto - mine, c->l);
   const LaneSequence q = sequence_at(c->lanes, c->l);
-  const Lengths len = lengths_of<BM>(p, q.n_q, q.n_kv);
+  const auto len = lengths_of<BM, MODE>(p, q.n_q, q.n_kv);
   int lo = 0, hi = row_tiles<BM>(q.n_q, p.group);  // the largest t with before(t) <= in
   while (hi - lo > 1) {
     const int t = (lo + hi) / 2;
@@ -253,7 +313,7 @@ __device__ __forceinline__ int cut_at(int64_t x, int64_t length, int key_tiles) 
 }
 
 // The next tile after the cursor's on the line; false: there is none.
-template <int BM, bool PAGES>
+template <int BM, bool PAGES, int MODE>
 __device__ __forceinline__ bool next_tile(ParamsRef p, int lane, Cursor* c) {
   const LaneSequence q = sequence_at(c->lanes, c->l);
   if (++c->tile < row_tiles<BM>(q.n_q, p.group)) return true;
@@ -265,10 +325,10 @@ __device__ __forceinline__ bool next_tile(ParamsRef p, int lane, Cursor* c) {
       c->l = __builtin_ctzll(have);
       return true;
     }
-    if (c->s0 + 64 >= p.seq.n_seq) return false;
+    if (c->s0 + 64 >= sequences<MODE>(p)) return false;
     c->s0 += 64;
     c->l = -1;
-    c->lanes = lane_sequence<PAGES>(p, c->s0 + lane);
+    c->lanes = lane_sequence<PAGES, MODE>(p, c->s0 + lane, c->prefix);
   }
 }
 

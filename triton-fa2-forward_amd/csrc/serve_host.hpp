@@ -184,12 +184,77 @@ int check_heads(int32_t h_q, int32_t h_kv, int32_t n_tokens, float qk_scale, con
   return FA2_OK;
 }
 
-// Launches a checked call whose heads, tensors and sequences are in p.
+int source_of(int32_t cache_dtype) { return cache_dtype == FA2_DTYPE_E4M3 ? fa2::kSourceE4m3 : fa2::kSourcePages; }
+
+// A call's arguments, checked, as the kernels take them.
+int packed_params(const void* q, const void* k, const void* v, void* out, const int64_t q_stride[2],
+                  const int64_t k_stride[2], const int64_t v_stride[2], const int64_t o_stride[2], const int32_t* cu,
+                  const int32_t* cu_kv, int32_t n_seq, int32_t n_tokens, int32_t kv_tokens, int32_t h_q, int32_t h_kv,
+                  int32_t head_dim, int32_t dtype, int32_t causal, float qk_scale, float* lse, fa2::RaggedParams* p) {
+  if (const int rc = check_type(head_dim, dtype)) return rc;
+  if (n_seq < 0 || n_tokens < 0 || kv_tokens < 0 || kv_tokens > kMaxKeys)
+    return fail(FA2_EINVAL, "bad sizes: n_seq=%d n_tokens=%d kv_tokens=%d", n_seq, n_tokens, kv_tokens);
+  if (!cu_kv && kv_tokens != n_tokens)
+    return fail(FA2_EINVAL, "k and v of %d rows for q of %d need their own cu_kv", kv_tokens, n_tokens);
+  if (const int rc = check_heads(h_q, h_kv, n_tokens, qk_scale, lse)) return rc;
+  if (n_seq == 0 || n_tokens == 0) return FA2_OK;  // (nothing to launch)
+  if (!cu) return fail(FA2_EINVAL, "null pointer: cu");
+  if (const int rc = check_rows("q", q, q_stride, 2, 8)) return rc;
+  if (const int rc = check_rows("out", out, o_stride, 2, 8)) return rc;
+  if (const int rc = check_written("out", {{n_tokens, o_stride[0]}, {h_q, o_stride[1]}})) return rc;
+  if (kv_tokens > 0) {  // (tensors of no rows may have no memory, and nothing of them is read)
+    if (const int rc = check_rows("k", k, k_stride, 2, 8)) return rc;
+    if (const int rc = check_rows("v", v, v_stride, 2, 8)) return rc;
+    if (k_stride[0] > kMaxRowStride || v_stride[0] > kMaxRowStride)
+      return fail(FA2_EINVAL, "a k/v row stride above %lld elements is not supported", (long long)kMaxRowStride);
+    p->kc.data = static_cast<char*>(const_cast<void*>(k));
+    p->kc.token = k_stride[0]; p->kc.head = k_stride[1];
+    p->vc.data = static_cast<char*>(const_cast<void*>(v));
+    p->vc.token = v_stride[0]; p->vc.head = v_stride[1];
+  }
+  p->q = static_cast<const uint16_t*>(q);
+  p->o = static_cast<uint16_t*>(out);
+  p->lse = lse;
+  p->sqt = q_stride[0]; p->sqh = q_stride[1];
+  p->sot = o_stride[0]; p->soh = o_stride[1];
+  p->seq.cu = cu;
+  p->seq.n_seq = n_seq;
+  p->seq.n_tokens = n_tokens;
+  p->cu_kv = cu_kv ? cu_kv : cu;
+  p->kv_tokens = kv_tokens;
+  p->h_kv = h_kv;
+  p->causal = causal != 0;
+  p->qk_scale = qk_scale;
+  return FA2_OK;
+}
+int paged_params(const void* q, void* out, const int64_t q_stride[2], const int64_t o_stride[2], const fa2_cache* cache,
+                 const fa2_sequences* seq, int32_t h_q, int32_t dtype, int32_t causal, float qk_scale, float* lse,
+                 fa2::RaggedParams* p) {
+  if (const int rc = check_cache(cache, seq, dtype, &p->kc, &p->vc, &p->seq)) return rc;
+  if (const int rc = check_heads(h_q, cache->h_kv, seq->n_tokens, qk_scale, lse)) return rc;
+  if (p->seq.n_seq == 0 || p->seq.n_tokens == 0) return FA2_OK;  // (nothing to launch)
+  if (const int rc = check_rows("q", q, q_stride, 2, 8)) return rc;
+  if (const int rc = check_rows("out", out, o_stride, 2, 8)) return rc;
+  if (const int rc = check_written("out", {{p->seq.n_tokens, o_stride[0]}, {h_q, o_stride[1]}})) return rc;
+  p->q = static_cast<const uint16_t*>(q);
+  p->o = static_cast<uint16_t*>(out);
+  p->lse = lse;
+  p->sqt = q_stride[0]; p->sqh = q_stride[1];
+  p->sot = o_stride[0]; p->soh = o_stride[1];
+  p->h_kv = cache->h_kv;
+  p->causal = causal != 0;
+  p->qk_scale = qk_scale;
+  return FA2_OK;
+}
+
+// Launches a checked call whose heads, tensors and sequences are in p. keys: see ragged_plan.
+template <int MODE = fa2::kModeAll>
 int launch_ragged(int32_t dtype, int32_t head_dim, int32_t h_q, fa2::RaggedParams& p, int source, int64_t keys, void* workspace,
                   size_t workspace_bytes, void* stream) {
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const Topology topo = device_topology(stream_device(s));
-  const RaggedPlan pl = ragged_plan(source, h_q, p.h_kv, head_dim, p.seq.n_tokens, p.seq.n_seq, keys, topo.cus);
+  const int32_t n_seq = MODE == fa2::kModePrefix ? 1 : p.seq.n_seq;
+  const RaggedPlan pl = ragged_plan(source, h_q, p.h_kv, head_dim, p.seq.n_tokens, n_seq, keys, topo.cus);
   if (pl.grid > 0x7fffffffLL) return fail(FA2_EINVAL, "grid of %lld workgroups is too large", (long long)pl.grid);
   if (pl.workspace) {
     if (!workspace || workspace_bytes < pl.workspace)
@@ -206,16 +271,49 @@ int launch_ragged(int32_t dtype, int32_t head_dim, int32_t h_q, fa2::RaggedParam
   const unsigned g = (unsigned)pl.grid;
   int e;
   switch (dtype * 4 + dim_index(head_dim)) {
-    case 0: e = fa2::launch_ragged<0, 16>(p, source, pl.row_waves, g, s); break;
-    case 1: e = fa2::launch_ragged<0, 32>(p, source, pl.row_waves, g, s); break;
-    case 2: e = fa2::launch_ragged<0, 64>(p, source, pl.row_waves, g, s); break;
-    case 3: e = fa2::launch_ragged<0, 128>(p, source, pl.row_waves, g, s); break;
-    case 4: e = fa2::launch_ragged<1, 16>(p, source, pl.row_waves, g, s); break;
-    case 5: e = fa2::launch_ragged<1, 32>(p, source, pl.row_waves, g, s); break;
-    case 6: e = fa2::launch_ragged<1, 64>(p, source, pl.row_waves, g, s); break;
-    default: e = fa2::launch_ragged<1, 128>(p, source, pl.row_waves, g, s);
+    case 0: e = fa2::launch_ragged<0, 16, MODE>(p, source, pl.row_waves, g, s); break;
+    case 1: e = fa2::launch_ragged<0, 32, MODE>(p, source, pl.row_waves, g, s); break;
+    case 2: e = fa2::launch_ragged<0, 64, MODE>(p, source, pl.row_waves, g, s); break;
+    case 3: e = fa2::launch_ragged<0, 128, MODE>(p, source, pl.row_waves, g, s); break;
+    case 4: e = fa2::launch_ragged<1, 16, MODE>(p, source, pl.row_waves, g, s); break;
+    case 5: e = fa2::launch_ragged<1, 32, MODE>(p, source, pl.row_waves, g, s); break;
+    case 6: e = fa2::launch_ragged<1, 64, MODE>(p, source, pl.row_waves, g, s); break;
+    default: e = fa2::launch_ragged<1, 128, MODE>(p, source, pl.row_waves, g, s);
   }
   return launched(e, "attention");
+}
+
+int write_params(const fa2_cache* cache, const fa2_sequences* seq, const void* k, const void* v, const int64_t k_stride[2],
+                 const int64_t v_stride[2], const void* q, void* q_out, const int64_t q_stride[2], const int64_t qo_stride[2],
+                 int32_t h_q, const fa2_rotation* rotation, int32_t dtype, fa2::CacheParams* p) {
+  if (const int rc = check_cache(cache, seq, dtype, &p->kc, &p->vc, &p->seq)) return rc;
+  if (const int rc = check_rotation(rotation, cache->head_dim, &p->rot)) return rc;
+  if (q && !rotation) return fail(FA2_EINVAL, "q is taken to be rotated: it needs a rotation");
+  if (q && h_q < 1) return fail(FA2_EINVAL, "bad sizes: h_q=%d", h_q);
+  if (cache->h_kv > (1 << 24) || h_q > (1 << 24)) return fail(FA2_EINVAL, "at most 2^24 heads");
+  if (p->seq.n_seq == 0 || p->seq.n_tokens == 0) return FA2_OK;  // (nothing to launch)
+  for (const int64_t* s : {cache->k_stride, cache->v_stride, p->kc.scale ? cache->k_scale_stride : cache->k_stride,
+                           p->kc.scale ? cache->v_scale_stride : cache->v_stride})
+    if (const int rc = check_written("the cache", {{cache->n_pages, s[0]}, {cache->h_kv, s[1]}, {cache->page_size, s[2]}}))
+      return rc;
+  if (const int rc = check_rows("k", k, k_stride, 2, 8)) return rc;
+  if (const int rc = check_rows("v", v, v_stride, 2, 8)) return rc;
+  if (q) {
+    if (const int rc = check_rows("q", q, q_stride, 2, 8)) return rc;
+    if (const int rc = check_rows("q_out", q_out, qo_stride, 2, 8)) return rc;
+    if (const int rc = check_written("q_out", {{p->seq.n_tokens, qo_stride[0]}, {h_q, qo_stride[1]}})) return rc;
+    p->q = static_cast<const uint16_t*>(q);
+    p->q_out = static_cast<uint16_t*>(q_out);
+    p->sqt = q_stride[0]; p->sqh = q_stride[1];
+    p->sot = qo_stride[0]; p->soh = qo_stride[1];
+    p->h_q = h_q;
+  }
+  p->k = static_cast<uint16_t*>(const_cast<void*>(k));
+  p->v = static_cast<uint16_t*>(const_cast<void*>(v));
+  p->skt = k_stride[0]; p->skh = k_stride[1];
+  p->svt = v_stride[0]; p->svh = v_stride[1];
+  p->h_kv = cache->h_kv;
+  return FA2_OK;
 }
 
 }  // namespace
@@ -263,33 +361,9 @@ int fa2_cache_write(const fa2_cache* cache, const fa2_sequences* seq, const void
                     const fa2_rotation* rotation, int32_t dtype, void* stream) {
   g_err[0] = '\0';
   fa2::CacheParams p{};
-  if (const int rc = check_cache(cache, seq, dtype, &p.kc, &p.vc, &p.seq)) return rc;
-  if (const int rc = check_rotation(rotation, cache->head_dim, &p.rot)) return rc;
-  if (q && !rotation) return fail(FA2_EINVAL, "q is taken to be rotated: it needs a rotation");
-  if (q && h_q < 1) return fail(FA2_EINVAL, "bad sizes: h_q=%d", h_q);
-  if (cache->h_kv > (1 << 24) || h_q > (1 << 24)) return fail(FA2_EINVAL, "at most 2^24 heads");
+  if (const int rc = write_params(cache, seq, k, v, k_stride, v_stride, q, q_out, q_stride, qo_stride, h_q, rotation, dtype, &p))
+    return rc;
   if (p.seq.n_seq == 0 || p.seq.n_tokens == 0) return FA2_OK;
-  for (const int64_t* s : {cache->k_stride, cache->v_stride, p.kc.scale ? cache->k_scale_stride : cache->k_stride,
-                           p.kc.scale ? cache->v_scale_stride : cache->v_stride})
-    if (const int rc = check_written("the cache", {{cache->n_pages, s[0]}, {cache->h_kv, s[1]}, {cache->page_size, s[2]}}))
-      return rc;
-  if (const int rc = check_rows("k", k, k_stride, 2, 8)) return rc;
-  if (const int rc = check_rows("v", v, v_stride, 2, 8)) return rc;
-  if (q) {
-    if (const int rc = check_rows("q", q, q_stride, 2, 8)) return rc;
-    if (const int rc = check_rows("q_out", q_out, qo_stride, 2, 8)) return rc;
-    if (const int rc = check_written("q_out", {{p.seq.n_tokens, qo_stride[0]}, {h_q, qo_stride[1]}})) return rc;
-    p.q = static_cast<const uint16_t*>(q);
-    p.q_out = static_cast<uint16_t*>(q_out);
-    p.sqt = q_stride[0]; p.sqh = q_stride[1];
-    p.sot = qo_stride[0]; p.soh = qo_stride[1];
-    p.h_q = h_q;
-  }
-  p.k = static_cast<uint16_t*>(const_cast<void*>(k));
-  p.v = static_cast<uint16_t*>(const_cast<void*>(v));
-  p.skt = k_stride[0]; p.skh = k_stride[1];
-  p.svt = v_stride[0]; p.svh = v_stride[1];
-  p.h_kv = cache->h_kv;
   const unsigned grid = cache_grid(&p, 2 * (int64_t)p.h_kv + p.h_q, cache->head_dim, kWriteWgs);
   return launched(fa2::launch_cache(true, dtype, cache->head_dim, cache->cache_dtype == FA2_DTYPE_E4M3, p, grid,
                                     static_cast<hipStream_t>(stream)),
@@ -325,40 +399,10 @@ int fa2_attn_packed(const void* q, const void* k, const void* v, void* out, cons
                     float* lse, void* stream) {
   g_err[0] = '\0';
   fa2::RaggedParams p{};
-  if (const int rc = check_type(head_dim, dtype)) return rc;
-  if (n_seq < 0 || n_tokens < 0 || kv_tokens < 0 || kv_tokens > kMaxKeys)
-    return fail(FA2_EINVAL, "bad sizes: n_seq=%d n_tokens=%d kv_tokens=%d", n_seq, n_tokens, kv_tokens);
-  if (!cu_kv && kv_tokens != n_tokens)
-    return fail(FA2_EINVAL, "k and v of %d rows for q of %d need their own cu_kv", kv_tokens, n_tokens);
-  if (const int rc = check_heads(h_q, h_kv, n_tokens, qk_scale, lse)) return rc;
+  if (const int rc = packed_params(q, k, v, out, q_stride, k_stride, v_stride, o_stride, cu, cu_kv, n_seq, n_tokens,
+                                   kv_tokens, h_q, h_kv, head_dim, dtype, causal, qk_scale, lse, &p))
+    return rc;
   if (n_seq == 0 || n_tokens == 0) return FA2_OK;
-  if (!cu) return fail(FA2_EINVAL, "null pointer: cu");
-  if (const int rc = check_rows("q", q, q_stride, 2, 8)) return rc;
-  if (const int rc = check_rows("out", out, o_stride, 2, 8)) return rc;
-  if (const int rc = check_written("out", {{n_tokens, o_stride[0]}, {h_q, o_stride[1]}})) return rc;
-  if (kv_tokens > 0) {  // (tensors of no rows may have no memory, and nothing of them is read)
-    if (const int rc = check_rows("k", k, k_stride, 2, 8)) return rc;
-    if (const int rc = check_rows("v", v, v_stride, 2, 8)) return rc;
-    if (k_stride[0] > kMaxRowStride || v_stride[0] > kMaxRowStride)
-      return fail(FA2_EINVAL, "a k/v row stride above %lld elements is not supported", (long long)kMaxRowStride);
-    p.kc.data = static_cast<char*>(const_cast<void*>(k));
-    p.kc.token = k_stride[0]; p.kc.head = k_stride[1];
-    p.vc.data = static_cast<char*>(const_cast<void*>(v));
-    p.vc.token = v_stride[0]; p.vc.head = v_stride[1];
-  }
-  p.q = static_cast<const uint16_t*>(q);
-  p.o = static_cast<uint16_t*>(out);
-  p.lse = lse;
-  p.sqt = q_stride[0]; p.sqh = q_stride[1];
-  p.sot = o_stride[0]; p.soh = o_stride[1];
-  p.seq.cu = cu;
-  p.seq.n_seq = n_seq;
-  p.seq.n_tokens = n_tokens;
-  p.cu_kv = cu_kv ? cu_kv : cu;
-  p.kv_tokens = kv_tokens;
-  p.h_kv = h_kv;
-  p.causal = causal != 0;
-  p.qk_scale = qk_scale;
   return launch_ragged(dtype, head_dim, h_q, p, fa2::kSourcePacked, kv_tokens, nullptr, 0, stream);
 }
 
@@ -367,28 +411,15 @@ int fa2_attn_paged(const void* q, void* out, const int64_t q_stride[2], const in
                    float qk_scale, float* lse, void* workspace, size_t workspace_bytes, void* stream) {
   g_err[0] = '\0';
   fa2::RaggedParams p{};
-  if (const int rc = check_cache(cache, seq, dtype, &p.kc, &p.vc, &p.seq)) return rc;
-  if (const int rc = check_heads(h_q, cache->h_kv, seq->n_tokens, qk_scale, lse)) return rc;
+  if (const int rc = paged_params(q, out, q_stride, o_stride, cache, seq, h_q, dtype, causal, qk_scale, lse, &p)) return rc;
   if (p.seq.n_seq == 0 || p.seq.n_tokens == 0) return FA2_OK;
-  if (const int rc = check_rows("q", q, q_stride, 2, 8)) return rc;
-  if (const int rc = check_rows("out", out, o_stride, 2, 8)) return rc;
-  if (const int rc = check_written("out", {{p.seq.n_tokens, o_stride[0]}, {h_q, o_stride[1]}})) return rc;
-  p.q = static_cast<const uint16_t*>(q);
-  p.o = static_cast<uint16_t*>(out);
-  p.lse = lse;
-  p.sqt = q_stride[0]; p.sqh = q_stride[1];
-  p.sot = o_stride[0]; p.soh = o_stride[1];
-  p.h_kv = cache->h_kv;
-  p.causal = causal != 0;
-  p.qk_scale = qk_scale;
-  return launch_ragged(dtype, cache->head_dim, h_q, p,
-                       cache->cache_dtype == FA2_DTYPE_E4M3 ? fa2::kSourceE4m3 : fa2::kSourcePages,
+  return launch_ragged(dtype, cache->head_dim, h_q, p, source_of(cache->cache_dtype),
                        (int64_t)p.seq.max_pages << p.seq.page_shift, workspace, workspace_bytes, stream);
 }
 
 size_t fa2_paged_workspace_bytes(int32_t h_q, int32_t h_kv, int32_t head_dim, int32_t cache_dtype, int32_t n_tokens,
                                  int32_t n_seq, int64_t max_keys, int32_t num_cus) {
-  const int source = cache_dtype == FA2_DTYPE_E4M3 ? fa2::kSourceE4m3 : fa2::kSourcePages;
+  const int source = source_of(cache_dtype);
   if (h_q <= 0 || h_kv <= 0 || h_q % h_kv || dim_index(head_dim) < 0 || n_tokens <= 0 || n_seq <= 0 || num_cus <= 0) return 0;
   return ragged_plan(source, h_q, h_kv, head_dim, n_tokens, n_seq, max_keys, num_cus).workspace;
 }

@@ -15,6 +15,12 @@ int launch_rotary(int dtype, int head_dim, const RotaryParams& p, unsigned grid,
 int launch_cache(bool write, int dtype, int head_dim, bool e4m3, const CacheParams& p, unsigned grid,
                  hipStream_t stream);
 
+int launch_rotary_qk(int dtype, int head_dim, const RotaryQkParams& p, unsigned grid, hipStream_t stream);
+int launch_cache_write_turn(int dtype, int head_dim, bool e4m3, const CacheTurnParams& p, unsigned grid, hipStream_t stream);
+
+int launch_pages_extend(const PagesParams& p, unsigned blocks, unsigned stripes, hipStream_t stream);
+int launch_pages_release(const ReleaseParams& p, hipStream_t stream);
+
 // Where K and V of a ragged attention launch lie: packed rows, 16-bit pages, e4m3 pages.
 constexpr int kSourcePacked = 0, kSourcePages = 1, kSourceE4m3 = 2;
 
@@ -30,12 +36,18 @@ constexpr int ragged_waves(int head_dim, int source, int row_waves) {
 
 // The ragged attention kernel with 32 * row_waves (1 or 4) rows per workgroup, and after it, with p.shares > 0,
 // the merge of the row tiles that its shares cut.
-template <int DT, int D>
+template <int DT, int D, int MODE>
 int launch_ragged(const RaggedParams& p, int source, int row_waves, unsigned grid, hipStream_t stream);
 
-#define FA2_DECLARE_RAGGED(DT, D) \
-  template <>                     \
-  int launch_ragged<DT, D>(const RaggedParams&, int, int, unsigned, hipStream_t);
+#define FA2_DECLARE_RAGGED(DT, D)                                                      \
+  template <>                                                                          \
+  int launch_ragged<DT, D, kModeAll>(const RaggedParams&, int, int, unsigned, hipStream_t);    \
+  template <>                                                                          \
+  int launch_ragged<DT, D, kModeWindow>(const RaggedParams&, int, int, unsigned, hipStream_t); \
+  template <>                                                                          \
+  int launch_ragged<DT, D, kModePrefix>(const RaggedParams&, int, int, unsigned, hipStream_t); \
+  template <>                                                                          \
+  int launch_ragged<DT, D, kModeOwn>(const RaggedParams&, int, int, unsigned, hipStream_t);
 FA2_DECLARE_RAGGED(0, 16)
 FA2_DECLARE_RAGGED(0, 32)
 FA2_DECLARE_RAGGED(0, 64)

@@ -64,7 +64,60 @@ struct CacheParams {
   RotaryPlan rot;
 };
 
+// What rows of q and k are turned by, beyond a rotation by one position: each head first divided by its root mean
+// square, x / sqrt(mean x^2 + eps) * weight (float32 [head_dim]; null: not), and pair i rotated by the position on
+// axis axes[i] of n_axes (null: all by the first; an entry outside them by the nearest).
+struct TurnParams {
+  const int32_t* axes;
+  int32_t n_axes;
+  int32_t positions64;
+  const void* positions;  // int32 or int64, element strides [axis, batch, token]; null: the place in the sequence
+  int64_t spa, spb, spn;
+  const float *q_weight, *k_weight;
+  double q_eps, k_eps;
+};
+
+struct RotaryQkParams {
+  const uint16_t *q, *k;
+  uint16_t *q_out, *k_out;
+  int64_t sqb, sqh, sqn, skb, skh, skn;
+  int64_t sqob, sqoh, sqon, skob, skoh, skon;
+  int32_t batch, h_q, h_k, n;
+  int32_t tokens_per_wg;
+  RotaryPlan rot;
+  TurnParams turn;
+};
+
+struct CacheTurnParams : CacheParams {
+  TurnParams turn;
+};
+
+// A step's pages (serve_pages.hip): free_pages[0 .. count) are free; results in memory of their own, but the table's.
+struct PagesParams {
+  const int32_t* free_pages;
+  const int32_t* count;
+  int32_t* table;
+  const int32_t *lens, *fresh;  // [n_seq]: tokens in the cache, and new ones
+  int64_t table_stride;
+  int32_t n_pages, n_seq, max_pages, page_shift, n_tokens;
+  int32_t *count_out, *lens_out, *cu_out, *positions;
+  int64_t* slots;
+};
+
+struct ReleaseParams {
+  int32_t* free_pages;
+  const int32_t *count, *table, *first, *last;
+  int64_t table_stride;
+  int32_t n_pages, n_seq, max_pages;
+  int32_t* count_out;
+  int32_t* counts;  // [n_seq + 1]
+};
+
 constexpr int kMergeBytes = 32;
+
+// What keys the rows of a ragged attention launch take: all up to their last; those of a window and the first
+// few; of sequences with a common prefix, the prefix's (all rows as those of one sequence), or their own behind it.
+constexpr int kModeAll = 0, kModeWindow = 1, kModePrefix = 2, kModeOwn = 3;
 
 // Attention of packed rows. K and V are packed rows too (source 0), pages of 16-bit elements (1) or of
 // e4m3 (2).
@@ -86,6 +139,12 @@ struct RaggedParams {
   double per_share;  // 1 / shares
   float* parts;  // [h_kv * shares][2][block_m][head_dim + 4]: O, then m, l, exact l
   void* merges;  // [h_kv * shares] of kMergeBytes: the tile that ends in each share
+  // kModeWindow: a row sees the `window` newest keys up to its last, and the first `sinks`
+  int32_t window, sinks;
+  // kModePrefix and kModeOwn: the leading tokens that all sequences have in common, on the device, and the results
+  // over them: [n_tokens * h_q][head_dim + 4] of O, m, l, exact l
+  const int32_t* shared;
+  float* prefix;
 };
 
 }  // namespace fa2

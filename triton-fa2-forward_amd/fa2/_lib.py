@@ -37,7 +37,13 @@ class Rotation(ctypes.Structure):
     _fields_ = [("freqs", _vp), ("half", _i32), ("interleaved", _i32), ("scale", ctypes.c_double)]
 
 
-_cachep, _seqp, _rotp = (ctypes.POINTER(t) for t in (Cache, Sequences, Rotation))
+class Turn(ctypes.Structure):
+    """fa2_turn"""
+    _fields_ = [("rotation", Rotation), ("axes", _vp), ("q_weight", _vp), ("k_weight", _vp), ("q_eps", ctypes.c_double),
+                ("k_eps", ctypes.c_double), ("n_axes", _i32)]
+
+
+_cachep, _seqp, _rotp, _turnp = (ctypes.POINTER(t) for t in (Cache, Sequences, Rotation, Turn))
 SIGNATURES = {
     "fa2_attn_fwd": (ctypes.c_int, [_vp, _vp, _vp, _vp, _i64p, _i64p, _i64p, _i64p,
                                     _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32,
@@ -67,6 +73,19 @@ SIGNATURES = {
     "fa2_attn_paged": (ctypes.c_int, [_vp, _vp, _i64p, _i64p, _cachep, _seqp, _i32, _i32, _i32, ctypes.c_float,
                                       _vp, _vp, ctypes.c_size_t, _vp]),
     "fa2_paged_workspace_bytes": (ctypes.c_size_t, [_i32] * 6 + [_i64, _i32]),
+    "fa2_attn_packed_window": (ctypes.c_int, [_vp, _vp, _vp, _vp, _i64p, _i64p, _i64p, _i64p, _vp, _vp, _i32, _i32, _i32,
+                                              _i32, _i32, _i32, _i32, _i32, _i32, ctypes.c_float, _vp, _vp]),
+    "fa2_attn_paged_window": (ctypes.c_int, [_vp, _vp, _i64p, _i64p, _cachep, _seqp, _i32, _i32, _i32, _i32, ctypes.c_float,
+                                             _vp, _vp, ctypes.c_size_t, _vp]),
+    "fa2_paged_window_workspace_bytes": (ctypes.c_size_t, [_i32] * 6 + [_i64, _i32, _i32, _i32]),
+    "fa2_attn_paged_shared": (ctypes.c_int, [_vp, _vp, _i64p, _i64p, _cachep, _seqp, _vp, _i32, _i32, _i32, ctypes.c_float,
+                                             _vp, _vp, ctypes.c_size_t, _vp]),
+    "fa2_paged_shared_workspace_bytes": (ctypes.c_size_t, [_i32] * 6 + [_i64, _i32]),
+    "fa2_rotary_qk": (ctypes.c_int, [_vp] * 4 + [_i64p] * 4 + [_vp, _i32, _i64p, _turnp] + [_i32] * 6 + [_vp]),
+    "fa2_cache_write_turned": (ctypes.c_int, [_cachep, _seqp, _vp, _vp, _i64p, _i64p, _vp, _vp, _i64p, _i64p, _i32, _vp,
+                                              _i32, _i64p, _turnp, _i32, _vp]),
+    "fa2_pages_extend": (ctypes.c_int, [_vp, _i32, _vp, _vp, _vp, _i64, _i32, _i32, _i32] + [_vp] * 6 + [_i32, _vp]),
+    "fa2_pages_release": (ctypes.c_int, [_vp, _i32, _vp, _vp, _vp, _i64, _i32, _i32, _vp, _vp, _vp, _vp]),
     "fa2_last_error": (ctypes.c_char_p, []),
     "fa2_version": (ctypes.c_char_p, []),
 }
@@ -301,3 +320,94 @@ def attn_paged(q, out, cache, seq, causal, qk_scale, lse, workspace, stream):
                                   ctypes.byref(seq), q.shape[1], DTYPE_CODE[q.dtype], int(bool(causal)), qk_scale,
                                   _ptr(lse), _ptr(workspace), 0 if workspace is None else workspace.numel(), stream),
              "fa2_attn_paged")
+
+
+# ---- a step beyond that: windows, a common prefix, normalised rotations of several axes, pages
+
+def turn_of(plan, freqs, axes, n_axes, q_norm, k_norm):
+    """The C description of a fa2.rotary.Rotary and the heads' norms (checked; None: no norm)."""
+    q_weight, q_eps = (None, 0.0) if q_norm is None else q_norm
+    k_weight, k_eps = (None, 0.0) if k_norm is None else k_norm
+    return Turn(Rotation(freqs.data_ptr(), freqs.numel(), plan.interleaved, plan.scale), _ptr(axes), _ptr(q_weight),
+                _ptr(k_weight), q_eps, k_eps, n_axes)
+
+
+def rotary_qk(q, k, q_out, k_out, positions, turn, stream):
+    """Call fa2_rotary_qk on [B, H, N, D] tensors (k and k_out may be None) and positions [axes, B, N]."""
+    B, H, N, D = q.shape
+    H_k = 0 if k is None else k.shape[1]
+    _int32(B=B, H_q=H, H_k=H_k, N=N)
+    none = (ctypes.c_int64 * 4)()
+    _checked(lib().fa2_rotary_qk(
+        q.data_ptr(), _ptr(k), q_out.data_ptr(), _ptr(k_out), _strides(q), none if k is None else _strides(k),
+        _strides(q_out), none if k is None else _strides(k_out), positions.data_ptr(), positions.element_size(),
+        (ctypes.c_int64 * 3)(*positions.stride()), ctypes.byref(turn), B, H, H_k, N, D, DTYPE_CODE[q.dtype], stream),
+        "fa2_rotary_qk")
+
+
+def cache_write_turned(cache, seq, k, v, q, q_out, positions, turn, stream):
+    """Call fa2_cache_write_turned; q and q_out, and positions [axes, T], may be None."""
+    _int32(H_q=0 if q is None else q.shape[1])
+    _checked(lib().fa2_cache_write_turned(
+        ctypes.byref(cache), ctypes.byref(seq), k.data_ptr(), v.data_ptr(), _strides(k), _strides(v), _ptr(q), _ptr(q_out),
+        None if q is None else _strides(q), None if q is None else _strides(q_out), 0 if q is None else q.shape[1],
+        _ptr(positions), 0 if positions is None else positions.element_size(),
+        None if positions is None else (ctypes.c_int64 * 2)(*positions.stride()), ctypes.byref(turn), DTYPE_CODE[k.dtype],
+        stream), "fa2_cache_write_turned")
+
+
+def attn_packed_window(q, k, v, out, cu, cu_kv, window, sinks, qk_scale, lse, stream):
+    """Call fa2_attn_packed_window; cu_kv and lse may be None."""
+    T, H_q, D = q.shape
+    _int32(T=T, H_q=H_q, T_kv=k.shape[0], H_kv=k.shape[1], sequences=cu.numel() - 1)
+    _checked(lib().fa2_attn_packed_window(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _strides(q), _strides(k), _strides(v),
+        _strides(out), cu.data_ptr(), _ptr(cu_kv), cu.numel() - 1, T, k.shape[0], H_q, k.shape[1], D,
+        DTYPE_CODE[q.dtype], window, sinks, qk_scale, _ptr(lse), stream), "fa2_attn_packed_window")
+
+
+def paged_window_workspace_bytes(H_q, H_kv, D, cache_dtype, n_tokens, n_seq, max_keys, window, sinks, num_cus):
+    return int(lib().fa2_paged_window_workspace_bytes(H_q, H_kv, D, CACHE_DTYPE_CODE[cache_dtype], n_tokens, n_seq, max_keys,
+                                                      window, sinks, num_cus))
+
+
+def attn_paged_window(q, out, cache, seq, window, sinks, qk_scale, lse, workspace, stream):
+    """Call fa2_attn_paged_window; lse and workspace (uint8) may be None."""
+    _int32(H_q=q.shape[1])
+    _checked(lib().fa2_attn_paged_window(
+        q.data_ptr(), out.data_ptr(), _strides(q), _strides(out), ctypes.byref(cache), ctypes.byref(seq), q.shape[1],
+        DTYPE_CODE[q.dtype], window, sinks, qk_scale, _ptr(lse), _ptr(workspace),
+        0 if workspace is None else workspace.numel(), stream), "fa2_attn_paged_window")
+
+
+def paged_shared_workspace_bytes(H_q, H_kv, D, cache_dtype, n_tokens, n_seq, max_keys, num_cus):
+    return int(lib().fa2_paged_shared_workspace_bytes(H_q, H_kv, D, CACHE_DTYPE_CODE[cache_dtype], n_tokens, n_seq, max_keys,
+                                                      num_cus))
+
+
+def attn_paged_shared(q, out, cache, seq, shared, causal, qk_scale, lse, workspace, stream):
+    """Call fa2_attn_paged_shared; lse may be None."""
+    _int32(H_q=q.shape[1])
+    _checked(lib().fa2_attn_paged_shared(
+        q.data_ptr(), out.data_ptr(), _strides(q), _strides(out), ctypes.byref(cache), ctypes.byref(seq), shared.data_ptr(),
+        q.shape[1], DTYPE_CODE[q.dtype], int(bool(causal)), qk_scale, _ptr(lse), _ptr(workspace), workspace.numel(), stream),
+        "fa2_attn_paged_shared")
+
+
+def pages_extend(free, count, count_out, table, page_size, lens, new_tokens, lens_out, cu_out, positions, slots, stream):
+    """Call fa2_pages_extend on int32 tensors (slots int64) that satisfy fa2.pages' checks."""
+    S, P = table.shape
+    _int32(pages=free.numel(), sequences=S, table_columns=P, page_size=page_size, n_tokens=slots.numel())
+    _checked(lib().fa2_pages_extend(
+        free.data_ptr(), free.numel(), count.data_ptr(), count_out.data_ptr(), table.data_ptr(), 0 if S == 1 else table.stride(0),
+        S, P, page_size, lens.data_ptr(), new_tokens.data_ptr(), lens_out.data_ptr(), cu_out.data_ptr(), positions.data_ptr(),
+        slots.data_ptr(), slots.numel(), stream), "fa2_pages_extend")
+
+
+def pages_release(free, count, count_out, table, first, last, workspace, stream):
+    """Call fa2_pages_release on int32 tensors that satisfy fa2.pages' checks."""
+    S, P = table.shape
+    _int32(pages=free.numel(), sequences=S, table_columns=P)
+    _checked(lib().fa2_pages_release(
+        free.data_ptr(), free.numel(), count.data_ptr(), count_out.data_ptr(), table.data_ptr(), 0 if S == 1 else table.stride(0),
+        S, P, first.data_ptr(), last.data_ptr(), workspace.data_ptr(), stream), "fa2_pages_release")

@@ -8,11 +8,14 @@ lengths that its tensors hold at each replay.
 """
 
 import math
+import operator
 
 import torch
 
 from . import _lib
 from .kernel import _MAX_KV_ROW_STRIDE, LOG2E
+
+_MOST = (1 << 31) - 1  # more tokens than any sequence has
 
 
 def _rows(t, max_row_stride=None):
@@ -40,6 +43,20 @@ def _scale(sm_scale, head_dim):
     return sm_scale * LOG2E
 
 
+def _window(window, sinks, causal):
+    """(window, sinks) of a call as the C ABI takes them; (None, 0): all keys."""
+    if window is None:
+        if sinks:
+            raise ValueError("sinks are the tokens that stay visible beside a window")
+        return None, 0
+    window, sinks = operator.index(window), operator.index(sinks)
+    if window < 1 or sinks < 0:
+        raise ValueError(f"window must be positive and sinks not negative, got {window} and {sinks}")
+    if not causal:
+        raise ValueError("a window needs the causal mask")
+    return min(window, _MOST), min(sinks, _MOST)
+
+
 def _output(q, out):
     """(the caller's out, the tensor the kernel writes): the same, or a copy that holds out's rows where the
     kernel cannot address out."""
@@ -51,8 +68,8 @@ def _output(q, out):
     return out, _rows(out)
 
 
-def attention_packed(q, k, v, cu_seqlens, cu_seqlens_kv=None, *, causal=True, sm_scale=None, return_lse=False,
-                     out=None):
+def attention_packed(q, k, v, cu_seqlens, cu_seqlens_kv=None, *, causal=True, window=None, sinks=0, sm_scale=None,
+                     return_lse=False, out=None):
     """softmax(Q K^T * sm_scale [+ causal mask]) V within each of the packed sequences.
 
     q: [T, H_q, D]; k, v: [T_kv, H_kv, D], fp16 or bf16, D in (16, 32, 64, 128), H_q % H_kv == 0; returns out
@@ -62,12 +79,14 @@ def attention_packed(q, k, v, cu_seqlens, cu_seqlens_kv=None, *, causal=True, sm
         out (undefined in a new one).
     causal: row i of a sequence sees its keys up to i + n_kv - n_q (with one cu_seqlens: up to its own).
         A row that sees no key gets 0, and a log-sum-exp of -inf.
+    window: (with causal) a row whose last key is n sees the `window` newest, n - window + 1 .. n, and the sequence's first
+        `sinks`; keys that no row sees are not read.
     return_lse: also return the natural-log log-sum-exp of every row's scaled scores, fp32 [H_q, T].
     out: of q's shape and type, in any layout without shared elements; q itself is allowed, and no other memory that
         the call reads.
     """
     if _lib.native is not None:  # the common call, made natively; None: not one of those
-        result = _lib.native.attn_packed(q, k, v, cu_seqlens, cu_seqlens_kv, causal, sm_scale, return_lse, out)
+        result = _lib.native.attn_packed(q, k, v, cu_seqlens, cu_seqlens_kv, causal, sm_scale, return_lse, out, window, sinks)
         if result is not None:
             return result if out is None else (out, result[1]) if return_lse else out
     assert q.dim() == k.dim() == v.dim() == 3
@@ -83,6 +102,7 @@ def attention_packed(q, k, v, cu_seqlens, cu_seqlens_kv=None, *, causal=True, sm
     else:
         assert cu_seqlens_kv.shape == cu_seqlens.shape, "cu_seqlens_kv holds as many entries as cu_seqlens"
     qk_scale = _scale(sm_scale, D)
+    window, sinks = _window(window, sinks, causal)
     if not (q.is_cuda and k.is_cuda and v.is_cuda):
         raise RuntimeError("fa2.packed.attention_packed runs on the GPU (gfx950 HIP kernel); got CPU tensors")
     if not q.device == k.device == v.device:
@@ -92,9 +112,13 @@ def attention_packed(q, k, v, cu_seqlens, cu_seqlens_kv=None, *, causal=True, sm
     out, o_ = _output(q, out)
     lse = torch.empty((H_q, T), dtype=torch.float32, device=q.device) if return_lse else None
     if out.numel():
+        tensors = (_rows(q), _rows(k, _MAX_KV_ROW_STRIDE), _rows(v, _MAX_KV_ROW_STRIDE), o_, cu, cu_kv)
         with torch.cuda.device(q.device):
-            _lib.attn_packed(_rows(q), _rows(k, _MAX_KV_ROW_STRIDE), _rows(v, _MAX_KV_ROW_STRIDE), o_, cu, cu_kv,
-                             causal, qk_scale, lse, torch.cuda.current_stream(q.device).cuda_stream)
+            stream = torch.cuda.current_stream(q.device).cuda_stream
+            if window is None:
+                _lib.attn_packed(*tensors, causal, qk_scale, lse, stream)
+            else:
+                _lib.attn_packed_window(*tensors, window, sinks, qk_scale, lse, stream)
         if o_ is not out:
             out.copy_(o_)
     return (out, lse) if return_lse else out

@@ -17,8 +17,8 @@ import torch
 
 from . import _lib
 from .kernel import _cu_count
-from .packed import _index, _output, _rows, _scale
-from .rotary import _check_plan
+from .packed import _index, _output, _rows, _scale, _window
+from .rotary import _check_axes, _check_norm, _check_plan, _positions
 
 _16BIT = (torch.float16, torch.bfloat16)
 
@@ -94,7 +94,8 @@ def _check_kv(cache, k, v):
         raise RuntimeError(f"k and v must be on {cache.k.device}, got {k.device} and {v.device}")
 
 
-def cache_write(cache, k, v, block_table, cu_seqlens, seqlens, *, rotary=None, q=None, q_out=None):
+def cache_write(cache, k, v, block_table, cu_seqlens, seqlens, *, rotary=None, q=None, q_out=None, q_norm=None,
+                k_norm=None, positions=None):
     """Write the new tokens' k and v [T, H_kv, D] into their places in the cache.
 
     block_table: int32 [S, pages], the pages of every sequence in order; cu_seqlens: int32 [S + 1], sequence s's new
@@ -102,15 +103,23 @@ def cache_write(cache, k, v, block_table, cu_seqlens, seqlens, *, rotary=None, q
     included (the first new one goes to position seqlens[s] minus their number).
     rotary: a fa2.rotary.Rotary; k is rotated by its position before it is written, and so is q [T, H_q, D], if given,
         into q_out (a new tensor; q_out=q rotates in place), which is returned.
+    q_norm, k_norm: a fa2.rotary.HeadNorm (with rotary): every head of q, or of k, is normalised before it is rotated.
+    positions: int32 or int64 [T], or with a plan's axes [axes, T] (which it needs): what q and k are rotated by, in the place
+        of the position in the sequence.
     An e4m3 cache rounds each token and head once, against its own power-of-two scale (the least that holds its
     largest finite value); what is not finite becomes NaN.
     Not written: tokens past the table or in a page outside the cache, rows of no sequence, and rows before their
     sequence's start (where it has more rows than tokens in the cache); q_out is left as it is at the last two (undefined
     in a new one). Two tokens in one place are the caller's to avoid.
     """
+    turned = positions is not None or q_norm is not None or k_norm is not None or (
+        rotary is not None and rotary.axes is not None)
     if _lib.native is not None:  # the common call, made natively; None: not one of those
-        result = _lib.native.cache_write(*cache, block_table, cu_seqlens, seqlens, k, v,
-                                         *((None, False, 1.0) if rotary is None else rotary), q, q_out)
+        args = (*cache, block_table, cu_seqlens, seqlens, k, v, *((None, False, 1.0, None) if rotary is None else rotary), q, q_out)
+        if turned:
+            result = _lib.native.cache_write_turned(*args, *(q_norm or (None, 0.0)), *(k_norm or (None, 0.0)), positions)
+        else:
+            result = _lib.native.cache_write(*args)
         if result is not None:
             return q_out if q is None or q_out is not None else result
     _check_cache(cache, k.dtype)
@@ -122,6 +131,18 @@ def cache_write(cache, k, v, block_table, cu_seqlens, seqlens, *, rotary=None, q
         keep = _check_plan(rotary, D, device)
         rotation = _lib.Rotation(keep.data_ptr(), keep.numel(), rotary.interleaved, rotary.scale)
     assert q is not None or q_out is None, "q_out is q's"
+    if turned:
+        assert rotary is not None, "norms and positions are of a rotation: they need a rotary plan"
+        assert q is not None or q_norm is None, "q_norm is q's"
+        axes = _check_axes(rotary, device)
+        norms = _check_norm(q_norm, "q_norm", D, device), _check_norm(k_norm, "k_norm", D, device)
+        if positions is not None:
+            if positions.device != device:
+                raise RuntimeError(f"positions must be on {device}, got {positions.device}")
+            positions = _positions(positions, rotary, 1, T, True)[:, 0]
+        elif axes is not None:
+            raise ValueError("a plan's axes need positions")
+        turn = _lib.turn_of(rotary, keep, axes, 1 if positions is None else positions.shape[0], *norms)
     o_ = None
     if q is not None:
         assert rotary is not None, "q is taken to be rotated: it needs a rotary plan"
@@ -131,9 +152,13 @@ def cache_write(cache, k, v, block_table, cu_seqlens, seqlens, *, rotary=None, q
         q_out, o_ = _output(q, q_out)
     c, s, alive = _step(cache, block_table, cu_seqlens, seqlens, T)
     if T:
+        rows = _rows(k), _rows(v), None if q is None else _rows(q), o_
         with torch.cuda.device(device):
-            _lib.cache_write(c, s, _rows(k), _rows(v), None if q is None else _rows(q), o_, rotation,
-                             torch.cuda.current_stream(device).cuda_stream)
+            stream = torch.cuda.current_stream(device).cuda_stream
+            if turned:
+                _lib.cache_write_turned(c, s, *rows, positions, turn, stream)
+            else:
+                _lib.cache_write(c, s, *rows, rotation, stream)
         if o_ is not q_out:
             q_out.copy_(o_)
     return q_out
@@ -175,8 +200,8 @@ def cache_read(cache, block_table, cu_seqlens, seqlens, n_tokens, *, dtype=None,
     return k, v
 
 
-def attention_paged(q, cache, block_table, cu_seqlens, seqlens, *, causal=True, sm_scale=None, return_lse=False,
-                    out=None):
+def attention_paged(q, cache, block_table, cu_seqlens, seqlens, *, causal=True, window=None, sinks=0, shared=None,
+                    sm_scale=None, return_lse=False, out=None):
     """Attention of the new tokens q [T, H_q, D] over all their sequences' tokens in the cache.
 
     block_table, cu_seqlens and seqlens as in cache_write, which has put the new tokens' own k and v there; one
@@ -186,12 +211,18 @@ def attention_paged(q, cache, block_table, cu_seqlens, seqlens, *, causal=True, 
     sequence are left as they are in out (undefined in a new one). A sequence of more tokens than its row of the
     table holds counts as one of as many. A page outside the cache makes the rows that see its tokens NaN, and may
     make other rows of its sequence NaN.
+    window: (with causal) a row whose last key is n sees the `window` newest, n - window + 1 .. n, and the sequence's first
+        `sinks`; entries of the table whose pages no row sees are not looked at, and their pages may be others' by now.
+    shared: int32 [1] on the GPU, a number of tokens that all sequences begin with and that lie in the same pages: those are
+        read once for the whole batch, from the table's row of the first sequence that has new tokens. As many count as
+        whole pages hold and as lie before every sequence's new tokens. Not with a window.
     return_lse: also return the natural-log log-sum-exp of every row's scaled scores, fp32 [H_q, T].
     out: of q's shape and type, in any layout without shared elements; q itself is allowed, and no other memory that
         the call reads.
     """
     if _lib.native is not None:  # the common call, made natively; None: not one of those
-        result = _lib.native.attn_paged(*cache, block_table, cu_seqlens, seqlens, q, causal, sm_scale, return_lse, out)
+        result = _lib.native.attn_paged(*cache, block_table, cu_seqlens, seqlens, q, causal, sm_scale, return_lse, out,
+                                        window, sinks, shared)
         if result is not None:
             return result if out is None else (out, result[1]) if return_lse else out
     assert q.dim() == 3
@@ -203,16 +234,34 @@ def attention_paged(q, cache, block_table, cu_seqlens, seqlens, *, causal=True, 
     if q.device != cache.k.device:
         raise RuntimeError(f"q must be on {cache.k.device}, got {q.device}")
     qk_scale = _scale(sm_scale, D)
+    window, sinks = _window(window, sinks, causal)
+    if shared is not None:
+        if window is not None:
+            raise ValueError("a shared prefix and a window exclude each other")
+        assert shared.dtype == torch.int32 and shared.numel() == 1, "shared is int32 [1]"
+        if shared.device != q.device:
+            raise RuntimeError(f"shared must be on {q.device}, got {shared.device}")
     out, o_ = _output(q, out)
     lse = torch.empty((H_q, T), dtype=torch.float32, device=q.device) if return_lse else None
     c, s, alive = _step(cache, block_table, cu_seqlens, seqlens, T)
     if out.numel():
-        n = _lib.paged_workspace_bytes(H_q, H_kv, D, cache.k.dtype, T, seqlens.numel(),
-                                       block_table.shape[1] * cache.k.shape[2], _cu_count(q.device))
+        sizes = (H_q, H_kv, D, cache.k.dtype, T, seqlens.numel(), block_table.shape[1] * cache.k.shape[2])
+        cus = _cu_count(q.device)
+        if shared is not None:
+            n = _lib.paged_shared_workspace_bytes(*sizes, cus)
+        elif window is not None:
+            n = _lib.paged_window_workspace_bytes(*sizes, window, sinks, cus)
+        else:
+            n = _lib.paged_workspace_bytes(*sizes, cus)
         ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
         with torch.cuda.device(q.device):
-            _lib.attn_paged(_rows(q), o_, c, s, causal, qk_scale, lse, ws,
-                            torch.cuda.current_stream(q.device).cuda_stream)
+            stream = torch.cuda.current_stream(q.device).cuda_stream
+            if shared is not None and seqlens.numel():
+                _lib.attn_paged_shared(_rows(q), o_, c, s, shared, causal, qk_scale, lse, ws, stream)
+            elif window is not None:
+                _lib.attn_paged_window(_rows(q), o_, c, s, window, sinks, qk_scale, lse, ws, stream)
+            else:
+                _lib.attn_paged(_rows(q), o_, c, s, causal, qk_scale, lse, ws, stream)
         if o_ is not out:
             out.copy_(o_)
     return (out, lse) if return_lse else out
