@@ -17,8 +17,10 @@ def norm(x, weight, eps):
 def turn(x, positions, freqs, interleaved=False, scale=1.0, axes=None, weight=None, eps=0.0):
     """x [T, H, D] normalised and rotated: (result, bound), both float64. positions [T], or [axes, T] with axes.
 
-    The bound of a kernel's value: it forms x * r * weight, and products of two of those with cos and sin and their sum, in
-    float32: at most 8 roundings of 2^-24, relative to |a cos| + |b sin|; then the rounding to the type."""
+    The bound of a kernel's value, in units of 2^-24 relative to |a cos| + |b sin|. The sum of D <= 128 squares: 8 products and
+    sums of a lane, at most 2 units each if they are cut off, and 4 sums of lanes, together 20, half of that in its root; the mean
+    and eps 1, the root's estimate 2 (one unit in its last place), x * r * weight 2, cos or sin, its product and the sum 3: 18, and 24 with
+    what second order adds. Then the rounding to the type."""
     half = freqs.numel()
     angle = (positions.double()[:, None] if axes is None else positions.double()[axes.long()].t()) * freqs.double()
     cos, sin = (torch.cos(angle) * scale)[:, None], (torch.sin(angle) * scale)[:, None]
@@ -31,7 +33,7 @@ def turn(x, positions, freqs, interleaved=False, scale=1.0, axes=None, weight=No
     size[..., b_at] = b.abs() * cos.abs() + a.abs() * sin.abs()
     y[..., a_at], y[..., b_at] = a * cos - b * sin, b * cos + a * sin
     u = serving.HALF_STEP[x.dtype]
-    return y, u * y.abs() * (1 + u) + 8 * serving.F32 * size + (2.0 ** -25 if x.dtype == torch.float16 else 0.0)
+    return y, u * y.abs() * (1 + u) + 24 * serving.F32 * size + (2.0 ** -25 if x.dtype == torch.float16 else 0.0)
 
 
 def release(free, count, table, first, last):

@@ -43,6 +43,8 @@ int check_turn(const fa2_turn* turn, int32_t head_dim, const void* positions, in
   return FA2_OK;
 }
 
+constexpr int64_t kTurnWgs = 1024, kTurnAngles = 512;
+
 // The keys that a row sees of n_kv at most, as the choice of a form counts them.
 int64_t window_keys(int64_t n_kv, int32_t window, int32_t sinks) { return std::min<int64_t>(n_kv, (int64_t)window + sinks + 128); }
 
@@ -81,7 +83,7 @@ int fa2_rotary_qk(const void* q, const void* k, void* q_out, void* k_out, const 
   if (const int rc = check_turn(turn, head_dim, positions, position_bytes, p_stride, 3, &p.rot, &p.turn)) return rc;
   if (batch < 0 || h_q < 0 || h_k < 0 || n < 0)
     return fail(FA2_EINVAL, "bad sizes: batch=%d h_q=%d h_k=%d n=%d", batch, h_q, h_k, n);
-  if (h_q > (1 << 24) || h_k > (1 << 24)) return fail(FA2_EINVAL, "at most 2^24 heads");
+  if (h_q > (1 << 18) || h_k > (1 << 18)) return fail(FA2_EINVAL, "at most 2^18 heads");  // (passes are the grid's second dimension)
   if (batch == 0 || n == 0 || h_q + h_k == 0) return FA2_OK;
   if (h_q) {
     if (const int rc = check_rows("q", q, q_stride, 3, 8)) return rc;
@@ -102,9 +104,11 @@ int fa2_rotary_qk(const void* q, const void* k, void* q_out, void* k_out, const 
     p.skob = ko_stride[0]; p.skoh = ko_stride[1]; p.skon = ko_stride[2];
   }
   p.batch = batch; p.h_q = h_q; p.h_k = h_k; p.n = n;
-  p.tokens_per_wg = fa2::serve_tokens_per_wg((int)std::min<int64_t>((int64_t)(h_q + h_k) * (head_dim / 8), 256),
-                                             (int64_t)batch * n, kRotaryWgs);
-  const int64_t grid = ((int64_t)batch * n + p.tokens_per_wg - 1) / p.tokens_per_wg;
+  // as many tokens as fill the lanes with rows, and, where workgroups are left for the CUs, with angles
+  p.tokens_per_wg = fa2::serve_tokens_per_wg((int)std::min<int64_t>(((int64_t)h_q + h_k) * (head_dim / 8), 256), n, kRotaryWgs);
+  while (p.tokens_per_wg < 16 && p.tokens_per_wg * p.rot.half < kTurnAngles && (int64_t)batch * n >= 2 * p.tokens_per_wg * kTurnWgs)
+    p.tokens_per_wg *= 2;
+  const int64_t grid = (int64_t)batch * (((int64_t)n + p.tokens_per_wg - 1) / p.tokens_per_wg);
   if (grid > 0x7fffffffLL) return fail(FA2_EINVAL, "grid of %lld workgroups is too large", (long long)grid);
   return launched(fa2::launch_rotary_qk(dtype, head_dim, p, (unsigned)grid, static_cast<hipStream_t>(stream)), "rotary");
 }

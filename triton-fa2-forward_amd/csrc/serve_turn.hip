@@ -16,53 +16,62 @@ namespace fa2 {
 
 namespace {
 
-// 16 bytes a lane, D / 8 lanes a row; rows of q and k of a group of tokens, which share the tokens' angles.
+// 16 bytes a lane, D / 8 lanes a row. A workgroup has a group of one batch row's tokens, which share their angles among the heads;
+// a lane has the same heads of every token (a pass of 256 lanes over a token's, or over several tokens' where they are few), so
+// that their places and weights are worked out once, and loads the next token's row while it turns this one's.
 template <int DT, int D>
-__global__ __launch_bounds__(256) void rotary_qk_kernel(const RotaryQkParams p) {
-  constexpr int LPR = D / 8, ROWS = kRowsAtOnce;
-  __shared__ float cs[kMaxTokensPerWg][kMaxHalf][2];
-  __shared__ float weights[2][D];
-  const int64_t total = (int64_t)p.batch * p.n;
-  const int64_t t0 = (int64_t)blockIdx.x * p.tokens_per_wg;
-  const int tokens = (int)min((int64_t)p.tokens_per_wg, total - t0);
-  const int chunk = threadIdx.x % LPR;
-  const int heads = p.h_q + p.h_k, rows = tokens * heads;
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(6))) void rotary_qk_kernel(const RotaryQkParams p) {
+  constexpr int LPR = D / 8, RP = 256 / LPR;  // lanes per row, rows of a pass
+  __shared__ alignas(16) float cs[kMaxTokensPerWg][kMaxHalf][2];
+  __shared__ alignas(16) float weights[2][D];
+  const int groups = (p.n + p.tokens_per_wg - 1) / p.tokens_per_wg;
+  const int b = (int)blockIdx.x / groups, t0 = ((int)blockIdx.x - b * groups) * p.tokens_per_wg;
+  const int tokens = min(p.tokens_per_wg, p.n - t0);
+  const int chunk = threadIdx.x % LPR, row = threadIdx.x / LPR;
+  const int heads = p.h_q + p.h_k;
   const int half = p.rot.half;
   const bool interleaved = p.rot.interleaved;
-  for (int base = 0; base < rows; base += ROWS * (256 / LPR)) {
-    Chunks in[ROWS];
-    uint16_t* dst[ROWS];
-    int token[ROWS];  // -1: nothing to do
-    bool is_k[ROWS];
-#pragma unroll
-    for (int u = 0; u < ROWS; ++u) {
-      const int r = base + u * (256 / LPR) + (int)threadIdx.x / LPR;
-      token[u] = -1;
-      if (r >= rows) continue;
-      const int t = r / heads, x = r - t * heads;
-      const int64_t b = (t0 + t) / p.n, i = (t0 + t) - b * p.n;
-      token[u] = t;
-      is_k[u] = x >= p.h_q;
-      const uint16_t* src = is_k[u] ? p.k + b * p.skb + (x - p.h_q) * p.skh + i * p.skn : p.q + b * p.sqb + x * p.sqh + i * p.sqn;
-      dst[u] = is_k[u] ? p.k_out + b * p.skob + (x - p.h_q) * p.skoh + i * p.skon
-                       : p.q_out + b * p.sqob + x * p.sqoh + i * p.sqon;
-      in[u] = load_chunks(src, chunk, half, interleaved);
-    }
-    if (base == 0) {  // while the first rows are on their way
-      fill_weights<D>(weights, p.turn);
-      fill_axes(cs, p.rot, p.turn, tokens, [&](int t, int axis) -> int64_t {
-        const int64_t b = (t0 + t) / p.n, i = (t0 + t) - b * p.n;
-        return position_at(p.turn, axis * p.turn.spa + b * p.turn.spb + i * p.turn.spn);
-      });
-      __syncthreads();
-    }
-#pragma unroll
-    for (int u = 0; u < ROWS; ++u) {
-      if (token[u] < 0) continue;
+  const int step = max(RP / heads, 1);                // tokens of a pass
+  const int sub = heads < RP ? row / heads : 0;       // this lane's
+  int head = row - sub * heads + (int)blockIdx.y * RP, t;
+  bool is_k = false;
+  const uint16_t* src = nullptr;
+  uint16_t* dst = nullptr;
+  int64_t sn = 0, son = 0;
+  Chunks next{};
+  auto begin = [&]() {  // on to `head`: its places, and the first token's row on its way
+    t = tokens;
+    if (head >= heads) return;
+    is_k = head >= p.h_q;
+    const int h = is_k ? head - p.h_q : head;
+    sn = is_k ? p.skn : p.sqn;
+    son = is_k ? p.skon : p.sqon;
+    src = (is_k ? p.k + b * p.skb + h * p.skh : p.q + b * p.sqb + h * p.sqh) + (t0 + sub) * sn;
+    dst = (is_k ? p.k_out + b * p.skob + h * p.skoh : p.q_out + b * p.sqob + h * p.sqoh) + (t0 + sub) * son + 8 * chunk;
+    if (sub < step) t = sub;
+    if (t < tokens) next = load_chunks(src, chunk, half, interleaved);
+    sn *= step;
+    son *= step;
+  };
+  begin();
+  fill_weights<D>(weights, p.turn);
+  fill_axes(cs, p.rot, p.turn, tokens, [&](int x, int axis) -> int64_t {
+    return position_at(p.turn, axis * p.turn.spa + b * p.turn.spb + (t0 + x) * p.turn.spn);
+  });
+  __syncthreads();
+  for (;;) {
+    for (; t < tokens; t += step) {
+      const Chunks in = next;
+      src += sn;
+      if (t + step < tokens) next = load_chunks(src, chunk, half, interleaved);
       float y[8];
-      turned8<DT, D, float>(p.turn, is_k[u], in[u], chunk, half, interleaved, cs[token[u]], weights, y);
-      *(u32x4*)(dst[u] + 8 * chunk) = pack8<DT>(y);
+      turned8<DT, D, float>(p.turn, is_k, in, chunk, half, interleaved, cs[t], weights, y);
+      *(u32x4*)dst = pack8<DT>(y);
+      dst += son;
     }
+    head += RP * (int)gridDim.y;
+    if (head >= heads) break;
+    begin();
   }
 }
 
@@ -75,9 +84,13 @@ int launch_write_d(bool e4m3, const CacheTurnParams& p, unsigned grid, hipStream
   return (int)hipGetLastError();
 }
 
+// Workgroups below which each pass over a token's heads is one of its own: few tokens wait for one pass after the other.
+constexpr unsigned kTurnFewWgs = 512;
 template <int DT, int D>
 int launch_qk_d(const RotaryQkParams& p, unsigned grid, hipStream_t s) {
-  hipLaunchKernelGGL((rotary_qk_kernel<DT, D>), dim3(grid), dim3(256), 0, s, p);
+  const int rows = 256 / (D / 8), heads = p.h_q + p.h_k;
+  const unsigned passes = grid < kTurnFewWgs && heads > rows ? (unsigned)((heads + rows - 1) / rows) : 1u;
+  hipLaunchKernelGGL((rotary_qk_kernel<DT, D>), dim3(grid, passes), dim3(256), 0, s, p);
   return (int)hipGetLastError();
 }
 
