@@ -391,8 +391,8 @@ FA2_API int fa2_attn_paged_shared(const void* q, void* out, const int64_t q_stri
                                   const fa2_cache* cache, const fa2_sequences* seq, const int32_t* shared,
                                   int32_t h_q, int32_t dtype, int32_t causal, float qk_scale, float* lse,
                                   void* workspace, size_t workspace_bytes, void* stream);
-FA2_API size_t fa2_paged_shared_workspace_bytes(int32_t h_q, int32_t h_kv, int32_t head_dim, int32_t cache_dtype,
-                                                int32_t n_tokens, int32_t n_seq, int64_t max_keys, int32_t num_cus);
+FA2_API size_t fa2_paged_shared_workspace_bytes(int32_t h_q, int32_t h_kv, int32_t head_dim, int32_t n_tokens,
+                                                int32_t n_seq, int32_t num_cus);
 
 /*
  * What rows of q and k are turned by: every head x of q first becomes x / sqrt(mean x^2 + q_eps) * q_weight (device

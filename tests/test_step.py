@@ -277,14 +277,14 @@ def test_c_shared_refusals():
     assert shared(n=None) == -1 and "shared" in _lib.last_error()
     assert shared(n=P + 2) == -2
     assert shared(q=None) == -1 and shared(h_q=3) == -1 and shared(lens=None) == -1
-    need = _lib.paged_shared_workspace_bytes(4, 2, 64, torch.bfloat16, 3, 2, 32, 256)
-    assert need >= 3 * 4 * 68 * 4  # a row's results over the prefix, in float
+    need = _lib.paged_shared_workspace_bytes(4, 2, 64, 3, 2, 256)
+    assert need >= 2 * 3 * 4 * 68 * 4  # a row's results over the prefix and behind it, in float
     assert shared(ws=None) == -1 and str(need) in _lib.last_error()
     assert shared(n_ws=need - 1) == -1 and str(need) in _lib.last_error()
     assert shared(ws=P + 128) == -2
     assert shared(tokens=0) == 0 and shared(n_seq=0) == 0
     for h_q, D, n, n_seq, cus in ((3, 64, 3, 2, 256), (4, 48, 3, 2, 256), (4, 64, 0, 2, 256), (4, 64, 3, 0, 256), (4, 64, 3, 2, 0)):
-        assert _lib.paged_shared_workspace_bytes(h_q, 2, D, torch.bfloat16, n, n_seq, 4096, cus) == 0
+        assert _lib.paged_shared_workspace_bytes(h_q, 2, D, n, n_seq, cus) == 0
 
 
 BAD_TURNS = [(dict(n_axes=0), -1), (dict(n_axes=3), -1), (dict(axes=P + 2, n_axes=3), -2), (dict(q_weight=P + 2, q_eps=1e-6), -2),

@@ -43,38 +43,38 @@ constexpr int ragged_block_n(int head_dim, int row_waves) {
   return row_waves == 4 ? (head_dim == 16 ? 128 : 64) : head_dim == 128 ? 32 : 64;
 }
 
-// A row's results over the keys before a common prefix's end, kept in float beside each other: O, then m, l and exact l
-template <int D>
-__device__ __forceinline__ float* prefix_row(ParamsRef p, int64_t token, int head) {
-  return p.prefix + (token * (p.h_kv * p.group) + head) * (D + 4);
+// A row's results over a common prefix, or over its own keys behind it: O, then m, l, exact l and a word that says more: bit 1, the row
+// sees no key; bit 0, they lie in pieces, and the words before it are the first and the last of the shares that have
+// one, and the row's place there.
+template <int D, int MODE>
+__device__ __forceinline__ float* row_results(ParamsRef p, int64_t token, int head) {
+  const int64_t h_q = p.h_kv * p.group;
+  return p.rows + ((MODE == kModeOwn ? p.seq.n_tokens * h_q : 0) + token * h_q + head) * (D + 4);
 }
-// Joined with the results (m, l, exact l) over the row's own keys: O = own * O_own + prefix * O_prefix. A NaN reference
-// makes the row NaN.
-struct Joined {
-  float own, prefix, lse;
-  __device__ Joined(float m, float l, float exact, const f32x4& of_prefix, bool no_key) {
-    const float M = fmaxf(m, of_prefix[0]);
-    const float a = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - M);
-    const float b = of_prefix[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(of_prefix[0] - M);
-    const float inv = no_key ? 0.f : 1.0f / (a * l + b * of_prefix[1]);
-    own = a * inv;
-    prefix = b * inv;
-    const bool nan = m != m || of_prefix[0] != of_prefix[0];
-    lse = !nan && M == INFINITY ? M : ((nan ? m + of_prefix[0] : M) + log2f(a * exact + b * of_prefix[2])) * kLn2;
-  }
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+// A workgroup's LDS
+template <int D, int GW>
+struct RaggedLds {
+  static constexpr int kBufs = GW == 1 ? 1 : 2, kGroups = 4 / GW;
+  static constexpr int kKvChunks = kGroups * kBufs * 2 * ragged_block_n(D, GW) * (D / 8);
+  static constexpr int kMergeChunks = kGroups > 1 ? 32 * GW * kGroups * (D / 4) : 0;
+  u32x4 kv[kKvChunks > kMergeChunks ? kKvChunks : kMergeChunks];
+  float sm[kGroups][kGroups > 1 ? 32 * GW : 1][3];  // m, l, exact l of every group's rows
+  int odd[kGroups > 1 ? 32 * GW : 1];               // rows whose sums are not finite
 };
 
 // LSE: with 128 rows, whether p.lse is set: known to the compiler, the sums it needs mix with the rest of the tile's
 // instructions, and cost nothing where they are not asked for.
 template <int DT, int D, int SRC, int GW, bool LSE, int MODE>
-__global__ __launch_bounds__(256)
-__attribute__((amdgpu_waves_per_eu(ragged_waves(D, SRC, GW))))
-void attn_ragged_kernel(const RaggedParams) {
+__device__ __forceinline__ void ragged_rows(RaggedLds<D, GW>& mem, int hkv, int rank, Cursor cur) {
   using E = Elem<DT>;
   ParamsRef p = params_here();
   constexpr bool kE4m3 = SRC == kSourceE4m3;
   constexpr bool kPages = SRC != kSourcePacked;
   constexpr bool kWindow = MODE == kModeWindow, kPrefix = MODE == kModePrefix, kOwn = MODE == kModeOwn;
+  constexpr bool kJoined = kPrefix || kOwn;  // results are kept in float, for attn_shared_join_kernel
   constexpr int EB = kE4m3 ? 1 : 2;      // bytes of a cached element
   constexpr int BN = ragged_block_n(D, GW);
   constexpr int BM = 32 * GW;            // rows per workgroup
@@ -95,11 +95,9 @@ void attn_ragged_kernel(const RaggedParams) {
   static_assert(NI >= 1 && BN % NI == 0, "a tile must be whole 1 KiB loads");
   constexpr int QPR = D / 4;             // 16-byte pieces of an fp32 output row
 
-  constexpr int kKvChunks = KG * BUFS * 2 * TCH;
-  constexpr int kMergeChunks = KG > 1 ? BM * KG * QPR : 0;
-  __shared__ u32x4 lds[kKvChunks > kMergeChunks ? kKvChunks : kMergeChunks];
-  __shared__ float sm[KG][KG > 1 ? BM : 1][3];  // m, l, exact l of every group's rows
-  __shared__ int odd[KG > 1 ? BM : 1];          // rows whose sums are not finite
+  auto& lds = mem.kv;
+  auto& sm = mem.sm;
+  auto& odd = mem.odd;
 
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -108,8 +106,6 @@ void attn_ragged_kernel(const RaggedParams) {
   const int g = lane >> 5;
   const int grp = wave / GW, gwave = wave % GW;
 
-  int hkv, rank;
-  head_and_rank(p, (int)blockIdx.x, &hkv, &rank);
   // ---- LDS operand reads, as in attn_fwd_kernel.hpp
   const FA2_LDS char* gbuf = (const FA2_LDS char*)(lds + grp * BUFS * 2 * TCH);
   auto kbuf = [&](int i) { return gbuf + (BUFS == 1 ? 0 : (i & 1) * TCH * 16); };
@@ -171,16 +167,16 @@ void attn_ragged_kernel(const RaggedParams) {
 
   const float qk_scale = p.qk_scale;
   const bool want_exact = GW == 1 ? p.lse != nullptr : LSE, causal = !kPrefix && p.causal != 0,
-             shared = kPages && p.shares > 0;
+             shared = kJoined || (kPages && p.shares > 0);
 
   // ---- the workgroup's work: the pieces of its share, or its one tile
-  Cursor cur;
-  if constexpr (kPrefix || kOwn) cur.prefix = common_prefix(p, lane);
   Share share = {0, 0, 0, 0};
   if (shared) {
     share = find_share<BM, kPages, MODE>(p, rank, lane, &cur);
     if (share.x >= share.end) {
-      if (tid == 0) merge_of(p, hkv, rank)->first = -1;
+      if constexpr (!kJoined) {
+        if (tid == 0) merge_of(p, hkv, rank)->first = -1;
+      }
       return;
     }
   } else if (!find_tile<BM, kPages, MODE>(p, rank, lane, &cur)) {
@@ -219,8 +215,19 @@ void attn_ragged_kernel(const RaggedParams) {
       // nothing between the cuts (a tile that sees no key at all belongs to the share that it starts in)
       const bool empty = all_tiles == 0 ? share.in > 0 : t_begin == t_end;
       const bool whole = t_begin == 0 && t_end == all_tiles;
-      if (!whole) part = part_of<BM, D>(p, hkv, rank, share.in == 0);
-      if (first_piece && tid == 0) {  // what the merge of a tile that ends here needs to know
+      if constexpr (kJoined) {
+        if (!whole) part = joined_part<D>(p, hkv, cur.first_share + rank, share.in == 0);
+        if (!whole && !empty && t_begin == 0 && tid < row_end - row0) {  // the first piece says where they all are
+          const int64_t start = share.x - share.in;
+          const int i = (row0 + tid) / p.group, head = hkv * p.group + (row0 + tid - i * p.group);
+          *(i32x4*)(row_results<D, MODE>(p, sq.first + i, head) + D) =
+              i32x4{cur.first_share + (int)(start / share.size), cur.first_share + (int)((start + length - 1) / share.size), tid,
+                    1 + (last_of(i) < 0 ? 2 : 0)};
+        }
+      } else if (!whole) {
+        part = part_of<BM, D>(p, hkv, rank, share.in == 0);
+      }
+      if (!kJoined && first_piece && tid == 0) {  // what the merge of a tile that ends here needs to know
         Merge m = {-1, row0, row_end - row0, sq.first, n_kv, shift};
         if (!empty && !whole && t_end == all_tiles) m.first = (int)((share.x - share.in) / share.size);
         *merge_of(p, hkv, rank) = m;
@@ -633,15 +640,9 @@ void attn_ragged_kernel(const RaggedParams) {
     auto put_sums = [&](int x, float m, float sum, float exact) {
       if (part) {
         *(f32x4*)(part + part_sums<BM, D>(x)) = f32x4{m, sum, exact, 0.f};
-      } else if (kPrefix) {
+      } else if (kJoined) {
         const RowPlace at = place(x);
-        *(f32x4*)(prefix_row<D>(pe, at.token, at.head) + D) = f32x4{m, sum, exact, 0.f};
-      } else if (kOwn) {
-        if (pe.lse) {
-          const RowPlace at = place(x);
-          const Joined j(m, sum, exact, *(const f32x4*)(prefix_row<D>(pe, at.token, at.head) + D), last_of(at.pos) < 0);
-          pe.lse[(int64_t)at.head * pe.seq.n_tokens + at.token] = j.lse;
-        }
+        *(f32x4*)(row_results<D, MODE>(pe, at.token, at.head) + D) = f32x4{m, sum, exact, __int_as_float(last_of(at.pos) < 0 ? 2 : 0)};
       } else if (pe.lse) {
         const RowPlace at = place(x);
         pe.lse[(int64_t)at.head * pe.seq.n_tokens + at.token] = (m + log2f(exact)) * kLn2;
@@ -720,19 +721,14 @@ void attn_ragged_kernel(const RaggedParams) {
       for (int o2 = 32; o2 >= 1; o2 /= 2) sum += __shfl_xor(sum, o2, 64);
       if (no_lse) m = __uint_as_float(0x7fc00000u);
       const float inv = last_of(at.pos) < 0 ? 0.f : 1.0f / sum;
-      const float* before = kPrefix || kOwn ? prefix_row<D>(pe, at.token, at.head) : nullptr;
-      const Joined j(m, sum, sum, kOwn && !part ? *(const f32x4*)(before + D) : f32x4{-INFINITY, 0.f, 0.f, 0.f}, last_of(at.pos) < 0);
 #pragma unroll
       for (int y = 0; y < (D + 63) / 64; ++y)
         if (lane + 64 * y < D) {
           const float v = nan ? m : o[y];
           if (part)
             part[part_index<GW, D>(x, lane + 64 * y)] = v;
-          else if (kPrefix)
-            const_cast<float*>(before)[lane + 64 * y] = v;
-          else if (kOwn)
-            pe.o[at.token * pe.sot + at.head * pe.soh + lane + 64 * y] =
-                (uint16_t)E::pack2(last_of(at.pos) < 0 ? 0.f : v * j.own + before[lane + 64 * y] * j.prefix, 0.f);
+          else if (kJoined)
+            row_results<D, MODE>(pe, at.token, at.head)[lane + 64 * y] = v;
           else
             pe.o[at.token * pe.sot + at.head * pe.soh + lane + 64 * y] =
                 (uint16_t)E::pack2(last_of(at.pos) < 0 ? 0.f : v * inv, 0.f);
@@ -750,32 +746,22 @@ void attn_ragged_kernel(const RaggedParams) {
         const RowPlace at = place(wr);
         uint16_t* orow = pe.o + at.token * pe.sot + at.head * pe.soh;
         const float nan_or_0 = m_i != m_i ? m_i : 0.f;
-        float* before = kPrefix || kOwn ? prefix_row<D>(pe, at.token, at.head) : nullptr;
-        const Joined j(m_i, l, l, kOwn && !part ? *(const f32x4*)(before + D) : f32x4{-INFINITY, 0.f, 0.f, 0.f}, last_key < 0);
+        float* kept = kJoined ? row_results<D, MODE>(pe, at.token, at.head) : nullptr;
 #pragma unroll
         for (int db = 0; db < DB; ++db)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const int d0 = 32 * db + 16 * h + 8 * g;
             if (d0 < D) {
-              if (part || kPrefix) {
+              if (part || kJoined) {
                 f32x4 lo, hi;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                   lo[i] = acc[db][8 * h + i];
                   hi[i] = acc[db][8 * h + 4 + i];
                 }
-                float* to = kPrefix && !part ? before + d0 : part + part_index<GW, D>(wr, d0);
-                *(f32x4*)to = lo;
-                *(f32x4*)(kPrefix && !part ? to + 4 : part + part_index<GW, D>(wr, d0 + 4)) = hi;
-              } else if (kOwn) {
-                float y[8];
-                const f32x4 lo = *(const f32x4*)(before + d0), hi = *(const f32x4*)(before + d0 + 4);
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                  y[i] = __builtin_fmaf(acc[db][8 * h + i], j.own, (i < 4 ? lo[i] : hi[i - 4]) * j.prefix) + nan_or_0;
-                *(u32x4*)(orow + d0) = u32x4{E::pack2(y[0], y[1]), E::pack2(y[2], y[3]), E::pack2(y[4], y[5]),
-                                             E::pack2(y[6], y[7])};
+                *(f32x4*)(kJoined && !part ? kept + d0 : part + part_index<GW, D>(wr, d0)) = lo;
+                *(f32x4*)(kJoined && !part ? kept + d0 + 4 : part + part_index<GW, D>(wr, d0 + 4)) = hi;
               } else {
                 float y[8];
 #pragma unroll
@@ -845,15 +831,8 @@ void attn_ragged_kernel(const RaggedParams) {
         const float m_nan = nan ? __uint_as_float(0x7fc00000u) : m;
         if (part) {
           *(f32x4*)(part + part_index<GW, D>(x, 4 * q)) = o;
-        } else if (kPrefix) {
-          *(f32x4*)(prefix_row<D>(pe, at.token, at.head) + 4 * q) = o;
-        } else if (kOwn) {
-          const float* before = prefix_row<D>(pe, at.token, at.head);
-          const Joined j(m_nan, ls, lxs, *(const f32x4*)(before + D), last_of(at.pos) < 0);
-          const f32x4 v = *(const f32x4*)(before + 4 * q);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(o[e], j.own, v[e] * j.prefix);
-          *(u32x2*)(pe.o + at.token * pe.sot + at.head * pe.soh + 4 * q) = u32x2{E::pack2(o[0], o[1]), E::pack2(o[2], o[3])};
+        } else if (kJoined) {
+          *(f32x4*)(row_results<D, MODE>(pe, at.token, at.head) + 4 * q) = o;
         } else {
           const float inv = last_of(at.pos) < 0 ? 0.f : 1.0f / ls;  // no key: 0
 #pragma unroll
@@ -873,6 +852,36 @@ void attn_ragged_kernel(const RaggedParams) {
     }
     more = shared && share.x < share.end && next_tile<BM, kPages, MODE>(params_here(), lane, &cur);
   }
+}
+
+template <int DT, int D, int SRC, int GW, bool LSE, int MODE>
+__global__ __launch_bounds__(256)
+__attribute__((amdgpu_waves_per_eu(ragged_waves(D, SRC, GW))))
+void attn_ragged_kernel(const RaggedParams) {
+  __shared__ RaggedLds<D, GW> mem;
+  int hkv, rank;
+  head_and_rank(params_here(), (int)blockIdx.x, &hkv, &rank);
+  ragged_rows<DT, D, SRC, GW, LSE, MODE>(mem, hkv, rank, Cursor{});
+}
+
+// Both passes of a batch with a common prefix in one launch: GWP row waves for the prefix's shares, whose rows are all of the
+// batch's, GWO for the others.
+template <int DT, int D, int SRC, int GWP, int GWO, bool LSE>
+__global__ __launch_bounds__(256)
+__attribute__((amdgpu_waves_per_eu(kSharedWaves)))
+void attn_shared_kernel(const RaggedParams) {
+  __shared__ union {
+    RaggedLds<D, GWP> prefix;
+    RaggedLds<D, GWO> own;
+  } mem;
+  ParamsRef p = params_here();
+  int hkv, rank;
+  head_and_rank(p, (int)blockIdx.x, &hkv, &rank);
+  Cursor cur{};
+  if (deal_shares<32 * GWP, 32 * GWO>(p, rank, threadIdx.x & 63, &cur))
+    ragged_rows<DT, D, SRC, GWP, LSE, kModePrefix>(mem.prefix, hkv, rank, cur);
+  else
+    ragged_rows<DT, D, SRC, GWO, LSE, kModeOwn>(mem.own, hkv, rank - cur.first_share, cur);
 }
 
 // Merges the pieces of the row tile that ends in share `rank` and starts in an earlier one: with M the largest of the
@@ -898,7 +907,7 @@ struct Merged {
     for (int e = 0; e < 4; ++e) o[e] = o[e] * a + (none ? 0.f : w * v[e]);
   }
 };
-template <int DT, int D, int GW, int MODE>
+template <int DT, int D, int GW>
 __global__ __launch_bounds__(combine_threads(D)) void attn_ragged_combine_kernel(const RaggedParams) {
   using E = Elem<DT>;
   ParamsRef p = params_here();
@@ -948,29 +957,78 @@ __global__ __launch_bounds__(combine_threads(D)) void attn_ragged_combine_kernel
   if (way > 0 || x >= at.rows) return;
   const int pos = (at.row0 + x) / p.group, head = hkv * p.group + (at.row0 + x - pos * p.group);
   const int64_t token = at.token + pos;
-  if constexpr (MODE == kModePrefix) {
-    float* row = prefix_row<D>(p, token, head);
-    *(f32x4*)(row + 4 * q) = r.o;
-    if (q == 0) *(f32x4*)(row + D) = f32x4{r.nan ? __uint_as_float(0x7fc00000u) : r.M, r.l, r.lx, 0.f};
-    return;
-  }
   const bool none = (p.causal ? min(pos + at.shift, at.n_kv - 1) : at.n_kv - 1) < 0;
-  if constexpr (MODE == kModeOwn) {
-    const float* before = prefix_row<D>(p, token, head);
-    const Joined j(r.nan ? __uint_as_float(0x7fc00000u) : r.M, r.l, r.lx, *(const f32x4*)(before + D), none);
-    const f32x4 v = *(const f32x4*)(before + 4 * q);
-    f32x4 o;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(r.o[e], j.own, v[e] * j.prefix);
-    *(u32x2*)(p.o + token * p.sot + head * p.soh + 4 * q) = u32x2{E::pack2(o[0], o[1]), E::pack2(o[2], o[3])};
-    if (p.lse && q == 0) p.lse[(int64_t)head * p.seq.n_tokens + token] = j.lse;
-    return;
-  }
   const float inv = none ? 0.f : 1.0f / r.l;
   *(u32x2*)(p.o + token * p.sot + head * p.soh + 4 * q) =
       u32x2{E::pack2(r.o[0] * inv, r.o[1] * inv), E::pack2(r.o[2] * inv, r.o[3] * inv)};
   if (p.lse && q == 0)  // (an infinite score has an infinite log-sum-exp, though the row has no weights)
     p.lse[(int64_t)head * p.seq.n_tokens + token] = !r.nan && r.M == INFINITY ? r.M : (r.M + log2f(r.lx)) * kLn2;
+}
+
+// Joins a row's results over a common prefix and over its own keys, each in one place or in pieces, as pieces are merged. 8
+// neighbouring rows a workgroup (those of 32 rows' pieces lie side by side), 4 dims of a row a thread, and as many threads in
+// turn for its pieces as 1024 have room for: bound by the latency of the pieces' loads.
+template <int DT, int D, int GWP, int GWO>
+__global__ __launch_bounds__(1024) void attn_shared_join_kernel(const RaggedParams) {
+  using E = Elem<DT>;
+  ParamsRef p = params_here();
+  constexpr int ROWS = 8, Q = D / 4, WAYS = 1024 / (ROWS * Q), STEP = 4;
+  __shared__ f32x4 values[1024], sums_of[1024];
+  const int blocks = (int)(((int64_t)p.seq.n_tokens * p.group + ROWS - 1) / ROWS);
+  const int hkv = (int)blockIdx.x / blocks, r = ((int)blockIdx.x - hkv * blocks) * ROWS + (int)(threadIdx.x % ROWS);
+  const int q = (int)threadIdx.x / ROWS % Q, way = (int)threadIdx.x / (ROWS * Q);
+  const int token = r / p.group, head = hkv * p.group + (r - token * p.group);
+  const bool mine = token >= row_bound(p.seq.cu, 0, p.seq.n_tokens) && token < row_bound(p.seq.cu, p.seq.n_seq, p.seq.n_tokens);
+  Merged m = {-INFINITY, 0.f, 0.f, f32x4{0.f, 0.f, 0.f, 0.f}, false};
+  bool no_key = false;
+  auto take = [&](const float* row, auto gw) {
+    constexpr int GW = decltype(gw)::value;
+    const f32x4 sums = *(const f32x4*)(row + D);
+    const int word = __float_as_int(sums[3]);
+    no_key = (word & 2) != 0;
+    if ((word & 1) == 0) {
+      if (way == 0) m.add(sums[0], sums[1], sums[2], *(const f32x4*)(row + 4 * q), sums[0] != sums[0]);
+      return;
+    }
+    // (held to the workspace, whatever lies there if the lengths changed under the launch)
+    const int first = min(max(__float_as_int(sums[0]), 0), p.shares - 1), last = min(max(__float_as_int(sums[1]), 0), p.shares - 1);
+    const int x = min(max(__float_as_int(sums[2]), 0), 32 * GW - 1);
+    for (int i0 = first + way; i0 <= last; i0 += STEP * WAYS) {
+      f32x4 s[STEP], v[STEP];
+#pragma unroll
+      for (int k = 0; k < STEP; ++k) {
+        const int i = min(i0 + k * WAYS, last);
+        const float* part = joined_part<D>(p, hkv, i, i == first);
+        s[k] = *(const f32x4*)(part + part_sums<32 * GW, D>(x));
+        v[k] = *(const f32x4*)(part + part_index<GW, D>(x, 4 * q));
+      }
+#pragma unroll
+      for (int k = 0; k < STEP; ++k) {
+        if (i0 + k * WAYS > last) break;
+        m.add(s[k][0], s[k][1], s[k][2], v[k], s[k][0] != s[k][0]);
+      }
+    }
+  };
+  if (mine) {
+    take(row_results<D, kModePrefix>(p, token, head), std::integral_constant<int, GWP>{});
+    take(row_results<D, kModeOwn>(p, token, head), std::integral_constant<int, GWO>{});  // (no_key is this one's)
+  }
+  if constexpr (WAYS > 1) {
+    values[threadIdx.x] = m.o;
+    sums_of[threadIdx.x] = f32x4{m.M, m.l, m.lx, m.nan ? 1.f : 0.f};
+    __syncthreads();
+    if (way == 0)
+      for (int y = 1; y < WAYS; ++y) {
+        const f32x4 s = sums_of[y * ROWS * Q + threadIdx.x];
+        m.add(s[0], s[1], s[2], values[y * ROWS * Q + threadIdx.x], s[3] != 0.f);
+      }
+  }
+  if (!mine || way > 0) return;
+  const float inv = no_key ? 0.f : 1.0f / m.l;
+  *(u32x2*)(p.o + token * p.sot + head * p.soh + 4 * q) =
+      u32x2{E::pack2(m.o[0] * inv, m.o[1] * inv), E::pack2(m.o[2] * inv, m.o[3] * inv)};
+  if (p.lse && q == 0)
+    p.lse[(int64_t)head * p.seq.n_tokens + token] = !m.nan && m.M == INFINITY ? m.M : (m.M + log2f(m.lx)) * kLn2;
 }
 
 }  // namespace fa2

@@ -6,9 +6,6 @@ namespace fa2 {
 
 namespace {
 
-// (a window's pieces merge as all keys' do)
-constexpr int kCombineMode = FA2_MODE == kModeWindow ? kModeAll : FA2_MODE;
-
 template <int SRC, int GW>
 int launch_form(const RaggedParams& p, unsigned grid, hipStream_t s) {
   if (GW > 1 && p.lse)
@@ -18,7 +15,7 @@ int launch_form(const RaggedParams& p, unsigned grid, hipStream_t s) {
   hipError_t e = hipGetLastError();
   if constexpr (SRC != kSourcePacked) {
     if (e == hipSuccess && p.shares > 0) {
-      hipLaunchKernelGGL((attn_ragged_combine_kernel<FA2_DT, FA2_D, GW, kCombineMode>), dim3(grid * GW), dim3(combine_threads(FA2_D)), 0, s, p);
+      hipLaunchKernelGGL((attn_ragged_combine_kernel<FA2_DT, FA2_D, GW>), dim3(grid * GW), dim3(combine_threads(FA2_D)), 0, s, p);
       e = hipGetLastError();
     }
   }
@@ -29,16 +26,15 @@ int launch_form(const RaggedParams& p, unsigned grid, hipStream_t s) {
 
 template <>
 int launch_ragged<FA2_DT, FA2_D, FA2_MODE>(const RaggedParams& p, int source, int row_waves, unsigned grid, hipStream_t s) {
-  constexpr int kNoPages = FA2_MODE == kModeAll || FA2_MODE == kModeWindow ? kSourcePacked : kSourcePages;  // (pages only)
   if (row_waves == 1) {
     switch (source) {
-      case kSourcePacked: return launch_form<kNoPages, 1>(p, grid, s);
+      case kSourcePacked: return launch_form<kSourcePacked, 1>(p, grid, s);
       case kSourcePages: return launch_form<kSourcePages, 1>(p, grid, s);
       default: return launch_form<kSourceE4m3, 1>(p, grid, s);
     }
   }
   switch (source) {
-    case kSourcePacked: return launch_form<kNoPages, 4>(p, grid, s);
+    case kSourcePacked: return launch_form<kSourcePacked, 4>(p, grid, s);
     case kSourcePages: return launch_form<kSourcePages, 4>(p, grid, s);
     default: return launch_form<kSourceE4m3, 4>(p, grid, s);
   }

@@ -3,7 +3,8 @@ measurement library libfa2_ablate.so beside it.
 
     python triton-fa2-forward_amd/csrc/build.py [-j 8] [--verbose]
 
-Compiles attn_fwd_inst.hip once per (dtype, head_dim) pair and attn_ragged_inst.hip once per pair and choice of keys, plus
+Compiles attn_fwd_inst.hip and attn_shared_inst.hip once per (dtype, head_dim) pair and attn_ragged_inst.hip once per pair and
+choice of keys (all, a window's), plus
 the split-KV combine pass (attn_fwd_combine.hip), the key-norm pass (attn_key_norm.hip), the rotary and cache kernels
 (serve_cache.hip, serve_turn.hip), the page kernels (serve_pages.hip) and the C-ABI file fa2_fwd.hip,
 in parallel, with hipcc for gfx950 only, and links them into
@@ -52,7 +53,7 @@ CAPI_DIR = os.path.join(ROOT, "tests", "capi")
 ARCH = "gfx950"
 DTYPES = (0, 1)            # 0 = fp16, 1 = bf16
 HEAD_DIMS = (16, 32, 64, 128)
-RAGGED_MODES = (0, 1, 2, 3)  # csrc/serve_params.hpp: all keys, a window's, a common prefix's, those behind it
+RAGGED_MODES = (0, 1)  # csrc/serve_params.hpp: all keys, a window's
 SERVE_UNITS = ("serve_cache", "serve_turn", "serve_pages")
 
 
@@ -103,17 +104,19 @@ _KERNELS = {
 _SERVING_KERNELS = {
     "attn_ragged_kernel": (re.compile(r"attn_ragged_kernelILi(\d)ELi(\d+)ELi(\d)ELi(\d)ELb([01])ELi0EEEv"),
                            ("source", "row_waves", "lse")),
-    "attn_ragged_combine_kernel": (re.compile(r"attn_ragged_combine_kernelILi(\d)ELi(\d+)ELi(\d)ELi0EEEv"), ("row_waves",)),
+    "attn_ragged_combine_kernel": (re.compile(r"attn_ragged_combine_kernelILi(\d)ELi(\d+)ELi(\d)EEEv"), ("row_waves",)),
     "rotary_kernel": (re.compile(r"rotary_kernelILi(\d)ELi(\d+)EEEv"), ()),
     "cache_write_kernel": (re.compile(r"cache_write_kernelILi(\d)ELi(\d+)ELb([01])ENS_11CacheParamsEEEv"), ("e4m3",)),
     "cache_read_kernel": (re.compile(r"cache_read_kernelILi(\d)ELi(\d+)ELb([01])EEEv"), ("e4m3",)),
 }
 # ... and those of a step beyond that (windows, common prefixes, normalised rotations, pages)
 _STEP_KERNELS = {
-    "attn_ragged_kernel": (re.compile(r"attn_ragged_kernelILi(\d)ELi(\d+)ELi(\d)ELi(\d)ELb([01])ELi([123])EEEv"),
-                           ("source", "row_waves", "lse", "mode")),
-    "attn_ragged_combine_kernel": (re.compile(r"attn_ragged_combine_kernelILi(\d)ELi(\d+)ELi(\d)ELi([123])EEEv"),
-                                   ("row_waves", "mode")),
+    "attn_ragged_kernel": (re.compile(r"attn_ragged_kernelILi(\d)ELi(\d+)ELi(\d)ELi(\d)ELb([01])ELi1EEEv"),
+                           ("source", "row_waves", "lse")),
+    "attn_shared_kernel": (re.compile(r"attn_shared_kernelILi(\d)ELi(\d+)ELi(\d)ELi(\d)ELi(\d)ELb([01])EEEv"),
+                           ("source", "prefix_waves", "own_waves", "lse")),
+    "attn_shared_join_kernel": (re.compile(r"attn_shared_join_kernelILi(\d)ELi(\d+)ELi(\d)ELi(\d)EEEv"),
+                                ("prefix_waves", "own_waves")),
     "rotary_qk_kernel": (re.compile(r"rotary_qk_kernelILi(\d)ELi(\d+)EEEv"), ()),
     "cache_write_kernel": (re.compile(r"cache_write_kernelILi(\d)ELi(\d+)ELb([01])ENS_15CacheTurnParamsEEEv"), ("e4m3",)),
     "pages_extend_kernel": (re.compile(r"pages_extend_kernelENS"), ()),
@@ -188,6 +191,9 @@ def build_variant(name, defines, jobs=8, verbose=False):
                 cmds.append([cc, *flags, f"-DFA2_DT={dt}", f"-DFA2_D={d}", f"-DFA2_MODE={mode}", "-c",
                              os.path.join(CSRC, "attn_ragged_inst.hip"), "-o",
                              os.path.join(obj_dir, f"attn_ragged_dt{dt}_d{d}_m{mode}.o")])
+            cmds.append([cc, *flags, f"-DFA2_DT={dt}", f"-DFA2_D={d}", "-c",
+                         os.path.join(CSRC, "attn_shared_inst.hip"), "-o",
+                         os.path.join(obj_dir, f"attn_shared_dt{dt}_d{d}.o")])
     for name_ in ("attn_fwd_combine", "attn_fwd_wavesplit", "attn_key_norm", *SERVE_UNITS, "fa2_fwd", "fa2_scratch"):
         cmds.append([cc, *flags, "-c", os.path.join(CSRC, name_ + ".hip"), "-o",
                      os.path.join(obj_dir, name_ + ".o")])
@@ -218,6 +224,9 @@ def build(jobs=8, verbose=False):
                 serve_units.append([cc, *common_flags(), "-Rpass-analysis=kernel-resource-usage", f"-DFA2_DT={dt}",
                                     f"-DFA2_D={d}", f"-DFA2_MODE={mode}", "-c",
                                     os.path.join(CSRC, "attn_ragged_inst.hip"), "-o", obj])
+            obj = os.path.join(OBJ_DIR, f"attn_shared_dt{dt}_d{d}.o")
+            serve_units.append([cc, *common_flags(), "-Rpass-analysis=kernel-resource-usage", f"-DFA2_DT={dt}",
+                                f"-DFA2_D={d}", "-c", os.path.join(CSRC, "attn_shared_inst.hip"), "-o", obj])
             obj = os.path.join(OBJ_DIR, f"attn_fwd_ablate_dt{dt}_d{d}.o")
             ablate_units.append([cc, *common_flags(), f"-DFA2_DT={dt}", f"-DFA2_D={d}", "-c",
                                  os.path.join(CSRC, "attn_fwd_ablate_inst.hip"), "-o", obj])

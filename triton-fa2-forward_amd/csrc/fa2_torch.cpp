@@ -718,7 +718,7 @@ PyObject* attn_paged(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   if (want_lse) lse = at::empty({hq, T}, q->options().dtype(at::kFloat));
   const int64_t keys = (int64_t)s.max_pages * c.page_size;
   const size_t n_ws =
-      shared   ? fa2_paged_shared_workspace_bytes(hq, c.h_kv, c.head_dim, c.cache_dtype, T, s.n_seq, keys, cus)
+      shared   ? fa2_paged_shared_workspace_bytes(hq, c.h_kv, c.head_dim, T, s.n_seq, cus)
       : window ? fa2_paged_window_workspace_bytes(hq, c.h_kv, c.head_dim, c.cache_dtype, T, s.n_seq, keys, window, sinks, cus)
                : fa2_paged_workspace_bytes(hq, c.h_kv, c.head_dim, c.cache_dtype, T, s.n_seq, keys, cus);
   if (n_ws) ws = at::empty({(int64_t)n_ws}, q->options().dtype(at::kByte));

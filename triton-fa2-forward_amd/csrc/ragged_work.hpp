@@ -168,8 +168,19 @@ __device__ __forceinline__ int64_t readlane64(int64_t x, int l) {
 struct Cursor {
   int s0, l, tile;
   LaneSequence lanes;
+  // Of a common prefix's passes: the prefix, and the shares of this pass among those of the head
   Prefix prefix;
+  int shares, first_share;
+  double per_share;
 };
+template <int MODE>
+__device__ __forceinline__ int shares_of(ParamsRef p, const Cursor& c) {
+  return MODE >= kModePrefix ? c.shares : p.shares;
+}
+template <int MODE>
+__device__ __forceinline__ double per_share_of(ParamsRef p, const Cursor& c) {
+  return MODE >= kModePrefix ? c.per_share : p.per_share;
+}
 
 // The rank-th row tile; false: there are fewer.
 template <int BM, bool PAGES, int MODE>
@@ -230,9 +241,9 @@ __device__ __forceinline__ int64_t wave_max(int64_t x) {
 // longest costs no more than a share and what sharing costs. With one workgroup a CU, half of those that
 // fit, a key takes 5/8 of the time. Measured on MI355X (32 / 8 heads of 128), whole tiles and shares: 4 prompts of 500
 // 25 and 41 us; a chunk of 500 behind 500 33 and 40, behind 2k 62 and 53; 4 of 500 behind 4k 146 and 161.
-__device__ __forceinline__ bool whole_tiles(ParamsRef p, int64_t tiles, int64_t total, int64_t longest) {
-  if (tiles > p.shares) return false;
-  return (2 * tiles <= p.shares ? 5 * longest / 8 : longest) <= (int64_t)((double)total * p.per_share) + kShareCost;
+__device__ __forceinline__ bool whole_tiles(int shares, double per_share, int64_t tiles, int64_t total, int64_t longest) {
+  if (tiles > shares) return false;
+  return (2 * tiles <= shares ? 5 * longest / 8 : longest) <= (int64_t)((double)total * per_share) + kShareCost;
 }
 
 // Share j: [x, end) of the line, the cursor at the tile that x lies in, `in` from its start; x >= end: nothing.
@@ -256,14 +267,14 @@ __device__ __forceinline__ Share find_share(ParamsRef p, int j, int lane, Cursor
   }
   Share w;
   // (the same for every workgroup; how it is rounded does not matter, as long as shares * size reaches the total)
-  w.size = max((int64_t)((double)total * p.per_share) + 1, (int64_t)kLeastShare);
+  w.size = max((int64_t)((double)total * per_share_of<MODE>(p, *c)) + 1, (int64_t)kLeastShare);
   w.x = w.size * j;
   w.end = min(w.x + w.size, total);
   w.in = 0;
   if (BM != 32 && sequences<MODE>(p) <= 64) {
     const auto len = lengths_of<BM, MODE>(p, c->lanes.n_q, c->lanes.n_kv);
     const int64_t tiles = row_tiles<BM>(c->lanes.n_q, p.group), tiles_upto = wave_scan(tiles, lane);
-    if (whole_tiles(p, readlane64(tiles_upto, 63), total, wave_max(tiles > 0 ? len.of(tiles - 1) : 0))) {
+    if (whole_tiles(shares_of<MODE>(p, *c), per_share_of<MODE>(p, *c), readlane64(tiles_upto, 63), total, wave_max(tiles > 0 ? len.of(tiles - 1) : 0))) {
       const uint64_t past = __builtin_amdgcn_ballot_w64(tiles_upto > j);
       w.end = w.x;
       if (!past) return w;
@@ -347,7 +358,33 @@ __device__ __forceinline__ void head_and_rank(ParamsRef p, int block, int* head,
   }
 }
 
+// The shares of a head dealt to a common prefix's keys and to those behind it, as their lines' lengths are, whose keys cost
+// a 128-row workgroup 3/2 of a 32-row one; true: share `rank` is one of the prefix's. (Every workgroup gets the same.)
+template <int BMP, int BMO>
+__device__ __forceinline__ bool deal_shares(ParamsRef p, int rank, int lane, Cursor* c) {
+  c->prefix = common_prefix(p, lane);
+  const int n_q = max(row_bound(p.seq.cu, p.seq.n_seq, p.seq.n_tokens) - row_bound(p.seq.cu, 0, p.seq.n_tokens), 0);
+  const int64_t cost = c->prefix.tokens == 0 ? 16 : c->prefix.tokens + kTileCost<BMP>;  // (no keys: only empty results to write)
+  double ours = (double)(row_tiles<BMP>(n_q, p.group) * cost) * (BMP > BMO ? 1.5 : 1.0), own = 0.0;
+  for (int s0 = 0; s0 < p.seq.n_seq; s0 += 64) {
+    const LaneSequence q = lane_sequence<true, kModeOwn>(p, s0 + lane, c->prefix);
+    own += (double)readlane64(
+        wave_scan(lengths_of<BMO, kModeOwn>(p, q.n_q, q.n_kv).before(row_tiles<BMO>(q.n_q, p.group)), lane), 63);
+  }
+  const double share = ours + own > 0.0 ? ours / (ours + own) : 0.5;
+  const int prefix = __builtin_amdgcn_readfirstlane(min(max((int)(share * p.shares + 0.5), 1), p.shares - 1));
+  const bool is_prefix = rank < prefix;
+  c->first_share = is_prefix ? 0 : prefix;
+  c->shares = is_prefix ? prefix : p.shares - prefix;
+  c->per_share = 1.0 / c->shares;
+  return is_prefix;
+}
+
 // A share's partial results: slot 1 of the tile that starts in it, slot 0 of the one that it goes on with.
+template <int D>
+__device__ __forceinline__ float* joined_part(ParamsRef p, int head, int share, int slot) {  // (of a common prefix's passes)
+  return p.parts + (((int64_t)head * p.shares + share) * 2 + slot) * (p.part_rows * (D + 4));
+}
 template <int BM, int D>
 __device__ __forceinline__ float* part_of(ParamsRef p, int head, int share, int slot) {
   return p.parts + (((int64_t)head * p.shares + share) * 2 + slot) * (BM * (D + 4));

@@ -253,8 +253,7 @@ int launch_ragged(int32_t dtype, int32_t head_dim, int32_t h_q, fa2::RaggedParam
                   size_t workspace_bytes, void* stream) {
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const Topology topo = device_topology(stream_device(s));
-  const int32_t n_seq = MODE == fa2::kModePrefix ? 1 : p.seq.n_seq;
-  const RaggedPlan pl = ragged_plan(source, h_q, p.h_kv, head_dim, p.seq.n_tokens, n_seq, keys, topo.cus);
+  const RaggedPlan pl = ragged_plan(source, h_q, p.h_kv, head_dim, p.seq.n_tokens, p.seq.n_seq, keys, topo.cus);
   if (pl.grid > 0x7fffffffLL) return fail(FA2_EINVAL, "grid of %lld workgroups is too large", (long long)pl.grid);
   if (pl.workspace) {
     if (!workspace || workspace_bytes < pl.workspace)

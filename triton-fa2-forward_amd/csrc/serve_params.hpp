@@ -141,10 +141,11 @@ struct RaggedParams {
   void* merges;  // [h_kv * shares] of kMergeBytes: the tile that ends in each share
   // kModeWindow: a row sees the `window` newest keys up to its last, and the first `sinks`
   int32_t window, sinks;
-  // kModePrefix and kModeOwn: the leading tokens that all sequences have in common, on the device, and the results
-  // over them: [n_tokens * h_q][head_dim + 4] of O, m, l, exact l
+  // kModePrefix and kModeOwn: the leading tokens that all sequences have in common, on the device; every row's results over
+  // them and over its own keys, [2][n_tokens * h_q][head_dim + 4]; the rows of a partial result
   const int32_t* shared;
-  float* prefix;
+  float* rows;
+  int32_t part_rows;
 };
 
 }  // namespace fa2

@@ -54,17 +54,22 @@ int check_window(int32_t causal, int32_t window, int32_t sinks) {
   return FA2_OK;
 }
 
-// The workspace of attention behind a common prefix: the rows' results over it, then what either pass needs, one after
-// the other.
+// The form of attention behind a common prefix: 128-row workgroups for the prefix where the batch has more rows of a KV head than one
+// wave takes, and for the keys behind it by the rows of a sequence, as ragged_plan chooses them; `shares` workgroups per
+// head, which the kernel deals to the two. Workspace: every row's results of both, then the pieces of cut row tiles.
 struct SharedPlan {
-  size_t rows = 0, passes = 0;
+  int prefix_waves = 4, own_waves = 4, shares = 0;
+  size_t rows = 0, workspace = 0;
 };
-SharedPlan shared_plan(int source, int32_t h_q, int32_t h_kv, int32_t head_dim, int32_t n_tokens, int32_t n_seq, int64_t keys,
-                       int cus) {
+SharedPlan shared_plan(int32_t h_q, int32_t h_kv, int32_t head_dim, int32_t n_tokens, int32_t n_seq, int cus) {
   SharedPlan pl;
-  pl.rows = ((size_t)n_tokens * h_q * (head_dim + 4) * sizeof(float) + 255) & ~(size_t)255;
-  pl.passes = std::max(ragged_plan(source, h_q, h_kv, head_dim, n_tokens, 1, keys, cus).workspace,
-                       ragged_plan(source, h_q, h_kv, head_dim, n_tokens, n_seq, keys, cus).workspace);
+  const int64_t rows = (int64_t)n_tokens * (h_q / h_kv);
+  pl.prefix_waves = rows <= 32 ? 1 : 4;
+  pl.own_waves = rows <= (int64_t)32 * n_seq ? 1 : 4;
+  pl.shares = std::max(2, fa2::kSharedWaves * cus / h_kv);
+  const size_t row = (size_t)(head_dim + 4) * sizeof(float);
+  pl.rows = (2 * (size_t)n_tokens * h_q * row + 255) & ~(size_t)255;
+  pl.workspace = pl.rows + (size_t)h_kv * pl.shares * 2 * 32 * pl.prefix_waves * row;
   return pl;
 }
 
@@ -182,26 +187,42 @@ int fa2_attn_paged_shared(const void* q, void* out, const int64_t q_stride[2], c
   if (!shared) return fail(FA2_EINVAL, "null pointer: shared");
   if (reinterpret_cast<uintptr_t>(shared) & 3u) return fail(FA2_EALIGN, "shared must be 4-byte aligned");
   const int source = source_of(cache->cache_dtype);
-  const int64_t keys = (int64_t)p.seq.max_pages << p.seq.page_shift;
-  const int cus = device_topology(stream_device(static_cast<hipStream_t>(stream))).cus;
-  const SharedPlan pl = shared_plan(source, h_q, p.h_kv, cache->head_dim, p.seq.n_tokens, p.seq.n_seq, keys, cus);
-  if (!workspace || workspace_bytes < pl.rows + pl.passes)
-    return fail(FA2_EINVAL, "the call needs a workspace of %zu bytes, got %zu", pl.rows + pl.passes,
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  const Topology topo = device_topology(stream_device(st));
+  const SharedPlan pl = shared_plan(h_q, p.h_kv, cache->head_dim, p.seq.n_tokens, p.seq.n_seq, topo.cus);
+  if (!workspace || workspace_bytes < pl.workspace)
+    return fail(FA2_EINVAL, "the call needs a workspace of %zu bytes, got %zu", pl.workspace,
                 workspace ? workspace_bytes : (size_t)0);
   if (reinterpret_cast<uintptr_t>(workspace) & 255u) return fail(FA2_EALIGN, "the workspace must be 256-byte aligned");
+  p.group = h_q / p.h_kv;
+  const int64_t grid = (int64_t)p.h_kv * pl.shares;
+  if (std::max(grid, ((int64_t)p.seq.n_tokens * p.group + 7) / 8 * p.h_kv) > 0x7fffffffLL)
+    return fail(FA2_EINVAL, "a grid of more than 2^31 workgroups is too large");
   p.shared = shared;
-  p.prefix = static_cast<float*>(workspace);
-  void* const rest = static_cast<char*>(workspace) + pl.rows;
-  if (const int rc = launch_ragged<fa2::kModePrefix>(dtype, cache->head_dim, h_q, p, source, keys, rest, pl.passes, stream))
-    return rc;
-  return launch_ragged<fa2::kModeOwn>(dtype, cache->head_dim, h_q, p, source, keys, rest, pl.passes, stream);
+  p.xcd_shift = topo.xcd_shift;
+  p.shares = pl.shares;
+  p.rows = static_cast<float*>(workspace);
+  p.parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + pl.rows);
+  p.part_rows = 32 * pl.prefix_waves;
+  const unsigned g = (unsigned)grid;
+  int e;
+  switch (dtype * 4 + dim_index(cache->head_dim)) {
+    case 0: e = fa2::launch_shared<0, 16>(p, source, pl.prefix_waves, pl.own_waves, g, st); break;
+    case 1: e = fa2::launch_shared<0, 32>(p, source, pl.prefix_waves, pl.own_waves, g, st); break;
+    case 2: e = fa2::launch_shared<0, 64>(p, source, pl.prefix_waves, pl.own_waves, g, st); break;
+    case 3: e = fa2::launch_shared<0, 128>(p, source, pl.prefix_waves, pl.own_waves, g, st); break;
+    case 4: e = fa2::launch_shared<1, 16>(p, source, pl.prefix_waves, pl.own_waves, g, st); break;
+    case 5: e = fa2::launch_shared<1, 32>(p, source, pl.prefix_waves, pl.own_waves, g, st); break;
+    case 6: e = fa2::launch_shared<1, 64>(p, source, pl.prefix_waves, pl.own_waves, g, st); break;
+    default: e = fa2::launch_shared<1, 128>(p, source, pl.prefix_waves, pl.own_waves, g, st);
+  }
+  return launched(e, "attention");
 }
 
-size_t fa2_paged_shared_workspace_bytes(int32_t h_q, int32_t h_kv, int32_t head_dim, int32_t cache_dtype, int32_t n_tokens,
-                                        int32_t n_seq, int64_t max_keys, int32_t num_cus) {
+size_t fa2_paged_shared_workspace_bytes(int32_t h_q, int32_t h_kv, int32_t head_dim, int32_t n_tokens, int32_t n_seq,
+                                        int32_t num_cus) {
   if (h_q <= 0 || h_kv <= 0 || h_q % h_kv || dim_index(head_dim) < 0 || n_tokens <= 0 || n_seq <= 0 || num_cus <= 0) return 0;
-  const SharedPlan pl = shared_plan(source_of(cache_dtype), h_q, h_kv, head_dim, n_tokens, n_seq, max_keys, num_cus);
-  return pl.rows + pl.passes;
+  return shared_plan(h_q, h_kv, head_dim, n_tokens, n_seq, num_cus).workspace;
 }
 
 int fa2_pages_extend(const int32_t* free_pages, int32_t n_pages, const int32_t* count, int32_t* count_out, int32_t* table,

@@ -80,7 +80,7 @@ SIGNATURES = {
     "fa2_paged_window_workspace_bytes": (ctypes.c_size_t, [_i32] * 6 + [_i64, _i32, _i32, _i32]),
     "fa2_attn_paged_shared": (ctypes.c_int, [_vp, _vp, _i64p, _i64p, _cachep, _seqp, _vp, _i32, _i32, _i32, ctypes.c_float,
                                              _vp, _vp, ctypes.c_size_t, _vp]),
-    "fa2_paged_shared_workspace_bytes": (ctypes.c_size_t, [_i32] * 6 + [_i64, _i32]),
+    "fa2_paged_shared_workspace_bytes": (ctypes.c_size_t, [_i32] * 6),
     "fa2_rotary_qk": (ctypes.c_int, [_vp] * 4 + [_i64p] * 4 + [_vp, _i32, _i64p, _turnp] + [_i32] * 6 + [_vp]),
     "fa2_cache_write_turned": (ctypes.c_int, [_cachep, _seqp, _vp, _vp, _i64p, _i64p, _vp, _vp, _i64p, _i64p, _i32, _vp,
                                               _i32, _i64p, _turnp, _i32, _vp]),
@@ -380,9 +380,8 @@ def attn_paged_window(q, out, cache, seq, window, sinks, qk_scale, lse, workspac
         0 if workspace is None else workspace.numel(), stream), "fa2_attn_paged_window")
 
 
-def paged_shared_workspace_bytes(H_q, H_kv, D, cache_dtype, n_tokens, n_seq, max_keys, num_cus):
-    return int(lib().fa2_paged_shared_workspace_bytes(H_q, H_kv, D, CACHE_DTYPE_CODE[cache_dtype], n_tokens, n_seq, max_keys,
-                                                      num_cus))
+def paged_shared_workspace_bytes(H_q, H_kv, D, n_tokens, n_seq, num_cus):
+    return int(lib().fa2_paged_shared_workspace_bytes(H_q, H_kv, D, n_tokens, n_seq, num_cus))
 
 
 def attn_paged_shared(q, out, cache, seq, shared, causal, qk_scale, lse, workspace, stream):

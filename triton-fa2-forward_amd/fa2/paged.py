@@ -248,7 +248,7 @@ def attention_paged(q, cache, block_table, cu_seqlens, seqlens, *, causal=True, 
         sizes = (H_q, H_kv, D, cache.k.dtype, T, seqlens.numel(), block_table.shape[1] * cache.k.shape[2])
         cus = _cu_count(q.device)
         if shared is not None:
-            n = _lib.paged_shared_workspace_bytes(*sizes, cus)
+            n = _lib.paged_shared_workspace_bytes(H_q, H_kv, D, T, seqlens.numel(), cus)
         elif window is not None:
             n = _lib.paged_window_workspace_bytes(*sizes, window, sinks, cus)
         else:
