@@ -878,7 +878,7 @@ void attn_shared_kernel(const RaggedParams) {
   int hkv, rank;
   head_and_rank(p, (int)blockIdx.x, &hkv, &rank);
   Cursor cur{};
-  if (deal_shares<32 * GWP, 32 * GWO>(p, rank, threadIdx.x & 63, &cur))
+  if (deal_shares<32 * GWP, 32 * GWO, SRC == kSourceE4m3>(p, rank, threadIdx.x & 63, &cur))
     ragged_rows<DT, D, SRC, GWP, LSE, kModePrefix>(mem.prefix, hkv, rank, cur);
   else
     ragged_rows<DT, D, SRC, GWO, LSE, kModeOwn>(mem.own, hkv, rank - cur.first_share, cur);

@@ -39,6 +39,11 @@ __device__ __forceinline__ ParamsRef params_here() {
 // 201 / 185 / 164 / 166 us; steps of 64 sequences of 1000 keys in 32-row tiles 46.5 / 47.8 / 48.0 / 49.0.
 template <int BM>
 constexpr int kTileCost = BM == 32 ? 64 : 256;
+// ... a 32-row tile's behind a common prefix, where keys are few and the chain of a tile's loads takes longest; and in e4m3 beside that, as
+// the shares are dealt. Measured on MI355X, 32 / 8 heads of 128, costs of 64 / 128 / 256 / 384 / 640: 32 steps of one 16-bit token of their own
+// behind 4096 shared 29.5 / 22.2 / 17.7 / 17.7 / 18.1 us, of up to 500 behind 8192 24.2 / 25.7 / 24.5 / 24.6 / 24.8; 16 drafts of one e4m3 token
+// of their own behind 64 29.4 / 19.9 / 13.6 / 13.9 / 15.8, of up to 300 behind 32k 51.0 / 54.7 / 53.0 / 50.2 / 49.8.
+constexpr int kOwnTileCost = 384, kOwnE4m3Cost = 448;
 // ... and what sharing the tiles out costs a 128-row workgroup: more pieces, the partial results, their merge
 constexpr int kShareCost = 640;
 // The most sequences whose tiles go by their index (above; at most 64, a lane each).
@@ -52,22 +57,38 @@ struct LaneSequence {
   int first, n_q, n_kv, kv_first;
 };
 
+template <bool PAGES>
+__device__ __forceinline__ LaneSequence lane_sequence(ParamsRef p, int s) {
+  LaneSequence q = {0, 0, 0, 0};
+  if (s >= p.seq.n_seq) return q;
+  q.first = row_bound(p.seq.cu, s, p.seq.n_tokens);
+  q.n_q = max(row_bound(p.seq.cu, s + 1, p.seq.n_tokens) - q.first, 0);
+  if constexpr (PAGES) {
+    q.n_kv = (int)min((int64_t)max(p.seq.lens[s], 0), (int64_t)p.seq.max_pages << p.seq.page_shift);
+  } else {
+    q.kv_first = row_bound(p.cu_kv, s, p.kv_tokens);
+    q.n_kv = max(row_bound(p.cu_kv, s + 1, p.kv_tokens) - q.kv_first, 0);
+  }
+  return q;
+}
+
 // The leading tokens that all sequences with new tokens have in common, and of whose rows of the table they are read. At
 // most p.shared says, whole pages, and none that is a row's own or behind it: every row of the call sees them all.
 // Everyone who asks gets the same answer, so that the two passes over the keys agree.
 struct Prefix {
   int tokens, row;
 };
-__device__ __forceinline__ Prefix common_prefix(ParamsRef p, int lane) {
-  const int64_t most = (int64_t)p.seq.max_pages << p.seq.page_shift;
-  int tokens = min((int64_t)max(p.shared[0], 0), most), row = p.seq.n_seq;
-  for (int s0 = 0; s0 < p.seq.n_seq; s0 += 64) {
-    const int s = s0 + lane;
-    if (s >= p.seq.n_seq) continue;
-    const int n_q = row_bound(p.seq.cu, s + 1, p.seq.n_tokens) - row_bound(p.seq.cu, s, p.seq.n_tokens);
-    if (n_q <= 0) continue;
-    tokens = min(tokens, max((int)min((int64_t)p.seq.lens[s], most) - n_q, 0));
-    row = min(row, s);
+__device__ __forceinline__ Prefix common_prefix(ParamsRef p, int lane, const LaneSequence& first) {
+  int tokens = (int)min((int64_t)max(p.shared[0], 0), (int64_t)p.seq.max_pages << p.seq.page_shift), row = p.seq.n_seq;
+  LaneSequence q = first;  // (of the first 64 sequences)
+  for (int s = lane;;) {
+    if (q.n_q > 0) {
+      tokens = min(tokens, max(q.n_kv - q.n_q, 0));
+      row = min(row, s);
+    }
+    s += 64;
+    if (s - lane >= p.seq.n_seq) break;
+    q = lane_sequence<true>(p, s);
   }
 #pragma unroll
   for (int off = 32; off >= 1; off /= 2) {
@@ -77,37 +98,6 @@ __device__ __forceinline__ Prefix common_prefix(ParamsRef p, int lane) {
   tokens = __builtin_amdgcn_readfirstlane(tokens) & ~((1 << p.seq.page_shift) - 1);
   row = __builtin_amdgcn_readfirstlane(row);
   return row == p.seq.n_seq ? Prefix{0, 0} : Prefix{tokens, row};
-}
-
-// Sequences whose tiles are dealt out
-template <int MODE>
-__device__ __forceinline__ int sequences(ParamsRef p) {
-  return MODE == kModePrefix ? min(p.seq.n_seq, 1) : p.seq.n_seq;
-}
-
-// kv_first: the first key's row in k and v, or, behind a common prefix, its position in the sequence
-template <bool PAGES, int MODE>
-__device__ __forceinline__ LaneSequence lane_sequence(ParamsRef p, int s, const Prefix& prefix) {
-  LaneSequence q = {0, 0, 0, 0};
-  if (s >= sequences<MODE>(p)) return q;
-  q.first = row_bound(p.seq.cu, s, p.seq.n_tokens);
-  if constexpr (MODE == kModePrefix) {
-    q.n_q = max(row_bound(p.seq.cu, p.seq.n_seq, p.seq.n_tokens) - q.first, 0);
-    q.n_kv = prefix.tokens;
-    return q;
-  }
-  q.n_q = max(row_bound(p.seq.cu, s + 1, p.seq.n_tokens) - q.first, 0);
-  if constexpr (PAGES) {
-    q.n_kv = (int)min((int64_t)max(p.seq.lens[s], 0), (int64_t)p.seq.max_pages << p.seq.page_shift);
-    if constexpr (MODE == kModeOwn) {
-      q.kv_first = prefix.tokens;
-      q.n_kv = max(q.n_kv - prefix.tokens, 0);
-    }
-  } else {
-    q.kv_first = row_bound(p.cu_kv, s, p.kv_tokens);
-    q.n_kv = max(row_bound(p.cu_kv, s + 1, p.kv_tokens) - q.kv_first, 0);
-  }
-  return q;
 }
 
 // The block's lane l, wave-uniform
@@ -144,9 +134,10 @@ __device__ __forceinline__ auto lengths_of(ParamsRef p, int n_q, int n_kv) {
     const int64_t full = base >= cap ? 0 : slope == 0 ? (int64_t)1 << 31 : (cap - base + slope - 1) / slope;
     return WindowLengths{base, slope, cap, full};
   } else {
-    if (MODE == kModePrefix || !p.causal) return Lengths{(int64_t)n_kv + kTileCost<BM>, 0};
+    constexpr int64_t kCost = MODE == kModeOwn && BM == 32 ? kOwnTileCost : kTileCost<BM>;
+    if (MODE == kModePrefix || !p.causal) return Lengths{(int64_t)n_kv + kCost, 0};
     const int64_t slope = BM / p.group;
-    return Lengths{(int64_t)max(n_kv - n_q, 0) + slope + kTileCost<BM>, slope};
+    return Lengths{(int64_t)max(n_kv - n_q, 0) + slope + kCost, slope};
   }
 }
 
@@ -168,11 +159,30 @@ __device__ __forceinline__ int64_t readlane64(int64_t x, int l) {
 struct Cursor {
   int s0, l, tile;
   LaneSequence lanes;
-  // Of a common prefix's passes: the prefix, and the shares of this pass among those of the head
+  // Of a common prefix's passes: the first 64 sequences (loaded once, by every lane for all passes), the rows of all, the prefix, and the
+  // shares of this pass among those of the head
+  LaneSequence raw;
+  int rows_first, rows;
   Prefix prefix;
   int shares, first_share;
   double per_share;
 };
+// Sequences whose tiles are dealt out
+template <int MODE>
+__device__ __forceinline__ int sequences(ParamsRef p) {
+  return MODE == kModePrefix ? min(p.seq.n_seq, 1) : p.seq.n_seq;
+}
+// Lane s of the sequences as the pass takes them: all rows as one sequence's over a prefix; or the keys behind it, kv_first being
+// the first one's position
+template <bool PAGES, int MODE>
+__device__ __forceinline__ LaneSequence lane_sequence(ParamsRef p, int s, const Cursor& c) {
+  if constexpr (MODE < kModePrefix) return lane_sequence<PAGES>(p, s);
+  if (MODE == kModePrefix) return s == 0 ? LaneSequence{c.rows_first, c.rows, c.prefix.tokens, 0} : LaneSequence{0, 0, 0, 0};
+  LaneSequence q = s < 64 ? c.raw : lane_sequence<true>(p, s);
+  q.kv_first = c.prefix.tokens;
+  q.n_kv = max(q.n_kv - c.prefix.tokens, 0);
+  return q;
+}
 template <int MODE>
 __device__ __forceinline__ int shares_of(ParamsRef p, const Cursor& c) {
   return MODE >= kModePrefix ? c.shares : p.shares;
@@ -185,7 +195,7 @@ __device__ __forceinline__ double per_share_of(ParamsRef p, const Cursor& c) {
 // The rank-th row tile; false: there are fewer.
 template <int BM, bool PAGES, int MODE>
 __device__ __forceinline__ bool find_tile(ParamsRef p, int rank, int lane, Cursor* c) {
-  c->lanes = lane_sequence<PAGES, MODE>(p, lane, c->prefix);
+  c->lanes = lane_sequence<PAGES, MODE>(p, lane, *c);
   if (sequences<MODE>(p) <= kFewSequences) {
     // Tiles of index t and above, over all sequences: A(t) = sum_s max(tiles_s - t, 0). The rank-th tile in the
     // order of falling t has the largest t with A(t) > rank; every lane tries a t of its own.
@@ -216,7 +226,7 @@ __device__ __forceinline__ bool find_tile(ParamsRef p, int rank, int lane, Curso
   }
   int64_t base = 0;
   for (int s0 = 0; s0 < sequences<MODE>(p); s0 += 64) {
-    if (s0) c->lanes = lane_sequence<PAGES, MODE>(p, s0 + lane, c->prefix);
+    if (s0) c->lanes = lane_sequence<PAGES, MODE>(p, s0 + lane, *c);
     const int64_t tiles = row_tiles<BM>(c->lanes.n_q, p.group);
     const int64_t upto = base + wave_scan(tiles, lane);
     const uint64_t past = __builtin_amdgcn_ballot_w64(upto > rank);
@@ -256,13 +266,13 @@ __device__ __forceinline__ Share find_share(ParamsRef p, int j, int lane, Cursor
   auto length = [&]() {
     return lengths_of<BM, MODE>(p, c->lanes.n_q, c->lanes.n_kv).before(row_tiles<BM>(c->lanes.n_q, p.group));
   };
-  c->lanes = lane_sequence<PAGES, MODE>(p, lane, c->prefix);
+  c->lanes = lane_sequence<PAGES, MODE>(p, lane, *c);
   c->s0 = 0;
   int64_t mine = length();
   int64_t upto = wave_scan(mine, lane);
   int64_t total = readlane64(upto, 63);
   for (int s0 = 64; s0 < sequences<MODE>(p); s0 += 64) {
-    c->lanes = lane_sequence<PAGES, MODE>(p, s0 + lane, c->prefix);
+    c->lanes = lane_sequence<PAGES, MODE>(p, s0 + lane, *c);
     total += readlane64(wave_scan(length(), lane), 63);
   }
   Share w;
@@ -286,7 +296,7 @@ __device__ __forceinline__ Share find_share(ParamsRef p, int j, int lane, Cursor
   }
   if (w.x >= w.end) return w;
   int64_t base = 0;
-  if (sequences<MODE>(p) > 64) c->lanes = lane_sequence<PAGES, MODE>(p, lane, c->prefix);
+  if (sequences<MODE>(p) > 64) c->lanes = lane_sequence<PAGES, MODE>(p, lane, *c);
   while (base + readlane64(upto, 63) <= w.x) {  // (w.x < total: ends within the sequences)
     base += readlane64(upto, 63);
     c->s0 += 64;
@@ -294,7 +304,7 @@ __device__ __forceinline__ Share find_share(ParamsRef p, int j, int lane, Cursor
       w.end = w.x;
       return w;
     }
-    c->lanes = lane_sequence<PAGES, MODE>(p, c->s0 + lane, c->prefix);
+    c->lanes = lane_sequence<PAGES, MODE>(p, c->s0 + lane, *c);
     mine = length();
     upto = wave_scan(mine, lane);
   }
@@ -339,7 +349,7 @@ __device__ __forceinline__ bool next_tile(ParamsRef p, int lane, Cursor* c) {
     if (c->s0 + 64 >= sequences<MODE>(p)) return false;
     c->s0 += 64;
     c->l = -1;
-    c->lanes = lane_sequence<PAGES, MODE>(p, c->s0 + lane, c->prefix);
+    c->lanes = lane_sequence<PAGES, MODE>(p, c->s0 + lane, *c);
   }
 }
 
@@ -360,16 +370,19 @@ __device__ __forceinline__ void head_and_rank(ParamsRef p, int block, int* head,
 
 // The shares of a head dealt to a common prefix's keys and to those behind it, as their lines' lengths are, whose keys cost
 // a 128-row workgroup 3/2 of a 32-row one; true: share `rank` is one of the prefix's. (Every workgroup gets the same.)
-template <int BMP, int BMO>
+template <int BMP, int BMO, bool E4M3>
 __device__ __forceinline__ bool deal_shares(ParamsRef p, int rank, int lane, Cursor* c) {
-  c->prefix = common_prefix(p, lane);
-  const int n_q = max(row_bound(p.seq.cu, p.seq.n_seq, p.seq.n_tokens) - row_bound(p.seq.cu, 0, p.seq.n_tokens), 0);
+  c->raw = lane_sequence<true>(p, lane);
+  c->rows_first = row_bound(p.seq.cu, 0, p.seq.n_tokens);
+  c->rows = max(row_bound(p.seq.cu, p.seq.n_seq, p.seq.n_tokens) - c->rows_first, 0);
+  c->prefix = common_prefix(p, lane, c->raw);
   const int64_t cost = c->prefix.tokens == 0 ? 16 : c->prefix.tokens + kTileCost<BMP>;  // (no keys: only empty results to write)
-  double ours = (double)(row_tiles<BMP>(n_q, p.group) * cost) * (BMP > BMO ? 1.5 : 1.0), own = 0.0;
+  double ours = (double)(row_tiles<BMP>(c->rows, p.group) * cost) * (BMP > BMO ? 1.5 : 1.0), own = 0.0;
   for (int s0 = 0; s0 < p.seq.n_seq; s0 += 64) {
-    const LaneSequence q = lane_sequence<true, kModeOwn>(p, s0 + lane, c->prefix);
-    own += (double)readlane64(
-        wave_scan(lengths_of<BMO, kModeOwn>(p, q.n_q, q.n_kv).before(row_tiles<BMO>(q.n_q, p.group)), lane), 63);
+    const LaneSequence q = lane_sequence<true, kModeOwn>(p, s0 + lane, *c);
+    const int64_t tiles = row_tiles<BMO>(q.n_q, p.group);
+    const int64_t line = lengths_of<BMO, kModeOwn>(p, q.n_q, q.n_kv).before(tiles) + (E4M3 ? kOwnE4m3Cost * tiles : 0);
+    own += (double)readlane64(wave_scan(line, lane), 63);
   }
   const double share = ours + own > 0.0 ? ours / (ours + own) : 0.5;
   const int prefix = __builtin_amdgcn_readfirstlane(min(max((int)(share * p.shares + 0.5), 1), p.shares - 1));
