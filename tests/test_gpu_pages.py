@@ -113,6 +113,18 @@ def test_release(n):
         assert t.tolist() == table and pool.count.tolist() == [count]
 
 
+def test_release_wide():
+    """Tables too wide for one launch: the same."""
+    from fa2.pages import pages_release
+    rng = random.Random(9)
+    n, columns = 300, 1000
+    free, count, table, lens = sequences(rng, n, 16, 2000, columns, 40 * n)
+    first, last = [rng.choice([0, 3]) for _ in range(n)], [rng.choice([0, -(-x // 16), columns]) for x in lens]
+    got = pages_release(pool_of(free, count), i32(table), i32(first), i32(last))
+    want, want_count = step_oracle.release(free, count, table, first, last)
+    assert got.count.tolist() == [want_count] and got.free.tolist() == want
+
+
 def test_release_more_than_the_pool_holds():
     from fa2.pages import pages_release
     pool = pool_of([0, 1, 2, 3], 3)

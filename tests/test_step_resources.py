@@ -25,7 +25,7 @@ def test_every_instance_is_recorded():
     # the two of pages, and 32 rows for both passes, or 128 and 32, or 128, these with and without the log-sum-exp
     assert count == {"attn_ragged_kernel": 8 * 3 * 3, "attn_shared_kernel": 8 * 2 * 5, "attn_shared_join_kernel": 8 * 3,
                      "rotary_qk_kernel": 8, "cache_write_kernel": 8 * 2, "pages_extend_kernel": 1, "pages_count_kernel": 1,
-                     "pages_release_kernel": 1}
+                     "pages_release_kernel": 1, "pages_release_once_kernel": 1}
 
 
 def test_as_many_workgroups_fit_a_cu_as_the_grids_count_on():

@@ -122,6 +122,7 @@ _STEP_KERNELS = {
     "pages_extend_kernel": (re.compile(r"pages_extend_kernelENS"), ()),
     "pages_count_kernel": (re.compile(r"pages_count_kernelENS"), ()),
     "pages_release_kernel": (re.compile(r"pages_release_kernelENS"), ()),
+    "pages_release_once_kernel": (re.compile(r"pages_release_once_kernelENS"), ()),
 }
 
 
