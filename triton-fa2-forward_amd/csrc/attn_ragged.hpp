@@ -54,15 +54,17 @@ __device__ __forceinline__ float* row_results(ParamsRef p, int64_t token, int he
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
-// A workgroup's LDS
+// A workgroup's LDS: K and V, and where four waves take a row's keys in turn, what they merge
 template <int D, int GW>
 struct RaggedLds {
-  static constexpr int kBufs = GW == 1 ? 1 : 2, kGroups = 4 / GW;
-  static constexpr int kKvChunks = kGroups * kBufs * 2 * ragged_block_n(D, GW) * (D / 8);
-  static constexpr int kMergeChunks = kGroups > 1 ? 32 * GW * kGroups * (D / 4) : 0;
+  u32x4 kv[2 * 2 * ragged_block_n(D, 4) * (D / 8)];
+};
+template <int D>
+struct RaggedLds<D, 1> {
+  static constexpr int kKvChunks = 4 * 2 * ragged_block_n(D, 1) * (D / 8), kMergeChunks = 32 * 4 * (D / 4);
   u32x4 kv[kKvChunks > kMergeChunks ? kKvChunks : kMergeChunks];
-  float sm[kGroups][kGroups > 1 ? 32 * GW : 1][3];  // m, l, exact l of every group's rows
-  int odd[kGroups > 1 ? 32 * GW : 1];               // rows whose sums are not finite
+  float sm[4][32][3];  // m, l, exact l of every group's rows
+  int odd[32];         // rows whose sums are not finite
 };
 
 // LSE: with 128 rows, whether p.lse is set: known to the compiler, the sums it needs mix with the rest of the tile's
@@ -96,8 +98,6 @@ __device__ __forceinline__ void ragged_rows(RaggedLds<D, GW>& mem, int hkv, int 
   constexpr int QPR = D / 4;             // 16-byte pieces of an fp32 output row
 
   auto& lds = mem.kv;
-  auto& sm = mem.sm;
-  auto& odd = mem.odd;
 
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -776,6 +776,8 @@ __device__ __forceinline__ void ragged_rows(RaggedLds<D, GW>& mem, int hkv, int 
       for (uint64_t todo = again_rows; todo; todo &= todo - 1)
         again(gwave * 32 + __builtin_ctzll(todo), m_i != m_i);
     } else {
+      auto& sm = mem.sm;
+      auto& odd = mem.odd;
       // ---- merge the groups through LDS: O^T blocks as 16-byte pieces [group][row][4 dims], then
       // every thread folds the groups of its pieces
       if (tid < BM) odd[tid] = 0;
@@ -981,13 +983,10 @@ __global__ __launch_bounds__(1024) void attn_shared_join_kernel(const RaggedPara
   const bool mine = token >= row_bound(p.seq.cu, 0, p.seq.n_tokens) && token < row_bound(p.seq.cu, p.seq.n_seq, p.seq.n_tokens);
   Merged m = {-INFINITY, 0.f, 0.f, f32x4{0.f, 0.f, 0.f, 0.f}, false};
   bool no_key = false;
-  auto take = [&](const float* row, auto gw) {
+  auto take = [&](const f32x4& sums, const f32x4& value, auto gw) {
     constexpr int GW = decltype(gw)::value;
-    const f32x4 sums = *(const f32x4*)(row + D);
-    const int word = __float_as_int(sums[3]);
-    no_key = (word & 2) != 0;
-    if ((word & 1) == 0) {
-      if (way == 0) m.add(sums[0], sums[1], sums[2], *(const f32x4*)(row + 4 * q), sums[0] != sums[0]);
+    if ((__float_as_int(sums[3]) & 1) == 0) {
+      if (way == 0) m.add(sums[0], sums[1], sums[2], value, sums[0] != sums[0]);
       return;
     }
     // (held to the workspace, whatever lies there if the lengths changed under the launch)
@@ -1010,8 +1009,13 @@ __global__ __launch_bounds__(1024) void attn_shared_join_kernel(const RaggedPara
     }
   };
   if (mine) {
-    take(row_results<D, kModePrefix>(p, token, head), std::integral_constant<int, GWP>{});
-    take(row_results<D, kModeOwn>(p, token, head), std::integral_constant<int, GWO>{});  // (no_key is this one's)
+    const float *of_prefix = row_results<D, kModePrefix>(p, token, head), *of_own = row_results<D, kModeOwn>(p, token, head);
+    const f32x4 a = *(const f32x4*)(of_prefix + D), b = *(const f32x4*)(of_own + D);
+    // (where a row is in pieces its place for values holds nothing, and is not looked at)
+    const f32x4 va = *(const f32x4*)(of_prefix + 4 * q), vb = *(const f32x4*)(of_own + 4 * q);
+    no_key = (__float_as_int(b[3]) & 2) != 0;
+    take(a, va, std::integral_constant<int, GWP>{});
+    take(b, vb, std::integral_constant<int, GWO>{});
   }
   if constexpr (WAYS > 1) {
     values[threadIdx.x] = m.o;

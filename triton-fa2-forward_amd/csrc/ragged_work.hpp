@@ -72,6 +72,43 @@ __device__ __forceinline__ LaneSequence lane_sequence(ParamsRef p, int s) {
   return q;
 }
 
+// Sums up to each lane, and the largest and least of a wave, by moves between neighbouring lanes (DPP): a step takes a few cycles
+// where one through LDS takes a hundred, and a workgroup's search for its work is a chain of them. Lanes that a move does not reach
+// take `old`.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int moved(int old, int x) {
+  return __builtin_amdgcn_update_dpp(old, x, CTRL, ROWS, 0xf, false);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int64_t moved64(int64_t old, int64_t x) {
+  const uint32_t lo = (uint32_t)moved<CTRL, ROWS>((int)(uint32_t)old, (int)(uint32_t)x);
+  const uint32_t hi = (uint32_t)moved<CTRL, ROWS>((int)(old >> 32), (int)(x >> 32));
+  return (int64_t)(((uint64_t)hi << 32) | lo);
+}
+// Every lane's value joined by f with those of the lanes before it: 1, 2, 4 and 8 lanes back in its row of 16, then the row's and the
+// half wave's before it
+template <class F>
+__device__ __forceinline__ int64_t wave_fold(int64_t x, bool sums, F&& f) {
+  x = f(x, moved64<0x111, 0xf>(sums ? 0 : x, x));
+  x = f(x, moved64<0x112, 0xf>(sums ? 0 : x, x));
+  x = f(x, moved64<0x114, 0xf>(sums ? 0 : x, x));
+  x = f(x, moved64<0x118, 0xf>(sums ? 0 : x, x));
+  x = f(x, moved64<0x142, 0xa>(sums ? 0 : x, x));
+  return f(x, moved64<0x143, 0xc>(sums ? 0 : x, x));
+}
+__device__ __forceinline__ int64_t wave_scan(int64_t x, int) {
+  return wave_fold(x, true, [](int64_t a, int64_t b) { return a + b; });
+}
+__device__ __forceinline__ int wave_min(int x) {
+  x = min(x, moved<0x111, 0xf>(x, x));
+  x = min(x, moved<0x112, 0xf>(x, x));
+  x = min(x, moved<0x114, 0xf>(x, x));
+  x = min(x, moved<0x118, 0xf>(x, x));
+  x = min(x, moved<0x142, 0xa>(x, x));
+  x = min(x, moved<0x143, 0xc>(x, x));
+  return __builtin_amdgcn_readlane(x, 63);
+}
+
 // The leading tokens that all sequences with new tokens have in common, and of whose rows of the table they are read. At
 // most p.shared says, whole pages, and none that is a row's own or behind it: every row of the call sees them all.
 // Everyone who asks gets the same answer, so that the two passes over the keys agree.
@@ -90,13 +127,8 @@ __device__ __forceinline__ Prefix common_prefix(ParamsRef p, int lane, const Lan
     if (s - lane >= p.seq.n_seq) break;
     q = lane_sequence<true>(p, s);
   }
-#pragma unroll
-  for (int off = 32; off >= 1; off /= 2) {
-    tokens = min(tokens, __shfl_xor(tokens, off, 64));
-    row = min(row, __shfl_xor(row, off, 64));
-  }
-  tokens = __builtin_amdgcn_readfirstlane(tokens) & ~((1 << p.seq.page_shift) - 1);
-  row = __builtin_amdgcn_readfirstlane(row);
+  tokens = wave_min(tokens) & ~((1 << p.seq.page_shift) - 1);
+  row = wave_min(row);
   return row == p.seq.n_seq ? Prefix{0, 0} : Prefix{tokens, row};
 }
 
@@ -141,14 +173,6 @@ __device__ __forceinline__ auto lengths_of(ParamsRef p, int n_q, int n_kv) {
   }
 }
 
-__device__ __forceinline__ int64_t wave_scan(int64_t x, int lane) {
-#pragma unroll
-  for (int off = 1; off < 64; off *= 2) {
-    const int64_t y = __shfl_up(x, off, 64);
-    if (lane >= off) x += y;
-  }
-  return x;
-}
 __device__ __forceinline__ int64_t readlane64(int64_t x, int l) {
   const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)x, l);
   const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)((uint64_t)x >> 32), l);
@@ -242,17 +266,18 @@ __device__ __forceinline__ bool find_tile(ParamsRef p, int rank, int lane, Curso
 }
 
 __device__ __forceinline__ int64_t wave_max(int64_t x) {
-#pragma unroll
-  for (int off = 32; off >= 1; off /= 2) x = max(x, (int64_t)__shfl_xor(x, off, 64));
-  return readlane64(x, 0);  // (a scalar: what is chosen by it stays one too)
+  return readlane64(wave_fold(x, false, [](int64_t a, int64_t b) { return max(a, b); }), 63);  // (a scalar: what is chosen by it stays one too)
 }
 
 // Whether a tile per workgroup takes no longer than equal shares, as estimated: as many tiles as workgroups at most, whose
 // longest costs no more than a share and what sharing costs. With one workgroup a CU, half of those that
 // fit, a key takes 5/8 of the time. Measured on MI355X (32 / 8 heads of 128), whole tiles and shares: 4 prompts of 500
-// 25 and 41 us; a chunk of 500 behind 500 33 and 40, behind 2k 62 and 53; 4 of 500 behind 4k 146 and 161.
+// 25 and 41 us; a chunk of 500 behind 500 33 and 40, behind 2k 62 and 53; 4 of 500 behind 4k 146 and 161. Behind a common prefix
+// 32-row tiles too, as a cut costs one more of their chains of loads: 32 steps of up to 500 behind 8192 shared 24.6 and 22.9.
+template <int BM>
 __device__ __forceinline__ bool whole_tiles(int shares, double per_share, int64_t tiles, int64_t total, int64_t longest) {
   if (tiles > shares) return false;
+  if (BM == 32) return longest <= (int64_t)((double)total * per_share) + 2 * kOwnTileCost;
   return (2 * tiles <= shares ? 5 * longest / 8 : longest) <= (int64_t)((double)total * per_share) + kShareCost;
 }
 
@@ -281,10 +306,10 @@ __device__ __forceinline__ Share find_share(ParamsRef p, int j, int lane, Cursor
   w.x = w.size * j;
   w.end = min(w.x + w.size, total);
   w.in = 0;
-  if (BM != 32 && sequences<MODE>(p) <= 64) {
+  if ((BM != 32 || MODE == kModeOwn) && sequences<MODE>(p) <= 64) {
     const auto len = lengths_of<BM, MODE>(p, c->lanes.n_q, c->lanes.n_kv);
     const int64_t tiles = row_tiles<BM>(c->lanes.n_q, p.group), tiles_upto = wave_scan(tiles, lane);
-    if (whole_tiles(shares_of<MODE>(p, *c), per_share_of<MODE>(p, *c), readlane64(tiles_upto, 63), total, wave_max(tiles > 0 ? len.of(tiles - 1) : 0))) {
+    if (whole_tiles<BM>(shares_of<MODE>(p, *c), per_share_of<MODE>(p, *c), readlane64(tiles_upto, 63), total, wave_max(tiles > 0 ? len.of(tiles - 1) : 0))) {
       const uint64_t past = __builtin_amdgcn_ballot_w64(tiles_upto > j);
       w.end = w.x;
       if (!past) return w;
