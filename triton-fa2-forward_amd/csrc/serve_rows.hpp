@@ -304,21 +304,47 @@ __global__ __launch_bounds__(256) void cache_write_kernel(const Params p) {
   __shared__ uint8_t scales[E4M3 ? kScalesAtOnce : 1];  // [K and V heads][tokens]
   const int t0 = (int)blockIdx.x * p.tokens_per_wg;
   const int tokens = min(p.tokens_per_wg, p.seq.n_tokens - t0);
-  const bool gather = E4M3 && tokens > 1 && (int64_t)tokens * 2 * p.h_kv <= kScalesAtOnce;
+  const bool gather = E4M3 && tokens > 1 && (!kTurn || gridDim.y == 1) && (int64_t)tokens * 2 * p.h_kv <= kScalesAtOnce;
   const int chunk = threadIdx.x % LPR;
   const int per_token = 2 * p.h_kv + (p.q ? p.h_q : 0);
   const int rows = tokens * per_token;
   const int half = p.rot.half;
   const bool interleaved = p.rot.interleaved;
-  for (int base = 0; base < rows; base += kRowsAtOnce * (256 / LPR)) {
+  auto look_up = [&]() {
+    LanePlace place;
+    int page = -1;
+    const bool looks_up = threadIdx.x < 64;
+    if (looks_up) {
+      place = find_positions(p.seq, t0, tokens, (int)threadIdx.x);
+      if ((int)threadIdx.x < tokens) places[threadIdx.x].pos = place.pos;
+      page = find_page(p.seq, place);  // on its way while the angles are computed
+    }
+    __syncthreads();
+    if constexpr (kTurn) {
+      fill_weights<D>(weights, p.turn);
+      fill_axes(cs, p.rot, p.turn, tokens, [&](int t, int axis) -> int64_t {
+        return p.turn.positions ? position_at(p.turn, axis * p.turn.spa + (t0 + t) * p.turn.spn) : (int64_t)places[t].pos;
+      });
+    } else {
+      if (p.rot.half) fill_angles(cs, p.rot, tokens, [&](int t) -> int64_t { return places[t].pos; });
+    }
+    if (looks_up && (int)threadIdx.x < tokens) places[threadIdx.x].page = page;
+    __syncthreads();
+  };
+  // Turned rows: the places and angles first, so that what they need does not stay in registers; few tokens' rows are dealt out to
+  // several workgroups, which each work those out.
+  const int share = kTurn ? (rows + (256 / LPR) * (int)gridDim.y - 1) / ((256 / LPR) * (int)gridDim.y) * (256 / LPR) : rows;
+  const int row0 = kTurn ? (int)blockIdx.y * share : 0, row_end = kTurn ? min(row0 + share, rows) : rows;
+  if constexpr (kTurn) look_up();
+  for (int base = row0; base < row_end; base += kRowsAtOnce * (256 / LPR)) {
     Chunks in[kRowsAtOnce];
     int token[kRowsAtOnce], which[kRowsAtOnce];  // row `which` of the token's; -1: nothing to do
 #pragma unroll
     for (int u = 0; u < kRowsAtOnce; ++u) {
       const int r = base + u * (256 / LPR) + (int)threadIdx.x / LPR;
       token[u] = r / per_token;
-      which[u] = r < rows ? r - token[u] * per_token : -1;
-      if (r >= rows) continue;
+      which[u] = r < row_end ? r - token[u] * per_token : -1;
+      if (r >= row_end) continue;
       const int x = which[u];
       const int64_t tok = t0 + token[u];
       const bool is_q = x >= 2 * p.h_kv, is_v = !is_q && x >= p.h_kv;
@@ -327,26 +353,8 @@ __global__ __launch_bounds__(256) void cache_write_kernel(const Params p) {
                          (is_q ? x - 2 * p.h_kv : is_v ? x - p.h_kv : x) * (is_q ? p.sqh : is_v ? p.svh : p.skh);
       in[u] = load_chunks(src + at, chunk, is_v ? 0 : half, interleaved);
     }
-    if (base == 0) {  // while the first rows are on their way
-      LanePlace place;
-      int page = -1;
-      const bool looks_up = threadIdx.x < 64;
-      if (looks_up) {
-        place = find_positions(p.seq, t0, tokens, (int)threadIdx.x);
-        if ((int)threadIdx.x < tokens) places[threadIdx.x].pos = place.pos;
-        page = find_page(p.seq, place);  // on its way while the angles are computed
-      }
-      __syncthreads();
-      if constexpr (kTurn) {
-        fill_weights<D>(weights, p.turn);
-        fill_axes(cs, p.rot, p.turn, tokens, [&](int t, int axis) -> int64_t {
-          return p.turn.positions ? position_at(p.turn, axis * p.turn.spa + (t0 + t) * p.turn.spn) : (int64_t)places[t].pos;
-        });
-      } else {
-        if (p.rot.half) fill_angles(cs, p.rot, tokens, [&](int t) -> int64_t { return places[t].pos; });
-      }
-      if (looks_up && (int)threadIdx.x < tokens) places[threadIdx.x].page = page;
-      __syncthreads();
+    if constexpr (!kTurn) {
+      if (base == 0) look_up();  // while the first rows are on their way
     }
 #pragma unroll
     for (int u = 0; u < kRowsAtOnce; ++u) {

@@ -9,6 +9,8 @@
 // Angles as in serve_cache.hip, in float64, once per token for all heads.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+
 #include "serve_launch.hpp"
 #include "serve_rows.hpp"
 
@@ -75,17 +77,20 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(6))) void r
   }
 }
 
+// Workgroups below which each pass over a token's heads is one of its own: few tokens wait for one pass after the other.
+constexpr unsigned kTurnFewWgs = 512;
 template <int DT, int D>
 int launch_write_d(bool e4m3, const CacheTurnParams& p, unsigned grid, hipStream_t s) {
+  const int rows = 256 / (D / 8);
+  const int64_t each = (2 * (int64_t)p.h_kv + p.h_q) * p.tokens_per_wg;
+  const unsigned passes = grid < kTurnFewWgs && each > rows ? (unsigned)std::min<int64_t>((each + rows - 1) / rows, 64) : 1u;
   if (e4m3)
-    hipLaunchKernelGGL((cache_write_kernel<DT, D, true, CacheTurnParams>), dim3(grid), dim3(256), 0, s, p);
+    hipLaunchKernelGGL((cache_write_kernel<DT, D, true, CacheTurnParams>), dim3(grid, passes), dim3(256), 0, s, p);
   else
-    hipLaunchKernelGGL((cache_write_kernel<DT, D, false, CacheTurnParams>), dim3(grid), dim3(256), 0, s, p);
+    hipLaunchKernelGGL((cache_write_kernel<DT, D, false, CacheTurnParams>), dim3(grid, passes), dim3(256), 0, s, p);
   return (int)hipGetLastError();
 }
 
-// Workgroups below which each pass over a token's heads is one of its own: few tokens wait for one pass after the other.
-constexpr unsigned kTurnFewWgs = 512;
 template <int DT, int D>
 int launch_qk_d(const RotaryQkParams& p, unsigned grid, hipStream_t s) {
   const int rows = 256 / (D / 8), heads = p.h_q + p.h_k;
