@@ -167,7 +167,7 @@ __device__ __forceinline__ void ragged_rows(RaggedLds<D, GW>& mem, int hkv, int 
 
   const float qk_scale = p.qk_scale;
   const bool want_exact = GW == 1 ? p.lse != nullptr : LSE, causal = !kPrefix && p.causal != 0,
-             shared = kJoined || (kPages && p.shares > 0);
+             shared = kJoined || (kPages && p.shares > 0 && !cur.by_tile);
 
   // ---- the workgroup's work: the pieces of its share, or its one tile
   Share share = {0, 0, 0, 0};
@@ -864,6 +864,30 @@ void attn_ragged_kernel(const RaggedParams) {
   int hkv, rank;
   head_and_rank(params_here(), (int)blockIdx.x, &hkv, &rank);
   ragged_rows<DT, D, SRC, GW, LSE, MODE>(mem, hkv, rank, Cursor{});
+}
+
+// A window over chunks of prompts beside single tokens, where the chunks' rows fill the GPU: their 128-row tiles are shared out as
+// ever, and each sequence of at most 32 rows has a 32-row workgroup of its own behind them. In 128-row tiles a token's row costs
+// what a chunk's 128 do. Measured on MI355X, a chunk of 2048 beside 24 steps, window 2048, 28 / 4 heads of 128: 92 and 17 us of merge in
+// 128-row tiles alone.
+template <int DT, int D, int SRC, bool LSE>
+__global__ __launch_bounds__(256)
+__attribute__((amdgpu_waves_per_eu(kSharedWaves)))
+void attn_window_mixed_kernel(const RaggedParams) {
+  __shared__ union {
+    RaggedLds<D, 4> many;
+    RaggedLds<D, 1> few;
+  } mem;
+  ParamsRef p = params_here();
+  int hkv, rank;
+  head_and_rank(p, (int)blockIdx.x, &hkv, &rank);
+  Cursor cur{};
+  cur.by_tile = rank >= p.shares;
+  cur.rows_of = cur.by_tile ? kFewRows : kManyRows;
+  if (cur.by_tile)
+    ragged_rows<DT, D, SRC, 1, LSE, kModeWindow>(mem.few, hkv, rank - p.shares, cur);
+  else
+    ragged_rows<DT, D, SRC, 4, LSE, kModeWindow>(mem.many, hkv, rank, cur);
 }
 
 // Both passes of a batch with a common prefix in one launch: GWP row waves for the prefix's shares, whose rows are all of the

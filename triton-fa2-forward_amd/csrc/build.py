@@ -3,7 +3,7 @@ measurement library libfa2_ablate.so beside it.
 
     python triton-fa2-forward_amd/csrc/build.py [-j 8] [--verbose]
 
-Compiles attn_fwd_inst.hip and attn_shared_inst.hip once per (dtype, head_dim) pair and attn_ragged_inst.hip once per pair and
+Compiles attn_fwd_inst.hip, attn_window_inst.hip and attn_shared_inst.hip once per (dtype, head_dim) pair and attn_ragged_inst.hip once per pair and
 choice of keys (all, a window's), plus
 the split-KV combine pass (attn_fwd_combine.hip), the key-norm pass (attn_key_norm.hip), the rotary and cache kernels
 (serve_cache.hip, serve_turn.hip), the page kernels (serve_pages.hip) and the C-ABI file fa2_fwd.hip,
@@ -54,6 +54,7 @@ ARCH = "gfx950"
 DTYPES = (0, 1)            # 0 = fp16, 1 = bf16
 HEAD_DIMS = (16, 32, 64, 128)
 RAGGED_MODES = (0, 1)  # csrc/serve_params.hpp: all keys, a window's
+STEP_UNITS = ("attn_window", "attn_shared")
 SERVE_UNITS = ("serve_cache", "serve_turn", "serve_pages")
 
 
@@ -113,6 +114,7 @@ _SERVING_KERNELS = {
 _STEP_KERNELS = {
     "attn_ragged_kernel": (re.compile(r"attn_ragged_kernelILi(\d)ELi(\d+)ELi(\d)ELi(\d)ELb([01])ELi1EEEv"),
                            ("source", "row_waves", "lse")),
+    "attn_window_mixed_kernel": (re.compile(r"attn_window_mixed_kernelILi(\d)ELi(\d+)ELi(\d)ELb([01])EEEv"), ("source", "lse")),
     "attn_shared_kernel": (re.compile(r"attn_shared_kernelILi(\d)ELi(\d+)ELi(\d)ELi(\d)ELi(\d)ELb([01])EEEv"),
                            ("source", "prefix_waves", "own_waves", "lse")),
     "attn_shared_join_kernel": (re.compile(r"attn_shared_join_kernelILi(\d)ELi(\d+)ELi(\d)ELi(\d)EEEv"),
@@ -192,9 +194,9 @@ def build_variant(name, defines, jobs=8, verbose=False):
                 cmds.append([cc, *flags, f"-DFA2_DT={dt}", f"-DFA2_D={d}", f"-DFA2_MODE={mode}", "-c",
                              os.path.join(CSRC, "attn_ragged_inst.hip"), "-o",
                              os.path.join(obj_dir, f"attn_ragged_dt{dt}_d{d}_m{mode}.o")])
-            cmds.append([cc, *flags, f"-DFA2_DT={dt}", f"-DFA2_D={d}", "-c",
-                         os.path.join(CSRC, "attn_shared_inst.hip"), "-o",
-                         os.path.join(obj_dir, f"attn_shared_dt{dt}_d{d}.o")])
+            for unit in STEP_UNITS:
+                cmds.append([cc, *flags, f"-DFA2_DT={dt}", f"-DFA2_D={d}", "-c", os.path.join(CSRC, unit + "_inst.hip"),
+                             "-o", os.path.join(obj_dir, f"{unit}_dt{dt}_d{d}.o")])
     for name_ in ("attn_fwd_combine", "attn_fwd_wavesplit", "attn_key_norm", *SERVE_UNITS, "fa2_fwd", "fa2_scratch"):
         cmds.append([cc, *flags, "-c", os.path.join(CSRC, name_ + ".hip"), "-o",
                      os.path.join(obj_dir, name_ + ".o")])
@@ -225,9 +227,10 @@ def build(jobs=8, verbose=False):
                 serve_units.append([cc, *common_flags(), "-Rpass-analysis=kernel-resource-usage", f"-DFA2_DT={dt}",
                                     f"-DFA2_D={d}", f"-DFA2_MODE={mode}", "-c",
                                     os.path.join(CSRC, "attn_ragged_inst.hip"), "-o", obj])
-            obj = os.path.join(OBJ_DIR, f"attn_shared_dt{dt}_d{d}.o")
-            serve_units.append([cc, *common_flags(), "-Rpass-analysis=kernel-resource-usage", f"-DFA2_DT={dt}",
-                                f"-DFA2_D={d}", "-c", os.path.join(CSRC, "attn_shared_inst.hip"), "-o", obj])
+            for unit in STEP_UNITS:
+                obj = os.path.join(OBJ_DIR, f"{unit}_dt{dt}_d{d}.o")
+                serve_units.append([cc, *common_flags(), "-Rpass-analysis=kernel-resource-usage", f"-DFA2_DT={dt}",
+                                    f"-DFA2_D={d}", "-c", os.path.join(CSRC, unit + "_inst.hip"), "-o", obj])
             obj = os.path.join(OBJ_DIR, f"attn_fwd_ablate_dt{dt}_d{d}.o")
             ablate_units.append([cc, *common_flags(), f"-DFA2_DT={dt}", f"-DFA2_D={d}", "-c",
                                  os.path.join(CSRC, "attn_fwd_ablate_inst.hip"), "-o", obj])

@@ -179,6 +179,9 @@ __device__ __forceinline__ int64_t readlane64(int64_t x, int l) {
   return (int64_t)(((uint64_t)hi << 32) | lo);
 }
 
+// Sequences by their rows of a KV head
+enum Rows { kAnyRows, kManyRows, kFewRows };  // more than 32, or at most 32
+
 // A place among the sequences: the block of 64 that starts at s0 is in `lanes`, the sequence is its lane l.
 struct Cursor {
   int s0, l, tile;
@@ -190,6 +193,9 @@ struct Cursor {
   Prefix prefix;
   int shares, first_share;
   double per_share;
+  // Of a window: the sequences that a workgroup takes, and whether it takes one row tile of them
+  Rows rows_of;
+  bool by_tile;
 };
 // Sequences whose tiles are dealt out
 template <int MODE>
@@ -200,7 +206,11 @@ __device__ __forceinline__ int sequences(ParamsRef p) {
 // the first one's position
 template <bool PAGES, int MODE>
 __device__ __forceinline__ LaneSequence lane_sequence(ParamsRef p, int s, const Cursor& c) {
-  if constexpr (MODE < kModePrefix) return lane_sequence<PAGES>(p, s);
+  if constexpr (MODE < kModePrefix) {
+    LaneSequence q = lane_sequence<PAGES>(p, s);
+    if (MODE == kModeWindow && c.rows_of != kAnyRows && (q.n_q * p.group <= 32) != (c.rows_of == kFewRows)) q.n_q = 0;
+    return q;
+  }
   if (MODE == kModePrefix) return s == 0 ? LaneSequence{c.rows_first, c.rows, c.prefix.tokens, 0} : LaneSequence{0, 0, 0, 0};
   LaneSequence q = s < 64 ? c.raw : lane_sequence<true>(p, s);
   q.kv_first = c.prefix.tokens;

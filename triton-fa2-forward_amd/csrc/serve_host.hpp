@@ -146,6 +146,7 @@ unsigned cache_grid(fa2::CacheParams* p, int64_t rows_per_token, int32_t head_di
 constexpr int64_t kShortKeys = 1536;
 struct RaggedPlan {
   int row_waves = 4;  // 32-row workgroups (1) or 128-row ones (4)
+  bool mixed = false;  // (of a window) 128-row workgroups' shares, and a 32-row one for each sequence of few rows
   int shares = 0;     // workgroups per KV head that share its work; 0: one per row tile
   int64_t grid = 0;
   size_t parts = 0, workspace = 0;  // bytes of the partial results, and with what their merge needs to know
@@ -169,6 +170,19 @@ RaggedPlan ragged_plan(int source, int32_t h_q, int32_t h_kv, int32_t head_dim, 
     pl.workspace = pl.parts + (size_t)h_kv * pl.shares * fa2::kMergeBytes;
   }
   pl.grid = (pl.shares ? pl.shares : n) * h_kv;
+  return pl;
+}
+// ... of a window over pages: mixed where sequences of few rows stand beside chunks whose row tiles give every CU one at least
+RaggedPlan window_plan(int source, int32_t h_q, int32_t h_kv, int32_t head_dim, int32_t n_tokens, int32_t n_seq, int64_t keys,
+                       int cus) {
+  RaggedPlan pl = ragged_plan(source, h_q, h_kv, head_dim, n_tokens, n_seq, keys, cus);
+  const int64_t rows = (int64_t)n_tokens * (h_q / h_kv);
+  if (source == fa2::kSourcePacked || pl.row_waves == 1 || !pl.shares || n_seq == 1 || rows / 128 * h_kv < cus) return pl;
+  pl.mixed = true;
+  pl.shares = std::max(1, fa2::kSharedWaves * cus / h_kv);
+  pl.parts = (size_t)h_kv * pl.shares * 2 * 128 * (head_dim + 4) * sizeof(float);
+  pl.workspace = pl.parts + (size_t)h_kv * pl.shares * fa2::kMergeBytes;
+  pl.grid = ((int64_t)pl.shares + n_seq) * h_kv;
   return pl;
 }
 
@@ -247,13 +261,20 @@ int paged_params(const void* q, void* out, const int64_t q_stride[2], const int6
   return FA2_OK;
 }
 
+template <int DT, int D, int MODE>
+int launch_form(const fa2::RaggedParams& p, int source, const RaggedPlan& pl, unsigned grid, hipStream_t s) {
+  if (MODE == fa2::kModeWindow && pl.mixed) return fa2::launch_window_mixed<DT, D>(p, source, grid, s);
+  return fa2::launch_ragged<DT, D, MODE>(p, source, pl.row_waves, grid, s);
+}
+
 // Launches a checked call whose heads, tensors and sequences are in p. keys: see ragged_plan.
 template <int MODE = fa2::kModeAll>
 int launch_ragged(int32_t dtype, int32_t head_dim, int32_t h_q, fa2::RaggedParams& p, int source, int64_t keys, void* workspace,
                   size_t workspace_bytes, void* stream) {
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const Topology topo = device_topology(stream_device(s));
-  const RaggedPlan pl = ragged_plan(source, h_q, p.h_kv, head_dim, p.seq.n_tokens, p.seq.n_seq, keys, topo.cus);
+  const RaggedPlan pl = (MODE == fa2::kModeWindow ? window_plan : ragged_plan)(source, h_q, p.h_kv, head_dim, p.seq.n_tokens,
+                                                                               p.seq.n_seq, keys, topo.cus);
   if (pl.grid > 0x7fffffffLL) return fail(FA2_EINVAL, "grid of %lld workgroups is too large", (long long)pl.grid);
   if (pl.workspace) {
     if (!workspace || workspace_bytes < pl.workspace)
@@ -270,14 +291,14 @@ int launch_ragged(int32_t dtype, int32_t head_dim, int32_t h_q, fa2::RaggedParam
   const unsigned g = (unsigned)pl.grid;
   int e;
   switch (dtype * 4 + dim_index(head_dim)) {
-    case 0: e = fa2::launch_ragged<0, 16, MODE>(p, source, pl.row_waves, g, s); break;
-    case 1: e = fa2::launch_ragged<0, 32, MODE>(p, source, pl.row_waves, g, s); break;
-    case 2: e = fa2::launch_ragged<0, 64, MODE>(p, source, pl.row_waves, g, s); break;
-    case 3: e = fa2::launch_ragged<0, 128, MODE>(p, source, pl.row_waves, g, s); break;
-    case 4: e = fa2::launch_ragged<1, 16, MODE>(p, source, pl.row_waves, g, s); break;
-    case 5: e = fa2::launch_ragged<1, 32, MODE>(p, source, pl.row_waves, g, s); break;
-    case 6: e = fa2::launch_ragged<1, 64, MODE>(p, source, pl.row_waves, g, s); break;
-    default: e = fa2::launch_ragged<1, 128, MODE>(p, source, pl.row_waves, g, s);
+    case 0: e = launch_form<0, 16, MODE>(p, source, pl, g, s); break;
+    case 1: e = launch_form<0, 32, MODE>(p, source, pl, g, s); break;
+    case 2: e = launch_form<0, 64, MODE>(p, source, pl, g, s); break;
+    case 3: e = launch_form<0, 128, MODE>(p, source, pl, g, s); break;
+    case 4: e = launch_form<1, 16, MODE>(p, source, pl, g, s); break;
+    case 5: e = launch_form<1, 32, MODE>(p, source, pl, g, s); break;
+    case 6: e = launch_form<1, 64, MODE>(p, source, pl, g, s); break;
+    default: e = launch_form<1, 128, MODE>(p, source, pl, g, s);
   }
   return launched(e, "attention");
 }

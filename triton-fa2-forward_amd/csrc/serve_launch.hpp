@@ -39,14 +39,18 @@ constexpr int ragged_waves(int head_dim, int source, int row_waves) {
 template <int DT, int D, int MODE>
 int launch_ragged(const RaggedParams& p, int source, int row_waves, unsigned grid, hipStream_t stream);
 
-// Workgroups per CU of the kernel for batches with a common prefix (two passes' code in one kernel: three would spill up to 64
-// registers at head_dim 64), and workgroups that join its rows' results (8 rows each)
+// Workgroups per CU of the kernels that hold two forms' code (three would spill up to 64 registers at head_dim 64), and workgroups that join its rows' results (8 rows each)
 constexpr int kSharedWaves = 2;
 inline unsigned shared_join_grid(const RaggedParams& p) {
   return (unsigned)(((int64_t)p.seq.n_tokens * p.group + 7) / 8 * p.h_kv);
 }
 
-// That kernel with 32 * prefix_waves rows per workgroup for the prefix and 32 * own_waves for the keys behind it (1 and 1, 4 and 1, or 4
+// Attention within a window over pages, chunks beside single tokens: p.shares workgroups per head for sequences of more than 32 rows, and
+// one for each sequence (grid: both), then the merge of the tiles that the shares cut.
+template <int DT, int D>
+int launch_window_mixed(const RaggedParams& p, int source, unsigned grid, hipStream_t stream);
+
+// The kernel for batches with a common prefix with 32 * prefix_waves rows per workgroup for the prefix and 32 * own_waves for the keys behind it (1 and 1, 4 and 1, or 4
 // and 4), and after it the join of its rows' results.
 template <int DT, int D>
 int launch_shared(const RaggedParams& p, int source, int prefix_waves, int own_waves, unsigned grid, hipStream_t stream);
@@ -56,6 +60,8 @@ int launch_shared(const RaggedParams& p, int source, int prefix_waves, int own_w
   int launch_ragged<DT, D, kModeAll>(const RaggedParams&, int, int, unsigned, hipStream_t);    \
   template <>                                                                                  \
   int launch_ragged<DT, D, kModeWindow>(const RaggedParams&, int, int, unsigned, hipStream_t); \
+  template <>                                                                                  \
+  int launch_window_mixed<DT, D>(const RaggedParams&, int, unsigned, hipStream_t);             \
   template <>                                                                                  \
   int launch_shared<DT, D>(const RaggedParams&, int, int, int, unsigned, hipStream_t);
 FA2_DECLARE_RAGGED(0, 16)

@@ -172,9 +172,11 @@ int fa2_attn_paged_window(const void* q, void* out, const int64_t q_stride[2], c
 
 size_t fa2_paged_window_workspace_bytes(int32_t h_q, int32_t h_kv, int32_t head_dim, int32_t cache_dtype, int32_t n_tokens,
                                         int32_t n_seq, int64_t max_keys, int32_t window, int32_t sinks, int32_t num_cus) {
-  if (window < 1 || sinks < 0) return 0;
-  return fa2_paged_workspace_bytes(h_q, h_kv, head_dim, cache_dtype, n_tokens, n_seq, window_keys(max_keys, window, sinks),
-                                   num_cus);
+  if (window < 1 || sinks < 0 || h_q <= 0 || h_kv <= 0 || h_q % h_kv || dim_index(head_dim) < 0 || n_tokens <= 0 || n_seq <= 0 ||
+      num_cus <= 0)
+    return 0;
+  return window_plan(source_of(cache_dtype), h_q, h_kv, head_dim, n_tokens, n_seq, window_keys(max_keys, window, sinks), num_cus)
+      .workspace;
 }
 
 int fa2_attn_paged_shared(const void* q, void* out, const int64_t q_stride[2], const int64_t o_stride[2],
