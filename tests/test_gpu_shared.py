@@ -105,20 +105,22 @@ def test_sequences_shorter_than_their_rows():
     assert (out[:2] == 0).all() and (lse[:, :2] == -math.inf).all()
 
 
+@pytest.mark.parametrize("which", ["k", "v"])
 @pytest.mark.parametrize("bad", [math.inf, math.nan])
 @pytest.mark.parametrize("where", [5, 270])  # in the prefix, behind it
-def test_not_finite(bad, where):
+def test_not_finite(which, bad, where):
     """An infinite or NaN value in a token: the rows that see it, of one sequence or of all, and no others."""
     from fa2.paged import attention_paged
     page_size, D, dtype = 16, 64, torch.bfloat16
     new, lens = [1, 3, 1], [300, 280, 400]
     pages, cache, cu, seqlens, table = batch(new, lens, 256, page_size, 2, D, dtype, False)
     page, row = pages.at(1, torch.tensor([where], device="cuda"))
-    cache.v[page, :, row] = bad
+    getattr(cache, which)[page, :, row] = bad
     q = randn((5, 8, D), dtype, 1)
     for columns in (0, 200):
         wide = torch.nn.functional.pad(table, (0, columns), value=-7)
         out, lse = attention_paged(q, cache, wide, cu, seqlens, shared=tokens(256), return_lse=True)
+        lse = None if which == "k" and math.isinf(bad) else lse  # (an infinite score's is infinite, a NaN one's NaN)
         check_paged_rows(out, lse, q, cache, pages, lens, cu, dtype, joined=JOINED)
 
 

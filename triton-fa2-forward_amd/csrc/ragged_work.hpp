@@ -411,7 +411,7 @@ __device__ __forceinline__ bool deal_shares(ParamsRef p, int rank, int lane, Cur
   c->rows_first = row_bound(p.seq.cu, 0, p.seq.n_tokens);
   c->rows = max(row_bound(p.seq.cu, p.seq.n_seq, p.seq.n_tokens) - c->rows_first, 0);
   c->prefix = common_prefix(p, lane, c->raw);
-  const int64_t cost = c->prefix.tokens == 0 ? 16 : c->prefix.tokens + kTileCost<BMP>;  // (no keys: only empty results to write)
+  const int64_t cost = c->prefix.tokens == 0 ? 128 : c->prefix.tokens + kTileCost<BMP>;  // (no keys: only empty results to write)
   double ours = (double)(row_tiles<BMP>(c->rows, p.group) * cost) * (BMP > BMO ? 1.5 : 1.0), own = 0.0;
   for (int s0 = 0; s0 < p.seq.n_seq; s0 += 64) {
     const LaneSequence q = lane_sequence<true, kModeOwn>(p, s0 + lane, *c);
