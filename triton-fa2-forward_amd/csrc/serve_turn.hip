@@ -4,9 +4,14 @@
 //   x_hat = x / sqrt(mean_d x_d^2 + eps) * weight_d
 //   (a, b) of pair i -> scale * (a cos t - b sin t, b cos t + a sin t),  t = freqs[i] * position[axes[i]]
 //
-// Squares and their sum are formed in float64 (a bf16 value's square is past float's range from 1.8e19 on), the
-// root's inverse too; products in float, or in float64 for keys on their way into an e4m3 cache, and rounded once.
+// Squares are summed in float where the sum is well inside its range (a bf16 value's square is past it from 1.8e19 on), in
+// float64 elsewhere; products in float, or all of it in float64 for keys on their way into an e4m3 cache, and rounded once.
 // Angles as in serve_cache.hip, in float64, once per token for all heads.
+//
+// Bound by HBM and, beside it, by the vector instructions (about 110 for 16 bytes of a row). Measured on MI355X: 16384 tokens of 32 + 8 heads of
+// 128, three axes, both normalised 82 us, 4.1 TB/s (the same with LDS conflicts of the angles 121, at 142 registers 113; a copy
+// reaches 4.8); 16 tokens 4.2 (7.0 with a token's heads in one workgroup, one pass after the other); a write of 5096 tokens of 28 + 2 x 4
+// heads 21 us, of 64 tokens into e4m3 6.1 (8.1 in one workgroup a token).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

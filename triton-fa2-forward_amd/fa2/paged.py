@@ -215,7 +215,9 @@ def attention_paged(q, cache, block_table, cu_seqlens, seqlens, *, causal=True, 
         `sinks`; entries of the table whose pages no row sees are not looked at, and their pages may be others' by now.
     shared: int32 [1] on the GPU, a number of tokens that all sequences begin with and that lie in the same pages: those are
         read once for the whole batch, from the table's row of the first sequence that has new tokens. As many count as
-        whole pages hold and as lie before every sequence's new tokens. Not with a window.
+        whole pages hold and as lie before every sequence's new tokens. Not with a window. It pays for long prefixes and few
+        new tokens a sequence; rows of hundreds share their sequence's keys as it is, and are faster without it. The workspace
+        holds every row's results twice in float, beside the pieces of cut row tiles.
     return_lse: also return the natural-log log-sum-exp of every row's scaled scores, fp32 [H_q, T].
     out: of q's shape and type, in any layout without shared elements; q itself is allowed, and no other memory that
         the call reads.

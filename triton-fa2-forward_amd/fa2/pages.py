@@ -3,8 +3,9 @@
 A PagePool holds the numbers of the pages that no sequence has. pages_extend() takes pages for a step's new tokens from
 it, enters them into the sequences' block table and gives what the step's other operators are called with (row starts,
 lengths, positions, slots); pages_release() gives pages back. Both work from lengths on the device: nothing is
-copied to the host. They change the block table and the pool's stack in place and return new lengths and a new count; a
-captured graph that goes on with those copies them to where it reads them. The HIP kernels are csrc/serve_pages.hip
+copied to the host. They change the block table and the pool's stack in place and return new lengths and a new count: go on
+with the pool that a call returns, the one it was given is used up. A captured graph copies the new lengths and count to
+where its next replay reads them. The HIP kernels are csrc/serve_pages.hip
 behind include/fa2_fwd.h.
 """
 

@@ -13,8 +13,8 @@ B 16, H 32/8, N_kv 4096, D 128, non-causal, default path: packed, automatic spli
 --shape X:B:Hq:Hkv:Nq:Nkv:D:causal:dtype[:lse] runs any other call of attention() on N(0, 1) inputs,
 with the log-sum-exp where it ends in lse.
 
---operators NAME,... (or all) runs the serving operators' measured cases of these names (perf/operators.py), one after the
-other.
+--operators NAME,... (or all) runs the serving operators' measured cases of these names (perf/operators.py and
+perf/more_operators.py), one after the other.
 
 --lib PATH runs another build of the product library (csrc/build.py --variant) through the same
 call attention() makes (ab.py's), for the counters of an A/B.
@@ -36,13 +36,14 @@ sys.path.insert(0, os.path.dirname(HERE))
 def run_operators(names, launches):
     import torch
 
-    import perf.operators as operators
+    import perf.more_operators
+    import perf.operators
 
-    operators.own = True
-    cases = [c for c in operators.listed() if names is None or c["name"] in names]
+    cases = [(m, c) for m in (perf.operators, perf.more_operators) for c in m.listed() if names is None or c["name"] in names]
     if len(cases) != len(names or cases):
         raise SystemExit(f"profile_target: no such case among {names}")
-    for case in cases:
+    for operators, case in cases:
+        operators.own = True
         print(f"profile_target: {case['name']}, {launches} launches", flush=True)
         state = operators.prepare(case, 1)
         for _ in range(launches):
