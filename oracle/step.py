@@ -20,7 +20,9 @@ def turn(x, positions, freqs, interleaved=False, scale=1.0, axes=None, weight=No
     The bound of a kernel's value, in units of 2^-24 relative to |a cos| + |b sin|. The sum of D <= 128 squares: 8 products and
     sums of a lane, at most 2 units each if they are cut off, and 4 sums of lanes, together 20, half of that in its root; the mean
     and eps 1, the root's estimate 2 (one unit in its last place), x * r * weight 2, cos or sin, its product and the sum 3: 18, and 24 with
-    what second order adds. Then the rounding to the type."""
+    what second order adds. Then the rounding to the type: half a step, which is at least half the type's least subnormal value
+    (2^-25 for fp16, 2^-134 for bf16, whose least normal value is float's own: there each of float's 8 roundings on the way is off by up to 2^-150,
+    with weights up to 16 together less than 2^-142)."""
     half = freqs.numel()
     angle = (positions.double()[:, None] if axes is None else positions.double()[axes.long()].t()) * freqs.double()
     cos, sin = (torch.cos(angle) * scale)[:, None], (torch.sin(angle) * scale)[:, None]
@@ -33,7 +35,7 @@ def turn(x, positions, freqs, interleaved=False, scale=1.0, axes=None, weight=No
     size[..., b_at] = b.abs() * cos.abs() + a.abs() * sin.abs()
     y[..., a_at], y[..., b_at] = a * cos - b * sin, b * cos + a * sin
     u = serving.HALF_STEP[x.dtype]
-    return y, u * y.abs() * (1 + u) + 24 * serving.F32 * size + (2.0 ** -25 if x.dtype == torch.float16 else 0.0)
+    return y, u * y.abs() * (1 + u) + 24 * serving.F32 * size + (2.0 ** -25 if x.dtype == torch.float16 else 2.0 ** -134 + 2.0 ** -142)
 
 
 def release(free, count, table, first, last):

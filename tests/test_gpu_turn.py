@@ -132,6 +132,23 @@ def test_norm_extremes(dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+def test_norm_of_small_values(dtype):
+    """Heads of values on both sides of the type's least normal one, whose squares are its sum; and of one large value among them."""
+    from fa2.rotary import HeadNorm, rotary_plan, rotary_qk
+    D = 128
+    least = torch.finfo(dtype).smallest_normal
+    g = torch.Generator().manual_seed(1)
+    x = ((torch.rand(40, 3, D, generator=g, dtype=torch.float64) - 0.5) * 4 * least).to(dtype).cuda()
+    x[:, 1, 5] = least
+    x[:, 2, 77] = 1.0
+    plan, norm = rotary_plan(64), HeadNorm(weight_of(D, 3), 1e-30 if dtype == torch.float16 else 1e-300)
+    positions = torch.arange(40, device="cuda")
+    got, _ = rotary_qk(x, None, positions, plan, q_norm=norm)
+    want, tol = step_oracle.turn(x, positions, plan.freqs, weight=norm.weight, eps=norm.eps)
+    assert ((got.double() - want).abs() <= tol).all(), ((got.double() - want).abs() / tol).max()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("e4m3", [False, True])
 @pytest.mark.parametrize("D,rot,interleaved", [(128, 128, False), (64, 32, True), (32, 16, False), (16, 16, True)])
 @pytest.mark.parametrize("axes", [1, 3])

@@ -36,6 +36,8 @@
 // 1/2 or 2 in the one line (121 -> 140, 125).
 #pragma once
 
+#include <type_traits>
+
 #include "attn_fwd_wavesplit.hpp"
 #include "ragged_work.hpp"
 
