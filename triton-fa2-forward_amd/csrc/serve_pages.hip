@@ -56,6 +56,7 @@ __global__ __launch_bounds__(256) void pages_extend_kernel(const PagesParams p) 
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int block = (int)blockIdx.x, stripe = (int)blockIdx.y, stripes = (int)gridDim.y;
   const int s0 = block * 256, s = s0 + tid;
+  const int stack = p.count[0];  // (on its way with the lengths)
   // ---- tokens and needs before the block's, of the block, and behind it
   int64_t sums[4] = {0, 0, 0, 0};  // tokens before, needs before, tokens in all, needs in all
   for (int i = tid; i < p.n_seq; i += 256) {
@@ -111,7 +112,7 @@ __global__ __launch_bounds__(256) void pages_extend_kernel(const PagesParams p) 
   }
   held_of[tid] = (int)mine.held;
   old_of[tid] = old;
-  const int64_t count = min(max(p.count[0], 0), p.n_pages), base = max(count - total, (int64_t)0);
+  const int64_t count = min(max(stack, 0), p.n_pages), base = max(count - total, (int64_t)0);
   auto clamp = [](int64_t x) { return (int32_t)min(x, (int64_t)0x7fffffff); };
   if (stripe == 0) {
     if (s < p.n_seq) {
@@ -229,6 +230,7 @@ __global__ __launch_bounds__(1024) void pages_release_once_kernel(const ReleaseP
   __shared__ int before[16], own[16];  // pages that a wave has counted
   const int lane = threadIdx.x & 63, wave = (int)(threadIdx.x >> 6);
   const int s0 = (int)blockIdx.x * 16, s = s0 + wave;
+  const int stack = p.count[0];
   const Range r = s < p.n_seq ? range_of(p, s) : Range{0, 0};
   int n = 0;
   Range next = range_of(p, min((int)(threadIdx.x >> 4), p.n_seq - 1));
@@ -248,7 +250,7 @@ __global__ __launch_bounds__(1024) void pages_release_once_kernel(const ReleaseP
     own[wave] = mine;
   }
   __syncthreads();
-  int64_t at = min(max(p.count[0], 0), p.n_pages);
+  int64_t at = min(max(stack, 0), p.n_pages);
   for (int w = 0; w < 16; ++w) at += before[w] + (w < wave ? own[w] : 0);
   at = push_pages(p, s, r, lane, at);
   if (s == p.n_seq - 1 && lane == 0) p.count_out[0] = (int32_t)min(at, (int64_t)p.n_pages);
