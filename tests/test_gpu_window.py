@@ -89,6 +89,25 @@ def test_as_all_keys():
     assert torch.equal(attention_packed(q, k, v, cu, window=(1 << 31) - 1, sinks=1 << 50), out)
 
 
+@pytest.mark.parametrize("window,sinks", [(1 << 40, 0), ((1 << 31) - 1, 3), ((1 << 31) - 20, 1 << 40)])
+@pytest.mark.parametrize("h_q", [2, 24])
+def test_largest_windows_of_rows_without_keys(window, sinks, h_q):
+    """The largest windows there are, in row tiles that begin with rows that see no key: packed rows with fewer keys than rows, and
+    sequences with fewer tokens in the cache than rows."""
+    from fa2.packed import attention_packed
+    from fa2.paged import attention_paged
+    n_q, n_kv, D, dtype = [40, 300, 7, 900], [10, 131, 0, 899], 64, torch.bfloat16
+    q, cu, cu_kv = randn((sum(n_q), h_q, D), dtype, 1), cumulative(n_q), cumulative(n_kv)
+    k, v = randn((sum(n_kv), 2, D), dtype, 2), randn((sum(n_kv), 2, D), dtype, 3)
+    out, lse = attention_packed(q, k, v, cu, cu_kv, window=window, sinks=sinks, return_lse=True)
+    check_rows(out, lse, q, of_rows(k, cu_kv), of_rows(v, cu_kv), cu, dtype, window=window, sinks=sinks)
+    pages = oracle.Pages(n_kv, 16, seed=1, device="cuda")
+    cache = make_cache(pages.n_pages, 2, 16, D, dtype, False, 5, "hnd")
+    seqlens = torch.tensor(n_kv, dtype=torch.int32, device="cuda")
+    out, lse = attention_paged(q, cache, pages.table, cu, seqlens, window=window, sinks=sinks, return_lse=True)
+    check_paged_rows(out, lse, q, cache, pages, n_kv, cu, dtype, window=window, sinks=sinks)
+
+
 # ------------------------------------------------------------------------------------------
 # pages
 # ------------------------------------------------------------------------------------------

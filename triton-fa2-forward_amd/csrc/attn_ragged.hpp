@@ -202,7 +202,8 @@ __device__ __forceinline__ void ragged_rows(RaggedLds<D, GW>& mem, int hkv, int 
     const int full_end = max(last_of(row0 / p.group) + 1, 0);
     // A window: the first key of a position (beside the sinks), the least and the largest of the tile's, and the key
     // tiles between the sinks' and the window's, which are skipped. Key tiles are counted without those.
-    auto first_of = [&](int i) { return kWindow ? max(last_of(i) - p.window + 1, 0) : 0; };
+    // (compared first: a window up to 2^31 - 1 less a negative last key, of a row that sees none, is no int)
+    auto first_of = [&](int i) { return kWindow && last_of(i) >= p.window ? last_of(i) - p.window + 1 : 0; };
     const int sinks = kWindow ? p.sinks : 0;
     const int see_begin = first_of(row0 / p.group), first_end = first_of((row_end - 1) / p.group);
     const int sink_tiles = kWindow ? (min(sinks, see_end) + BN - 1) / BN : 0;
