@@ -149,6 +149,30 @@ def test_norm_of_small_values(dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("eps", [5e-324, 1e-300, 1e-78, 1e-76, 1e-40, 1e300])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_norm_least_values(dtype, eps, interleaved):
+    """The least eps there are, and the largest: rows of zeros are zeros, rows of the type's least values as any others."""
+    from fa2.rotary import HeadNorm, rotary_plan, rotary_qk
+    D = 64
+    least = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+    g = torch.Generator().manual_seed(2)
+    x = torch.zeros(60, 2, D, dtype=torch.float64)
+    for t in range(1, 60):  # (with one value, a few and all; up to 2^40 times the least)
+        n = (1, 5, D)[t % 3]
+        x[t, 0, torch.randperm(D, generator=g)[:n]] = torch.randint(-9, 10, (n,), generator=g).double() * least * 2.0 ** (t * 2 // 3)
+        x[t, 1] = least * (1 if t % 2 else -3)
+    x = x.to(dtype).cuda()
+    plan, norm = rotary_plan(48, interleaved=interleaved), HeadNorm(weight_of(D, 3), eps)
+    positions = torch.arange(60, device="cuda")
+    got, _ = rotary_qk(x, None, positions, plan, q_norm=norm)
+    want, tol = step_oracle.turn(x, positions, plan.freqs, interleaved, weight=norm.weight, eps=norm.eps)
+    assert (got[0] == 0).all() and torch.equal(got.isnan(), want.isnan())
+    fine = ~want.isnan()  # (fp16's largest rows hold infinities)
+    assert fine[:40].all() and ((got.double() - want).abs() <= tol)[fine].all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("e4m3", [False, True])
 @pytest.mark.parametrize("D,rot,interleaved", [(128, 128, False), (64, 32, True), (32, 16, False), (16, 16, True)])
 @pytest.mark.parametrize("axes", [1, 3])

@@ -177,9 +177,16 @@ __device__ __forceinline__ float row_sum(float x) {
   if constexpr (LANES >= 16) with(std::integral_constant<int, 0x140>{});
   return x;
 }
-// 1 / sqrt(mean x^2 + eps) of the row, in float64, or in float where the squares' sum is well inside its range
+// Two bf16 values below 2^-113 times 2^16: exact
+__device__ __forceinline__ uint32_t raised(uint32_t pair) {
+  const float lo = __uint_as_float(pair << 16) * 65536.f, hi = __uint_as_float(pair & 0xffff0000u) * 65536.f;
+  return (__float_as_uint(lo) >> 16) | (__float_as_uint(hi) & 0xffff0000u);
+}
+
+// 1 / sqrt(mean x^2 + eps) of the row, in float64, or in float where the squares' sum is well inside its range. As a float it may
+// be past its range for rows of zeros, whatever it is, and for bf16 rows below 2^-126, whose values take 2^16 of it.
 template <int DT, int D, class T>
-__device__ __forceinline__ T inverse_rms(const Chunks& in, double eps) {
+__device__ __forceinline__ T inverse_rms(Chunks& in, double eps) {
   if constexpr (sizeof(T) == 4) {
     float sum = 0.f;
 #pragma unroll
@@ -195,7 +202,19 @@ __device__ __forceinline__ T inverse_rms(const Chunks& in, double eps) {
   }
 #pragma unroll
   for (int off = D / 16; off >= 1; off /= 2) sum += __shfl_xor(sum, off, 64);
-  return (T)inverse_root<sizeof(T) == 8 ? 3 : 1>(sum * (1.0 / D) + eps);
+  double r = inverse_root<sizeof(T) == 8 ? 3 : 1>(sum * (1.0 / D) + eps);
+  if (sizeof(T) == 4 && r > 0x1p126) {
+    if constexpr (DT == 1) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        in.own[i] = raised(in.own[i]);
+        in.other[i] = raised(in.other[i]);
+      }
+      r *= 0x1p-16;
+    }
+    r = fmin(r, 0x1p126);
+  }
+  return (T)r;
 }
 
 // Where pair f's angle and dim d's weight lie in LDS: in units of 16 bytes, the i-th units of all chunks side by side, so that
@@ -214,7 +233,7 @@ __device__ __forceinline__ int weight_slot(int chunk, int i) {
 // This lane's 8 values of a row (D / 8 lanes hold it) normalised (NORM) and rotated: rotated8 of
 // x / sqrt(mean x^2 + eps) * weight
 template <int DT, int D, class T, bool NORM, class A>
-__device__ __forceinline__ void normed_rotated8(const Chunks& in, int chunk, int half, bool interleaved, const A (*cs)[2],
+__device__ __forceinline__ void normed_rotated8(Chunks in, int chunk, int half, bool interleaved, const A (*cs)[2],
                                                 const float* weight, double eps, float (&y)[8]) {
   T r = 1;
   if constexpr (NORM) r = inverse_rms<DT, D, T>(in, eps);
