@@ -196,7 +196,7 @@ def rotary_qk(q, k, positions, plan, *, q_norm=None, k_norm=None, q_out=None, k_
 
     q: fp16 or bf16 [B, H_q, N, D], k [B, H_k, N, D], or packed [T, H_q, D] and [T, H_k, D]; k may be None.
     positions as for rotary(). Returns (q_out, k_out), laid out like q and k; q_out=q and k_out=k work in place, and no other
-    memory that the call reads may be written. Squares are summed in float64, and a value is rounded once.
+    memory that the call reads may be written. Sums and products are held in 32 bits or more, and a value is rounded once.
     """
     if _lib.native is not None:  # the common call, made natively; None: not one of those
         result = _lib.native.rotary_qk(q, k, positions, *plan, *(q_norm or (None, 0.0)), *(k_norm or (None, 0.0)), q_out, k_out)
