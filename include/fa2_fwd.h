@@ -397,8 +397,8 @@ FA2_API size_t fa2_paged_shared_workspace_bytes(int32_t h_q, int32_t h_kv, int32
 /*
  * What rows of q and k are turned by: every head x of q first becomes x / sqrt(mean x^2 + q_eps) * q_weight (device
  * float[head_dim]; NULL: it stays), k likewise, and then pair i is rotated by freqs[i] times the position on axis axes[i]
- * (device int32[half], 0 .. n_axes - 1, others count as the nearest; NULL: all on axis 0, n_axes 1). Squares and their sum
- * are formed in float64.
+ * (device int32[half], 0 .. n_axes - 1, others count as the nearest; NULL: all on axis 0, n_axes 1). Squares are summed in
+ * float, or in float64 where the sum is near the ends of float's range and for keys of an e4m3 cache.
  */
 typedef struct fa2_turn {
   fa2_rotation rotation;
