@@ -243,6 +243,7 @@ FA2_API int fa2_should_pack_gqa(int32_t n_q, int32_t group, int32_t block_m);
  * strides non-negative multiples of 8 elements, K and V rows at most 2^22 elements apart. What a call writes
  * has no stride of 0 over more than one row and overlaps nothing that the call reads, but out of attention
  * and rotary may be q and x, and q_out q.
+ * A call whose launch would hold 2^32 threads or more is refused.
  */
 
 /* Element type of a cache that holds e4m3 (OCP, no infinities), with a scale byte per row. */

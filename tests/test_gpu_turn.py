@@ -284,3 +284,24 @@ def test_graph_and_streams():
                 got.append((rotary_qk(*c, plan, **norms), w))
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for g, w in got for a, b in zip(g, w))
+
+
+@pytest.mark.parametrize("shape", ["packed", "batch"])
+def test_most_tokens(shape):
+    """As many tokens of one head of 16 as a launch holds threads for, 8 GiB written: every group of tokens is its own, the last,
+    partial one too."""
+    from fa2.rotary import HeadNorm, rotary_qk
+    N, D = 16 * (((1 << 32) - 1) // 256) - 5, 16
+    x = randn((1, 1, D), torch.bfloat16, 1)
+    plan, norm = plan_of(D, 1), HeadNorm(weight_of(D, 1))
+    out = torch.full((N, 1, D), 9.0, dtype=x.dtype, device="cuda")
+    positions = torch.tensor([7], device="cuda")  # every token's
+    q, o = x.expand(N, 1, D), out
+    if shape == "batch":
+        q, o = (t.transpose(0, 1).unsqueeze(0) for t in (q, o))
+    made, _ = rotary_qk(q, None, positions.expand(N), plan, q_norm=norm, q_out=o)
+    assert made is o
+    want, _ = rotary_qk(x, None, positions, plan, q_norm=norm)
+    check(want, x, positions, plan, norm)
+    for rows in out.split(1 << 24):
+        assert torch.equal(rows, want.expand(rows.shape))

@@ -14,7 +14,7 @@ int launch_form(const RaggedParams& p, unsigned grid, hipStream_t s) {
     hipLaunchKernelGGL((attn_shared_kernel<FA2_DT, FA2_D, SRC, GWP, GWO, false>), dim3(grid), dim3(256), 0, s, p);
   hipError_t e = hipGetLastError();
   if (e == hipSuccess) {
-    hipLaunchKernelGGL((attn_shared_join_kernel<FA2_DT, FA2_D, GWP, GWO>), dim3(shared_join_grid(p)), dim3(1024), 0, s, p);
+    hipLaunchKernelGGL((attn_shared_join_kernel<FA2_DT, FA2_D, GWP, GWO>), dim3((unsigned)shared_join_grid(p)), dim3(1024), 0, s, p);
     e = hipGetLastError();
   }
   return (int)e;

@@ -116,6 +116,12 @@ int check_cache(const fa2_cache* c, const fa2_sequences* q, int32_t dtype, fa2::
   return FA2_OK;
 }
 
+// A launch holds fewer than 2^32 threads. (So rows, and the kernels' counts of their groups, stay far inside 32 bits.)
+int check_grid(int64_t wgs, int threads = 256) {
+  if (wgs > 0xffffffffLL / threads) return fail(FA2_EINVAL, "a grid of %lld workgroups is too large", (long long)wgs);
+  return FA2_OK;
+}
+
 int launched(int e, const char* what) {
   return e == hipSuccess ? FA2_OK : fail(FA2_ELAUNCH, "%s launch failed: %s", what, hipGetErrorString((hipError_t)e));
 }
@@ -125,10 +131,10 @@ int launched(int e, const char* what) {
 // 1274 workgroups 20.0, 16.8 and 16.4 us; a read of 57071 tokens of 2 x 8 e4m3 heads of 128 in 57071, 7134 and
 // 3567 112, 73 and 81 us. The rotary kernel has no such lookup, and takes as few tokens as fill its lanes.
 constexpr int64_t kWriteWgs = 1024, kReadWgs = 4096, kRotaryWgs = int64_t(1) << 40;
-unsigned cache_grid(fa2::CacheParams* p, int64_t rows_per_token, int32_t head_dim, int64_t least_wgs) {
+int64_t cache_grid(fa2::CacheParams* p, int64_t rows_per_token, int32_t head_dim, int64_t least_wgs) {
   p->tokens_per_wg = fa2::serve_tokens_per_wg((int)std::min<int64_t>(rows_per_token * (head_dim / 8), 256),
                                               p->seq.n_tokens, least_wgs);
-  return (unsigned)(((int64_t)p->seq.n_tokens + p->tokens_per_wg - 1) / p->tokens_per_wg);
+  return ((int64_t)p->seq.n_tokens + p->tokens_per_wg - 1) / p->tokens_per_wg;
 }
 
 // The form of a ragged attention call (attn_ragged.hpp, ragged_work.hpp), from what the host knows of it: the
@@ -275,7 +281,7 @@ int launch_ragged(int32_t dtype, int32_t head_dim, int32_t h_q, fa2::RaggedParam
   const Topology topo = device_topology(stream_device(s));
   const RaggedPlan pl = (MODE == fa2::kModeWindow ? window_plan : ragged_plan)(source, h_q, p.h_kv, head_dim, p.seq.n_tokens,
                                                                                p.seq.n_seq, keys, topo.cus);
-  if (pl.grid > 0x7fffffffLL) return fail(FA2_EINVAL, "grid of %lld workgroups is too large", (long long)pl.grid);
+  if (const int rc = check_grid(pl.grid)) return rc;
   if (pl.workspace) {
     if (!workspace || workspace_bytes < pl.workspace)
       return fail(FA2_EINVAL, "the call needs a workspace of %zu bytes, got %zu", pl.workspace,
@@ -371,7 +377,7 @@ int fa2_rotary(const void* x, void* out, const int64_t x_stride[3], const int64_
   p.tokens_per_wg = fa2::serve_tokens_per_wg((int)std::min<int64_t>((int64_t)heads * (head_dim / 8), 256),
                                              (int64_t)batch * n, kRotaryWgs);
   const int64_t grid = ((int64_t)batch * n + p.tokens_per_wg - 1) / p.tokens_per_wg;
-  if (grid > 0x7fffffffLL) return fail(FA2_EINVAL, "grid of %lld workgroups is too large", (long long)grid);
+  if (const int rc = check_grid(grid)) return rc;
   return launched(fa2::launch_rotary(dtype, head_dim, p, (unsigned)grid, static_cast<hipStream_t>(stream)), "rotary");
 }
 
@@ -384,8 +390,9 @@ int fa2_cache_write(const fa2_cache* cache, const fa2_sequences* seq, const void
   if (const int rc = write_params(cache, seq, k, v, k_stride, v_stride, q, q_out, q_stride, qo_stride, h_q, rotation, dtype, &p))
     return rc;
   if (p.seq.n_seq == 0 || p.seq.n_tokens == 0) return FA2_OK;
-  const unsigned grid = cache_grid(&p, 2 * (int64_t)p.h_kv + p.h_q, cache->head_dim, kWriteWgs);
-  return launched(fa2::launch_cache(true, dtype, cache->head_dim, cache->cache_dtype == FA2_DTYPE_E4M3, p, grid,
+  const int64_t grid = cache_grid(&p, 2 * (int64_t)p.h_kv + p.h_q, cache->head_dim, kWriteWgs);
+  if (const int rc = check_grid(grid)) return rc;
+  return launched(fa2::launch_cache(true, dtype, cache->head_dim, cache->cache_dtype == FA2_DTYPE_E4M3, p, (unsigned)grid,
                                     static_cast<hipStream_t>(stream)),
                   "cache write");
 }
@@ -406,8 +413,9 @@ int fa2_cache_read(const fa2_cache* cache, const fa2_sequences* seq, void* k, vo
   p.skt = k_stride[0]; p.skh = k_stride[1];
   p.svt = v_stride[0]; p.svh = v_stride[1];
   p.h_kv = cache->h_kv;
-  const unsigned grid = cache_grid(&p, 2 * (int64_t)p.h_kv, cache->head_dim, kReadWgs);
-  return launched(fa2::launch_cache(false, dtype, cache->head_dim, cache->cache_dtype == FA2_DTYPE_E4M3, p, grid,
+  const int64_t grid = cache_grid(&p, 2 * (int64_t)p.h_kv, cache->head_dim, kReadWgs);
+  if (const int rc = check_grid(grid)) return rc;
+  return launched(fa2::launch_cache(false, dtype, cache->head_dim, cache->cache_dtype == FA2_DTYPE_E4M3, p, (unsigned)grid,
                                     static_cast<hipStream_t>(stream)),
                   "cache read");
 }

@@ -41,8 +41,8 @@ int launch_ragged(const RaggedParams& p, int source, int row_waves, unsigned gri
 
 // Workgroups per CU of the kernels that hold two forms' code (three would spill up to 64 registers at head_dim 64), and workgroups that join its rows' results (8 rows each)
 constexpr int kSharedWaves = 2;
-inline unsigned shared_join_grid(const RaggedParams& p) {
-  return (unsigned)(((int64_t)p.seq.n_tokens * p.group + 7) / 8 * p.h_kv);
+inline int64_t shared_join_grid(const RaggedParams& p) {
+  return ((int64_t)p.seq.n_tokens * p.group + 7) / 8 * p.h_kv;
 }
 
 // Attention within a window over pages, chunks beside single tokens: p.shares workgroups per head for sequences of more than 32 rows, and

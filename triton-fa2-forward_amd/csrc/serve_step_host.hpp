@@ -114,7 +114,7 @@ int fa2_rotary_qk(const void* q, const void* k, void* q_out, void* k_out, const 
   while (p.tokens_per_wg < 16 && p.tokens_per_wg * p.rot.half < kTurnAngles && (int64_t)batch * n >= 2 * p.tokens_per_wg * kTurnWgs)
     p.tokens_per_wg *= 2;
   const int64_t grid = (int64_t)batch * (((int64_t)n + p.tokens_per_wg - 1) / p.tokens_per_wg);
-  if (grid > 0x7fffffffLL) return fail(FA2_EINVAL, "grid of %lld workgroups is too large", (long long)grid);
+  if (const int rc = check_grid(grid)) return rc;
   return launched(fa2::launch_rotary_qk(dtype, head_dim, p, (unsigned)grid, static_cast<hipStream_t>(stream)), "rotary");
 }
 
@@ -131,8 +131,9 @@ int fa2_cache_write_turned(const fa2_cache* cache, const fa2_sequences* seq, con
   if (const int rc = check_turn(turn, cache->head_dim, positions, position_bytes, p_stride, 2, &p.rot, &p.turn)) return rc;
   if (!positions && turn->n_axes != 1) return fail(FA2_EINVAL, "a rotation by %d axes needs positions", turn->n_axes);
   if (p.seq.n_seq == 0 || p.seq.n_tokens == 0) return FA2_OK;
-  const unsigned grid = cache_grid(&p, 2 * (int64_t)p.h_kv + p.h_q, cache->head_dim, kWriteWgs);
-  return launched(fa2::launch_cache_write_turn(dtype, cache->head_dim, cache->cache_dtype == FA2_DTYPE_E4M3, p, grid,
+  const int64_t grid = cache_grid(&p, 2 * (int64_t)p.h_kv + p.h_q, cache->head_dim, kWriteWgs);
+  if (const int rc = check_grid(grid)) return rc;
+  return launched(fa2::launch_cache_write_turn(dtype, cache->head_dim, cache->cache_dtype == FA2_DTYPE_E4M3, p, (unsigned)grid,
                                                static_cast<hipStream_t>(stream)),
                   "cache write");
 }
@@ -192,14 +193,14 @@ int fa2_attn_paged_shared(const void* q, void* out, const int64_t q_stride[2], c
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const Topology topo = device_topology(stream_device(st));
   const SharedPlan pl = shared_plan(h_q, p.h_kv, cache->head_dim, p.seq.n_tokens, p.seq.n_seq, topo.cus);
+  p.group = h_q / p.h_kv;
+  const int64_t grid = (int64_t)p.h_kv * pl.shares;
+  for (const auto& [wgs, threads] : {std::pair<int64_t, int>{grid, 256}, {fa2::shared_join_grid(p), 1024}})
+    if (const int rc = check_grid(wgs, threads)) return rc;
   if (!workspace || workspace_bytes < pl.workspace)
     return fail(FA2_EINVAL, "the call needs a workspace of %zu bytes, got %zu", pl.workspace,
                 workspace ? workspace_bytes : (size_t)0);
   if (reinterpret_cast<uintptr_t>(workspace) & 255u) return fail(FA2_EALIGN, "the workspace must be 256-byte aligned");
-  p.group = h_q / p.h_kv;
-  const int64_t grid = (int64_t)p.h_kv * pl.shares;
-  if (std::max(grid, ((int64_t)p.seq.n_tokens * p.group + 7) / 8 * p.h_kv) > 0x7fffffffLL)
-    return fail(FA2_EINVAL, "a grid of more than 2^31 workgroups is too large");
   p.shared = shared;
   p.xcd_shift = topo.xcd_shift;
   p.shares = pl.shares;
