@@ -243,7 +243,7 @@ FA2_API int fa2_should_pack_gqa(int32_t n_q, int32_t group, int32_t block_m);
  * strides non-negative multiples of 8 elements, K and V rows at most 2^22 elements apart. What a call writes
  * has no stride of 0 over more than one row and overlaps nothing that the call reads, but out of attention
  * and rotary may be q and x, and q_out q.
- * A call whose launch would hold 2^32 threads or more is refused.
+ * A call whose launch would hold 2^32 threads or more is refused, and so is one of more than 2^31 - 2049 sequences.
  */
 
 /* Element type of a cache that holds e4m3 (OCP, no infinities), with a scale byte per row. */
@@ -431,7 +431,8 @@ FA2_API int fa2_cache_write_turned(const fa2_cache* cache, const fa2_sequences* 
                                    const fa2_turn* turn, int32_t dtype, void* stream);
 
 /*
- * fa2_pages_extend - the pages of new_tokens[s] more tokens of every sequence of lens[s] (negative ones count as 0).
+ * fa2_pages_extend - the pages of new_tokens[s] more tokens of every sequence of lens[s] (negative ones count as 0). n_seq is at
+ * most 2^20, here and in fa2_pages_release.
  * free_pages[0 .. count[0]) are free, of n_pages. Needs are counted in the order of the sequences; with N in all,
  * the i-th gets free_pages[max(count - N, 0) + i], or -1 where that is not free; the page is entered into its place of the
  * table [n_seq, max_pages] (tokens past the row need none). Writes count_out[0], what is left of the free ones; lens_out

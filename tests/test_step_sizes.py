@@ -37,8 +37,33 @@ def test_other_launches():
              lambda: _lib.lib().fa2_cache_read(cache, seq, P, P, s, s, 1, None),
              lambda: _lib.lib().fa2_cache_write_turned(cache, seq, P, P, s, s, None, None, s, s, 0, None, 0, strides(0, 0), turn, 1, None),
              lambda: _lib.lib().fa2_attn_paged_shared(P, P, s, s, cache, seq, P, 4, 1, 1, 0.1, None, P, 1 << 62, None),
-             lambda: _lib.lib().fa2_attn_packed(P, P, P, P, s, s, s, s, P, P, 2 ** 31 - 2048, 2 ** 30, 3, 2, 2, 64, 1, 1, 0.1, None, None),
-             lambda: _lib.lib().fa2_attn_packed_window(P, P, P, P, s, s, s, s, P, P, 2 ** 31 - 2048, 2 ** 30, 3, 2, 2, 64, 1, 9, 0, 0.1,
+             lambda: _lib.lib().fa2_attn_packed(P, P, P, P, s, s, s, s, P, P, 2 ** 31 - 2049, 2 ** 30, 3, 2, 2, 64, 1, 1, 0.1, None, None),
+             lambda: _lib.lib().fa2_attn_packed_window(P, P, P, P, s, s, s, s, P, P, 2 ** 31 - 2049, 2 ** 30, 3, 2, 2, 64, 1, 9, 0, 0.1,
                                                        None, None)]
     for call in calls:
         assert call() == -1 and "too large" in _lib.last_error()
+
+
+@needs_lib
+@pytest.mark.parametrize("n", [2 ** 31 - 1, 2 ** 31 - 64])
+def test_more_sequences_than_are_counted_in_32_bits(n):
+    """The kernels go through the sequences 64 at a time, up to 64 past the last."""
+    s = strides(256, 64)
+    seq = ctypes.byref(c_seq(n_seq=n))
+    calls = [lambda: _lib.lib().fa2_attn_packed(P, P, P, P, s, s, s, s, P, P, n, 3, 3, 4, 4, 64, 1, 1, 0.1, None, None),
+             lambda: _lib.lib().fa2_attn_packed_window(P, P, P, P, s, s, s, s, P, P, n, 3, 3, 4, 4, 64, 1, 9, 0, 0.1, None, None),
+             lambda: _lib.lib().fa2_attn_paged(P, P, s, s, ctypes.byref(c_cache()), seq, 4, 1, 1, 0.1, None, P, 1 << 62, None),
+             lambda: _lib.lib().fa2_attn_paged_window(P, P, s, s, ctypes.byref(c_cache()), seq, 4, 1, 9, 0, 0.1, None, P, 1 << 62, None),
+             lambda: _lib.lib().fa2_attn_paged_shared(P, P, s, s, ctypes.byref(c_cache()), seq, P, 4, 1, 1, 0.1, None, P, 1 << 62, None)]
+    for call in calls:
+        assert call() == -1 and "n_seq" in _lib.last_error()
+
+
+@needs_lib
+@pytest.mark.parametrize("n", [2 ** 31 - 1, 2 ** 31 - 256, 2 ** 20 + 1])
+def test_more_sequences_than_a_step_has(n):
+    """Every workgroup of the pages' kernels goes through all sequences, in 32 bits."""
+    assert _lib.lib().fa2_pages_extend(P, 8, P, P, None, 0, n, 0, 16, P, P, P, P, P, P, 4, None) == -1
+    assert "2^20" in _lib.last_error()
+    assert _lib.lib().fa2_pages_release(P, 8, P, P, None, 0, n, 0, P, P, P, None) == -1
+    assert "2^20" in _lib.last_error()

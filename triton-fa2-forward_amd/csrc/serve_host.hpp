@@ -57,6 +57,12 @@ int check_rotation(const fa2_rotation* r, int32_t head_dim, fa2::RotaryPlan* out
   return FA2_OK;
 }
 
+// The kernels count sequences in 32 bits, 64 at a time.
+int check_sequences(int32_t n_seq) {
+  if (n_seq > kMaxKeys) return fail(FA2_EINVAL, "n_seq must be at most %d", kMaxKeys);
+  return FA2_OK;
+}
+
 // The cache and the sequences over it, checked, as the kernels take them.
 int check_cache(const fa2_cache* c, const fa2_sequences* q, int32_t dtype, fa2::CacheTensor* kc,
                 fa2::CacheTensor* vc, fa2::Sequences* seq) {
@@ -98,6 +104,7 @@ int check_cache(const fa2_cache* c, const fa2_sequences* q, int32_t dtype, fa2::
     return fail(FA2_EINVAL, "bad sizes: n_seq=%d n_tokens=%d max_pages=%d table_stride=%lld", q->n_seq, q->n_tokens,
                 q->max_pages, (long long)q->table_stride);
   if (q->n_tokens > kMaxKeys) return fail(FA2_EINVAL, "n_tokens must be at most %d", kMaxKeys);
+  if (const int rc = check_sequences(q->n_seq)) return rc;
   if ((int64_t)q->max_pages * c->page_size > kMaxKeys)
     return fail(FA2_EINVAL, "max_pages * page_size must be at most %d (32-bit key positions), got %lld", kMaxKeys,
                 (long long)q->max_pages * c->page_size);
@@ -214,6 +221,7 @@ int packed_params(const void* q, const void* k, const void* v, void* out, const 
   if (const int rc = check_type(head_dim, dtype)) return rc;
   if (n_seq < 0 || n_tokens < 0 || kv_tokens < 0 || kv_tokens > kMaxKeys)
     return fail(FA2_EINVAL, "bad sizes: n_seq=%d n_tokens=%d kv_tokens=%d", n_seq, n_tokens, kv_tokens);
+  if (const int rc = check_sequences(n_seq)) return rc;
   if (!cu_kv && kv_tokens != n_tokens)
     return fail(FA2_EINVAL, "k and v of %d rows for q of %d need their own cu_kv", kv_tokens, n_tokens);
   if (const int rc = check_heads(h_q, h_kv, n_tokens, qk_scale, lse)) return rc;

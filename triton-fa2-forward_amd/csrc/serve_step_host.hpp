@@ -73,6 +73,13 @@ SharedPlan shared_plan(int32_t h_q, int32_t h_kv, int32_t head_dim, int32_t n_to
   return pl;
 }
 
+// Every workgroup of the pages' kernels goes through the lengths, or counts, of all sequences before its own, 256 or 64 at a time.
+constexpr int32_t kMostStepSequences = 1 << 20;
+int check_step_sequences(int32_t n_seq) {
+  if (n_seq > kMostStepSequences) return fail(FA2_EINVAL, "at most 2^20 sequences, got %d", n_seq);
+  return FA2_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -236,6 +243,7 @@ int fa2_pages_extend(const int32_t* free_pages, int32_t n_pages, const int32_t* 
   if (n_pages < 0 || n_seq < 1 || max_pages < 0 || n_tokens < 0 || table_stride < 0)
     return fail(FA2_EINVAL, "bad sizes: n_pages=%d n_seq=%d max_pages=%d n_tokens=%d table_stride=%lld", n_pages, n_seq,
                 max_pages, n_tokens, (long long)table_stride);
+  if (const int rc = check_step_sequences(n_seq)) return rc;
   if (!power_of_two(page_size) || page_size > (1 << 20))
     return fail(FA2_EINVAL, "page_size must be a power of two up to 2^20, got %d", page_size);
   if (!count || !count_out || !lens || !new_tokens || !lens_out || !cu_out || (n_pages > 0 && !free_pages) ||
@@ -267,6 +275,7 @@ int fa2_pages_release(int32_t* free_pages, int32_t n_pages, const int32_t* count
   if (n_pages < 0 || n_seq < 1 || max_pages < 0 || table_stride < 0)
     return fail(FA2_EINVAL, "bad sizes: n_pages=%d n_seq=%d max_pages=%d table_stride=%lld", n_pages, n_seq, max_pages,
                 (long long)table_stride);
+  if (const int rc = check_step_sequences(n_seq)) return rc;
   if (!count || !count_out || !first || !last || !workspace || (n_pages > 0 && !free_pages) || (max_pages > 0 && !table))
     return fail(FA2_EINVAL, "null pointer");
   for (const void* x : {(const void*)free_pages, (const void*)count, (const void*)count_out, (const void*)table,

@@ -63,7 +63,7 @@ def _check(pool, block_table):
 def pages_extend(pool, block_table, seqlens, new_tokens, page_size, n_tokens):
     """Pages for the new tokens of a step: a Step.
 
-    block_table: int32 [S, pages], whose rows hold the pages of seqlens[s] tokens in order; the new ones are entered
+    block_table: int32 [S, pages] (S up to 2^20), whose rows hold the pages of seqlens[s] tokens in order; the new ones are entered
     behind them, in place. seqlens: int32 [S], tokens in the cache; new_tokens: int32 [S], to be added to each (negative
     numbers count as 0). page_size: a power of two up to 2^20. n_tokens: rows of positions and slots (the sum of new_tokens, which is
     not copied to the host to find out; or more).
