@@ -115,7 +115,8 @@ def cache_write(cache, k, v, block_table, cu_seqlens, seqlens, *, rotary=None, q
     turned = positions is not None or q_norm is not None or k_norm is not None or (
         rotary is not None and rotary.axes is not None)
     if _lib.native is not None:  # the common call, made natively; None: not one of those
-        args = (*cache, block_table, cu_seqlens, seqlens, k, v, *((None, False, 1.0, None) if rotary is None else rotary), q, q_out)
+        plan = (None, False, 1.0, None) if rotary is None else (rotary.freqs, rotary.interleaved, rotary.scale, rotary.axes)
+        args = (*cache, block_table, cu_seqlens, seqlens, k, v, *plan, q, q_out)
         if turned:
             result = _lib.native.cache_write_turned(*args, *(q_norm or (None, 0.0)), *(k_norm or (None, 0.0)), positions)
         else:

@@ -20,7 +20,20 @@ from . import _lib
 from .kernel import _loadable
 
 
-class Rotary(NamedTuple):
+class _Plan(NamedTuple):
+    freqs: torch.Tensor
+    interleaved: bool = False
+    scale: float = 1.0
+
+
+class _AxesPlan(NamedTuple):
+    freqs: torch.Tensor
+    interleaved: bool = False
+    scale: float = 1.0
+    axes: Optional[torch.Tensor] = None
+
+
+class Rotary(_Plan):
     """Frequencies and form of a rotation, kept by the caller for every layer.
 
     freqs: float64 [rot_dim / 2] on the GPU, radians per position; rot_dim a multiple of 16, at most head_dim.
@@ -28,11 +41,24 @@ class Rotary(NamedTuple):
     scale: factor on the rotated values (scaled contexts).
     axes: int32 [rot_dim / 2] on the GPU, the axis by whose position each pair is rotated (below the number of axes of the
         positions it is used with; others count as the nearest). None: one position a token.
+
+    A named tuple of the first three, and of all four (an AxesRotary) with axes.
     """
-    freqs: torch.Tensor
-    interleaved: bool = False
-    scale: float = 1.0
-    axes: Optional[torch.Tensor] = None
+    __slots__ = ()
+    axes = None
+
+    def __new__(cls, freqs, interleaved=False, scale=1.0, axes=None):
+        if axes is not None:
+            return AxesRotary(freqs, interleaved, scale, axes)
+        return super().__new__(cls, freqs, interleaved, scale)
+
+    def _replace(self, *, axes=None, **values):
+        return Rotary(*super()._replace(**values), axes)
+
+
+class AxesRotary(_AxesPlan, Rotary):
+    """A Rotary with axes."""
+    __slots__ = ()
 
 
 class HeadNorm(NamedTuple):
@@ -199,7 +225,8 @@ def rotary_qk(q, k, positions, plan, *, q_norm=None, k_norm=None, q_out=None, k_
     memory that the call reads may be written. Sums and products are held in 32 bits or more, and a value is rounded once.
     """
     if _lib.native is not None:  # the common call, made natively; None: not one of those
-        result = _lib.native.rotary_qk(q, k, positions, *plan, *(q_norm or (None, 0.0)), *(k_norm or (None, 0.0)), q_out, k_out)
+        result = _lib.native.rotary_qk(q, k, positions, plan.freqs, plan.interleaved, plan.scale, plan.axes,
+                                       *(q_norm or (None, 0.0)), *(k_norm or (None, 0.0)), q_out, k_out)
         if result is not None:
             return result[0] if q_out is None else q_out, result[1] if k_out is None else k_out
     assert q.dim() in (3, 4) and q.dtype in (torch.float16, torch.bfloat16)
