@@ -173,6 +173,25 @@ def test_norm_least_values(dtype, eps, interleaved):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("eps", [1e29, 1e31, 1e38, 1e39, 1e60, 1e72, 1e76, 1e100, 1e200, 1.7e308])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_norm_large_eps(dtype, eps, interleaved):
+    """An eps past float's range, beside ordinary values and the type's largest: results are small, not zero."""
+    from fa2.rotary import HeadNorm, rotary_plan, rotary_qk
+    D = 64
+    g = torch.Generator().manual_seed(2)
+    top = torch.finfo(dtype).max
+    size = torch.tensor([1.0, 2.0 ** 15, top, top / 2, *([2.0 ** 60, 2.0 ** 100, 2.0 ** 120, 2.0 ** -60] if dtype == torch.bfloat16 else [0.1])],
+                        dtype=torch.float64)[:, None, None]
+    x = (size * (torch.rand(len(size), 2, D, generator=g, dtype=torch.float64) * 2 - 1)).to(dtype).cuda()
+    plan, norm = rotary_plan(48, interleaved=interleaved), HeadNorm(weight_of(D, 3), eps)
+    positions = torch.arange(len(x), device="cuda")
+    got, _ = rotary_qk(x, None, positions, plan, q_norm=norm)
+    want, tol = step_oracle.turn(x, positions, plan.freqs, interleaved, weight=norm.weight, eps=norm.eps)
+    assert ((got.double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("e4m3", [False, True])
 @pytest.mark.parametrize("D,rot,interleaved", [(128, 128, False), (64, 32, True), (32, 16, False), (16, 16, True)])
 @pytest.mark.parametrize("axes", [1, 3])

@@ -177,14 +177,17 @@ __device__ __forceinline__ float row_sum(float x) {
   if constexpr (LANES >= 16) with(std::integral_constant<int, 0x140>{});
   return x;
 }
-// Two bf16 values below 2^-113 times 2^16: exact
-__device__ __forceinline__ uint32_t raised(uint32_t pair) {
-  const float lo = __uint_as_float(pair << 16) * 65536.f, hi = __uint_as_float(pair & 0xffff0000u) * 65536.f;
+// Two bf16 values times 2^k: exact, but where a product leaves bf16's normal numbers at their lower end
+__device__ __forceinline__ uint32_t scaled(uint32_t pair, int k) {
+  const float lo = __builtin_amdgcn_ldexpf(__uint_as_float(pair << 16), k);
+  const float hi = __builtin_amdgcn_ldexpf(__uint_as_float(pair & 0xffff0000u), k);
   return (__float_as_uint(lo) >> 16) | (__float_as_uint(hi) & 0xffff0000u);
 }
 
-// 1 / sqrt(mean x^2 + eps) of the row, in float64, or in float where the squares' sum is well inside its range. As a float it may
-// be past its range for rows of zeros, whatever it is, and for bf16 rows below 2^-126, whose values take 2^16 of it.
+// 1 / sqrt(mean x^2 + eps) of the row, in float64, or in float where the squares' sum and eps are well inside its range. As a float it
+// may be past its range: above for rows of zeros, whatever it is, and for bf16 rows below 2^-126, whose values take 2^16 of it; below for
+// the largest bf16 rows and for an eps from 2^240 on, where bf16 values take as much of it as leaves it at 2^-64 (values that are
+// no normal numbers then are results below 2^-189; of fp16 all results are below 2^-104).
 template <int DT, int D, class T>
 __device__ __forceinline__ T inverse_rms(Chunks& in, double eps) {
   if constexpr (sizeof(T) == 4) {
@@ -192,7 +195,7 @@ __device__ __forceinline__ T inverse_rms(Chunks& in, double eps) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) sum = Elem<DT>::sumsq2(in.own[i], sum);
     sum = row_sum<D / 8>(sum);
-    if (sum > 1e-30f && sum < 1e30f) return __builtin_amdgcn_rsqf(__builtin_fmaf(sum, 1.0f / D, (float)eps));
+    if (sum > 1e-30f && sum < 1e30f && eps < 1e30) return __builtin_amdgcn_rsqf(__builtin_fmaf(sum, 1.0f / D, (float)eps));
   }
   double sum = 0.0;
 #pragma unroll
@@ -203,16 +206,18 @@ __device__ __forceinline__ T inverse_rms(Chunks& in, double eps) {
 #pragma unroll
   for (int off = D / 16; off >= 1; off /= 2) sum += __shfl_xor(sum, off, 64);
   double r = inverse_root<sizeof(T) == 8 ? 3 : 1>(sum * (1.0 / D) + eps);
-  if (sizeof(T) == 4 && r > 0x1p126) {
-    if constexpr (DT == 1) {
+  if constexpr (sizeof(T) == 4) {
+    const bool above = r > 0x1p126, below = r > 0.0 && r < 0x1p-120;  // (0: of an infinite value)
+    if (DT == 1 && (above || below)) {
+      const int k = above ? 16 : 64 + __builtin_amdgcn_frexp_exp(r);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        in.own[i] = raised(in.own[i]);
-        in.other[i] = raised(in.other[i]);
+        in.own[i] = scaled(in.own[i], k);
+        in.other[i] = scaled(in.other[i], k);
       }
-      r *= 0x1p-16;
+      r = __builtin_amdgcn_ldexp(r, -k);
     }
-    r = fmin(r, 0x1p126);
+    if (above) r = fmin(r, 0x1p126);
   }
   return (T)r;
 }
