@@ -11,6 +11,8 @@
 // Measured on MI355X: 256 sequences of one new token 4.2 us, 50 of up to 2048 6.7.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+
 #include "serve_launch.hpp"
 
 namespace fa2 {
@@ -209,10 +211,8 @@ __global__ __launch_bounds__(256) void pages_release_kernel(const ReleaseParams 
   if (s == p.n_seq - 1 && lane == 0) p.count_out[0] = (int32_t)min(at, (int64_t)p.n_pages);
 }
 
-// Both in one launch, for tables of at most kOneRelease entries (more would be read too often): a wave a sequence, 16 a workgroup,
+// Both in one launch, where few rounds count what lies before the last sequences (one_release): a wave a sequence, 16 a workgroup,
 // which counts the pages of all sequences before its own for itself, 16 lanes a sequence and 16 entries a lane at once.
-// Measured on MI355X, in two launches and in one: 8 of 256 sequences of up to 512 pages 2.3 + 3.5 and 7.6 us, 50 of 100 of up to 64 2.4 +
-// 3.1 and 6.0; the whole calls, and an extension after them, 15.4 and 12.8 both times: the host's launch is what counts.
 template <int LANES, int STEP>
 __device__ __forceinline__ int count_pages(const ReleaseParams& p, int s, const Range& r, int lane) {
   int n = 0;
@@ -255,7 +255,19 @@ __global__ __launch_bounds__(1024) void pages_release_once_kernel(const ReleaseP
   at = push_pages(p, s, r, lane, at);
   if (s == p.n_seq - 1 && lane == 0) p.count_out[0] = (int32_t)min(at, (int64_t)p.n_pages);
 }
-constexpr int64_t kOneRelease = 1 << 18;
+
+// One launch while the last workgroup counts the others' pages in at most 8 rounds of 64 sequences and 256 entries, which all wait for
+// their loads. Each workgroup counts for itself, so that the time grows with the square of the sequences; what it saves is a launch,
+// about 2.5 us of the host. Measured on MI355X, one launch and two, with a 32nd of the sequences or all of them ended, in a captured
+// graph: 16 sequences of up to 4096 pages (no rounds) 12.9 and 18.3, 18.1 and 20.2 us; 128 of 256 (2) 4.3 and 5.0, 5.9 and 5.5; 256 of
+// 64 (4) 5.9 and 5.0, 8.4 and 5.6; 256 of 512 (8) 8.6 and 6.3, 13.3 and 6.7 - made call after call with an extension behind it, where
+// the host is what counts, 12.8 and 15.4 -; 512 of 512 (16) 14.8 and 7.1, 22 and 7.9; 1024 of 4 (16) 15 and 8.3, 23 and 8.9; 16384 of
+// 4 470 and 65, 775 and 67.
+constexpr int64_t kOneReleaseRounds = 8;
+bool one_release(const ReleaseParams& p) {
+  const int64_t before = (p.n_seq - 1) / 16 * 16, entries = std::max(p.max_pages, 1);
+  return (before + 63) / 64 * ((entries + 255) / 256) <= kOneReleaseRounds;
+}
 
 }  // namespace
 
@@ -265,7 +277,7 @@ int launch_pages_extend(const PagesParams& p, unsigned blocks, unsigned stripes,
 }
 
 int launch_pages_release(const ReleaseParams& p, hipStream_t s) {
-  if ((int64_t)p.n_seq * p.max_pages <= kOneRelease) {
+  if (one_release(p)) {
     hipLaunchKernelGGL(pages_release_once_kernel, dim3((unsigned)((p.n_seq + 15) / 16)), dim3(1024), 0, s, p);
     return (int)hipGetLastError();
   }
