@@ -49,8 +49,8 @@ class Rotary(_Plan):
 
     def __new__(cls, freqs, interleaved=False, scale=1.0, axes=None):
         if axes is not None:
-            return AxesRotary(freqs, interleaved, scale, axes)
-        return super().__new__(cls, freqs, interleaved, scale)
+            return tuple.__new__(AxesRotary, (freqs, interleaved, scale, axes))
+        return tuple.__new__(cls, (freqs, interleaved, scale))
 
     def _replace(self, *, axes=None, **values):
         return Rotary(*super()._replace(**values), axes)
