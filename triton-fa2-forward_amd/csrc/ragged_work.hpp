@@ -34,18 +34,11 @@ __device__ __forceinline__ ParamsRef params_here() {
   return *p;
 }
 
-// Keys that a tile costs beside its own: its rows' loads, its merge and stores. Measured on MI355X, in keys of cost
-// 64 / 128 / 256 / 384: 4 prompts of 2000 in 128-row tiles (a share of short tiles alone holds many of them)
-// 201 / 185 / 164 / 166 us; steps of 64 sequences of 1000 keys in 32-row tiles 46.5 / 47.8 / 48.0 / 49.0.
-template <int BM>
-constexpr int kTileCost = BM == 32 ? 64 : 256;
-// ... a 32-row tile's behind a common prefix, where keys are few and the chain of a tile's loads takes longest; and in e4m3 beside that, as
+// kTileCost of a 32-row tile behind a common prefix, where keys are few and the chain of a tile's loads takes longest; and in e4m3 beside that, as
 // the shares are dealt. Measured on MI355X, 32 / 8 heads of 128, costs of 64 / 128 / 256 / 384 / 640: 32 steps of one 16-bit token of their own
 // behind 4096 shared 29.5 / 22.2 / 17.7 / 17.7 / 18.1 us, of up to 500 behind 8192 24.2 / 25.7 / 24.5 / 24.6 / 24.8; 16 drafts of one e4m3 token
 // of their own behind 64 29.4 / 19.9 / 13.6 / 13.9 / 15.8, of up to 300 behind 32k 51.0 / 54.7 / 53.0 / 50.2 / 49.8.
 constexpr int kOwnTileCost = 384, kOwnE4m3Cost = 448;
-// ... and what sharing the tiles out costs a 128-row workgroup: more pieces, the partial results, their merge
-constexpr int kShareCost = 640;
 // The most sequences whose tiles go by their index (above; at most 64, a lane each).
 constexpr int kFewSequences = 8;
 // Keys of the smallest share: four tiles of 64, or two of 32 for each of four waves. Measured on MI355X, 128 / 256 / 512: steps of

@@ -185,14 +185,29 @@ RaggedPlan ragged_plan(int source, int32_t h_q, int32_t h_kv, int32_t head_dim, 
   pl.grid = (pl.shares ? pl.shares : n) * h_kv;
   return pl;
 }
-// ... of a window over pages: mixed where sequences of few rows stand beside chunks whose row tiles give every CU one at least
+// ... of a window over pages: mixed where sequences of few rows stand beside chunks whose row tiles give every CU one at least.
+// Measured on MI355X, window 2048, a chunk beside single tokens behind 6000, 128-row tiles alone and mixed, us: heads of 16, 32 / 8, a
+// chunk of 1024 beside 24 51 and 40, of 2048 64 and 52, of 4096 beside 64 124 and 99; of 64, 28 / 4, of 2048 beside 24 71 and 60, of 3000
+// 76 and 91; e4m3 of 128, 28 / 4, of 1024 beside 24 86 and 71, of 2048 115 and 94, of 4096 186 and 184, 32 / 8 220 and 184.
+// 16-bit heads of 128, where a single token's workgroup takes longest, only where the few would take the row tiles past one round of the
+// workgroups, which then share all of them and merge the pieces, while the chunk's alone are a tile a workgroup (ragged_work.hpp's
+// whole_tiles), and where the few are no more than the CUs:
+//   * so: 28 / 4 heads, a chunk of 2048 (112 tiles on 128 workgroups a head) beside 24 97 and 86, 40 105 and 104; 32 / 8, 2048 (64 on
+//     64) beside 24 119 and 112.
+//   * all of them in one round: 28 / 4, 1500 (82 tiles) beside 24 70 and 90; 32 / 8, 1200 (37) 70 and 111.
+//   * the chunk past a round: 28 / 4, 2500 (136) beside 24 116 and 123, 4096 159 and 170; 32 / 8, 3000 (93) 151 and 181.
+//   * more of the few: 28 / 4, 2048 beside 64 121 and 153, 100 144 and 192; 32 / 8 beside 40 134 and 153.
 RaggedPlan window_plan(int source, int32_t h_q, int32_t h_kv, int32_t head_dim, int32_t n_tokens, int32_t n_seq, int64_t keys,
                        int cus) {
   RaggedPlan pl = ragged_plan(source, h_q, h_kv, head_dim, n_tokens, n_seq, keys, cus);
-  const int64_t rows = (int64_t)n_tokens * (h_q / h_kv);
-  if (source == fa2::kSourcePacked || pl.row_waves == 1 || !pl.shares || n_seq == 1 || rows / 128 * h_kv < cus) return pl;
+  const int64_t tiles = (int64_t)n_tokens * (h_q / h_kv) / 128, shares = std::max(1, fa2::kSharedWaves * cus / h_kv);
+  if (source == fa2::kSourcePacked || pl.row_waves == 1 || !pl.shares || n_seq == 1 || tiles * h_kv < cus) return pl;
+  if (head_dim == 128 && source == fa2::kSourcePages) {
+    const bool whole = tiles <= shares && (keys + fa2::kTileCost<128>) * (shares - tiles) <= fa2::kShareCost * shares;
+    if (!whole || tiles + n_seq <= pl.shares || (int64_t)n_seq * h_kv > cus) return pl;
+  }
   pl.mixed = true;
-  pl.shares = std::max(1, fa2::kSharedWaves * cus / h_kv);
+  pl.shares = (int)shares;
   pl.parts = (size_t)h_kv * pl.shares * 2 * 128 * (head_dim + 4) * sizeof(float);
   pl.workspace = pl.parts + (size_t)h_kv * pl.shares * fa2::kMergeBytes;
   pl.grid = ((int64_t)pl.shares + n_seq) * h_kv;

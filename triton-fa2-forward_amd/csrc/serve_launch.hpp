@@ -34,6 +34,14 @@ constexpr int ragged_waves(int head_dim, int source, int row_waves) {
   return head_dim == 128 || source == kSourceE4m3 ? 2 : source == kSourcePages ? 3 : 4;
 }
 
+// Keys that a tile costs beside its own: its rows' loads, its merge and stores. Measured on MI355X, in keys of cost
+// 64 / 128 / 256 / 384: 4 prompts of 2000 in 128-row tiles (a share of short tiles alone holds many of them)
+// 201 / 185 / 164 / 166 us; steps of 64 sequences of 1000 keys in 32-row tiles 46.5 / 47.8 / 48.0 / 49.0.
+template <int BM>
+constexpr int kTileCost = BM == 32 ? 64 : 256;
+// ... and what sharing the tiles out costs a 128-row workgroup: more pieces, the partial results, their merge
+constexpr int kShareCost = 640;
+
 // The ragged attention kernel with 32 * row_waves (1 or 4) rows per workgroup, and after it, with p.shares > 0,
 // the merge of the row tiles that its shares cut.
 template <int DT, int D, int MODE>
