@@ -82,13 +82,16 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(6))) void r
   }
 }
 
-// Workgroups below which each pass over a token's heads is one of its own: few tokens wait for one pass after the other.
-constexpr unsigned kTurnFewWgs = 512;
+// Workgroups below which each pass over a token's heads is one of its own, of rotations and of writes: few tokens wait for one pass after
+// the other. Measured on MI355X, one workgroup a token and one a pass: 32 + 8 heads of 128, 3 passes, 16 tokens 6.4 and 4.6 us, 256 6.8 and
+// 5.5, 384 7.6 and 6.7, 512 7.8 and 7.4, 700 8.7 and 9.8; written into e4m3 (32 + 2 x 8) 16 7.5 and 6.2, 256 8.3 and 7.2, 320 9.3 and 8.4,
+// 384 9.5 and 10.4, 511 9.8 and 12.1; into 16 bits 256 6.8 and 6.2, 320 7.5 and 6.8, 384 7.5 and 7.5, 511 8.0 and 9.7.
+constexpr unsigned kTurnFewWgs = 512, kWriteFewWgs = 352;
 template <int DT, int D>
 int launch_write_d(bool e4m3, const CacheTurnParams& p, unsigned grid, hipStream_t s) {
   const int rows = 256 / (D / 8);
   const int64_t each = (2 * (int64_t)p.h_kv + p.h_q) * p.tokens_per_wg;
-  const unsigned passes = grid < kTurnFewWgs && each > rows ? (unsigned)std::min<int64_t>((each + rows - 1) / rows, 64) : 1u;
+  const unsigned passes = grid < kWriteFewWgs && each > rows ? (unsigned)std::min<int64_t>((each + rows - 1) / rows, 64) : 1u;
   if (e4m3)
     hipLaunchKernelGGL((cache_write_kernel<DT, D, true, CacheTurnParams>), dim3(grid, passes), dim3(256), 0, s, p);
   else
