@@ -28,7 +28,8 @@
 //     spilled, 7 of them with 32 rows). 2 e4m3 chunks of up to 2048 behind 12k and 32k: 1218 us, 930 TFLOP/s, and 17 of merge.
 //     One of 500 beside 24 steps of up to 8k: 88 us and 12 of merge.
 //   * windows: the same, and the tiles at both ends, of which a row tile sees parts: 4 packed prompts of up to 8192, window 1024 and 4 sinks, 32 / 8
-//     heads of 128, bf16, with the log-sum-exp: 265 us, 825 TFLOP/s of the pairs that are seen, matrix cores 42% busy.
+//     heads of 128, bf16, with the log-sum-exp: 275 to 295 us (the least and the median of 60 in a row, up to 357 as the clock gives), 740 to
+//     800 TFLOP/s of the pairs that are seen, matrix cores 42% busy.
 //   * steps: reading K and V. 16 of up to 4095 tokens, 32 / 8 heads of 128, bf16, pages of 16: 28 us, 4.7 TB/s, and 4.5 of
 //     merge; 64 of up to 16000, e4m3: 198 us, 5.3 TB/s.
 // Tried and dropped: writing e4m3's converted pairs in an order without bank conflicts (10% of the cycles have one; the
@@ -875,7 +876,7 @@ void attn_ragged_kernel(const RaggedParams) {
 // A window over chunks of prompts beside single tokens, where the chunks' rows fill the GPU: their 128-row tiles are shared out as
 // ever, and each sequence of at most 32 rows has a 32-row workgroup of its own behind them. In 128-row tiles a token's row costs
 // what a chunk's 128 do. Measured on MI355X, a chunk of 2048 beside 24 steps, window 2048, 28 / 4 heads of 128: 92 us and 17 of merge in
-// 128-row tiles alone, 89 and 5 (no tile is cut) with both.
+// 128-row tiles alone, 89 and 5 (no tile is cut) with both. When it is chosen, with other batches' times: serve_host.hpp, window_plan.
 template <int DT, int D, int SRC, bool LSE>
 __global__ __launch_bounds__(256)
 __attribute__((amdgpu_waves_per_eu(kSharedWaves)))
@@ -902,7 +903,8 @@ void attn_window_mixed_kernel(const RaggedParams) {
 // sequence. Measured on MI355X, 32 steps behind 8192 shared tokens and up to 500 of their own, 32 / 8 heads of 128, bf16: 21.6 us and 7 of join
 // (one launch after the other, each with its merge: 18 + 25 + 19 + 5; without sharing 63); bound by the chain of loads that finds a
 // workgroup's work, its pages and its first keys (11 us with hardly a key). 16 drafts of up to 5 behind 32k, 28 / 4 heads, e4m3: 41 and 8; the
-// loads of a tile, one ahead, and registers spilled at two workgroups a CU (matrix cores 19% busy).
+// loads of a tile, one ahead, and registers spilled at two workgroups a CU (34 of them; in e4m3 at head_dim 128 20 to 50; matrix
+// cores 19% busy).
 template <int DT, int D, int SRC, int GWP, int GWO, bool LSE>
 __global__ __launch_bounds__(256)
 __attribute__((amdgpu_waves_per_eu(kSharedWaves)))

@@ -9,7 +9,9 @@
 //     keys, so the longest start first. More sequences go one after the other, each from its highest tile down: its tiles
 //     share its K and V in an L2, and the search is shorter. Measured on MI355X, by index and by sequence: 4 of up to
 //     8192, 16 heads of 64 with the log-sum-exp, 231 and 256 us; 8 of up to 2048, 32 / 8 heads of 128, 116 and 115 to 119;
-//     16 of 512 78 and 65; 64 of 128 77 and 46, of 1024 1012 and 689.
+//     16 of 512 78 and 65; 64 of 128 77 and 46, of 1024 1012 and 689. Windows, whose tiles are nearly even, have the same rule: 4 of up to
+//     8192, window 1024, 32 / 8 heads of 128, 513 and 495; 8 of 4096 577 and 557; 8 of 2000, window 128, 16 heads of 64, 44.0 and 42.6; of 8192, 3000
+//     and twice 100, window 512, 49.6 and 53.9; 16 of 2048, window 1024, 523 and 494.
 //   * `shares` workgroups per head, each an equal share of the head's tiles laid end to end, a tile's length being
 //     its keys (an estimate, linear in the tile's index, so that a sequence's sum is a closed form; it only
 //     decides where the cuts lie). A share starts and ends inside tiles: a tile cut by a share's end leaves
@@ -37,7 +39,9 @@ __device__ __forceinline__ ParamsRef params_here() {
 // kTileCost of a 32-row tile behind a common prefix, where keys are few and the chain of a tile's loads takes longest; and in e4m3 beside that, as
 // the shares are dealt. Measured on MI355X, 32 / 8 heads of 128, costs of 64 / 128 / 256 / 384 / 640: 32 steps of one 16-bit token of their own
 // behind 4096 shared 29.5 / 22.2 / 17.7 / 17.7 / 18.1 us, of up to 500 behind 8192 24.2 / 25.7 / 24.5 / 24.6 / 24.8; 16 drafts of one e4m3 token
-// of their own behind 64 29.4 / 19.9 / 13.6 / 13.9 / 15.8, of up to 300 behind 32k 51.0 / 54.7 / 53.0 / 50.2 / 49.8.
+// of their own behind 64 29.4 / 19.9 / 13.6 / 13.9 / 15.8, of up to 300 behind 32k 51.0 / 54.7 / 53.0 / 50.2 / 49.8. In 16 bits, a whole call with its
+// join: 128 steps of up to 300 behind 8192 62 / 55 / 50 / 50 / 53, with heads of 64 54 / 47 / 46 / 42 / 40, of 32 46 / 43 / 39 / 39 / 34, 16 / 16 heads of
+// 64 50 / 49 / 46 / 46 / 52; 16 drafts of 5 and up to 300 behind 8192 50 / 48 / 42 / 37 / 33, of 64 39 / 36 / 34 / 30 / 27, of 32 31 / 30 / 27 / 27 / 24.
 constexpr int kOwnTileCost = 384, kOwnE4m3Cost = 448;
 // The most sequences whose tiles go by their index (above; at most 64, a lane each).
 constexpr int kFewSequences = 8;
@@ -404,7 +408,9 @@ __device__ __forceinline__ bool deal_shares(ParamsRef p, int rank, int lane, Cur
   c->rows_first = row_bound(p.seq.cu, 0, p.seq.n_tokens);
   c->rows = max(row_bound(p.seq.cu, p.seq.n_seq, p.seq.n_tokens) - c->rows_first, 0);
   c->prefix = common_prefix(p, lane, c->raw);
-  const int64_t cost = c->prefix.tokens == 0 ? 128 : c->prefix.tokens + kTileCost<BMP>;  // (no keys: only empty results to write)
+  // (no keys: only empty results to write. Measured on MI355X, 32 / 8 heads of 128, costs of 16 / 128 / 512: 32 steps of 500 to 1000 keys
+  // 30.1 / 30.6 / 30.3 us, 128 of 100 to 200 33.1 / 32.9 / 31.5, 16 drafts of 5 20.7 / 20.4 / 20.4)
+  const int64_t cost = c->prefix.tokens == 0 ? 128 : c->prefix.tokens + kTileCost<BMP>;
   double ours = (double)(row_tiles<BMP>(c->rows, p.group) * cost) * (BMP > BMO ? 1.5 : 1.0), own = 0.0;
   for (int s0 = 0; s0 < p.seq.n_seq; s0 += 64) {
     const LaneSequence q = lane_sequence<true, kModeOwn>(p, s0 + lane, *c);

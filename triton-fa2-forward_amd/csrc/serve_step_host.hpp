@@ -43,6 +43,10 @@ int check_turn(const fa2_turn* turn, int32_t head_dim, const void* positions, in
   return FA2_OK;
 }
 
+// Workgroups that are left at least where rotary_qk gathers tokens, and angles a workgroup forms from which on it gathers no more. Measured on
+// MI355X, 32 + 8 heads of 128, three axes: 2048 tokens, one / two / four a workgroup 17.1 / 14.3 / 16.1 us, 4096 27.1 / 22.5 / 20.8 (and 26.1 of
+// eight); 16384, one / four / eight / sixteen 127 / 79.4 / 78.7 / 81.5. 16 + 4 heads of 64: 16384 tokens, one / eight / sixteen 47.1 / 23.1 /
+// 22.2.
 constexpr int64_t kTurnWgs = 1024, kTurnAngles = 512;
 
 // The keys that a row sees of n_kv at most, as the choice of a form counts them.
