@@ -28,8 +28,8 @@
 //     spilled, 7 of them with 32 rows). 2 e4m3 chunks of up to 2048 behind 12k and 32k: 1218 us, 930 TFLOP/s, and 17 of merge.
 //     One of 500 beside 24 steps of up to 8k: 88 us and 12 of merge.
 //   * windows: the same, and the tiles at both ends, of which a row tile sees parts: 4 packed prompts of up to 8192, window 1024 and 4 sinks, 32 / 8
-//     heads of 128, bf16, with the log-sum-exp: 275 to 295 us (the least and the median of 60 in a row, up to 357 as the clock gives), 740 to
-//     800 TFLOP/s of the pairs that are seen, matrix cores 42% busy.
+//     heads of 128, bf16, with the log-sum-exp: 267 to 294 us (the least and the median of 60 in a row, up to 357 as the clock gives), 745 to
+//     820 TFLOP/s of the pairs that are seen, matrix cores 42% busy.
 //   * steps: reading K and V. 16 of up to 4095 tokens, 32 / 8 heads of 128, bf16, pages of 16: 28 us, 4.7 TB/s, and 4.5 of
 //     merge; 64 of up to 16000, e4m3: 198 us, 5.3 TB/s.
 // Tried and dropped: writing e4m3's converted pairs in an order without bank conflicts (10% of the cycles have one; the
